@@ -517,6 +517,39 @@ typedef struct b200_xent_args {
 int b200_xent_fwd(const b200_xent_args *args, void *stream);
 int b200_xent_bwd(const b200_xent_args *args, void *stream);
 
+/* ------------------------------------------------------------------------
+ * Softmax cross entropy of hidden weight^T without the logits (lrnnx has no loss: its LM
+ * returns logits, lrnnx/architectures/language_model.py:615-727).  With z = hidden weight^T:
+ *   lse[r] = log sum_v exp z[r, v],   loss of a row = lse[r] - z[r, labels[r]]
+ * A row whose label is ignore_index, or outside [0, classes), has no loss and no gradient.
+ *   hidden (rows, features), weight (classes, features): dtype, features contiguous
+ *   labels int64 (rows);  lse float32 (rows): written by the forward, read by the backward
+ *   reduction 0: loss float32 (rows), dloss float32 (rows)
+ *             1: loss and dloss float32 (1), the mean over the labels that are not ignore_index;
+ *                count float32 (1), their number and at least 1, written by the forward, read by the backward
+ *             2: loss and dloss float32 (1), the sum
+ *   backward: dhidden (rows, features), dweight (classes, features), either nullable, written whole
+ *   work: device workspace, 256-byte aligned, b200_lce_{fwd,bwd}_work_bytes() bytes (for the
+ *   backward with dhidden / dweight set as for the call)
+ * ------------------------------------------------------------------------ */
+typedef struct b200_lce_args {
+  int64_t rows, ignore_index;
+  int32_t classes, features, dtype, reduction;
+  const void *hidden, *weight, *labels;
+  int64_t hidden_rs, weight_rs;
+  void *lse, *loss, *count;
+  const void *dloss;
+  void *dhidden, *dweight;
+  int64_t dhidden_rs, dweight_rs;
+  void *work;
+  int64_t work_bytes;
+} b200_lce_args;
+
+int64_t b200_lce_fwd_work_bytes(const b200_lce_args *args);
+int64_t b200_lce_bwd_work_bytes(const b200_lce_args *args);
+int b200_lce_fwd(const b200_lce_args *args, void *stream);
+int b200_lce_bwd(const b200_lce_args *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

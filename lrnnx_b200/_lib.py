@@ -23,6 +23,7 @@ LIB_PATH = _PKG / "lib" / "liblrnnx_b200.so"
 ENTRY_POINTS = (
     "b200_last_error", "b200_abi_version", "b200_sizeof", "b200_device_status", "b200_s4_bwd_scratch_bytes",
     "b200_selscan_stage_states", "b200_selscan_bwd_work_bytes",
+    "b200_lce_fwd_work_bytes", "b200_lce_bwd_work_bytes",
     "b200_selscan_fwd", "b200_selscan_bwd", "b200_selscan_fixup", "b200_selscan_fold",
     "b200_selscan_adjoint_summary",
     "b200_simpscan_fwd", "b200_simpscan_bwd",
@@ -31,6 +32,7 @@ ENTRY_POINTS = (
     "b200_conv1d_fwd", "b200_conv1d_bwd", "b200_conv1d_update", "b200_rmsnorm_fwd", "b200_rmsnorm_bwd",
     "b200_cgemm_wx", "b200_cgemm_planes", "b200_cgemm_grad",
     "b200_xent_fwd", "b200_xent_bwd", "b200_skinny_linear",
+    "b200_lce_fwd", "b200_lce_bwd",
 )
 
 _SCALARS = {"int32_t": ctypes.c_int32, "int64_t": ctypes.c_int64, "uint32_t": ctypes.c_uint32,
@@ -120,9 +122,14 @@ def lib() -> ctypes.CDLL:
     handle.b200_s4_bwd_scratch_bytes.argtypes = [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32]
     handle.b200_selscan_stage_states.restype = ctypes.c_int
     handle.b200_selscan_stage_states.argtypes = [ctypes.c_void_p]
-    handle.b200_selscan_bwd_work_bytes.restype = ctypes.c_int64
-    handle.b200_selscan_bwd_work_bytes.argtypes = [ctypes.c_void_p]
-    for fn in ENTRY_POINTS[7:]:
+    sizes = [fn for fn in ENTRY_POINTS if fn.endswith("_work_bytes")]
+    for fn in sizes:
+        f = getattr(handle, fn)
+        f.restype = ctypes.c_int64
+        f.argtypes = [ctypes.c_void_p]
+    for fn in ENTRY_POINTS[6:]:
+        if fn in sizes:
+            continue
         f = getattr(handle, fn)
         f.restype = ctypes.c_int
         f.argtypes = [ctypes.c_void_p, ctypes.c_void_p]

@@ -42,7 +42,7 @@ using namespace b200;
 extern "C" {
 
 const char *b200_last_error(void) { return g_err; }
-int b200_abi_version(void) { return 7; }
+int b200_abi_version(void) { return 8; }
 
 // size of an argument block as this library was compiled; lets a binding
 // verify its own struct layout before the first call
@@ -62,6 +62,7 @@ int b200_sizeof(const char *name) {
   if (!strcmp(name, "b200_cgemm_planes_args")) return (int)sizeof(b200_cgemm_planes_args);
   if (!strcmp(name, "b200_cgemm_grad_args")) return (int)sizeof(b200_cgemm_grad_args);
   if (!strcmp(name, "b200_xent_args")) return (int)sizeof(b200_xent_args);
+  if (!strcmp(name, "b200_lce_args")) return (int)sizeof(b200_lce_args);
   if (!strcmp(name, "b200_skinny_linear_args")) return (int)sizeof(b200_skinny_linear_args);
   return -1;
 }

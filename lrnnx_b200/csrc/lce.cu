@@ -1,0 +1,767 @@
+// Softmax cross entropy of hidden W^T without the logits (b200_lce_fwd / b200_lce_bwd), sm_100a.
+//
+//     z = H W^T   (rows x classes, H rows x features, W classes x features)
+//     lse_r = log sum_v exp z_rv,     loss_r = lse_r - z_{r, label_r}
+//     dz_rv = s_r (exp(z_rv - lse_r) - [v = label_r]),     dH = dz W,     dW = dz^T H
+//
+// The forward is one product whose tiles never leave the SM: each 128 x 256 tile of z is reduced to a running maximum
+// and sum of a row's half (float32, natural units scaled by log2 e), a second kernel joins them.  The backward makes z
+// again in pieces of the vocabulary, writes a piece of dz in the operands' type and multiplies it from both sides; the
+// piece's columns are chosen so that dz stays below kPieceBytes.  dz is kept in units of the largest |s_r|, so that a
+// float16 dz neither overflows under a scaled loss nor vanishes under a mean over many rows; the products are scaled back
+// in 32 bits.  s_r = 0 (ignored labels) makes an exact zero row.
+//
+// The products run on tcgen05 with accumulators in TMEM, one kernel with three epilogues.  Persistent thread blocks take
+// tiles in turn: warp 0 issues TMA loads into a 4-stage ring (64 of the contraction a stage), warp 1 issues the MMAs,
+// warps 4-11 empty one of two 256-column accumulators while the other is filled.  Either operand may have the contraction
+// along its rows (z) or across them (dz W, dz^T H): both are 128-byte swizzled tiles, of K-major or of MN-major layout.
+//
+// float32 operands are split into three bfloat16 (8 bits of mantissa each) and multiplied as six products of the
+// planes, the small ones first; what is left out is below 2^-24.  The tensor core truncates when it adds into its
+// accumulator, an error to one side that grows with the length of the chain, so that long contractions are cut into
+// chains of kSegSteps whose sums are added up in float32, rounded to nearest.  (An infinite float32 operand gives NaN
+// where its product with the rest of a split is none.)
+#include "common.cuh"
+#include "dispatch.h"
+#include "tc_common.cuh"
+#include <cstring>
+
+namespace b200 {
+namespace {
+
+using namespace tc;
+
+__device__ int g_lce_status = 0;
+
+constexpr int TM = 128, TN = 256, TK = 64;       // tile of the result, contraction of a stage
+constexpr int NST = 4;
+constexpr int A_BYTES = TM * TK * 2, B_BYTES = TN * TK * 2;
+constexpr int ST_BYTES = A_BYTES + B_BYTES;      // 48 KB
+constexpr int STAGING = 32 * 128;                // a warp's 32 rows x 64 columns of dz on their way out
+constexpr int LCE_THREADS = 384;                 // 4 warps that issue, 8 that empty accumulators
+constexpr int LCE_SMEM = NST * ST_BYTES + 8 * STAGING + 1024;
+constexpr uint32_t LCE_WAIT = 1u << 24;
+constexpr int64_t kPieceBytes = int64_t(1) << 30;
+constexpr int kSegSteps = 16;                    // float32 only: stages (of 64) in one accumulation chain's leading product
+
+enum { EPI_LSE = 0, EPI_DZ = 1, EPI_OUT = 2 };
+
+struct LceGemm {
+  CUtensorMap a, b, out;       // (inner, rows, plane); out: dz
+  int mt, nt, nk;              // tiles, stages of 64 along the contraction
+  int seg;                     // stages a chain, nk where it is not cut
+  int passes;                  // 1, or 6 products of the planes of a split
+  int a_mn, b_mn;              // operand has the contraction across its rows
+  int b_row0;                  // first row (K-major) of the piece within W
+  int bk_row0;                 // the same where W's rows are the contraction
+  uint32_t idesc;
+  // epilogues
+  int rows, cols;              // of the result
+  int64_t classes, ignore_index;
+  const int64_t *labels;
+  float2 *part;                // LSE: (slot, rows)
+  float *target;               // LSE: (rows)
+  const float *lse, *rs, *common;
+  int col0;                    // first class of this piece
+  int dtype;                   // of the operands and gradients
+  float *acc;                  // OUT: float32 sums, pitch acc_rs
+  int64_t acc_rs;
+  void *dst;
+  int64_t dst_rs;
+  int add, last;               // OUT: acc holds earlier pieces; this is the last one
+};
+
+__device__ __forceinline__ void tma_st_3d(const CUtensorMap *map, const void *src, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x),
+               "r"(y), "r"(z), "r"(smem_u32(src))
+               : "memory");
+}
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0)
+      : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+struct LcePipe {
+  uint64_t full[NST], empty[NST], acc_full[2], acc_empty[2];
+  uint32_t tmem_base;
+  int fail;
+};
+
+// planes of a product of splits: the small ones first
+__device__ __forceinline__ int plane_a(int passes, int p) { return passes == 1 ? 0 : (0x021010 >> (4 * (5 - p))) & 15; }
+__device__ __forceinline__ int plane_b(int passes, int p) { return passes == 1 ? 0 : (0x201100 >> (4 * (5 - p))) & 15; }
+
+// The largest |s_r|, which dz is kept in units of; 1 where there is none to divide by.
+__device__ __forceinline__ float unit_of(const float *common) {
+  const float c = *common;
+  return c > 0.f && c < INFINITY ? c : 1.f;
+}
+
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+
+// 64 columns of this warp's 32 rows, a row per lane, into the swizzled staging tile and out
+template <typename T>
+__device__ __forceinline__ void store_dz(const LceGemm &p, unsigned char *staging, const float (&v)[64], int col, int row, int plane, int lane) {
+  if (lane == 0) bulk_wait_read<0>();
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    uint4 w;
+    w.x = pack2<T>(v[8 * j], v[8 * j + 1]);
+    w.y = pack2<T>(v[8 * j + 2], v[8 * j + 3]);
+    w.z = pack2<T>(v[8 * j + 4], v[8 * j + 5]);
+    w.w = pack2<T>(v[8 * j + 6], v[8 * j + 7]);
+    *reinterpret_cast<uint4 *>(staging + lane * 128 + ((j ^ (lane & 7)) << 4)) = w;
+  }
+  fence_proxy_async();
+  __syncwarp();
+  if (lane == 0 && col < p.cols && row < p.rows) {
+    tma_st_3d(&p.out, staging, col, row, plane);
+    bulk_commit();
+  }
+}
+
+template <typename T> __device__ __forceinline__ void store_row(T *dst, const float (&v)[32], int n, bool vec);
+template <> __device__ __forceinline__ void store_row<float>(float *dst, const float (&v)[32], int n, bool vec) {
+  if (vec && n >= 32) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) reinterpret_cast<float4 *>(dst)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j < n) dst[j] = v[j];
+  }
+}
+template <typename T> __device__ __forceinline__ void store_row16(T *dst, const float (&v)[32], int n, bool vec) {
+  if (vec && n >= 32) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      reinterpret_cast<uint4 *>(dst)[j] = make_uint4(pack2<T>(v[8 * j], v[8 * j + 1]), pack2<T>(v[8 * j + 2], v[8 * j + 3]),
+                                                     pack2<T>(v[8 * j + 4], v[8 * j + 5]), pack2<T>(v[8 * j + 6], v[8 * j + 7]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j < n) {
+        const uint32_t w = pack2<T>(v[j], 0.f);
+        reinterpret_cast<uint16_t *>(dst)[j] = (uint16_t)w;
+      }
+  }
+}
+
+template <int EPI>
+__global__ void __launch_bounds__(LCE_THREADS, 1) lce_gemm_kernel(const __grid_constant__ LceGemm p) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ LcePipe pipe;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tiles = p.mt * p.nt;
+  if (tid == 0) {
+    for (int s = 0; s < NST; ++s) {
+      mbar_init(&pipe.full[s], 1);
+      mbar_init(&pipe.empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&pipe.acc_full[s], 1);
+      mbar_init(&pipe.acc_empty[s], 8);
+    }
+    pipe.fail = 0;
+    mbar_fence_init();
+    fence_proxy_async();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&pipe.tmem_base)), "r"(2 * TN) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = pipe.tmem_base;
+  // z and dz: neighbouring blocks share W's tile; products of dz: they share dz's
+  const auto m_of = [&](int t) { return EPI == EPI_OUT ? t / p.nt : t % p.mt; };
+  const auto n_of = [&](int t) { return EPI == EPI_OUT ? t % p.nt : t / p.mt; };
+
+  if (warp == 0 && lane == 0) {
+    // ------------------------------------------------------------------ loads
+    int g = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      const int m0 = m_of(t) * TM, n0 = n_of(t) * TN;
+      for (int k0 = 0; k0 < p.nk && ok; k0 += p.seg) {
+        const int k1 = min(p.nk, k0 + p.seg);
+        for (int ps = 0; ps < p.passes && ok; ++ps) {
+          const int pa = plane_a(p.passes, ps), pb = plane_b(p.passes, ps);
+          for (int k = k0; k < k1; ++k, ++g) {
+            const int s = g % NST;
+            if (g >= NST && !mbar_wait(&pipe.empty[s], ((g / NST) - 1) & 1, LCE_WAIT)) { ok = false; break; }
+            unsigned char *st = smem + (size_t)s * ST_BYTES;
+            mbar_expect_tx(&pipe.full[s], ST_BYTES);
+            if (p.a_mn) {
+#pragma unroll
+              for (int j = 0; j < TM / 64; ++j) tma_3d(st + j * 8192, &p.a, m0 + 64 * j, k * TK, pa, &pipe.full[s]);
+            } else {
+              tma_3d(st, &p.a, k * TK, m0, pa, &pipe.full[s]);
+            }
+            if (p.b_mn) {
+#pragma unroll
+              for (int j = 0; j < TN / 64; ++j) tma_3d(st + A_BYTES + j * 8192, &p.b, n0 + 64 * j, p.bk_row0 + k * TK, pb, &pipe.full[s]);
+            } else {
+              tma_3d(st + A_BYTES, &p.b, k * TK, p.b_row0 + n0, pb, &pipe.full[s]);
+            }
+          }
+        }
+      }
+    }
+    if (!ok) {
+      atomicExch(&pipe.fail, 1);
+      for (int i = max(0, g - NST); i < g; ++i) mbar_wait(&pipe.full[i % NST], (i / NST) & 1, 1u << 16);     // copies in flight
+    }
+  } else if (warp == 1 && lane == 0) {
+    // ------------------------------------------------------------------ products
+    int g = 0, ch = 0;
+    bool ok = true;
+    const uint32_t a_lbo = p.a_mn ? 8192 : 16, b_lbo = p.b_mn ? 8192 : 16;
+    const uint32_t a_step = p.a_mn ? 2048 : 32, b_step = p.b_mn ? 2048 : 32;      // bytes to the next 16 of the contraction
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      for (int k0 = 0; k0 < p.nk && ok; k0 += p.seg, ++ch) {
+        const int n = (min(p.nk, k0 + p.seg) - k0) * p.passes;
+        const uint32_t d = tmem + (ch & 1) * TN;
+        if (ch >= 2 && !mbar_wait(&pipe.acc_empty[ch & 1], ((ch >> 1) - 1) & 1, LCE_WAIT)) { ok = false; break; }
+        tc_fence_after();
+        for (int i = 0; i < n; ++i, ++g) {
+          const int s = g % NST;
+          if (!mbar_wait(&pipe.full[s], (g / NST) & 1, LCE_WAIT)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t st = smem_u32(smem + (size_t)s * ST_BYTES);
+#pragma unroll
+          for (int kk = 0; kk < TK / 16; ++kk)
+            mma_f16(d, smem_desc(st + kk * a_step, a_lbo, 1024, 2), smem_desc(st + A_BYTES + kk * b_step, b_lbo, 1024, 2), p.idesc, i > 0 || kk > 0 ? 1u : 0u);
+          mma_commit(&pipe.empty[s]);
+        }
+        if (ok) mma_commit(&pipe.acc_full[ch & 1]);
+      }
+    }
+    if (!ok) atomicExch(&pipe.fail, 1);
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------------ epilogues
+    const int q = warp & 3, half = (warp - 4) >> 2;
+    unsigned char *staging = smem + NST * ST_BYTES + (warp - 4) * STAGING;
+    int ch = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      const int m0 = m_of(t) * TM, n0 = n_of(t) * TN;
+      const int row = m0 + q * 32 + lane, c0 = n0 + half * (TN / 2);      // this thread's row and 128 columns
+      const bool in = row < p.rows;
+      for (int k0 = 0; k0 < p.nk; k0 += p.seg, ++ch) {
+        // what the epilogue needs besides is loaded before the wait
+        float lse2 = 0.f, sc = 0.f;
+        int at = -1;                                                     // the label's column within this thread's columns
+        if (EPI != EPI_OUT && in) {
+          const int64_t label = p.labels[row];
+          if (label != p.ignore_index && label >= 0 && label < p.classes) {
+            const int64_t c = label - p.col0 - c0;
+            if (c >= 0 && c < TN / 2) at = (int)c;
+          }
+          if (EPI == EPI_DZ) {
+            lse2 = p.lse[row] * kLog2e;
+            sc = p.rs[row] / unit_of(p.common);
+          }
+        }
+        if (!mbar_wait(&pipe.acc_full[ch & 1], (ch >> 1) & 1, LCE_WAIT)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t ta = tmem + (ch & 1) * TN + ((uint32_t)(q * 32) << 16) + half * (TN / 2);
+        if constexpr (EPI == EPI_LSE) {
+          float m = -INFINITY, sum = 0.f, target = 0.f;                   // m in units of log2
+#pragma unroll
+          for (int c = 0; c < TN / 64; ++c) {
+            float v[32];
+            __syncwarp();
+            tmem_ld32(ta + c * 32, v);
+            const int left = p.cols - (c0 + c * 32);
+            if (left < 32) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = j < left ? v[j] : -INFINITY;
+            }
+            if ((at >> 5) == c) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) target = j == (at & 31) ? v[j] : target;
+            }
+            float vm = v[0];
+#pragma unroll
+            for (int j = 1; j < 32; ++j) vm = fmaxf(vm, v[j]);
+            const float nm = fmaxf(m, vm * kLog2e), off = nm == -INFINITY ? 0.f : nm;
+            float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              s0 += ex2(fmaf(v[j], kLog2e, -off));
+              s1 += ex2(fmaf(v[j + 1], kLog2e, -off));
+            }
+            sum = fmaf(sum, ex2(m - off), s0 + s1);                       // the first time 0 * 2^-inf
+            m = nm;
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&pipe.acc_empty[ch & 1]);
+          if (in) {
+            p.part[(int64_t)(n_of(t) * 2 + half) * p.rows + row] = make_float2(m, sum);
+            if (at >= 0) p.target[row] = target;
+          }
+        } else if constexpr (EPI == EPI_DZ) {
+#pragma unroll 1
+          for (int c = 0; c < TN / 128; ++c) {
+            float v[64];
+            __syncwarp();
+            tmem_ld32(ta + c * 64, *reinterpret_cast<float(*)[32]>(v));
+            tmem_ld32(ta + c * 64 + 32, *reinterpret_cast<float(*)[32]>(v + 32));
+#pragma unroll
+            for (int j = 0; j < 64; ++j) v[j] = ex2(fmaf(v[j], kLog2e, -lse2));
+            if ((at >> 6) == c) {
+#pragma unroll
+              for (int j = 0; j < 64; ++j) v[j] = j == (at & 63) ? v[j] - 1.f : v[j];
+            }
+#pragma unroll
+            for (int j = 0; j < 64; ++j) v[j] = sc == 0.f ? 0.f : v[j] * sc;
+            const int col = c0 + c * 64, r0 = m0 + q * 32;
+            if (p.dtype == B200_BF16) store_dz<__nv_bfloat16>(p, staging, v, col, r0, 0, lane);
+            else if (p.dtype == B200_F16) store_dz<__half>(p, staging, v, col, r0, 0, lane);
+            else {
+#pragma unroll 1
+              for (int pl = 0; pl < 3; ++pl) {
+                store_dz<__nv_bfloat16>(p, staging, v, col, r0, pl, lane);
+#pragma unroll
+                for (int j = 0; j < 64; ++j) v[j] -= __bfloat162float(__float2bfloat16_rn(v[j]));
+              }
+            }
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&pipe.acc_empty[ch & 1]);
+        } else {
+          const bool first = k0 == 0 && !p.add, last = k0 + p.seg >= p.nk && p.last;
+          const float unit = unit_of(p.common);
+          const bool vec = (p.dst_rs * (p.dtype == B200_F32 ? 4 : 2)) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.dst) & 15) == 0;
+#pragma unroll 1
+          for (int c = 0; c < TN / 64; ++c) {
+            float v[32];
+            __syncwarp();
+            tmem_ld32(ta + c * 32, v);
+            const int col = c0 + c * 32, n = min(32, p.cols - col);
+            if (!in || n <= 0) continue;
+            if (!first) {
+              const float4 *o = reinterpret_cast<const float4 *>(p.acc + (int64_t)row * p.acc_rs + col);
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (4 * j < n) {
+                  const float4 w = o[j];
+                  v[4 * j] += w.x;
+                  v[4 * j + 1] += w.y;
+                  v[4 * j + 2] += w.z;
+                  v[4 * j + 3] += w.w;
+                }
+            }
+            if (!last) {
+              float4 *o = reinterpret_cast<float4 *>(p.acc + (int64_t)row * p.acc_rs + col);
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (4 * j < n) o[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] *= unit;
+              const int64_t i = (int64_t)row * p.dst_rs + col;
+              if (p.dtype == B200_F32) store_row<float>(reinterpret_cast<float *>(p.dst) + i, v, n, vec);
+              else if (p.dtype == B200_BF16) store_row16<__nv_bfloat16>(reinterpret_cast<__nv_bfloat16 *>(p.dst) + i, v, n, vec);
+              else store_row16<__half>(reinterpret_cast<__half *>(p.dst) + i, v, n, vec);
+            }
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&pipe.acc_empty[ch & 1]);
+        }
+      }
+    }
+    if (EPI == EPI_DZ && lane == 0) bulk_wait<0>();
+    if (!ok) atomicExch(&pipe.fail, 1);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * TN) : "memory");
+  if (tid == 0 && pipe.fail) atomicExch(&g_lce_status, 7);
+}
+
+// Rows of 16-byte pitch from rows of any: a copy for 16-bit types, three bfloat16 planes for float32.
+__global__ void __launch_bounds__(256) lce_pack_kernel(const void *src, int64_t rs, int64_t rows, int cols, int pitch, int split, uint16_t *dst) {
+  const int64_t n = rows * (pitch / 2);
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / (pitch / 2);
+    const int c = (int)(i - r * (pitch / 2)) * 2;
+    if (!split) {
+      const uint16_t *s = reinterpret_cast<const uint16_t *>(src) + r * rs;
+      const uint32_t lo = c < cols ? s[c] : 0, hi = c + 1 < cols ? s[c + 1] : 0;
+      *reinterpret_cast<uint32_t *>(dst + r * pitch + c) = lo | hi << 16;
+    } else {
+      const float *s = reinterpret_cast<const float *>(src) + r * rs;
+      float a = c < cols ? s[c] : 0.f, b = c + 1 < cols ? s[c + 1] : 0.f;
+#pragma unroll
+      for (int pl = 0; pl < 3; ++pl) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+        *reinterpret_cast<__nv_bfloat162 *>(dst + ((int64_t)pl * rows + r) * pitch + c) = v;
+        a = isfinite(a) ? a - __bfloat162float(v.x) : 0.f;
+        b = isfinite(b) ? b - __bfloat162float(v.y) : 0.f;
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ bool is_target(int64_t label, int64_t ignore, int classes) { return label != ignore && label >= 0 && label < classes; }
+
+// Joins the partial maxima and sums of 32 rows: a warp reads the same slot of 32 rows.
+__global__ void __launch_bounds__(256) lce_join_kernel(const float2 *part, const float *target, const int64_t *labels, int64_t ignore, int classes, int rows,
+                                                      int slots, float *lse, float *loss) {
+  __shared__ float2 sh[8][32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, row = blockIdx.x * 32 + lane;
+  float m = -INFINITY, s = 0.f;
+  if (row < rows) {
+#pragma unroll 4
+    for (int i = w; i < slots; i += 8) {
+      const float2 v = part[(int64_t)i * rows + row];
+      const float nm = fmaxf(m, v.x), off = nm == -INFINITY ? 0.f : nm;
+      s = s * ex2(m - off) + v.y * ex2(v.x - off);
+      m = nm;
+    }
+  }
+  sh[w][lane] = make_float2(m, s);
+  __syncthreads();
+  if (w == 0 && row < rows) {
+    for (int i = 1; i < 8; ++i) {
+      const float2 v = sh[i][lane];
+      const float nm = fmaxf(m, v.x), off = nm == -INFINITY ? 0.f : nm;
+      s = s * ex2(m - off) + v.y * ex2(v.x - off);
+      m = nm;
+    }
+    const float l = m / kLog2e + logf(s);
+    lse[row] = l;
+    loss[row] = is_target(labels[row], ignore, classes) ? l - target[row] : 0.f;
+  }
+}
+
+// Sum of the rows' losses (over the count of labels that are not ignored), one block in a fixed order.
+__global__ void __launch_bounds__(1024) lce_sum_kernel(const float *loss, const int64_t *labels, int64_t ignore, int rows, int mean, float *out, float *count) {
+  __shared__ double ss[32];
+  __shared__ int sc[32];
+  double s = 0.0;
+  int n = 0;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < rows; i += 1024) {
+    s += (double)loss[i];
+    n += labels[i] != ignore;
+  }
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    s += __shfl_xor_sync(0xffffffffu, s, o);
+    n += __shfl_xor_sync(0xffffffffu, n, o);
+  }
+  if (lane == 0) { ss[w] = s; sc[w] = n; }
+  __syncthreads();
+  if (w == 0) {
+    s = ss[lane];
+    n = sc[lane];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      s += __shfl_xor_sync(0xffffffffu, s, o);
+      n += __shfl_xor_sync(0xffffffffu, n, o);
+    }
+    if (lane == 0) {
+      const int c = n > 0 ? n : 1;
+      if (count) *count = (float)c;
+      if (out) *out = (float)(mean ? s / c : s);
+    }
+  }
+}
+
+// s_r, and the largest |s_r| by an atomic maximum of its bits (any order gives the same; the word was cleared).
+__global__ void __launch_bounds__(256) lce_scale_kernel(const float *dloss, int per_row, const float *count, const int64_t *labels, int64_t ignore, int classes,
+                                                       int rows, float *rs, unsigned *common) {
+  const int r = blockIdx.x * 256 + threadIdx.x;
+  float s = 0.f;
+  if (r < rows) {
+    if (is_target(labels[r], ignore, classes)) s = dloss[per_row ? r : 0] / (count ? *count : 1.f);
+    rs[r] = s;
+  }
+  const unsigned m = __reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(s)));
+  if ((threadIdx.x & 31) == 0 && m) atomicMax(common, m);
+}
+
+// ------------------------------------------------------------------------------------------------ host
+
+int64_t up(int64_t n, int64_t unit) { return (n + unit - 1) / unit * unit; }
+
+bool map16(CUtensorMap *m, int dtype, const void *base, uint64_t inner, uint64_t rows, uint64_t pitch, int planes, uint32_t box_rows) {
+  EncodeTiledFn enc = encoder();
+  if (!enc) return false;
+  const cuuint64_t dims[3] = {inner, rows, (cuuint64_t)planes};
+  const cuuint64_t strides[2] = {pitch * 2, pitch * 2 * rows};
+  const cuuint32_t box[3] = {64, box_rows, 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  return enc(m, dtype == B200_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(base), dims, strides, box, estr,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// how the operands are read: in place where their rows allow TMA, else from packed (or split) copies
+struct Plan {
+  int planes, Dp;
+  bool pack_h, pack_w;
+  int64_t pack_bytes_h, pack_bytes_w;
+  int piece, n_pieces;            // columns of dz at a time (a multiple of 256), pieces
+  int64_t dz_pitch, dz_bytes, acc_h_bytes, acc_w_bytes;
+  int64_t Da;                     // pitch of the float32 sums
+  int seg;
+};
+
+bool in_place(const void *p, int64_t rs, int cols) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && rs % 8 == 0 && rs >= cols && rs < (int64_t(1) << 36);
+}
+
+Plan plan_of(const b200_lce_args &a) {
+  Plan q;
+  const bool f32 = a.dtype == B200_F32;
+  q.planes = f32 ? 3 : 1;
+  q.Dp = (int)up(a.features, 8);
+  q.pack_h = f32 || !in_place(a.hidden, a.hidden_rs, a.features);
+  q.pack_w = f32 || !in_place(a.weight, a.weight_rs, a.features);
+  q.pack_bytes_h = q.pack_h ? up(2 * q.planes * a.rows * q.Dp, 256) : 0;
+  q.pack_bytes_w = q.pack_w ? up(2 * q.planes * (int64_t)a.classes * q.Dp, 256) : 0;
+  q.seg = f32 ? kSegSteps : 1 << 30;
+  q.Da = up(a.features, 4);
+  int64_t most = kPieceBytes / (2 * q.planes * a.rows) / TN * TN;
+  if (most < TN) most = TN;
+  q.n_pieces = (int)((a.classes + most - 1) / most);
+  q.piece = (int)up((a.classes + q.n_pieces - 1) / q.n_pieces, TN);
+  q.n_pieces = (a.classes + q.piece - 1) / q.piece;
+  q.dz_pitch = q.piece;
+  q.dz_bytes = up(2 * q.planes * a.rows * q.dz_pitch, 256);
+  // float32 sums: of dH over the pieces and the chains, of dW over the chains
+  q.acc_h_bytes = f32 || q.n_pieces > 1 ? up(4 * a.rows * q.Da, 256) : 0;
+  q.acc_w_bytes = f32 && (a.rows + TK - 1) / TK > q.seg ? up(4 * (int64_t)q.piece * q.Da, 256) : 0;
+  return q;
+}
+
+int slots_of(const b200_lce_args &a) { return (a.classes + TN - 1) / TN * 2; }
+
+int check_lce(const b200_lce_args &a) {
+  B200_REQUIRE(a.hidden && a.weight && a.labels, B200_ERR_NULL, "lce: hidden, weight and labels must be non-null");
+  B200_REQUIRE(a.rows > 0 && a.classes > 0 && a.features > 0, B200_ERR_SHAPE, "lce: sizes must be positive");
+  B200_REQUIRE(a.dtype == B200_F32 || a.dtype == B200_F16 || a.dtype == B200_BF16, B200_ERR_DTYPE, "lce: unknown dtype %d", a.dtype);
+  B200_REQUIRE(a.reduction >= 0 && a.reduction <= 2, B200_ERR_DTYPE, "lce: unknown reduction %d", a.reduction);
+  B200_REQUIRE(a.rows < (int64_t(1) << 30) && a.classes < (1 << 30) && a.features <= (1 << 20) &&
+                   ((a.rows + TM - 1) / TM) * ((int64_t)(a.classes + TN - 1) / TN) < (int64_t(1) << 30),
+               B200_ERR_SHAPE, "lce: sizes too large (rows %lld, classes %d, features %d)", (long long)a.rows, a.classes, a.features);
+  B200_REQUIRE(a.hidden_rs >= a.features && a.weight_rs >= a.features, B200_ERR_SHAPE, "lce: row pitches must be at least the features");
+  B200_REQUIRE((reinterpret_cast<uintptr_t>(a.work) & 255) == 0, B200_ERR_ALIGN, "lce: work must be 256-byte aligned");
+  return 0;
+}
+
+int pack(const void *src, int64_t rs, int64_t rows, const b200_lce_args &a, const Plan &q, void *dst, cudaStream_t st) {
+  const int64_t n = rows * (q.Dp / 2);
+  const int64_t blocks = (n + 255) / 256, most = (int64_t)sm_count_current() * 32;
+  lce_pack_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, st>>>(src, rs, rows, a.features, q.Dp, a.dtype == B200_F32,
+                                                                            reinterpret_cast<uint16_t *>(dst));
+  return launch_status();
+}
+
+template <int EPI> int launch_gemm(const LceGemm &g, cudaStream_t st) {
+  cudaError_t e = cudaFuncSetAttribute(lce_gemm_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, LCE_SMEM);
+  if (e != cudaSuccess) { set_error("cudaFuncSetAttribute: %s", cudaGetErrorString(e)); return (int)e; }
+  const int tiles = g.mt * g.nt, sms = sm_count_current();
+  lce_gemm_kernel<EPI><<<(unsigned)(tiles < sms ? tiles : sms), LCE_THREADS, LCE_SMEM, st>>>(g);
+  return launch_status();
+}
+
+uint32_t idesc_of(int dtype, bool a_mn, bool b_mn) {
+  const uint32_t f = dtype == B200_F16 ? 0u : 1u;
+  return (1u << 4) | (f << 7) | (f << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((TN >> 3) << 17) | ((TM >> 4) << 24);
+}
+
+struct Operands { const void *h, *w; int64_t h_pitch, w_pitch; };
+
+// z = H W^T for classes c0 .. c0 + cols
+int gemm_z(LceGemm &g, const b200_lce_args &a, const Plan &q, const Operands &o, int c0, int cols) {
+  memset(&g, 0, sizeof(g));
+  B200_REQUIRE(map16(&g.a, a.dtype, o.h, a.features, a.rows, o.h_pitch, q.planes, TM) && map16(&g.b, a.dtype, o.w, a.features, a.classes, o.w_pitch, q.planes, TN),
+               B200_ERR_UNSUPPORTED, "lce: tensor-map encoding failed");
+  g.mt = (int)((a.rows + TM - 1) / TM);
+  g.nt = (cols + TN - 1) / TN;
+  g.nk = (a.features + TK - 1) / TK;
+  g.seg = g.nk;
+  g.passes = q.planes == 3 ? 6 : 1;
+  g.b_row0 = c0;
+  g.idesc = idesc_of(a.dtype, false, false);
+  g.rows = (int)a.rows;
+  g.cols = cols;
+  g.classes = a.classes;
+  g.ignore_index = a.ignore_index;
+  g.labels = reinterpret_cast<const int64_t *>(a.labels);
+  g.col0 = c0;
+  g.dtype = a.dtype;
+  return 0;
+}
+
+}  // namespace
+
+int lce_status_read() {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_lce_status, sizeof(int)) != cudaSuccess) return -1;
+  return v;
+}
+
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" int64_t b200_lce_fwd_work_bytes(const b200_lce_args *args) {
+  if (!args || check_lce(*args)) return 0;
+  const b200_lce_args &a = *args;
+  const Plan q = plan_of(a);
+  return q.pack_bytes_h + q.pack_bytes_w + up(8 * a.rows * slots_of(a), 256) + 2 * up(4 * a.rows, 256);
+}
+
+extern "C" int64_t b200_lce_bwd_work_bytes(const b200_lce_args *args) {
+  if (!args || check_lce(*args)) return 0;
+  const b200_lce_args &a = *args;
+  const Plan q = plan_of(a);
+  return q.pack_bytes_h + q.pack_bytes_w + q.dz_bytes + (a.dhidden ? q.acc_h_bytes : 0) + (a.dweight ? q.acc_w_bytes : 0) + up(4 * a.rows, 256) + 256;
+}
+
+extern "C" int b200_lce_fwd(const b200_lce_args *args, void *stream) {
+  B200_REQUIRE(args, B200_ERR_NULL, "lce_fwd: null argument block");
+  const b200_lce_args &a = *args;
+  if (int e = check_lce(a)) return e;
+  B200_REQUIRE(a.lse && a.loss && a.work && (a.reduction != 1 || a.count), B200_ERR_NULL, "lce_fwd: lse, loss, work and (for a mean) count must be non-null");
+  const Plan q = plan_of(a);
+  B200_REQUIRE(a.work_bytes >= b200_lce_fwd_work_bytes(args), B200_ERR_TOO_LARGE, "lce_fwd: work has %lld bytes, %lld are needed", (long long)a.work_bytes,
+               (long long)b200_lce_fwd_work_bytes(args));
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  unsigned char *w = reinterpret_cast<unsigned char *>(a.work);
+  Operands o = {a.hidden, a.weight, a.hidden_rs, a.weight_rs};
+  if (q.pack_h) { o.h = w; o.h_pitch = q.Dp; if (int e = pack(a.hidden, a.hidden_rs, a.rows, a, q, w, st)) return e; }
+  w += q.pack_bytes_h;
+  if (q.pack_w) { o.w = w; o.w_pitch = q.Dp; if (int e = pack(a.weight, a.weight_rs, a.classes, a, q, w, st)) return e; }
+  w += q.pack_bytes_w;
+  LceGemm g;
+  if (int e = gemm_z(g, a, q, o, 0, a.classes)) return e;
+  g.part = reinterpret_cast<float2 *>(w);
+  w += up(8 * a.rows * slots_of(a), 256);
+  g.target = reinterpret_cast<float *>(w);
+  w += up(4 * a.rows, 256);
+  float *row_loss = a.reduction == 0 ? reinterpret_cast<float *>(a.loss) : reinterpret_cast<float *>(w);
+  if (int e = launch_gemm<EPI_LSE>(g, st)) return e;
+  lce_join_kernel<<<(unsigned)((a.rows + 31) / 32), 256, 0, st>>>(g.part, g.target, g.labels, a.ignore_index, a.classes, (int)a.rows, slots_of(a),
+                                                                reinterpret_cast<float *>(a.lse), row_loss);
+  if (int e = launch_status()) return e;
+  if (a.reduction != 0)
+    lce_sum_kernel<<<1, 1024, 0, st>>>(row_loss, g.labels, a.ignore_index, (int)a.rows, a.reduction == 1, reinterpret_cast<float *>(a.loss),
+                                       reinterpret_cast<float *>(a.count));
+  return launch_status();
+}
+
+extern "C" int b200_lce_bwd(const b200_lce_args *args, void *stream) {
+  B200_REQUIRE(args, B200_ERR_NULL, "lce_bwd: null argument block");
+  const b200_lce_args &a = *args;
+  if (int e = check_lce(a)) return e;
+  B200_REQUIRE(a.lse && a.dloss && a.work && (a.reduction != 1 || a.count), B200_ERR_NULL, "lce_bwd: lse, dloss, work and (for a mean) count must be non-null");
+  B200_REQUIRE(a.dhidden || a.dweight, B200_ERR_NULL, "lce_bwd: dhidden or dweight must be non-null");
+  B200_REQUIRE((!a.dhidden || a.dhidden_rs >= a.features) && (!a.dweight || a.dweight_rs >= a.features), B200_ERR_SHAPE,
+               "lce_bwd: row pitches must be at least the features");
+  const Plan q = plan_of(a);
+  B200_REQUIRE(a.work_bytes >= b200_lce_bwd_work_bytes(args), B200_ERR_TOO_LARGE, "lce_bwd: work has %lld bytes, %lld are needed", (long long)a.work_bytes,
+               (long long)b200_lce_bwd_work_bytes(args));
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  unsigned char *w = reinterpret_cast<unsigned char *>(a.work);
+  Operands o = {a.hidden, a.weight, a.hidden_rs, a.weight_rs};
+  if (q.pack_h) { o.h = w; o.h_pitch = q.Dp; if (int e = pack(a.hidden, a.hidden_rs, a.rows, a, q, w, st)) return e; }
+  w += q.pack_bytes_h;
+  if (q.pack_w) { o.w = w; o.w_pitch = q.Dp; if (int e = pack(a.weight, a.weight_rs, a.classes, a, q, w, st)) return e; }
+  w += q.pack_bytes_w;
+  void *dz = w;
+  w += q.dz_bytes;
+  float *acc_h = reinterpret_cast<float *>(w);
+  if (a.dhidden) w += q.acc_h_bytes;
+  float *acc_w = reinterpret_cast<float *>(w);
+  if (a.dweight) w += q.acc_w_bytes;
+  float *rs = reinterpret_cast<float *>(w);
+  w += up(4 * a.rows, 256);
+  float *common = reinterpret_cast<float *>(w);
+  cudaError_t ce = cudaMemsetAsync(common, 0, 4, st);
+  if (ce != cudaSuccess) { set_error("cudaMemsetAsync: %s", cudaGetErrorString(ce)); return (int)ce; }
+  lce_scale_kernel<<<(unsigned)((a.rows + 255) / 256), 256, 0, st>>>(reinterpret_cast<const float *>(a.dloss), a.reduction == 0,
+                                                                    a.reduction == 1 ? reinterpret_cast<const float *>(a.count) : nullptr,
+                                                                    reinterpret_cast<const int64_t *>(a.labels), a.ignore_index, a.classes, (int)a.rows, rs,
+                                                                    reinterpret_cast<unsigned *>(common));
+  if (int e = launch_status()) return e;
+  const int esz = a.dtype == B200_F32 ? 4 : 2;
+  for (int pc = 0; pc < q.n_pieces; ++pc) {
+    const int c0 = pc * q.piece, cols = a.classes - c0 < q.piece ? a.classes - c0 : q.piece;
+    LceGemm g;
+    if (int e = gemm_z(g, a, q, o, c0, cols)) return e;
+    B200_REQUIRE(map16(&g.out, a.dtype, dz, cols, a.rows, q.dz_pitch, q.planes, 32), B200_ERR_UNSUPPORTED, "lce: tensor-map encoding failed");
+    g.lse = reinterpret_cast<const float *>(a.lse);
+    g.rs = rs;
+    g.common = common;
+    if (int e = launch_gemm<EPI_DZ>(g, st)) return e;
+    g.seg = q.seg;
+    g.nt = (a.features + TN - 1) / TN;
+    g.cols = a.features;
+    g.acc_rs = q.Da;
+    g.b_mn = 1;
+    g.b_row0 = 0;
+    if (a.dhidden) {                                             // dz W: contraction over the piece's classes
+      B200_REQUIRE(map16(&g.a, a.dtype, dz, cols, a.rows, q.dz_pitch, q.planes, TM) && map16(&g.b, a.dtype, o.w, a.features, a.classes, o.w_pitch, q.planes, 64),
+                   B200_ERR_UNSUPPORTED, "lce: tensor-map encoding failed");
+      g.nk = (cols + TK - 1) / TK;
+      if (g.seg > g.nk) g.seg = g.nk;
+      g.a_mn = 0;
+      g.bk_row0 = c0;
+      g.idesc = idesc_of(a.dtype, false, true);
+      g.acc = acc_h;
+      g.dst = a.dhidden;
+      g.dst_rs = a.dhidden_rs;
+      g.add = pc > 0;
+      g.last = pc == q.n_pieces - 1;
+      if (int e = launch_gemm<EPI_OUT>(g, st)) return e;
+    }
+    if (a.dweight) {                                             // dz^T H: contraction over the rows
+      B200_REQUIRE(map16(&g.a, a.dtype, dz, cols, a.rows, q.dz_pitch, q.planes, 64) && map16(&g.b, a.dtype, o.h, a.features, a.rows, o.h_pitch, q.planes, 64),
+                   B200_ERR_UNSUPPORTED, "lce: tensor-map encoding failed");
+      g.mt = (cols + TM - 1) / TM;
+      g.nk = (int)((a.rows + TK - 1) / TK);
+      g.seg = q.seg < g.nk ? q.seg : g.nk;
+      g.a_mn = 1;
+      g.bk_row0 = 0;
+      g.idesc = idesc_of(a.dtype, true, true);
+      g.rows = cols;
+      g.acc = acc_w;
+      g.dst = reinterpret_cast<unsigned char *>(a.dweight) + (int64_t)c0 * a.dweight_rs * esz;
+      g.dst_rs = a.dweight_rs;
+      g.add = 0;
+      g.last = 1;
+      if (int e = launch_gemm<EPI_OUT>(g, st)) return e;
+    }
+  }
+  return 0;
+}
