@@ -550,6 +550,32 @@ int64_t b200_lce_bwd_work_bytes(const b200_lce_args *args);
 int b200_lce_fwd(const b200_lce_args *args, void *stream);
 int b200_lce_bwd(const b200_lce_args *args, void *stream);
 
+/* ------------------------------------------------------------------------
+ * Embedding lookup with a scale, and its gradient by sorted tokens; replaces nn.Embedding in
+ * lrnnx's backbone (lrnnx/architectures/language_model.py:198-240) and the scatter of its backward.
+ *   out[t] = scale weight[ids[t]];  an id outside [0, classes) reads nothing and gives NaN
+ *   dweight[v] = scale sum_{t: ids[t] = v} dout[t], float32 sums in the order of t; zero for other
+ *   rows and for padding_idx (-1: none)
+ *   ids (tokens) int64 (ids_wide 1) or int32;  weight, dweight (classes, features), out, dout
+ *   (tokens, features): dtype, features contiguous;  dweight dense, written whole
+ *   work: device workspace of the backward, 256-byte aligned, b200_embed_bwd_work_bytes() bytes
+ * ------------------------------------------------------------------------ */
+typedef struct b200_embed_args {
+  int64_t tokens, padding_idx;
+  int32_t classes, features, dtype, ids_wide;
+  float scale;
+  int32_t reserved0;
+  const void *ids, *weight, *dout;
+  void *out, *dweight;
+  int64_t weight_rs, out_rs, dout_rs, dweight_rs;
+  void *work;
+  int64_t work_bytes;
+} b200_embed_args;
+
+int64_t b200_embed_bwd_work_bytes(const b200_embed_args *args);
+int b200_embed_fwd(const b200_embed_args *args, void *stream);
+int b200_embed_bwd(const b200_embed_args *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

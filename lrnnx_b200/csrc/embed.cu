@@ -1,0 +1,355 @@
+// Embedding lookup with a scale, and its gradient by sorted tokens (b200_embed_fwd / b200_embed_bwd), sm_100a.
+//
+//     out[t] = scale W[ids[t]],        dW[v] = scale sum over t with ids[t] = v of dout[t]
+//
+// Forward: a copy of rows, 16 bytes a thread; bound by HBM, and by the launch for the few tokens of a decoding step.
+// Backward: the (id, position) pairs are sorted by id, stably (least significant digit first, up to 9 bits a pass), so
+// that rows of one id are added in the order of their positions: no atomics, the same bits every time.  Every 32 sorted
+// pairs are a piece, whatever ids they hold, so a frequent token does not make one block slow: a thread block adds up the
+// runs of equal ids in its piece in float32 and writes a run that lies inside it; what a run crossing borders has in a piece goes to
+// the workspace and is joined by the piece where the run begins.  Each row is rounded once.  Ids outside [0, classes) and the padding id
+// sort behind all others and are not summed.
+#include "common.cuh"
+#include "dispatch.h"
+#include <cstring>
+
+namespace b200 {
+namespace {
+
+constexpr int PIECE = 32;             // sorted pairs a piece
+constexpr int SORT_T = 256, SORT_TILE = 2048, SORT_PER = SORT_TILE / SORT_T;
+constexpr int MAX_BITS = 9, MAX_BINS = 1 << MAX_BITS;
+constexpr int ROW_T = 128;
+
+template <typename T, int VEC> struct Row {
+  // VEC consecutive elements as floats, by one access of 16 bytes where VEC > 1
+  static __device__ __forceinline__ void load(const T *p, float (&v)[VEC]) {
+    if constexpr (VEC == 1) v[0] = (float)*p;
+    else {
+      const uint4 w = __ldg(reinterpret_cast<const uint4 *>(p));
+      const T *e = reinterpret_cast<const T *>(&w);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[i] = (float)e[i];
+    }
+  }
+  static __device__ __forceinline__ void store(T *p, const float (&v)[VEC]) {
+    if constexpr (VEC == 1) *p = T(v[0]);
+    else {
+      uint4 w;
+      T *e = reinterpret_cast<T *>(&w);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) e[i] = T(v[i]);
+      *reinterpret_cast<uint4 *>(p) = w;
+    }
+  }
+};
+
+__device__ __forceinline__ int64_t id_at(const void *ids, int wide, int64_t t) {
+  return wide ? reinterpret_cast<const int64_t *>(ids)[t] : reinterpret_cast<const int32_t *>(ids)[t];
+}
+
+template <typename T, int VEC> __global__ void __launch_bounds__(256) embed_fwd_kernel(const b200_embed_args p) {
+  const int per = (p.features + VEC - 1) / VEC;
+  const int64_t n = p.tokens * per;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t t = n <= 0xffffffffll ? (int64_t)((uint32_t)i / (uint32_t)per) : i / per;
+    const int c = (int)(i - t * per) * VEC;
+    const int64_t id = id_at(p.ids, p.ids_wide, t);
+    float v[VEC];
+    if (id >= 0 && id < p.classes) {
+      Row<T, VEC>::load(reinterpret_cast<const T *>(p.weight) + id * p.weight_rs + c, v);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[j] *= p.scale;
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[j] = __int_as_float(0x7fffffff);      // no such row: NaN
+    }
+    Row<T, VEC>::store(reinterpret_cast<T *>(p.out) + t * p.out_rs + c, v);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ sort
+
+__device__ __forceinline__ uint32_t key_of(const b200_embed_args &p, int64_t t) {
+  const int64_t id = id_at(p.ids, p.ids_wide, t);
+  return id >= 0 && id < p.classes && id != p.padding_idx ? (uint32_t)id : (uint32_t)p.classes;
+}
+
+// Digit counts of a tile, digit-major (the scan over all of them gives each tile's place for each digit).
+__global__ void __launch_bounds__(SORT_T) embed_count_kernel(const b200_embed_args p, const uint32_t *keys, int shift, int bits, uint32_t *hist) {
+  __shared__ uint32_t h[MAX_BINS];
+  const int bins = 1 << bits;
+  for (int i = threadIdx.x; i < bins; i += SORT_T) h[i] = 0;
+  __syncthreads();
+  const int64_t t0 = (int64_t)blockIdx.x * SORT_TILE;
+#pragma unroll
+  for (int i = 0; i < SORT_PER; ++i) {
+    const int64_t t = t0 + i * SORT_T + threadIdx.x;
+    if (t < p.tokens) atomicAdd(&h[((keys ? keys[t] : key_of(p, t)) >> shift) & (bins - 1)], 1u);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < bins; i += SORT_T) hist[(int64_t)i * gridDim.x + blockIdx.x] = h[i];
+}
+
+// Exclusive sums of n counts by one block.
+__global__ void __launch_bounds__(1024) embed_scan_kernel(uint32_t *x, int64_t n) {
+  __shared__ uint32_t ws[32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  uint32_t carry = 0;
+  for (int64_t i0 = 0; i0 < n; i0 += 4096) {
+    const int64_t i = i0 + threadIdx.x * 4;
+    uint32_t v[4], s = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { v[j] = i + j < n ? x[i + j] : 0; s += v[j]; }
+    uint32_t inc = s;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t u = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += u;
+    }
+    if (lane == 31) ws[w] = inc;
+    __syncthreads();
+    uint32_t before = 0, all = 0;
+    for (int j = 0; j < 32; ++j) { const uint32_t u = ws[j]; before += j < w ? u : 0; all += u; }
+    uint32_t e = carry + before + inc - s;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { if (i + j < n) x[i + j] = e; e += v[j]; }
+    carry += all;
+    __syncthreads();
+  }
+}
+
+// Stable placement: a warp takes 256 consecutive pairs, 32 at a time, and counts what it has placed of each digit.
+__global__ void __launch_bounds__(SORT_T) embed_place_kernel(const b200_embed_args p, const uint32_t *keys, const uint32_t *pos, int shift, int bits,
+                                                            const uint32_t *hist, uint32_t *keys_out, uint32_t *pos_out) {
+  __shared__ uint32_t cnt[SORT_T / 32][MAX_BINS];
+  const int bins = 1 << bits, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  for (int i = threadIdx.x; i < bins * (SORT_T / 32); i += SORT_T) cnt[i >> bits][i & (bins - 1)] = 0;
+  __syncthreads();
+  const int64_t t0 = (int64_t)blockIdx.x * SORT_TILE + w * (SORT_PER * 32);
+  uint32_t k[SORT_PER], at[SORT_PER];
+#pragma unroll
+  for (int i = 0; i < SORT_PER; ++i) {
+    const int64_t t = t0 + i * 32 + lane;
+    const bool in = t < p.tokens;
+    k[i] = in ? (keys ? keys[t] : key_of(p, t)) : 0;
+    const uint32_t d = in ? (k[i] >> shift) & (bins - 1) : 0xffffffffu;
+    const uint32_t peers = __match_any_sync(0xffffffffu, d);
+    const uint32_t before = in ? cnt[w][d] : 0;
+    __syncwarp();
+    if (in && (peers >> lane) == 1u) cnt[w][d] = before + __popc(peers);        // the last of the equal lanes
+    __syncwarp();
+    at[i] = before + __popc(peers & ((1u << lane) - 1));
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < bins; i += SORT_T) {
+    uint32_t s = hist[(int64_t)i * gridDim.x + blockIdx.x];
+    for (int j = 0; j < SORT_T / 32; ++j) { const uint32_t c = cnt[j][i]; cnt[j][i] = s; s += c; }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < SORT_PER; ++i) {
+    const int64_t t = t0 + i * 32 + lane;
+    if (t < p.tokens) {
+      const uint32_t o = cnt[w][(k[i] >> shift) & (bins - 1)] + at[i];
+      keys_out[o] = k[i];
+      pos_out[o] = pos ? pos[t] : (uint32_t)t;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ sums
+
+// One piece, ROW_T * VEC columns.  head[piece]: sum of the run that came in from the piece before; tail[piece]: sum of the run that
+// begins here and goes on.  A run that covers the whole piece is a head.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(ROW_T) embed_sum_kernel(const b200_embed_args p, const uint32_t *keys, const uint32_t *pos, float *head, float *tail) {
+  __shared__ uint32_t k[PIECE + 2], at[PIECE];
+  const int64_t s0 = (int64_t)blockIdx.x * PIECE;
+  const int n = (int)min((int64_t)PIECE, p.tokens - s0);
+  if (threadIdx.x < PIECE + 2) {
+    const int64_t i = s0 + threadIdx.x - 1;
+    k[threadIdx.x] = i >= 0 && i < p.tokens ? keys[i] : 0xffffffffu;
+    if (threadIdx.x >= 1 && threadIdx.x <= PIECE) at[threadIdx.x - 1] = i < p.tokens ? pos[i] : 0;
+  }
+  __syncthreads();
+  const int c = (blockIdx.y * ROW_T + threadIdx.x) * VEC;
+  if (c >= p.features) return;
+  const T *dout = reinterpret_cast<const T *>(p.dout) + c;
+  T *dw = reinterpret_cast<T *>(p.dweight) + c;
+  float acc[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
+  bool came_in = k[0] == k[1];
+  for (int i0 = 0; i0 < n; i0 += 8) {
+    float v[8][VEC];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i0 + i < n && k[i0 + i + 1] < (uint32_t)p.classes) Row<T, VEC>::load(dout + (int64_t)at[i0 + i] * p.dout_rs, v[i]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i0 + i >= n) break;
+      const uint32_t key = k[i0 + i + 1];
+      if (key >= (uint32_t)p.classes) return;                 // these sort behind all others
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) acc[j] += v[i][j];
+      const bool ends = k[i0 + i + 2] != key;
+      if (!ends && i0 + i + 1 < n) continue;
+      if (ends && !came_in) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) acc[j] *= p.scale;
+        Row<T, VEC>::store(dw + (int64_t)key * p.dweight_rs, acc);
+      } else {
+        float *o = (came_in ? head : tail) + (int64_t)blockIdx.x * p.features + c;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) o[j] = acc[j];
+      }
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
+      came_in = false;
+    }
+  }
+}
+
+// The runs that cross borders: the piece where one begins adds up its parts, eight interleaved shares of them.
+template <typename T>
+__global__ void __launch_bounds__(256) embed_join_kernel(const b200_embed_args p, const uint32_t *keys, const float *head, const float *tail, int pieces) {
+  __shared__ float sh[8][32];
+  __shared__ int ends;
+  const int piece = blockIdx.x;
+  const int64_t last = (int64_t)piece * PIECE + PIECE - 1;              // of this piece
+  if (last + 1 >= p.tokens) return;
+  const uint32_t key = keys[last];
+  if (key >= (uint32_t)p.classes || keys[last + 1] != key) return;      // nothing goes on
+  const int64_t first = (int64_t)piece * PIECE;
+  if (first > 0 && keys[first - 1] == key) return;                      // it began earlier
+  // the piece that the run ends in: the last whose entry border still has the key
+  if (threadIdx.x == 0) {
+    int lo = piece + 1, hi = pieces - 1;                                // keys are sorted
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (keys[(int64_t)mid * PIECE] == key) lo = mid;
+      else hi = mid - 1;
+    }
+    ends = lo;
+  }
+  __syncthreads();
+  const int to = ends, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  for (int c0 = 0; c0 < p.features; c0 += 32) {
+    const int c = c0 + lane;
+    float s = 0.f;
+    if (c < p.features) {
+      if (w == 0) s = tail[(int64_t)piece * p.features + c];
+#pragma unroll 4
+      for (int i = piece + 1 + w; i <= to; i += 8) s += head[(int64_t)i * p.features + c];
+    }
+    sh[w][lane] = s;
+    __syncthreads();
+    if (w == 0 && c < p.features) {
+#pragma unroll
+      for (int i = 1; i < 8; ++i) s += sh[i][lane];
+      reinterpret_cast<T *>(p.dweight)[(int64_t)key * p.dweight_rs + c] = T(s * p.scale);
+    }
+    __syncthreads();
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+
+int64_t up(int64_t n, int64_t unit) { return (n + unit - 1) / unit * unit; }
+
+struct Sort { int passes, bits; int64_t tiles, pieces; };
+
+Sort sort_of(const b200_embed_args &a) {
+  Sort s;
+  int width = 1;
+  while ((int64_t(1) << width) <= a.classes) ++width;           // keys reach classes
+  s.passes = (width + MAX_BITS - 1) / MAX_BITS;
+  s.bits = (width + s.passes - 1) / s.passes;
+  s.tiles = (a.tokens + SORT_TILE - 1) / SORT_TILE;
+  s.pieces = (a.tokens + PIECE - 1) / PIECE;
+  return s;
+}
+
+int check_embed(const b200_embed_args &a, bool bwd) {
+  B200_REQUIRE(a.ids && (bwd ? a.dout && a.dweight : a.weight && a.out), B200_ERR_NULL, "embed: null operand");
+  B200_REQUIRE(a.tokens > 0 && a.classes > 0 && a.features > 0 && a.tokens < (int64_t(1) << 31) - SORT_TILE && a.classes < (1 << 30), B200_ERR_SHAPE,
+               "embed: sizes must be positive and tokens below 2^31 (tokens %lld, classes %d, features %d)", (long long)a.tokens, a.classes, a.features);
+  B200_REQUIRE(a.dtype == B200_F32 || a.dtype == B200_F16 || a.dtype == B200_BF16, B200_ERR_DTYPE, "embed: unknown dtype %d", a.dtype);
+  return 0;
+}
+
+bool al16(const void *p, int64_t rs, int esz) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && rs * esz % 16 == 0; }
+
+template <typename T> int run_fwd(const b200_embed_args &a, cudaStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  const bool vec = a.features % V == 0 && al16(a.weight, a.weight_rs, sizeof(T)) && al16(a.out, a.out_rs, sizeof(T));
+  const int64_t n = a.tokens * (vec ? a.features / V : a.features), blocks = (n + 255) / 256, most = int64_t(1) << 22;
+  if (vec) embed_fwd_kernel<T, V><<<(unsigned)(blocks < most ? blocks : most), 256, 0, st>>>(a);
+  else embed_fwd_kernel<T, 1><<<(unsigned)(blocks < most ? blocks : most), 256, 0, st>>>(a);
+  return launch_status();
+}
+
+template <typename T> int run_sums(const b200_embed_args &a, const Sort &s, const uint32_t *keys, const uint32_t *pos, float *head, float *tail, cudaStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  const bool vec = a.features % V == 0 && al16(a.dout, a.dout_rs, sizeof(T)) && al16(a.dweight, a.dweight_rs, sizeof(T));
+  const int cols = ROW_T * (vec ? V : 1);
+  const dim3 grid((unsigned)s.pieces, (unsigned)((a.features + cols - 1) / cols));
+  if (vec) embed_sum_kernel<T, V><<<grid, ROW_T, 0, st>>>(a, keys, pos, head, tail);
+  else embed_sum_kernel<T, 1><<<grid, ROW_T, 0, st>>>(a, keys, pos, head, tail);
+  if (int e = launch_status()) return e;
+  if (s.pieces > 1) embed_join_kernel<T><<<(unsigned)s.pieces, 256, 0, st>>>(a, keys, head, tail, (int)s.pieces);
+  return launch_status();
+}
+
+}  // namespace
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" int b200_embed_fwd(const b200_embed_args *args, void *stream) {
+  B200_REQUIRE(args, B200_ERR_NULL, "embed_fwd: null argument block");
+  if (int e = check_embed(*args, false)) return e;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (args->dtype == B200_F32) return run_fwd<float>(*args, st);
+  return args->dtype == B200_F16 ? run_fwd<__half>(*args, st) : run_fwd<__nv_bfloat16>(*args, st);
+}
+
+extern "C" int64_t b200_embed_bwd_work_bytes(const b200_embed_args *args) {
+  if (!args || check_embed(*args, true)) return 0;
+  const Sort s = sort_of(*args);
+  return 4 * up(4 * args->tokens, 256) + up(4 * (s.tiles << s.bits), 256) + 2 * up(4 * s.pieces * args->features, 256);
+}
+
+extern "C" int b200_embed_bwd(const b200_embed_args *args, void *stream) {
+  B200_REQUIRE(args, B200_ERR_NULL, "embed_bwd: null argument block");
+  const b200_embed_args &a = *args;
+  if (int e = check_embed(a, true)) return e;
+  B200_REQUIRE(a.work, B200_ERR_NULL, "embed_bwd: work must be non-null");
+  B200_REQUIRE((reinterpret_cast<uintptr_t>(a.work) & 255) == 0, B200_ERR_ALIGN, "embed_bwd: work must be 256-byte aligned");
+  B200_REQUIRE(a.work_bytes >= b200_embed_bwd_work_bytes(args), B200_ERR_TOO_LARGE, "embed_bwd: work has %lld bytes, %lld are needed", (long long)a.work_bytes,
+               (long long)b200_embed_bwd_work_bytes(args));
+  B200_REQUIRE(a.dweight_rs == a.features, B200_ERR_SHAPE, "embed_bwd: dweight must be dense");
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const Sort s = sort_of(a);
+  unsigned char *w = reinterpret_cast<unsigned char *>(a.work);
+  const int64_t arr = up(4 * a.tokens, 256);
+  uint32_t *keys[2] = {reinterpret_cast<uint32_t *>(w), reinterpret_cast<uint32_t *>(w + arr)};
+  uint32_t *pos[2] = {reinterpret_cast<uint32_t *>(w + 2 * arr), reinterpret_cast<uint32_t *>(w + 3 * arr)};
+  uint32_t *hist = reinterpret_cast<uint32_t *>(w + 4 * arr);
+  float *head = reinterpret_cast<float *>(w + 4 * arr + up(4 * (s.tiles << s.bits), 256));
+  float *tail = head + up(4 * s.pieces * a.features, 256) / 4;
+  cudaError_t ce = cudaMemsetAsync(a.dweight, 0, (size_t)a.classes * a.features * act_size(a.dtype), st);
+  if (ce != cudaSuccess) { set_error("cudaMemsetAsync: %s", cudaGetErrorString(ce)); return (int)ce; }
+  const uint32_t *k = nullptr, *q = nullptr;
+  for (int i = 0; i < s.passes; ++i) {
+    embed_count_kernel<<<(unsigned)s.tiles, SORT_T, 0, st>>>(a, k, i * s.bits, s.bits, hist);
+    embed_scan_kernel<<<1, 1024, 0, st>>>(hist, s.tiles << s.bits);
+    embed_place_kernel<<<(unsigned)s.tiles, SORT_T, 0, st>>>(a, k, q, i * s.bits, s.bits, hist, keys[i & 1], pos[i & 1]);
+    if (int e = launch_status()) return e;
+    k = keys[i & 1];
+    q = pos[i & 1];
+  }
+  if (a.dtype == B200_F32) return run_sums<float>(a, s, k, q, head, tail, st);
+  return a.dtype == B200_F16 ? run_sums<__half>(a, s, k, q, head, tail, st) : run_sums<__nv_bfloat16>(a, s, k, q, head, tail, st);
+}

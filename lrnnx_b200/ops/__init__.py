@@ -1,5 +1,6 @@
 """Autograd wrappers with the names and signatures of ``lrnnx.ops``
 (lrnnx/ops/__init__.py:1-25)."""
+from .embedding import TokenEmbeddingFn, token_embedding
 from .linear_cross_entropy import LinearCrossEntropyFn, linear_cross_entropy
 from .rglru_scan import RGLRUScanFn, rglru_scan_fn
 from .s4 import cauchy_mult, log_vandermonde_cuda, log_vandermonde_fast
@@ -12,4 +13,4 @@ from .simplified_scan import S5InnerFn, SimplifiedScanFn, s5_inner_fn, simplifie
 __all__ = ["SelectiveScanFn", "selective_scan_fn", "RGLRUScanFn", "rglru_scan_fn", "S7ScanFn", "s7_scan_fn",
            "SimplifiedScanFn", "simplified_scan_fn", "S5InnerFn", "s5_inner_fn",
            "selective_state_update", "simplified_state_update", "cauchy_mult", "log_vandermonde_cuda", "log_vandermonde_fast",
-           "LinearCrossEntropyFn", "linear_cross_entropy"]
+           "LinearCrossEntropyFn", "linear_cross_entropy", "TokenEmbeddingFn", "token_embedding"]
