@@ -576,6 +576,52 @@ int64_t b200_embed_bwd_work_bytes(const b200_embed_args *args);
 int b200_embed_fwd(const b200_embed_args *args, void *stream);
 int b200_embed_bwd(const b200_embed_args *args, void *stream);
 
+/* ------------------------------------------------------------------------
+ * Linear attention with a decay for each head (no counterpart in lrnnx; the matrix-state sibling of
+ * its selective scan):  S_t = exp(g_t) S_{t-1} + k_t v_t^T,  out_t = scale S_t^T q_t.
+ *   q, k (batch, seqlen, groups, dk), v, out (batch, seqlen, heads, dv): dtype, sizes contiguous, dk and dv up to
+ *   128; head h reads group h / (heads / groups)
+ *   g (batch, seqlen, heads): log decays, float32 or dtype, any strides (0 for a decay per head); -inf empties the state
+ *   s0 float32 (batch, heads, dk, dv), dv contiguous, nullable (zeros); last float32, dense: nullable
+ *   backward: dout like out; dlast float32, dense, nullable; last: the forward's, needed with dlast and dg;
+ *   dq, dk_out, dv_out dense, dtype; dg (nullable) of g's dtype, dense (batch, seqlen, heads), or (heads) with
+ *   g_heads 1; ds0 (nullable) float32, dense
+ *   work: device workspace, 256-byte aligned, b200_linattn_{fwd,bwd}_work_bytes() bytes (0: none)
+ * ------------------------------------------------------------------------ */
+typedef struct b200_linattn_args {
+  int32_t batch, seqlen, heads, groups, dk, dv, dtype, g_dtype;
+  float scale;
+  int32_t g_heads;
+  const void *q, *k, *v, *g, *s0;
+  void *out, *last;
+  int64_t q_bs, q_ls, q_hs, k_bs, k_ls, k_hs, v_bs, v_ls, v_hs, g_bs, g_ls, g_hs, s0_bs, s0_hs, s0_ks, out_bs, out_ls, out_hs;
+  const void *dout, *dlast;
+  int64_t dout_bs, dout_ls, dout_hs;
+  void *dq, *dk_out, *dv_out, *dg, *ds0;
+  void *work;
+  int64_t work_bytes;
+} b200_linattn_args;
+
+/* One token: state (slots, heads, dk, dv) float32 or dtype, dv contiguous, updated in place; q, k (batch, groups, dk),
+ * v, out (batch, heads, dv), g (batch, heads).  state_batch_indices (batch) int32, nullable: the slot of each batch entry, no
+ * slot twice; an entry outside [0, slots) has no state: its out is zero. */
+typedef struct b200_linattn_step_args {
+  int32_t batch, heads, groups, dk, dv, dtype, g_dtype, state_dtype;
+  float scale;
+  int32_t slots;
+  void *state;
+  const void *q, *k, *v, *g;
+  const int32_t *state_batch_indices;
+  void *out;
+  int64_t state_bs, state_hs, state_ks, q_bs, q_gs, k_bs, k_gs, v_bs, v_hs, g_bs, g_hs, out_bs, out_hs;
+} b200_linattn_step_args;
+
+int64_t b200_linattn_fwd_work_bytes(const b200_linattn_args *args);
+int64_t b200_linattn_bwd_work_bytes(const b200_linattn_args *args);
+int b200_linattn_fwd(const b200_linattn_args *args, void *stream);
+int b200_linattn_bwd(const b200_linattn_args *args, void *stream);
+int b200_linattn_step(const b200_linattn_step_args *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

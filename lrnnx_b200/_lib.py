@@ -24,6 +24,7 @@ ENTRY_POINTS = (
     "b200_last_error", "b200_abi_version", "b200_sizeof", "b200_device_status", "b200_s4_bwd_scratch_bytes",
     "b200_selscan_stage_states", "b200_selscan_bwd_work_bytes",
     "b200_lce_fwd_work_bytes", "b200_lce_bwd_work_bytes", "b200_embed_bwd_work_bytes",
+    "b200_linattn_fwd_work_bytes", "b200_linattn_bwd_work_bytes",
     "b200_selscan_fwd", "b200_selscan_bwd", "b200_selscan_fixup", "b200_selscan_fold",
     "b200_selscan_adjoint_summary",
     "b200_simpscan_fwd", "b200_simpscan_bwd",
@@ -33,6 +34,7 @@ ENTRY_POINTS = (
     "b200_cgemm_wx", "b200_cgemm_planes", "b200_cgemm_grad",
     "b200_xent_fwd", "b200_xent_bwd", "b200_skinny_linear",
     "b200_lce_fwd", "b200_lce_bwd", "b200_embed_fwd", "b200_embed_bwd",
+    "b200_linattn_fwd", "b200_linattn_bwd", "b200_linattn_step",
 )
 
 _SCALARS = {"int32_t": ctypes.c_int32, "int64_t": ctypes.c_int64, "uint32_t": ctypes.c_uint32,

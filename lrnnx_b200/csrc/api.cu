@@ -64,6 +64,8 @@ int b200_sizeof(const char *name) {
   if (!strcmp(name, "b200_xent_args")) return (int)sizeof(b200_xent_args);
   if (!strcmp(name, "b200_lce_args")) return (int)sizeof(b200_lce_args);
   if (!strcmp(name, "b200_embed_args")) return (int)sizeof(b200_embed_args);
+  if (!strcmp(name, "b200_linattn_args")) return (int)sizeof(b200_linattn_args);
+  if (!strcmp(name, "b200_linattn_step_args")) return (int)sizeof(b200_linattn_step_args);
   if (!strcmp(name, "b200_skinny_linear_args")) return (int)sizeof(b200_skinny_linear_args);
   return -1;
 }

@@ -1,0 +1,710 @@
+// Linear attention with a decay for each head (b200_linattn_fwd / bwd / step), sm_100a.
+//
+//     S_t = exp(g_t) S_{t-1} + k_t v_t^T   (dk x dv, float32),      o_t = scale S_t^T q_t
+//
+// A sequence is walked in chunks of 64 steps.  With G_i the sum of g from the chunk's start to step i, S the state before the chunk,
+//     o_i = exp(G_i) q_i S + sum_{j <= i} exp(G_i - G_j) (q_i . k_j) v_j,
+//     S' = exp(G_end) S + sum_j exp(G_end - G_j) k_j v_j^T,
+// products of small matrices.  Every exponent is a difference of sums of the same chunk and is formed from sums that are kept
+// to 48 bits (a head and a tail in float32), so that strong decays do not cost the weak ones their precision; a decay of
+// -inf (an empty state) counts as one of -300, whose exponential is zero in float32 all the same.
+//
+// All the gradients are the same walk with the operands in other roles:
+//     dq: (q, k, v) -> (do, v, k) forwards;   dk: (v, do, q) backwards;   dv: (k, q, do) backwards,
+// where backwards in time the decay of a step is that of the step after it.  d G_t = q_t . dq_t - k_t . dk_t, taken from the float32
+// results before they are rounded, and dg_t is the sum of these from t on (plus what the last state gives).
+//
+// One thread block walks 64 output columns of a (batch, head); where these are too few for the GPU the
+// sequence is cut into segments: a first pass forms each segment's own state, a scan joins them, and every segment then
+// starts from the state that the earlier ones lead to.
+#include "common.cuh"
+#include "dispatch.h"
+#include <cstring>
+
+namespace b200 {
+namespace {
+
+constexpr int CH = 64;                    // steps of a chunk
+constexpr int DO = 64;                    // output columns of a block
+constexpr int WT = 256;
+constexpr int MAX_D = 128;
+constexpr int PP = CH + 4, PV = DO + 8;   // pitches of scores and of values / state (in floats)
+constexpr float kNoDecay = -300.f * 1.4426950408889634f;
+
+struct Walk {
+  // operands (batch, length, heads or groups, size), sizes contiguous; strides in elements
+  const void *q, *k, *v, *x;              // x: dotted with the result
+  int64_t q_bs, q_ls, q_hs, k_bs, k_ls, k_hs, v_bs, v_ls, v_hs, x_bs, x_ls, x_hs;
+  int q_div, k_div, v_div, x_div;         // head / div: which of the operand's heads
+  const void *g;
+  int64_t g_bs, g_ls, g_hs;
+  int g_dtype;
+  int batch, length, heads, di, dout;     // sizes of q, k and of v
+  int rev;
+  float s_inter, s_intra, s_update;
+  const float *s0;                        // state at the start: (batch, heads, di, dout) by strides
+  int64_t s0_bs, s0_hs, s0_is, s0_os;
+  float *last;                            // state at the end, nullable
+  int64_t last_bs, last_hs, last_is, last_os;
+  int last_decay;                         // rev: times exp(g_0)
+  void *out;
+  int64_t o_bs, o_ls, o_hs;
+  int out_f32;
+  float *dot;                             // (tile, batch heads, length), nullable
+  int tiles, nseg, seg_chunks;            // blocks for a sequence's columns; segments and their chunks
+  float *seg;                             // (batch heads, nseg, di, dout): states
+  double *seg_g;                          // (batch heads, nseg): sums of g
+};
+
+__device__ __forceinline__ float ex2a(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float load_g(const void *g, int dtype, int64_t i) { return ld_act(g, dtype, i); }
+
+// a in log2 units, bounded below
+__device__ __forceinline__ double log2_decay(const Walk &p, int b, int h, int i) {
+  if (i >= p.length) return 0.0;
+  int t = i;
+  if (p.rev) {
+    if (i == 0) return 0.0;
+    t = p.length - i;
+  }
+  const float g = load_g(p.g, p.g_dtype, b * p.g_bs + t * p.g_ls + h * p.g_hs);
+  return (double)fmaxf(g, -300.f) * 1.4426950408889634 + (g != g ? (double)g : 0.0);
+}
+
+// One 16 x 8 x 8 product on TF32 operands given as float32 bit patterns.
+__device__ __forceinline__ void mma8(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+__device__ __forceinline__ uint32_t tf32(float x) {
+  uint32_t y;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(y) : "f"(x));
+  return y;
+}
+
+// acc (16 x 32 of a warp, four 8-column tiles) += A (16 x K) B (K x 32).  A(m, k) = a[m * am + k * ak] * wk[k] (wk nullable), B(k, n) = b[k * bk + n * bn].
+// An operand whose values have at most 11 bits (16-bit inputs) is exact in TF32; others are split in two: a b ~ a_hi b_hi + a_lo b_hi + a_hi b_lo.
+template <bool SPLIT_A, bool SPLIT_B>
+__device__ __forceinline__ void product(float (&acc)[4][4], const float *a, int am, int ak, const float *wk, const float *b, int bk, int bn, int K, int lane) {
+  const int g = lane >> 2, t = lane & 3;
+  for (int k0 = 0; k0 < K; k0 += 8) {
+    float av[4];
+    av[0] = a[g * am + (k0 + t) * ak];
+    av[1] = a[(g + 8) * am + (k0 + t) * ak];
+    av[2] = a[g * am + (k0 + t + 4) * ak];
+    av[3] = a[(g + 8) * am + (k0 + t + 4) * ak];
+    if (wk) {
+      const float w0 = wk[k0 + t], w1 = wk[k0 + t + 4];
+      av[0] *= w0;
+      av[1] *= w0;
+      av[2] *= w1;
+      av[3] *= w1;
+    }
+    uint32_t ah[4], al[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      ah[i] = SPLIT_A ? tf32(av[i]) : __float_as_uint(av[i]);
+      al[i] = SPLIT_A ? __float_as_uint(av[i] - __uint_as_float(ah[i])) : 0u;
+    }
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      float bv[2];
+      bv[0] = b[(k0 + t) * bk + (n * 8 + g) * bn];
+      bv[1] = b[(k0 + t + 4) * bk + (n * 8 + g) * bn];
+      uint32_t bh[2], bl[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        bh[i] = SPLIT_B ? tf32(bv[i]) : __float_as_uint(bv[i]);
+        bl[i] = SPLIT_B ? __float_as_uint(bv[i] - __uint_as_float(bh[i])) : 0u;
+      }
+      if (SPLIT_A) mma8(acc[n], al, bh);
+      if (SPLIT_B) mma8(acc[n], ah, bl);
+      mma8(acc[n], ah, bh);
+    }
+  }
+}
+
+// 64 rows of an operand from step i0 on into shared memory as float32, zero past the sequence and past its size.
+template <typename T>
+__device__ __forceinline__ void load_rows(const Walk &p, const void *base, int64_t off, int64_t ls, int i0, int col0, int size, int width, int pitch, float *dst) {
+  const T *src = reinterpret_cast<const T *>(base) + off;
+  const bool vec = ((reinterpret_cast<uintptr_t>(src + col0) | (uintptr_t)(ls * sizeof(T))) & (4 * sizeof(T) - 1)) == 0;
+  const int per = width / 4;
+  for (int e = threadIdx.x; e < CH * per; e += WT) {
+    const int r = e / per, c = e % per * 4, i = i0 + r;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (i < p.length) {
+      const T *s = src + (int64_t)(p.rev ? p.length - 1 - i : i) * ls + col0 + c;
+      const int left = size - col0 - c;
+      if (vec && left >= 4) {
+        if constexpr (sizeof(T) == 4) {
+          const float4 w = *reinterpret_cast<const float4 *>(s);
+          v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
+        } else {
+          const uint2 w = *reinterpret_cast<const uint2 *>(s);
+          const T *x = reinterpret_cast<const T *>(&w);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = (float)x[j];
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (j < left) v[j] = (float)s[j];
+      }
+    }
+    *reinterpret_cast<float4 *>(dst + r * pitch + c) = make_float4(v[0], v[1], v[2], v[3]);
+  }
+}
+
+template <typename T, bool STATE_ONLY> __global__ void __launch_bounds__(WT) linattn_walk_kernel(const Walk p) {
+  constexpr bool F32 = sizeof(T) == 4;
+  extern __shared__ __align__(16) float sm[];
+  const int dip = (p.di + 15) / 16 * 16, PQ = dip + 4;
+  float *sq = sm, *sk = sq + (STATE_ONLY ? 0 : CH * PQ), *sv = sk + CH * PQ, *S = sv + CH * PV, *sp = S + dip * PV;
+  __shared__ float gh[CH], gl[CH], eg[CH], wu[CH], dots[2][CH];
+  __shared__ double g_total;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gq = lane >> 2, tq = lane & 3;
+  const int tile = blockIdx.x % p.tiles, bh = blockIdx.x / p.tiles % (p.batch * p.heads), seg = blockIdx.x / p.tiles / (p.batch * p.heads);
+  const int b = bh / p.heads, h = bh % p.heads, col0 = tile * DO;
+  const int i_begin = seg * p.seg_chunks * CH, i_end = min(p.length, (seg + 1) * p.seg_chunks * CH);
+  // the state before the first step
+  for (int e = tid; e < dip * DO; e += WT) {
+    const int r = e / DO, c = e % DO;
+    float s = 0.f;
+    if (!STATE_ONLY && r < p.di && col0 + c < p.dout) {
+      if (p.nseg > 1) s = p.seg[(((int64_t)bh * p.nseg + seg) * p.di + r) * p.dout + col0 + c];
+      else if (p.s0) s = p.s0[b * p.s0_bs + h * p.s0_hs + r * p.s0_is + (col0 + c) * p.s0_os];
+    }
+    S[r * PV + c] = s;
+  }
+  double total = 0.0;
+  for (int i0 = i_begin; i0 < i_end; i0 += CH) {
+    __syncthreads();                                 // the last chunk's reads are done
+    if (warp == 0) {                                 // sums of the decays, two steps a lane
+      const double a0 = log2_decay(p, b, h, i0 + 2 * lane), a1 = log2_decay(p, b, h, i0 + 2 * lane + 1);
+      double s = a0 + a1;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double u = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += u;
+      }
+      const double end = __shfl_sync(0xffffffffu, s, 31), first = s - a1;
+      const double G[2] = {first, s};
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float hi = (float)G[j];
+        gh[2 * lane + j] = hi;
+        gl[2 * lane + j] = (float)(G[j] - (double)hi);
+        eg[2 * lane + j] = ex2a(hi);
+        wu[2 * lane + j] = ex2a((float)(end - G[j])) * p.s_update;
+      }
+      if (lane == 0) g_total = end;
+    }
+    if (!STATE_ONLY) load_rows<T>(p, p.q, b * p.q_bs + h / p.q_div * p.q_hs, p.q_ls, i0, 0, p.di, dip, PQ, sq);
+    load_rows<T>(p, p.k, b * p.k_bs + h / p.k_div * p.k_hs, p.k_ls, i0, 0, p.di, dip, PQ, sk);
+    load_rows<T>(p, p.v, b * p.v_bs + h / p.v_div * p.v_hs, p.v_ls, i0, col0, p.dout, DO, PV, sv);
+    __syncthreads();
+    const int m0 = (warp & 3) * 16, n0 = (warp >> 2) * 32;      // this warp's 16 x 32 of scores and of results
+    if (!STATE_ONLY) {
+      float acc[4][4] = {};
+      if (n0 <= m0 + 15) product<F32, F32>(acc, sq + m0 * PQ, PQ, 1, nullptr, sk + n0 * PQ, 1, PQ, dip, lane);
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = m0 + gq + (e >> 1) * 8, c = n0 + n * 8 + tq * 2 + (e & 1);
+          sp[r * PP + c] = c <= r ? acc[n][e] * ex2a((gh[r] - gh[c]) + (gl[r] - gl[c])) * p.s_intra : 0.f;
+        }
+      __syncthreads();
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
+      product<F32, true>(acc, sq + m0 * PQ, PQ, 1, nullptr, S + n0, PV, 1, dip, lane);
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[n][e] *= eg[m0 + gq + (e >> 1) * 8] * p.s_inter;
+      product<true, F32>(acc, sp + m0 * PP, PP, 1, nullptr, sv + n0, PV, 1, min(CH, m0 + 16), lane);
+      // out, and its product with x
+      float dsum[2] = {0.f, 0.f};
+#pragma unroll
+      for (int e2 = 0; e2 < 2; ++e2) {
+        const int i = i0 + m0 + gq + e2 * 8;
+        if (i >= p.length) continue;
+        const int64_t t = p.rev ? p.length - 1 - i : i;
+        const int64_t o = b * p.o_bs + t * p.o_ls + h * p.o_hs;
+        const T *x = p.dot ? reinterpret_cast<const T *>(p.x) + b * p.x_bs + t * p.x_ls + h / p.x_div * p.x_hs : nullptr;
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int e1 = 0; e1 < 2; ++e1) {
+            const int c = col0 + n0 + n * 8 + tq * 2 + e1;
+            if (c >= p.dout) continue;
+            const float v = acc[n][e2 * 2 + e1];
+            if (p.out_f32) reinterpret_cast<float *>(p.out)[o + c] = v;
+            else reinterpret_cast<T *>(p.out)[o + c] = T(v);
+            if (x) dsum[e2] = fmaf(v, (float)x[c], dsum[e2]);
+          }
+      }
+      if (p.dot) {
+#pragma unroll
+        for (int e2 = 0; e2 < 2; ++e2) {
+          dsum[e2] += __shfl_xor_sync(0xffffffffu, dsum[e2], 1);
+          dsum[e2] += __shfl_xor_sync(0xffffffffu, dsum[e2], 2);
+          if (tq == 0) dots[warp >> 2][m0 + gq + e2 * 8] = dsum[e2];
+        }
+      }
+    }
+    __syncthreads();                                 // all have read the state
+    if (!STATE_ONLY && p.dot && tid < CH && i0 + tid < p.length)
+      p.dot[((int64_t)tile * p.batch * p.heads + bh) * p.length + (p.rev ? p.length - 1 - i0 - tid : i0 + tid)] = dots[0][tid] + dots[1][tid];
+    total += g_total;
+    const float keep = ex2a((float)g_total);
+    for (int u = warp; u < dip / 16 * 2; u += 8) {
+      const int r0 = u / 2 * 16, c0 = u % 2 * 32;
+      float acc[4][4] = {};
+      product<true, F32>(acc, sk + r0, 1, PQ, wu, sv + c0, PV, 1, CH, lane);
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float *s = S + (r0 + gq + (e >> 1) * 8) * PV + c0 + n * 8 + tq * 2 + (e & 1);
+          *s = fmaf(*s, keep, acc[n][e]);
+        }
+    }
+  }
+  __syncthreads();
+  if (STATE_ONLY) {
+    for (int e = tid; e < p.di * DO; e += WT) {
+      const int r = e / DO, c = e % DO;
+      if (col0 + c < p.dout) p.seg[(((int64_t)bh * p.nseg + seg) * p.di + r) * p.dout + col0 + c] = S[r * PV + c];
+    }
+    if (tile == 0 && tid == 0) p.seg_g[(int64_t)bh * p.nseg + seg] = total;
+  } else if (p.last && seg == p.nseg - 1) {
+    float f = 1.f;
+    if (p.last_decay) f = ex2a((float)((double)fmaxf(load_g(p.g, p.g_dtype, b * p.g_bs + h * p.g_hs), -300.f) * 1.4426950408889634));
+    for (int e = tid; e < p.di * DO; e += WT) {
+      const int r = e / DO, c = e % DO;
+      if (col0 + c < p.dout) p.last[b * p.last_bs + h * p.last_hs + r * p.last_is + (col0 + c) * p.last_os] = S[r * PV + c] * f;
+    }
+  }
+}
+
+// Each segment's own state becomes the state before it.
+__global__ void __launch_bounds__(256) linattn_join_kernel(const Walk p) {
+  const int64_t per = (int64_t)p.di * p.dout, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int bh = blockIdx.y, b = bh / p.heads, h = bh % p.heads;
+  if (i >= per) return;
+  float s = 0.f;
+  if (p.s0) s = p.s0[b * p.s0_bs + h * p.s0_hs + i / p.dout * p.s0_is + i % p.dout * p.s0_os];
+  for (int n = 0; n < p.nseg; ++n) {
+    float *at = p.seg + ((int64_t)bh * p.nseg + n) * per + i;
+    const float own = n < p.nseg - 1 ? *at : 0.f;
+    *at = s;
+    if (n < p.nseg - 1) s = fmaf(s, ex2a((float)p.seg_g[(int64_t)bh * p.nseg + n]), own);
+  }
+}
+
+// Gradients of operands that several heads share: the sum over the heads of a group.
+template <typename T>
+__global__ void __launch_bounds__(256) linattn_fold_kernel(const float *src, int64_t rows, int heads, int groups, int d, T *dst) {
+  const int64_t n = rows * groups * d;
+  const int per = heads / groups;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t rg = i / d;
+    const int c = (int)(i - rg * d);
+    const float *s = src + rg * per * d + c;
+    float v = 0.f;
+    for (int j = 0; j < per; ++j) v += s[(int64_t)j * d];
+    dst[i] = T(v);
+  }
+}
+
+// dg from the dots: one block a (batch, head), each thread a run of steps, sums in 64 bits.
+__global__ void __launch_bounds__(256) linattn_dg_kernel(const b200_linattn_args p, const float *dot_q, int tiles_q, const float *dot_k, int tiles_k, double *per_head) {
+  __shared__ double sh[256];
+  __shared__ double end_s;
+  const int bh = blockIdx.x, b = bh / p.heads, h = bh % p.heads, tid = threadIdx.x;
+  const int64_t plane = (int64_t)p.batch * p.heads * p.seqlen;
+  dot_q += (int64_t)bh * p.seqlen;
+  dot_k += (int64_t)bh * p.seqlen;
+  const auto d_at = [&](int t) {
+    double s = 0.0;
+    for (int i = 0; i < tiles_q; ++i) s += (double)dot_q[i * plane + t];
+    for (int i = 0; i < tiles_k; ++i) s -= (double)dot_k[i * plane + t];
+    return s;
+  };
+  double e = 0.0;                                     // what the last state gives all steps
+  if (p.dlast) {
+    const float *S = reinterpret_cast<const float *>(p.last) + (int64_t)bh * p.dk * p.dv;
+    const float *D = reinterpret_cast<const float *>(p.dlast) + (int64_t)bh * p.dk * p.dv;
+    for (int i = tid; i < p.dk * p.dv; i += 256) e += (double)S[i] * (double)D[i];
+  }
+  sh[tid] = e;
+  __syncthreads();
+  for (int o = 128; o > 0; o >>= 1) {
+    if (tid < o) sh[tid] += sh[tid + o];
+    __syncthreads();
+  }
+  if (tid == 0) end_s = sh[0];
+  __syncthreads();
+  const int run = (p.seqlen + 255) / 256, t0 = tid * run, t1 = min(p.seqlen, t0 + run);
+  double s = 0.0;
+  for (int t = t0; t < t1; ++t) s += d_at(t);
+  sh[tid] = s;
+  __syncthreads();
+  if (tid == 0) {
+    double a = end_s;
+    for (int i = 255; i >= 0; --i) { const double v = sh[i]; sh[i] = a; a += v; }
+  }
+  __syncthreads();
+  double a = sh[tid], sum = 0.0;
+  for (int t = t1 - 1; t >= t0; --t) {
+    a += d_at(t);
+    const int64_t gi = b * p.g_bs + t * p.g_ls + h * p.g_hs;
+    const double v = load_g(p.g, p.g_dtype, gi) == -INFINITY ? 0.0 : a;
+    if (per_head) sum += v;
+    else st_act(p.dg, p.g_dtype, ((int64_t)b * p.seqlen + t) * p.heads + h, (float)v);
+  }
+  if (per_head) {
+    __syncthreads();
+    sh[tid] = sum;
+    __syncthreads();
+    if (tid == 0) {
+      double x = 0.0;
+      for (int i = 0; i < 256; ++i) x += sh[i];
+      per_head[bh] = x;
+    }
+  }
+}
+__global__ void linattn_dg_heads_kernel(const b200_linattn_args p, const double *per_head) {
+  const int h = blockIdx.x * blockDim.x + threadIdx.x;
+  if (h >= p.heads) return;
+  double s = 0.0;
+  for (int b = 0; b < p.batch; ++b) s += per_head[(int64_t)b * p.heads + h];
+  st_act(p.dg, p.g_dtype, h, (float)s);
+}
+
+// ------------------------------------------------------------------------------------------------ one token
+
+// A block takes a (batch entry, head): the state is read and written once, 16 bytes an access where its rows allow it.  Threads
+// along the state's rows of dv, and groups of them along dk whose sums are joined in shared memory.
+template <typename TS, typename T, int VEC> __global__ void __launch_bounds__(128) linattn_step_kernel(const b200_linattn_step_args p) {
+  __shared__ float sh[128 * VEC], sq[MAX_D], sk[MAX_D];
+  const int b = blockIdx.x / p.heads, h = blockIdx.x % p.heads, grp = h / (p.heads / p.groups), tid = threadIdx.x;
+  const T *v = reinterpret_cast<const T *>(p.v) + b * p.v_bs + h * p.v_hs;
+  T *out = reinterpret_cast<T *>(p.out) + b * p.out_bs + h * p.out_hs;
+  int64_t slot = b;
+  if (p.state_batch_indices) {
+    slot = p.state_batch_indices[b];
+    if (slot < 0 || slot >= p.slots) {                    // no state: padding of the batch
+      for (int c = tid; c < p.dv; c += 128) out[c] = T(0.f);
+      return;
+    }
+  }
+  for (int i = tid; i < p.dk; i += 128) {
+    sq[i] = (float)reinterpret_cast<const T *>(p.q)[b * p.q_bs + grp * p.q_gs + i] * p.scale;
+    sk[i] = (float)reinterpret_cast<const T *>(p.k)[b * p.k_bs + grp * p.k_gs + i];
+  }
+  const float a = expf(load_g(p.g, p.g_dtype, b * p.g_bs + h * p.g_hs));
+  const int across = (p.dv + VEC - 1) / VEC, along = 128 / across;           // threads along dv (at most 128) and along dk
+  const int cx = tid % across, ry = tid / across, c0 = cx * VEC;
+  TS *S = reinterpret_cast<TS *>(p.state) + slot * p.state_bs + h * p.state_hs + c0;
+  __syncthreads();
+  float acc[VEC], vv[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) {
+    acc[j] = 0.f;
+    vv[j] = (float)v[c0 + j];
+  }
+  if (ry < along) {
+#pragma unroll 4
+    for (int r = ry; r < p.dk; r += along) {
+      TS *s = S + (int64_t)r * p.state_ks;
+      TS e[VEC];
+      if constexpr (VEC > 1) *reinterpret_cast<uint4 *>(e) = *reinterpret_cast<const uint4 *>(s);
+      else e[0] = *s;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float x = fmaf(a, (float)e[j], sk[r] * vv[j]);
+        acc[j] = fmaf(sq[r], x, acc[j]);
+        e[j] = TS(x);
+      }
+      if constexpr (VEC > 1) *reinterpret_cast<uint4 *>(s) = *reinterpret_cast<const uint4 *>(e);
+      else *s = e[0];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) sh[tid * VEC + j] = acc[j];
+  __syncthreads();
+  for (int c = tid; c < p.dv; c += 128) {
+    float s = 0.f;
+    for (int r = 0; r < along; ++r) s += sh[(r * across) * VEC + c];
+    out[c] = T(s);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+
+int64_t up(int64_t n, int64_t unit) { return (n + unit - 1) / unit * unit; }
+
+int walk_smem(int di, bool state_only) {
+  const int dip = (int)up(di, 16);
+  return 4 * ((state_only ? 1 : 2) * CH * (dip + 4) + CH * PV + dip * PV + (state_only ? 0 : CH * PP));
+}
+
+// Segments: as many as make the walk shortest, counted in chunks that one SM goes through, a first pass over segments at 0.45 of a walk.
+int segments(int64_t blocks, int chunks) {
+  const int sms = sm_count_current();
+  int best = 1;
+  double cost = 1e30;
+  for (int n = 1; n <= 64 && n <= chunks; ++n) {
+    const int per = (chunks + n - 1) / n;
+    if ((int64_t)(n - 1) * per >= chunks) continue;
+    const double waves = (double)((blocks * n + sms - 1) / sms);
+    const double c = waves * per * (n > 1 ? 1.45 : 1.0) + (n > 1 ? 2 : 0);
+    if (c < cost * 0.97) { cost = c; best = n; }
+  }
+  return best;
+}
+
+void cut(Walk &w) {
+  const int chunks = (w.length + CH - 1) / CH;
+  w.tiles = (w.dout + DO - 1) / DO;
+  const int n = segments((int64_t)w.batch * w.heads * w.tiles, chunks);
+  w.seg_chunks = (chunks + n - 1) / n;
+  w.nseg = (chunks + w.seg_chunks - 1) / w.seg_chunks;
+}
+int64_t seg_bytes(int64_t bh, int nseg, int di, int dout) { return nseg > 1 ? up(4 * bh * nseg * di * dout, 256) + up(8 * bh * nseg, 256) : 0; }
+
+template <typename T> int walk(Walk &w, unsigned char *work, cudaStream_t st) {
+  const int64_t bh = (int64_t)w.batch * w.heads;
+  if (w.nseg > 1) {
+    w.seg = reinterpret_cast<float *>(work);
+    w.seg_g = reinterpret_cast<double *>(work + up(4 * bh * w.nseg * w.di * w.dout, 256));
+    const int sm0 = walk_smem(w.di, true);
+    cudaError_t e = cudaFuncSetAttribute(linattn_walk_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, sm0);
+    if (e != cudaSuccess) { set_error("cudaFuncSetAttribute: %s", cudaGetErrorString(e)); return (int)e; }
+    linattn_walk_kernel<T, true><<<(unsigned)(bh * w.tiles * (w.nseg - 1)), WT, sm0, st>>>(w);
+    const int64_t per = (int64_t)w.di * w.dout;
+    linattn_join_kernel<<<dim3((unsigned)((per + 255) / 256), (unsigned)bh), 256, 0, st>>>(w);
+    if (int r = launch_status()) return r;
+  }
+  const int sm1 = walk_smem(w.di, false);
+  cudaError_t e = cudaFuncSetAttribute(linattn_walk_kernel<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, sm1);
+  if (e != cudaSuccess) { set_error("cudaFuncSetAttribute: %s", cudaGetErrorString(e)); return (int)e; }
+  linattn_walk_kernel<T, false><<<(unsigned)(bh * w.tiles * w.nseg), WT, sm1, st>>>(w);
+  return launch_status();
+}
+int run_walk(int dtype, Walk &w, unsigned char *work, cudaStream_t st) {
+  if (dtype == B200_F32) return walk<float>(w, work, st);
+  return dtype == B200_F16 ? walk<__half>(w, work, st) : walk<__nv_bfloat16>(w, work, st);
+}
+
+int check_linattn(const b200_linattn_args &a) {
+  B200_REQUIRE(a.q && a.k && a.v && a.g, B200_ERR_NULL, "linattn: q, k, v and g must be non-null");
+  B200_REQUIRE(a.batch > 0 && a.seqlen > 0 && a.heads > 0 && a.groups > 0 && a.dk > 0 && a.dv > 0, B200_ERR_SHAPE, "linattn: sizes must be positive");
+  B200_REQUIRE(a.dk <= MAX_D && a.dv <= MAX_D, B200_ERR_SHAPE, "linattn: head sizes up to %d (got dk=%d dv=%d)", MAX_D, a.dk, a.dv);
+  B200_REQUIRE(a.heads % a.groups == 0, B200_ERR_SHAPE, "linattn: heads (%d) must be a multiple of groups (%d)", a.heads, a.groups);
+  B200_REQUIRE((int64_t)a.batch * a.heads <= 65535 && a.seqlen <= (1 << 30), B200_ERR_SHAPE, "linattn: batch * heads up to 65535 (got %d * %d)", a.batch, a.heads);
+  B200_REQUIRE(a.dtype == B200_F32 || a.dtype == B200_F16 || a.dtype == B200_BF16, B200_ERR_DTYPE, "linattn: unknown dtype %d", a.dtype);
+  B200_REQUIRE(a.g_dtype == B200_F32 || a.g_dtype == a.dtype, B200_ERR_DTYPE, "linattn: g is float32 or of the dtype of q, k, v");
+  B200_REQUIRE((reinterpret_cast<uintptr_t>(a.work) & 255) == 0, B200_ERR_ALIGN, "linattn: work must be 256-byte aligned");
+  return 0;
+}
+
+Walk base_walk(const b200_linattn_args &a) {
+  Walk w;
+  memset(&w, 0, sizeof(w));
+  w.g = a.g; w.g_bs = a.g_bs; w.g_ls = a.g_ls; w.g_hs = a.g_hs; w.g_dtype = a.g_dtype;
+  w.batch = a.batch; w.length = a.seqlen; w.heads = a.heads;
+  w.q_div = w.k_div = w.v_div = w.x_div = 1;
+  return w;
+}
+#define ROLE(slot, from)                                          \
+  do {                                                            \
+    w.slot = a.from;                                              \
+    w.slot##_bs = a.from##_bs;                                    \
+    w.slot##_ls = a.from##_ls;                                    \
+    w.slot##_hs = a.from##_hs;                                    \
+  } while (0)
+
+// the walks: o, dq, dk, dv
+Walk walk_o(const b200_linattn_args &a) {
+  Walk w = base_walk(a);
+  ROLE(q, q); ROLE(k, k); ROLE(v, v);
+  w.q_div = w.k_div = a.heads / a.groups;
+  w.di = a.dk; w.dout = a.dv;
+  w.s_inter = w.s_intra = a.scale; w.s_update = 1.f;
+  w.s0 = reinterpret_cast<const float *>(a.s0);
+  w.s0_bs = a.s0_bs; w.s0_hs = a.s0_hs; w.s0_is = a.s0_ks; w.s0_os = 1;
+  w.out = a.out; w.o_bs = a.out_bs; w.o_ls = a.out_ls; w.o_hs = a.out_hs;
+  w.last = reinterpret_cast<float *>(a.last);
+  w.last_bs = (int64_t)a.heads * a.dk * a.dv; w.last_hs = (int64_t)a.dk * a.dv; w.last_is = a.dv; w.last_os = 1;
+  cut(w);
+  return w;
+}
+Walk walk_dq(const b200_linattn_args &a) {
+  Walk w = base_walk(a);
+  ROLE(q, dout); ROLE(k, v); ROLE(v, k); ROLE(x, q);
+  w.v_div = w.x_div = a.heads / a.groups;
+  w.di = a.dv; w.dout = a.dk;
+  w.s_inter = w.s_intra = a.scale; w.s_update = 1.f;
+  w.s0 = reinterpret_cast<const float *>(a.s0);
+  w.s0_bs = a.s0_bs; w.s0_hs = a.s0_hs; w.s0_is = 1; w.s0_os = a.s0_ks;
+  cut(w);
+  return w;
+}
+Walk walk_dk(const b200_linattn_args &a) {
+  Walk w = base_walk(a);
+  ROLE(q, v); ROLE(k, dout); ROLE(v, q); ROLE(x, k);
+  w.v_div = w.x_div = a.heads / a.groups;
+  w.di = a.dv; w.dout = a.dk;
+  w.rev = 1;
+  w.s_inter = 1.f; w.s_intra = w.s_update = a.scale;
+  w.s0 = reinterpret_cast<const float *>(a.dlast);
+  w.s0_bs = (int64_t)a.heads * a.dk * a.dv; w.s0_hs = (int64_t)a.dk * a.dv; w.s0_is = 1; w.s0_os = a.dv;
+  cut(w);
+  return w;
+}
+Walk walk_dv(const b200_linattn_args &a) {
+  Walk w = base_walk(a);
+  ROLE(q, k); ROLE(k, q); ROLE(v, dout);
+  w.q_div = w.k_div = a.heads / a.groups;
+  w.di = a.dk; w.dout = a.dv;
+  w.rev = 1;
+  w.s_inter = 1.f; w.s_intra = w.s_update = a.scale;
+  w.s0 = reinterpret_cast<const float *>(a.dlast);
+  w.s0_bs = (int64_t)a.heads * a.dk * a.dv; w.s0_hs = (int64_t)a.dk * a.dv; w.s0_is = a.dv; w.s0_os = 1;
+  w.out = a.dv_out; w.o_bs = (int64_t)a.seqlen * a.heads * a.dv; w.o_ls = (int64_t)a.heads * a.dv; w.o_hs = a.dv;
+  w.last = reinterpret_cast<float *>(a.ds0);
+  w.last_bs = w.s0_bs; w.last_hs = w.s0_hs; w.last_is = a.dv; w.last_os = 1;
+  w.last_decay = 1;
+  cut(w);
+  return w;
+}
+
+struct BwdPlan { int64_t seg, part, dot_q, dot_k, heads, total; };
+BwdPlan bwd_plan(const b200_linattn_args &a) {
+  BwdPlan q;
+  const int64_t bh = (int64_t)a.batch * a.heads;
+  const Walk ws[3] = {walk_dq(a), walk_dk(a), walk_dv(a)};
+  q.seg = 0;
+  for (const Walk &w : ws) {
+    const int64_t s = seg_bytes(bh, w.nseg, w.di, w.dout);
+    if (s > q.seg) q.seg = s;
+  }
+  q.part = a.heads != a.groups ? up(4 * bh * a.seqlen * a.dk, 256) : 0;
+  q.dot_q = a.dg ? up(4 * bh * a.seqlen * ws[0].tiles, 256) : 0;
+  q.dot_k = a.dg ? up(4 * bh * a.seqlen * ws[1].tiles, 256) : 0;
+  q.heads = a.dg && a.g_heads ? up(8 * bh, 256) : 0;
+  q.total = q.seg + q.part + q.dot_q + q.dot_k + q.heads;
+  return q;
+}
+
+int fold(const b200_linattn_args &a, const float *src, void *dst, cudaStream_t st) {
+  const int64_t rows = (int64_t)a.batch * a.seqlen, n = rows * a.groups * a.dk, most = (int64_t)sm_count_current() * 16;
+  const unsigned grid = (unsigned)((n + 255) / 256 < most ? (n + 255) / 256 : most);
+  if (a.dtype == B200_F32) linattn_fold_kernel<float><<<grid, 256, 0, st>>>(src, rows, a.heads, a.groups, a.dk, reinterpret_cast<float *>(dst));
+  else if (a.dtype == B200_F16) linattn_fold_kernel<__half><<<grid, 256, 0, st>>>(src, rows, a.heads, a.groups, a.dk, reinterpret_cast<__half *>(dst));
+  else linattn_fold_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(src, rows, a.heads, a.groups, a.dk, reinterpret_cast<__nv_bfloat16 *>(dst));
+  return launch_status();
+}
+
+template <typename TS, typename T> int run_step(const b200_linattn_step_args &a, cudaStream_t st) {
+  constexpr int V = 16 / sizeof(TS);
+  const bool vec = a.dv % V == 0 && (reinterpret_cast<uintptr_t>(a.state) & 15) == 0 && a.state_bs % V == 0 && a.state_hs % V == 0 && a.state_ks % V == 0;
+  const unsigned grid = (unsigned)((int64_t)a.batch * a.heads);
+  if (vec) linattn_step_kernel<TS, T, V><<<grid, 128, 0, st>>>(a);
+  else linattn_step_kernel<TS, T, 1><<<grid, 128, 0, st>>>(a);
+  return launch_status();
+}
+
+}  // namespace
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" int64_t b200_linattn_fwd_work_bytes(const b200_linattn_args *args) {
+  if (!args || check_linattn(*args)) return 0;
+  const Walk w = walk_o(*args);
+  return seg_bytes((int64_t)w.batch * w.heads, w.nseg, w.di, w.dout);
+}
+
+extern "C" int64_t b200_linattn_bwd_work_bytes(const b200_linattn_args *args) {
+  if (!args || check_linattn(*args)) return 0;
+  return bwd_plan(*args).total;
+}
+
+extern "C" int b200_linattn_fwd(const b200_linattn_args *args, void *stream) {
+  B200_REQUIRE(args, B200_ERR_NULL, "linattn_fwd: null argument block");
+  const b200_linattn_args &a = *args;
+  if (int e = check_linattn(a)) return e;
+  B200_REQUIRE(a.out, B200_ERR_NULL, "linattn_fwd: out must be non-null");
+  const int64_t need = b200_linattn_fwd_work_bytes(args);
+  B200_REQUIRE(a.work_bytes >= need && (a.work || !need), B200_ERR_TOO_LARGE, "linattn_fwd: work has %lld bytes, %lld are needed", (long long)a.work_bytes, (long long)need);
+  Walk w = walk_o(a);
+  return run_walk(a.dtype, w, reinterpret_cast<unsigned char *>(a.work), reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" int b200_linattn_bwd(const b200_linattn_args *args, void *stream) {
+  B200_REQUIRE(args, B200_ERR_NULL, "linattn_bwd: null argument block");
+  const b200_linattn_args &a = *args;
+  if (int e = check_linattn(a)) return e;
+  B200_REQUIRE(a.dout && a.dq && a.dk_out && a.dv_out, B200_ERR_NULL, "linattn_bwd: dout, dq, dk_out and dv_out must be non-null");
+  B200_REQUIRE(!a.dg || !a.dlast || a.last, B200_ERR_NULL, "linattn_bwd: with dlast and dg the last state must be non-null");
+  const BwdPlan q = bwd_plan(a);
+  B200_REQUIRE(a.work_bytes >= q.total && (a.work || !q.total), B200_ERR_TOO_LARGE, "linattn_bwd: work has %lld bytes, %lld are needed", (long long)a.work_bytes,
+               (long long)q.total);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  unsigned char *work = reinterpret_cast<unsigned char *>(a.work);
+  float *part = reinterpret_cast<float *>(work + q.seg), *dot_q = reinterpret_cast<float *>(work + q.seg + q.part);
+  float *dot_k = dot_q + q.dot_q / 4;
+  double *heads = reinterpret_cast<double *>(work + q.seg + q.part + q.dot_q + q.dot_k);
+  const bool shared = a.heads != a.groups;
+  int tiles[2];
+  for (int i = 0; i < 2; ++i) {
+    Walk w = i == 0 ? walk_dq(a) : walk_dk(a);
+    void *dst = i == 0 ? a.dq : a.dk_out;
+    w.out = shared ? part : dst;
+    w.out_f32 = shared;
+    w.o_bs = (int64_t)a.seqlen * a.heads * a.dk;
+    w.o_ls = (int64_t)a.heads * a.dk;
+    w.o_hs = a.dk;
+    if (a.dg) w.dot = i == 0 ? dot_q : dot_k;
+    tiles[i] = w.tiles;
+    if (int e = run_walk(a.dtype, w, work, st)) return e;
+    if (shared)
+      if (int e = fold(a, part, dst, st)) return e;
+  }
+  Walk w = walk_dv(a);
+  if (int e = run_walk(a.dtype, w, work, st)) return e;
+  if (a.dg) {
+    linattn_dg_kernel<<<(unsigned)(a.batch * a.heads), 256, 0, st>>>(a, dot_q, tiles[0], dot_k, tiles[1], a.g_heads ? heads : nullptr);
+    if (a.g_heads) linattn_dg_heads_kernel<<<(unsigned)((a.heads + 127) / 128), 128, 0, st>>>(a, heads);
+  }
+  return launch_status();
+}
+
+extern "C" int b200_linattn_step(const b200_linattn_step_args *args, void *stream) {
+  B200_REQUIRE(args, B200_ERR_NULL, "linattn_step: null argument block");
+  const b200_linattn_step_args &a = *args;
+  B200_REQUIRE(a.state && a.q && a.k && a.v && a.g && a.out, B200_ERR_NULL, "linattn_step: state, q, k, v, g and out must be non-null");
+  B200_REQUIRE(a.batch > 0 && a.heads > 0 && a.groups > 0 && a.dk > 0 && a.dv > 0 && a.heads % a.groups == 0, B200_ERR_SHAPE,
+               "linattn_step: sizes must be positive, heads a multiple of groups");
+  B200_REQUIRE(a.dk <= MAX_D && a.dv <= MAX_D, B200_ERR_SHAPE, "linattn_step: head sizes up to %d (got dk=%d dv=%d)", MAX_D, a.dk, a.dv);
+  B200_REQUIRE((int64_t)a.batch * a.heads < (int64_t(1) << 31), B200_ERR_SHAPE, "linattn_step: batch * heads too large");
+  B200_REQUIRE(a.dtype == B200_F32 || a.dtype == B200_F16 || a.dtype == B200_BF16, B200_ERR_DTYPE, "linattn_step: unknown dtype %d", a.dtype);
+  B200_REQUIRE((a.state_dtype == B200_F32 || a.state_dtype == a.dtype) && (a.g_dtype == B200_F32 || a.g_dtype == a.dtype), B200_ERR_DTYPE,
+               "linattn_step: the state and g are float32 or of the dtype of q, k, v");
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (a.dtype == B200_F32) return run_step<float, float>(a, st);
+  if (a.dtype == B200_F16) return a.state_dtype == B200_F32 ? run_step<float, __half>(a, st) : run_step<__half, __half>(a, st);
+  return a.state_dtype == B200_F32 ? run_step<float, __nv_bfloat16>(a, st) : run_step<__nv_bfloat16, __nv_bfloat16>(a, st);
+}
