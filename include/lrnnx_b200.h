@@ -583,7 +583,7 @@ int b200_embed_bwd(const b200_embed_args *args, void *stream);
  *   128; head h reads group h / (heads / groups)
  *   g (batch, seqlen, heads): log decays, float32 or dtype, any strides (0 for a decay per head); -inf empties the state
  *   s0 float32 (batch, heads, dk, dv), dv contiguous, nullable (zeros); last float32, dense: nullable
- *   backward: dout like out; dlast float32, dense, nullable; last: the forward's, needed with dlast and dg;
+ *   backward: dout like out; dlast float32, dense, nullable;
  *   dq, dk_out, dv_out dense, dtype; dg (nullable) of g's dtype, dense (batch, seqlen, heads), or (heads) with
  *   g_heads 1; ds0 (nullable) float32, dense
  *   work: device workspace, 256-byte aligned, b200_linattn_{fwd,bwd}_work_bytes() bytes (0: none)

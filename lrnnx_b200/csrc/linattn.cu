@@ -11,8 +11,11 @@
 //
 // All the gradients are the same walk with the operands in other roles:
 //     dq: (q, k, v) -> (do, v, k) forwards;   dk: (v, do, q) backwards;   dv: (k, q, do) backwards,
-// where backwards in time the decay of a step is that of the step after it.  d G_t = q_t . dq_t - k_t . dk_t, taken from the float32
-// results before they are rounded, and dg_t is the sum of these from t on (plus what the last state gives).
+// where backwards in time the decay of a step is that of the step after it.  dg_t is the sum over all pairs of a step s before t and a step r not
+// before it of (what s puts into the state) . (what r takes from it), decayed from s to r.  Sums of q . dq - k . dk
+// would give it too, but as a small difference of long sums; instead, for a chunk: pairs within it, from the products of their two scores;
+// pairs with one step outside, from the dots of q with the state's part of dq and of k with that of dk; and pairs on
+// both sides of it, from the product of the two walks' states, which they save at every eighth border.
 //
 // One thread block walks 64 output columns of a (batch, head); where these are too few for the GPU the
 // sequence is cut into segments: a first pass forms each segment's own state, a scan joins them, and every segment then
@@ -29,7 +32,7 @@ constexpr int DO = 64;                    // output columns of a block
 constexpr int WT = 256;
 constexpr int MAX_D = 128;
 constexpr int PP = CH + 4, PV = DO + 8;   // pitches of scores and of values / state (in floats)
-constexpr float kNoDecay = -300.f * 1.4426950408889634f;
+constexpr int kSnap = 8;                  // chunks between the states that the gradient of g is anchored at
 
 struct Walk {
   // operands (batch, length, heads or groups, size), sizes contiguous; strides in elements
@@ -40,7 +43,7 @@ struct Walk {
   int64_t g_bs, g_ls, g_hs;
   int g_dtype;
   int batch, length, heads, di, dout;     // sizes of q, k and of v
-  int rev;
+  int chunks, rev;                        // rev: from the last chunk to the first, and backwards within each
   float s_inter, s_intra, s_update;
   const float *s0;                        // state at the start: (batch, heads, di, dout) by strides
   int64_t s0_bs, s0_hs, s0_is, s0_os;
@@ -50,7 +53,10 @@ struct Walk {
   void *out;
   int64_t o_bs, o_ls, o_hs;
   int out_f32;
-  float *dot;                             // (tile, batch heads, length), nullable
+  // for the gradient of g, nullable together (x is given then)
+  float *run;                             // (tile, batch heads, length): what the pairs of steps across each step give, within its chunk
+  float *sum;                             // (tile, batch heads, chunks): sums of the dots of a chunk
+  float *snap;                            // (batch heads, snapshots, di, dout): states at every kSnap-th border of chunks
   int tiles, nseg, seg_chunks;            // blocks for a sequence's columns; segments and their chunks
   float *seg;                             // (batch heads, nseg, di, dout): states
   double *seg_g;                          // (batch heads, nseg): sums of g
@@ -63,16 +69,71 @@ __device__ __forceinline__ float ex2a(float x) {
 }
 __device__ __forceinline__ float load_g(const void *g, int dtype, int64_t i) { return ld_act(g, dtype, i); }
 
-// a in log2 units, bounded below
-__device__ __forceinline__ double log2_decay(const Walk &p, int b, int h, int i) {
-  if (i >= p.length) return 0.0;
-  int t = i;
-  if (p.rev) {
-    if (i == 0) return 0.0;
-    t = p.length - i;
-  }
+// the time of the walk's step i (past the sequence's end where there is none)
+__device__ __forceinline__ int time_of(const Walk &p, int i) { return p.rev ? p.chunks * CH - 1 - i : i; }
+
+// a log decay in units of log2, bounded below; NaN stays
+__device__ __forceinline__ double log2_of(const Walk &p, int b, int h, int t) {
   const float g = load_g(p.g, p.g_dtype, b * p.g_bs + t * p.g_ls + h * p.g_hs);
-  return (double)fmaxf(g, -300.f) * 1.4426950408889634 + (g != g ? (double)g : 0.0);
+  return g != g ? (double)g : (double)fmaxf(g, -300.f) * 1.4426950408889634;
+}
+// the decay before the walk's step i: backwards that of the step after it in time
+__device__ __forceinline__ double log2_decay(const Walk &p, int b, int h, int i) {
+  const int t = p.rev ? p.chunks * CH - i : i;
+  return t < p.length ? log2_of(p, b, h, t) : 0.0;
+}
+
+// What the chunk's decays come to, by one warp, two steps a lane: sums from the chunk's start in two floats, their
+// exponentials, and what is left of each step at the chunk's end.
+struct Decays {
+  float hi[CH], lo[CH], in[CH], out[CH];
+  float keep;
+  double total;
+};
+__device__ __forceinline__ void chunk_decays(const Walk &p, int b, int h, int i0, int lane, Decays &d) {
+  const double a0 = log2_decay(p, b, h, i0 + 2 * lane), a1 = log2_decay(p, b, h, i0 + 2 * lane + 1);
+  double s = a0 + a1;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double u = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += u;
+  }
+  const double end = __shfl_sync(0xffffffffu, s, 31);
+  const double G[2] = {s - a1, s};
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int i = 2 * lane + j;
+    const float hi = (float)G[j];
+    d.hi[i] = hi;
+    d.lo[i] = (float)(G[j] - (double)hi);
+    d.in[i] = ex2a(hi);
+    d.out[i] = ex2a((float)(end - G[j])) * p.s_update;
+  }
+  if (lane == 0) {
+    d.keep = ex2a((float)end);
+    d.total = end;
+  }
+}
+// exp(G_r - G_c)
+__device__ __forceinline__ float decay_between(const Decays &d, int r, int c) { return ex2a((d.hi[r] - d.hi[c]) + (d.lo[r] - d.lo[c])); }
+
+// The dots of a chunk's steps become what the pairs of steps on both sides of a step give to its decay, by one warp, in 64
+// bits.  Forwards (x . dq, pairs whose earlier step is before the chunk): the sum from the step on.  Backwards (x . dk, pairs whose later step is after
+// the chunk, and pairs within it, by row and column sums without the diagonal): the sum over the steps before it in time.
+__device__ __forceinline__ void chunk_runs(const Walk &p, int tile, int bh, int i0, int lane, double v0, double v1, float dots) {
+  double s = v0 + v1;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double u = __shfl_down_sync(0xffffffffu, s, o);
+    if (lane + o < 32) s += u;
+  }
+  const int64_t row = (int64_t)tile * p.batch * p.heads + bh;
+  const double r0 = p.rev ? s - v0 : s, r1 = p.rev ? s - v0 - v1 : s - v0;
+  const int t0 = time_of(p, i0 + 2 * lane), t1 = time_of(p, i0 + 2 * lane + 1);
+  if (t0 < p.length) p.run[row * p.length + t0] = (float)r0;
+  if (t1 < p.length) p.run[row * p.length + t1] = (float)r1;
+  dots = warp_sum(dots);
+  if (lane == 0) p.sum[row * p.chunks + (p.rev ? p.chunks - 1 - i0 / CH : i0 / CH)] = dots;
 }
 
 // One 16 x 8 x 8 product on TF32 operands given as float32 bit patterns.
@@ -136,10 +197,10 @@ __device__ __forceinline__ void load_rows(const Walk &p, const void *base, int64
   const bool vec = ((reinterpret_cast<uintptr_t>(src + col0) | (uintptr_t)(ls * sizeof(T))) & (4 * sizeof(T) - 1)) == 0;
   const int per = width / 4;
   for (int e = threadIdx.x; e < CH * per; e += WT) {
-    const int r = e / per, c = e % per * 4, i = i0 + r;
+    const int r = e / per, c = e % per * 4, i = time_of(p, i0 + r);
     float v[4] = {0.f, 0.f, 0.f, 0.f};
     if (i < p.length) {
-      const T *s = src + (int64_t)(p.rev ? p.length - 1 - i : i) * ls + col0 + c;
+      const T *s = src + (int64_t)i * ls + col0 + c;
       const int left = size - col0 - c;
       if (vec && left >= 4) {
         if constexpr (sizeof(T) == 4) {
@@ -165,13 +226,20 @@ template <typename T, bool STATE_ONLY> __global__ void __launch_bounds__(WT) lin
   constexpr bool F32 = sizeof(T) == 4;
   extern __shared__ __align__(16) float sm[];
   const int dip = (p.di + 15) / 16 * 16, PQ = dip + 4;
-  float *sq = sm, *sk = sq + (STATE_ONLY ? 0 : CH * PQ), *sv = sk + CH * PQ, *S = sv + CH * PV, *sp = S + dip * PV;
-  __shared__ float gh[CH], gl[CH], eg[CH], wu[CH], dots[2][CH];
-  __shared__ double g_total;
+  float *sk = sm, *sv = sk + CH * PQ, *S = sv + CH * PV, *sq = S + dip * PV, *sp = sq + CH * PQ, *sx = sp + CH * PP;
+  __shared__ Decays d;
+  __shared__ float dots[2][CH], rows_[2][CH], cols_[4][CH];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gq = lane >> 2, tq = lane & 3;
   const int tile = blockIdx.x % p.tiles, bh = blockIdx.x / p.tiles % (p.batch * p.heads), seg = blockIdx.x / p.tiles / (p.batch * p.heads);
   const int b = bh / p.heads, h = bh % p.heads, col0 = tile * DO;
-  const int i_begin = seg * p.seg_chunks * CH, i_end = min(p.length, (seg + 1) * p.seg_chunks * CH);
+  const int i_begin = seg * p.seg_chunks * CH, i_end = min(p.chunks, (seg + 1) * p.seg_chunks) * CH;
+  const int snaps = (p.chunks + kSnap - 1) / kSnap;
+  const auto snapshot = [&](int c, float f) {            // at the border before chunk c in time
+    for (int e = tid; e < p.di * DO; e += WT) {
+      const int r = e / DO, col = e % DO;
+      if (col0 + col < p.dout) p.snap[(((int64_t)bh * snaps + c / kSnap) * p.di + r) * p.dout + col0 + col] = S[r * PV + col] * f;
+    }
+  };
   // the state before the first step
   for (int e = tid; e < dip * DO; e += WT) {
     const int r = e / DO, c = e % DO;
@@ -184,42 +252,57 @@ template <typename T, bool STATE_ONLY> __global__ void __launch_bounds__(WT) lin
   }
   double total = 0.0;
   for (int i0 = i_begin; i0 < i_end; i0 += CH) {
-    __syncthreads();                                 // the last chunk's reads are done
-    if (warp == 0) {                                 // sums of the decays, two steps a lane
-      const double a0 = log2_decay(p, b, h, i0 + 2 * lane), a1 = log2_decay(p, b, h, i0 + 2 * lane + 1);
-      double s = a0 + a1;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double u = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s += u;
-      }
-      const double end = __shfl_sync(0xffffffffu, s, 31), first = s - a1;
-      const double G[2] = {first, s};
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float hi = (float)G[j];
-        gh[2 * lane + j] = hi;
-        gl[2 * lane + j] = (float)(G[j] - (double)hi);
-        eg[2 * lane + j] = ex2a(hi);
-        wu[2 * lane + j] = ex2a((float)(end - G[j])) * p.s_update;
-      }
-      if (lane == 0) g_total = end;
-    }
-    if (!STATE_ONLY) load_rows<T>(p, p.q, b * p.q_bs + h / p.q_div * p.q_hs, p.q_ls, i0, 0, p.di, dip, PQ, sq);
+    __syncthreads();                                 // the last chunk's reads and writes are done
+    const int chunk = p.rev ? p.chunks - 1 - i0 / CH : i0 / CH;
+    if (!STATE_ONLY && p.run && !p.rev && chunk % kSnap == 0) snapshot(chunk, 1.f);
+    if (warp == 0) chunk_decays(p, b, h, i0, lane, d);
     load_rows<T>(p, p.k, b * p.k_bs + h / p.k_div * p.k_hs, p.k_ls, i0, 0, p.di, dip, PQ, sk);
     load_rows<T>(p, p.v, b * p.v_bs + h / p.v_div * p.v_hs, p.v_ls, i0, col0, p.dout, DO, PV, sv);
+    if (!STATE_ONLY) {
+      load_rows<T>(p, p.q, b * p.q_bs + h / p.q_div * p.q_hs, p.q_ls, i0, 0, p.di, dip, PQ, sq);
+      if (p.run) load_rows<T>(p, p.x, b * p.x_bs + h / p.x_div * p.x_hs, p.x_ls, i0, col0, p.dout, DO, PP, sx);
+    }
     __syncthreads();
     const int m0 = (warp & 3) * 16, n0 = (warp >> 2) * 32;      // this warp's 16 x 32 of scores and of results
     if (!STATE_ONLY) {
       float acc[4][4] = {};
-      if (n0 <= m0 + 15) product<F32, F32>(acc, sq + m0 * PQ, PQ, 1, nullptr, sk + n0 * PQ, 1, PQ, dip, lane);
+      const bool any = n0 <= m0 + 15;
+      if (any) product<F32, F32>(acc, sq + m0 * PQ, PQ, 1, nullptr, sk + n0 * PQ, 1, PQ, dip, lane);
 #pragma unroll
       for (int n = 0; n < 4; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int r = m0 + gq + (e >> 1) * 8, c = n0 + n * 8 + tq * 2 + (e & 1);
-          sp[r * PP + c] = c <= r ? acc[n][e] * ex2a((gh[r] - gh[c]) + (gl[r] - gl[c])) * p.s_intra : 0.f;
+          acc[n][e] = c <= r ? acc[n][e] * decay_between(d, r, c) * p.s_intra : 0.f;
+          sp[r * PP + c] = acc[n][e];
         }
+      if (p.run && p.rev) {                          // products of a pair's two scores, without the diagonal
+        float x[4][4] = {};
+        if (any) product<F32, F32>(x, sx + m0 * PP, PP, 1, nullptr, sv + n0 * PV, 1, PV, DO, lane);
+        float row[2] = {0.f, 0.f};
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int e1 = 0; e1 < 2; ++e1) {
+            const int c = n0 + n * 8 + tq * 2 + e1;
+            float col = 0.f;
+#pragma unroll
+            for (int e2 = 0; e2 < 2; ++e2) {
+              const float m = c == m0 + gq + e2 * 8 ? 0.f : acc[n][e2 * 2 + e1] * x[n][e2 * 2 + e1];
+              row[e2] += m;
+              col += m;
+            }
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) col += __shfl_xor_sync(0xffffffffu, col, o);
+            if (gq == 0) cols_[warp & 3][c] = col;
+          }
+#pragma unroll
+        for (int e2 = 0; e2 < 2; ++e2) {
+          row[e2] += __shfl_xor_sync(0xffffffffu, row[e2], 1);
+          row[e2] += __shfl_xor_sync(0xffffffffu, row[e2], 2);
+          if (tq == 0) rows_[warp >> 2][m0 + gq + e2 * 8] = row[e2];
+        }
+      }
       __syncthreads();
 #pragma unroll
       for (int n = 0; n < 4; ++n)
@@ -229,17 +312,27 @@ template <typename T, bool STATE_ONLY> __global__ void __launch_bounds__(WT) lin
 #pragma unroll
       for (int n = 0; n < 4; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[n][e] *= eg[m0 + gq + (e >> 1) * 8] * p.s_inter;
+        for (int e = 0; e < 4; ++e) acc[n][e] *= d.in[m0 + gq + (e >> 1) * 8] * p.s_inter;
+      if (p.run) {
+#pragma unroll
+        for (int e2 = 0; e2 < 2; ++e2) {
+          const int r = m0 + gq + e2 * 8;
+          float s = 0.f;
+#pragma unroll
+          for (int n = 0; n < 4; ++n)
+#pragma unroll
+            for (int e1 = 0; e1 < 2; ++e1) s = fmaf(acc[n][e2 * 2 + e1], sx[r * PP + n0 + n * 8 + tq * 2 + e1], s);
+          s += __shfl_xor_sync(0xffffffffu, s, 1);
+          s += __shfl_xor_sync(0xffffffffu, s, 2);
+          if (tq == 0) dots[warp >> 2][r] = s;
+        }
+      }
       product<true, F32>(acc, sp + m0 * PP, PP, 1, nullptr, sv + n0, PV, 1, min(CH, m0 + 16), lane);
-      // out, and its product with x
-      float dsum[2] = {0.f, 0.f};
 #pragma unroll
       for (int e2 = 0; e2 < 2; ++e2) {
-        const int i = i0 + m0 + gq + e2 * 8;
-        if (i >= p.length) continue;
-        const int64_t t = p.rev ? p.length - 1 - i : i;
+        const int t = time_of(p, i0 + m0 + gq + e2 * 8);
+        if (t >= p.length) continue;
         const int64_t o = b * p.o_bs + t * p.o_ls + h * p.o_hs;
-        const T *x = p.dot ? reinterpret_cast<const T *>(p.x) + b * p.x_bs + t * p.x_ls + h / p.x_div * p.x_hs : nullptr;
 #pragma unroll
         for (int n = 0; n < 4; ++n)
 #pragma unroll
@@ -249,27 +342,29 @@ template <typename T, bool STATE_ONLY> __global__ void __launch_bounds__(WT) lin
             const float v = acc[n][e2 * 2 + e1];
             if (p.out_f32) reinterpret_cast<float *>(p.out)[o + c] = v;
             else reinterpret_cast<T *>(p.out)[o + c] = T(v);
-            if (x) dsum[e2] = fmaf(v, (float)x[c], dsum[e2]);
           }
-      }
-      if (p.dot) {
-#pragma unroll
-        for (int e2 = 0; e2 < 2; ++e2) {
-          dsum[e2] += __shfl_xor_sync(0xffffffffu, dsum[e2], 1);
-          dsum[e2] += __shfl_xor_sync(0xffffffffu, dsum[e2], 2);
-          if (tq == 0) dots[warp >> 2][m0 + gq + e2 * 8] = dsum[e2];
-        }
       }
     }
     __syncthreads();                                 // all have read the state
-    if (!STATE_ONLY && p.dot && tid < CH && i0 + tid < p.length)
-      p.dot[((int64_t)tile * p.batch * p.heads + bh) * p.length + (p.rev ? p.length - 1 - i0 - tid : i0 + tid)] = dots[0][tid] + dots[1][tid];
-    total += g_total;
-    const float keep = ex2a((float)g_total);
+    if (!STATE_ONLY && p.run && warp == 0) {
+      double v[2];
+      float s = 0.f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int i = 2 * lane + j;
+        const float dot = dots[0][i] + dots[1][i];
+        s += dot;
+        v[j] = dot;
+        if (p.rev) v[j] += ((double)rows_[0][i] + rows_[1][i]) - (((double)cols_[0][i] + cols_[1][i]) + ((double)cols_[2][i] + cols_[3][i]));
+      }
+      chunk_runs(p, tile, bh, i0, lane, v[0], v[1], s);
+    }
+    total += d.total;
+    const float keep = d.keep;
     for (int u = warp; u < dip / 16 * 2; u += 8) {
       const int r0 = u / 2 * 16, c0 = u % 2 * 32;
       float acc[4][4] = {};
-      product<true, F32>(acc, sk + r0, 1, PQ, wu, sv + c0, PV, 1, CH, lane);
+      product<true, F32>(acc, sk + r0, 1, PQ, d.out, sv + c0, PV, 1, CH, lane);
 #pragma unroll
       for (int n = 0; n < 4; ++n)
 #pragma unroll
@@ -277,6 +372,10 @@ template <typename T, bool STATE_ONLY> __global__ void __launch_bounds__(WT) lin
           float *s = S + (r0 + gq + (e >> 1) * 8) * PV + c0 + n * 8 + tq * 2 + (e & 1);
           *s = fmaf(*s, keep, acc[n][e]);
         }
+    }
+    if (!STATE_ONLY && p.run && p.rev && chunk % kSnap == 0) {
+      __syncthreads();
+      snapshot(chunk, ex2a((float)log2_of(p, b, h, chunk * CH)));
     }
   }
   __syncthreads();
@@ -287,8 +386,7 @@ template <typename T, bool STATE_ONLY> __global__ void __launch_bounds__(WT) lin
     }
     if (tile == 0 && tid == 0) p.seg_g[(int64_t)bh * p.nseg + seg] = total;
   } else if (p.last && seg == p.nseg - 1) {
-    float f = 1.f;
-    if (p.last_decay) f = ex2a((float)((double)fmaxf(load_g(p.g, p.g_dtype, b * p.g_bs + h * p.g_hs), -300.f) * 1.4426950408889634));
+    const float f = p.last_decay ? ex2a((float)log2_of(p, b, h, 0)) : 1.f;
     for (int e = tid; e < p.di * DO; e += WT) {
       const int r = e / DO, c = e % DO;
       if (col0 + c < p.dout) p.last[b * p.last_bs + h * p.last_hs + r * p.last_is + (col0 + c) * p.last_os] = S[r * PV + c] * f;
@@ -326,61 +424,69 @@ __global__ void __launch_bounds__(256) linattn_fold_kernel(const float *src, int
   }
 }
 
-// dg from the dots: one block a (batch, head), each thread a run of steps, sums in 64 bits.
-__global__ void __launch_bounds__(256) linattn_dg_kernel(const b200_linattn_args p, const float *dot_q, int tiles_q, const float *dot_k, int tiles_k, double *per_head) {
-  __shared__ double sh[256];
-  __shared__ double end_s;
-  const int bh = blockIdx.x, b = bh / p.heads, h = bh % p.heads, tid = threadIdx.x;
-  const int64_t plane = (int64_t)p.batch * p.heads * p.seqlen;
-  dot_q += (int64_t)bh * p.seqlen;
-  dot_k += (int64_t)bh * p.seqlen;
-  const auto d_at = [&](int t) {
-    double s = 0.0;
-    for (int i = 0; i < tiles_q; ++i) s += (double)dot_q[i * plane + t];
-    for (int i = 0; i < tiles_k; ++i) s -= (double)dot_k[i * plane + t];
-    return s;
-  };
-  double e = 0.0;                                     // what the last state gives all steps
-  if (p.dlast) {
-    const float *S = reinterpret_cast<const float *>(p.last) + (int64_t)bh * p.dk * p.dv;
-    const float *D = reinterpret_cast<const float *>(p.dlast) + (int64_t)bh * p.dk * p.dv;
-    for (int i = tid; i < p.dk * p.dv; i += 256) e += (double)S[i] * (double)D[i];
-  }
-  sh[tid] = e;
-  __syncthreads();
-  for (int o = 128; o > 0; o >>= 1) {
-    if (tid < o) sh[tid] += sh[tid + o];
-    __syncthreads();
-  }
-  if (tid == 0) end_s = sh[0];
-  __syncthreads();
-  const int run = (p.seqlen + 255) / 256, t0 = tid * run, t1 = min(p.seqlen, t0 + run);
+// What the pairs of steps on both sides of a whole chunk give: at every kSnap-th border all pairs across it are the product of
+// the two states there, and from border to border the sums of the chunk's dots are taken off and added on.
+__global__ void __launch_bounds__(256) linattn_across_kernel(const float *snap_q, const float *snap_k, const float *sum_q, const float *sum_k, int tiles, int64_t per,
+                                                            int chunks, int snaps, int bhs, double *across) {
+  __shared__ double sh[8];
+  const int bh = blockIdx.x / snaps, sn = blockIdx.x % snaps, tid = threadIdx.x;
+  const float *a = snap_q + (int64_t)blockIdx.x * per, *c = snap_k + (int64_t)blockIdx.x * per;
   double s = 0.0;
-  for (int t = t0; t < t1; ++t) s += d_at(t);
-  sh[tid] = s;
+  for (int64_t i = tid; i < per; i += 256) s += (double)a[i] * (double)c[i];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if ((tid & 31) == 0) sh[tid >> 5] = s;
   __syncthreads();
   if (tid == 0) {
-    double a = end_s;
-    for (int i = 255; i >= 0; --i) { const double v = sh[i]; sh[i] = a; a += v; }
+    double x = 0.0;
+    for (int i = 0; i < 8; ++i) x += sh[i];
+    for (int n = sn * kSnap; n < min(chunks, (sn + 1) * kSnap); ++n) {
+      double q = 0.0, k = 0.0;
+      for (int t = 0; t < tiles; ++t) {
+        q += (double)sum_q[((int64_t)t * bhs + bh) * chunks + n];
+        k += (double)sum_k[((int64_t)t * bhs + bh) * chunks + n];
+      }
+      x -= q;
+      across[(int64_t)bh * chunks + n] = x;
+      x += k;
+    }
+  }
+}
+
+__device__ __forceinline__ double dg_at(const b200_linattn_args &p, const float *run_q, const float *run_k, int tiles, const double *across, int chunks, int bh, int t) {
+  const int b = bh / p.heads, h = bh % p.heads;
+  if (load_g(p.g, p.g_dtype, b * p.g_bs + t * p.g_ls + h * p.g_hs) == -INFINITY) return 0.0;      // a decay of nothing has no slope
+  const int64_t plane = (int64_t)p.batch * p.heads * p.seqlen, i = (int64_t)bh * p.seqlen + t;
+  double s = across[(int64_t)bh * chunks + t / CH];
+  for (int n = 0; n < tiles; ++n) s += (double)run_q[n * plane + i] + (double)run_k[n * plane + i];
+  return s;
+}
+// 32 steps x 8 heads a block, so that both layouts are read and written in runs
+__global__ void __launch_bounds__(256) linattn_dg_kernel(const b200_linattn_args p, const float *run_q, const float *run_k, int tiles, const double *across, int chunks) {
+  __shared__ float sh[8][33];
+  const int b = blockIdx.z, t0 = blockIdx.x * 32, h0 = blockIdx.y * 8;
+  {
+    const int t = t0 + (threadIdx.x & 31), h = h0 + (threadIdx.x >> 5);
+    sh[threadIdx.x >> 5][threadIdx.x & 31] = t < p.seqlen && h < p.heads ? (float)dg_at(p, run_q, run_k, tiles, across, chunks, b * p.heads + h, t) : 0.f;
   }
   __syncthreads();
-  double a = sh[tid], sum = 0.0;
-  for (int t = t1 - 1; t >= t0; --t) {
-    a += d_at(t);
-    const int64_t gi = b * p.g_bs + t * p.g_ls + h * p.g_hs;
-    const double v = load_g(p.g, p.g_dtype, gi) == -INFINITY ? 0.0 : a;
-    if (per_head) sum += v;
-    else st_act(p.dg, p.g_dtype, ((int64_t)b * p.seqlen + t) * p.heads + h, (float)v);
-  }
-  if (per_head) {
-    __syncthreads();
-    sh[tid] = sum;
-    __syncthreads();
-    if (tid == 0) {
-      double x = 0.0;
-      for (int i = 0; i < 256; ++i) x += sh[i];
-      per_head[bh] = x;
-    }
+  const int t = t0 + (threadIdx.x >> 3), h = h0 + (threadIdx.x & 7);
+  if (t < p.seqlen && h < p.heads) st_act(p.dg, p.g_dtype, ((int64_t)b * p.seqlen + t) * p.heads + h, sh[threadIdx.x & 7][threadIdx.x >> 3]);
+}
+// a decay for each head: the sum over a (batch, head), then over the batch
+__global__ void __launch_bounds__(256) linattn_dg_sum_kernel(const b200_linattn_args p, const float *run_q, const float *run_k, int tiles, const double *across, int chunks,
+                                                            double *per_head) {
+  __shared__ double sh[8];
+  double s = 0.0;
+  for (int t = threadIdx.x; t < p.seqlen; t += 256) s += dg_at(p, run_q, run_k, tiles, across, chunks, blockIdx.x, t);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = 0.0;
+    for (int i = 0; i < 8; ++i) s += sh[i];
+    per_head[blockIdx.x] = s;
   }
 }
 __global__ void linattn_dg_heads_kernel(const b200_linattn_args p, const double *per_head) {
@@ -454,9 +560,9 @@ template <typename TS, typename T, int VEC> __global__ void __launch_bounds__(12
 
 int64_t up(int64_t n, int64_t unit) { return (n + unit - 1) / unit * unit; }
 
-int walk_smem(int di, bool state_only) {
+int walk_smem(int di, bool state_only, bool with_x) {
   const int dip = (int)up(di, 16);
-  return 4 * ((state_only ? 1 : 2) * CH * (dip + 4) + CH * PV + dip * PV + (state_only ? 0 : CH * PP));
+  return 4 * (CH * (dip + 4) + CH * PV + dip * PV + (state_only ? 0 : CH * (dip + 4) + (with_x ? 2 : 1) * CH * PP));
 }
 
 // Segments: as many as make the walk shortest, counted in chunks that one SM goes through, a first pass over segments at 0.45 of a walk.
@@ -475,7 +581,7 @@ int segments(int64_t blocks, int chunks) {
 }
 
 void cut(Walk &w) {
-  const int chunks = (w.length + CH - 1) / CH;
+  const int chunks = w.chunks;
   w.tiles = (w.dout + DO - 1) / DO;
   const int n = segments((int64_t)w.batch * w.heads * w.tiles, chunks);
   w.seg_chunks = (chunks + n - 1) / n;
@@ -488,7 +594,7 @@ template <typename T> int walk(Walk &w, unsigned char *work, cudaStream_t st) {
   if (w.nseg > 1) {
     w.seg = reinterpret_cast<float *>(work);
     w.seg_g = reinterpret_cast<double *>(work + up(4 * bh * w.nseg * w.di * w.dout, 256));
-    const int sm0 = walk_smem(w.di, true);
+    const int sm0 = walk_smem(w.di, true, false);
     cudaError_t e = cudaFuncSetAttribute(linattn_walk_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, sm0);
     if (e != cudaSuccess) { set_error("cudaFuncSetAttribute: %s", cudaGetErrorString(e)); return (int)e; }
     linattn_walk_kernel<T, true><<<(unsigned)(bh * w.tiles * (w.nseg - 1)), WT, sm0, st>>>(w);
@@ -496,7 +602,7 @@ template <typename T> int walk(Walk &w, unsigned char *work, cudaStream_t st) {
     linattn_join_kernel<<<dim3((unsigned)((per + 255) / 256), (unsigned)bh), 256, 0, st>>>(w);
     if (int r = launch_status()) return r;
   }
-  const int sm1 = walk_smem(w.di, false);
+  const int sm1 = walk_smem(w.di, false, w.run != nullptr);
   cudaError_t e = cudaFuncSetAttribute(linattn_walk_kernel<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, sm1);
   if (e != cudaSuccess) { set_error("cudaFuncSetAttribute: %s", cudaGetErrorString(e)); return (int)e; }
   linattn_walk_kernel<T, false><<<(unsigned)(bh * w.tiles * w.nseg), WT, sm1, st>>>(w);
@@ -524,6 +630,7 @@ Walk base_walk(const b200_linattn_args &a) {
   memset(&w, 0, sizeof(w));
   w.g = a.g; w.g_bs = a.g_bs; w.g_ls = a.g_ls; w.g_hs = a.g_hs; w.g_dtype = a.g_dtype;
   w.batch = a.batch; w.length = a.seqlen; w.heads = a.heads;
+  w.chunks = (a.seqlen + CH - 1) / CH;
   w.q_div = w.k_div = w.v_div = w.x_div = 1;
   return w;
 }
@@ -590,7 +697,7 @@ Walk walk_dv(const b200_linattn_args &a) {
   return w;
 }
 
-struct BwdPlan { int64_t seg, part, dot_q, dot_k, heads, total; };
+struct BwdPlan { int64_t seg, part, run, sum, snap, across, heads, total; };
 BwdPlan bwd_plan(const b200_linattn_args &a) {
   BwdPlan q;
   const int64_t bh = (int64_t)a.batch * a.heads;
@@ -600,11 +707,14 @@ BwdPlan bwd_plan(const b200_linattn_args &a) {
     const int64_t s = seg_bytes(bh, w.nseg, w.di, w.dout);
     if (s > q.seg) q.seg = s;
   }
+  const int64_t chunks = ws[0].chunks;
   q.part = a.heads != a.groups ? up(4 * bh * a.seqlen * a.dk, 256) : 0;
-  q.dot_q = a.dg ? up(4 * bh * a.seqlen * ws[0].tiles, 256) : 0;
-  q.dot_k = a.dg ? up(4 * bh * a.seqlen * ws[1].tiles, 256) : 0;
+  q.run = a.dg ? up(4 * bh * a.seqlen * ws[0].tiles, 256) : 0;
+  q.sum = a.dg ? up(4 * bh * chunks * ws[0].tiles, 256) : 0;
+  q.snap = a.dg ? up(4 * bh * ((chunks + kSnap - 1) / kSnap) * a.dk * a.dv, 256) : 0;
+  q.across = a.dg ? up(8 * bh * chunks, 256) : 0;
   q.heads = a.dg && a.g_heads ? up(8 * bh, 256) : 0;
-  q.total = q.seg + q.part + q.dot_q + q.dot_k + q.heads;
+  q.total = q.seg + q.part + 2 * (q.run + q.sum + q.snap) + q.across + q.heads;
   return q;
 }
 
@@ -658,17 +768,24 @@ extern "C" int b200_linattn_bwd(const b200_linattn_args *args, void *stream) {
   const b200_linattn_args &a = *args;
   if (int e = check_linattn(a)) return e;
   B200_REQUIRE(a.dout && a.dq && a.dk_out && a.dv_out, B200_ERR_NULL, "linattn_bwd: dout, dq, dk_out and dv_out must be non-null");
-  B200_REQUIRE(!a.dg || !a.dlast || a.last, B200_ERR_NULL, "linattn_bwd: with dlast and dg the last state must be non-null");
+  B200_REQUIRE(!a.dg || (int64_t)a.batch * a.heads * ((a.seqlen + CH * kSnap - 1) / (CH * kSnap)) < (int64_t(1) << 31), B200_ERR_SHAPE, "linattn_bwd: sizes too large");
   const BwdPlan q = bwd_plan(a);
   B200_REQUIRE(a.work_bytes >= q.total && (a.work || !q.total), B200_ERR_TOO_LARGE, "linattn_bwd: work has %lld bytes, %lld are needed", (long long)a.work_bytes,
                (long long)q.total);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   unsigned char *work = reinterpret_cast<unsigned char *>(a.work);
-  float *part = reinterpret_cast<float *>(work + q.seg), *dot_q = reinterpret_cast<float *>(work + q.seg + q.part);
-  float *dot_k = dot_q + q.dot_q / 4;
-  double *heads = reinterpret_cast<double *>(work + q.seg + q.part + q.dot_q + q.dot_k);
+  unsigned char *at = work + q.seg;
+  const auto take = [&](int64_t bytes) { unsigned char *r = at; at += bytes; return r; };
+  float *part = reinterpret_cast<float *>(take(q.part));
+  float *run[2], *sum[2], *snap[2];
+  for (int i = 0; i < 2; ++i) {
+    run[i] = reinterpret_cast<float *>(take(q.run));
+    sum[i] = reinterpret_cast<float *>(take(q.sum));
+    snap[i] = reinterpret_cast<float *>(take(q.snap));
+  }
+  double *across = reinterpret_cast<double *>(take(q.across)), *heads = reinterpret_cast<double *>(take(q.heads));
   const bool shared = a.heads != a.groups;
-  int tiles[2];
+  int tiles = 0, chunks = 0;
   for (int i = 0; i < 2; ++i) {
     Walk w = i == 0 ? walk_dq(a) : walk_dk(a);
     void *dst = i == 0 ? a.dq : a.dk_out;
@@ -677,8 +794,13 @@ extern "C" int b200_linattn_bwd(const b200_linattn_args *args, void *stream) {
     w.o_bs = (int64_t)a.seqlen * a.heads * a.dk;
     w.o_ls = (int64_t)a.heads * a.dk;
     w.o_hs = a.dk;
-    if (a.dg) w.dot = i == 0 ? dot_q : dot_k;
-    tiles[i] = w.tiles;
+    if (a.dg) {
+      w.run = run[i];
+      w.sum = sum[i];
+      w.snap = snap[i];
+    }
+    tiles = w.tiles;
+    chunks = w.chunks;
     if (int e = run_walk(a.dtype, w, work, st)) return e;
     if (shared)
       if (int e = fold(a, part, dst, st)) return e;
@@ -686,8 +808,15 @@ extern "C" int b200_linattn_bwd(const b200_linattn_args *args, void *stream) {
   Walk w = walk_dv(a);
   if (int e = run_walk(a.dtype, w, work, st)) return e;
   if (a.dg) {
-    linattn_dg_kernel<<<(unsigned)(a.batch * a.heads), 256, 0, st>>>(a, dot_q, tiles[0], dot_k, tiles[1], a.g_heads ? heads : nullptr);
-    if (a.g_heads) linattn_dg_heads_kernel<<<(unsigned)((a.heads + 127) / 128), 128, 0, st>>>(a, heads);
+    const int bh = a.batch * a.heads, snaps = (chunks + kSnap - 1) / kSnap;
+    linattn_across_kernel<<<(unsigned)((int64_t)bh * snaps), 256, 0, st>>>(snap[0], snap[1], sum[0], sum[1], tiles, (int64_t)a.dk * a.dv, chunks, snaps, bh, across);
+    if (a.g_heads) {
+      linattn_dg_sum_kernel<<<(unsigned)bh, 256, 0, st>>>(a, run[0], run[1], tiles, across, chunks, heads);
+      linattn_dg_heads_kernel<<<(unsigned)((a.heads + 127) / 128), 128, 0, st>>>(a, heads);
+    } else {
+      linattn_dg_kernel<<<dim3((unsigned)((a.seqlen + 31) / 32), (unsigned)((a.heads + 7) / 8), (unsigned)a.batch), 256, 0, st>>>(a, run[0], run[1], tiles, across,
+                                                                                                                             chunks);
+    }
   }
   return launch_status();
 }

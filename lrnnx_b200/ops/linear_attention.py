@@ -69,14 +69,14 @@ class LinearAttentionFn(torch.autograd.Function):
             work = _work(a, "b200_linattn_fwd_work_bytes", q)
             _lib.call("b200_linattn_fwd", a, _stream(q))
             del work
-        ctx.save_for_backward(q, k, v, g, s0, last)
+        ctx.save_for_backward(q, k, v, g, s0)
         ctx.scale = scale
         ctx.set_materialize_grads(False)
         return (out, last) if return_last_state else out
 
     @staticmethod
     def backward(ctx, dout, dlast=None):
-        q, k, v, g, s0, last = ctx.saved_tensors
+        q, k, v, g, s0 = ctx.saved_tensors
         if dout is None and dlast is None:
             return None, None, None, None, None, None, None
         a = _lib.struct("b200_linattn_args")()
@@ -87,7 +87,7 @@ class LinearAttentionFn(torch.autograd.Function):
             a.dout_bs, a.dout_ls, a.dout_hs, _ = dout.stride()
             if dlast is not None:
                 dlast = dlast.contiguous()
-                a.dlast, a.last = dlast.data_ptr(), last.data_ptr()
+                a.dlast = dlast.data_ptr()
             new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
             dq, dk, dv = new(q), new(k), new(v)
             a.dq, a.dk_out, a.dv_out = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
