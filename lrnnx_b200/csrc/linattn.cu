@@ -394,6 +394,438 @@ template <typename T, bool STATE_ONLY> __global__ void __launch_bounds__(WT) lin
   }
 }
 
+// ------------------------------------------------------------------------------------------------ bfloat16
+//
+// The same walk on bfloat16 m16n8k16 products, eight warps a block.  A warp has 16 steps of a chunk and 32 of the 64 columns: scores
+// become the left operand of the product with v without leaving its registers (the two warps of a row each form them).
+// The state lives in the warps' accumulators (a quarter of its rows, half of its columns each) and is scaled and added to
+// there; what is multiplied with q are its bfloat16 terms in shared memory, written once a chunk.  The terms of a float32 number are
+// its bfloat16 rounding, that of the rest, and so on: two keep 2^-17 of it, which a bfloat16 result does not see, three all
+// of it.  Scores are kept in two, the state that q meets in two (three where its dots with x go into the float32 gradient of
+// g), decayed values in two (three where the state is itself a result or goes into such a dot).  float16 stays with the
+// TF32 kernel: its states may exceed what it can hold.
+//
+// Loads are asynchronous copies: queries and values of the next chunk are on their way while the state is brought up to
+// date, its keys while values are decayed and q meets the state.
+
+constexpr int BT = 256;                     // threads
+constexpr int VP = DO * 2 + 16;             // bytes: rows of 64 columns, shifted by 16 bytes from row to row
+
+__device__ __forceinline__ void ldsm(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// the next bfloat16 term of two numbers, which keep their rest
+__device__ __forceinline__ uint32_t term(float &a, float &b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  const uint32_t w = *reinterpret_cast<const uint32_t *>(&v);
+  a -= __uint_as_float(w << 16);
+  b -= __uint_as_float(w & 0xffff0000u);
+  return w;
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, uint32_t bytes) {      // the rest of 16 bytes is zero
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// An operand's tile: 64 rows of W columns (64 or 128) from step i0 on, zero past the sequence and past its size
+struct Tile {
+  const __nv_bfloat16 *src;
+  int64_t ls;
+  int left;                                 // columns there are
+  bool vec;
+};
+__device__ __forceinline__ Tile tile_of(const void *base, int64_t off, int64_t ls, int col0, int size) {
+  Tile t;
+  t.src = reinterpret_cast<const __nv_bfloat16 *>(base) + off + col0;
+  t.ls = ls;
+  t.left = size - col0;
+  t.vec = ((reinterpret_cast<uintptr_t>(t.src) | (uintptr_t)(ls * 2)) & 15) == 0;
+  return t;
+}
+template <int W> __device__ __forceinline__ void load_tile(const Walk &p, const Tile &o, int i0, int pitch, unsigned char *dst) {
+  constexpr int PER = W / 8, ROWS = BT / PER;            // 16-byte pieces of a row, rows a pass
+  const int r0 = threadIdx.x / PER, c = threadIdx.x % PER * 8, left = o.left - c;
+#pragma unroll
+  for (int i = 0; i < CH / ROWS; ++i) {
+    const int r = r0 + i * ROWS, t = time_of(p, i0 + r);
+    const bool in = t < p.length && left > 0;
+    const __nv_bfloat16 *s = o.src + (int64_t)(in ? t : 0) * o.ls + (in ? c : 0);
+    unsigned char *at = dst + r * pitch + c * 2;
+    if (o.vec) copy16(smem_u32(at), s, in ? (left >= 8 ? 16u : (uint32_t)left * 2) : 0u);
+    else {
+      uint16_t x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = in && j < left ? reinterpret_cast<const uint16_t *>(s)[j] : 0;
+      *reinterpret_cast<uint4 *>(at) = make_uint4(x[0] | (uint32_t)x[1] << 16, x[2] | (uint32_t)x[3] << 16, x[4] | (uint32_t)x[5] << 16, x[6] | (uint32_t)x[7] << 16);
+    }
+  }
+}
+
+// a chunk's decays, and from each 16 steps' start back to the steps before (what lies between two blocks of 16 steps is
+// the product of two factors of at most one)
+struct Decays16 {
+  Decays d;
+  float back[3][CH];
+};
+__device__ __forceinline__ void chunk_decays16(const Walk &p, int b, int h, int i0, int lane, Decays16 &x) {
+  chunk_decays(p, b, h, i0, lane, x.d);
+  __syncwarp();
+#pragma unroll
+  for (int j = 1; j < 4; ++j)
+    for (int c = lane; c < 16 * j; c += 32) x.back[j - 1][c] = decay_between(x.d, 16 * j, c);
+}
+
+template <int DI, bool STATE_ONLY> __global__ void __launch_bounds__(BT, 2) linattn_walk16_kernel(const Walk p, const int ts, const int tu) {
+  constexpr int QP = DI * 2 + 16, MS = DI / 64;          // bytes of a row of q and k; 16-row tiles of the state for each warp
+  extern __shared__ __align__(16) unsigned char sb[];
+  unsigned char *sk = sb, *sv = sk + CH * QP, *su = sv + CH * VP, *ss = su + tu * CH * VP, *sq = ss + ts * DI * VP, *sx = sq + CH * QP;
+  __shared__ Decays16 dd[2];
+  __shared__ float dots[2][CH], rows_[2][CH], cols_[4][CH];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gq = lane >> 2, tq = lane & 3;
+  const int tile = blockIdx.x % p.tiles, bh = blockIdx.x / p.tiles % (p.batch * p.heads), seg = blockIdx.x / p.tiles / (p.batch * p.heads);
+  const int b = bh / p.heads, h = bh % p.heads, col0 = tile * DO;
+  const int i_begin = seg * p.seg_chunks * CH, i_end = min(p.chunks, (seg + 1) * p.seg_chunks) * CH;
+  const int snaps = (p.chunks + kSnap - 1) / kSnap;
+  const int wr = warp & 3, wc = warp >> 2;               // this warp's 16 steps (quarter of the state's rows), half of the columns
+  const int d0 = wr * (DI / 4), m0 = wr * 16, n0 = wc * 32;
+  const bool grad = !STATE_ONLY && p.run, cross = grad && p.rev;
+  // ldmatrix addresses of a lane within a 16 x 16 tile: by rows; two 8-row tiles side by side along the rows
+  const int a_row = lane & 15, a_col = (lane >> 4) * 8;
+  const int b_row = (lane & 7) + ((lane >> 4) << 3), b_col = ((lane >> 3) & 1) * 8;
+
+  float S[MS][4][4];
+  const auto each = [&](auto f) {                        // all elements of the state within its size: row, column, value
+#pragma unroll
+    for (int m = 0; m < MS; ++m)
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = d0 + m * 16 + gq + (e >> 1) * 8, c = col0 + n0 + n * 8 + tq * 2 + (e & 1);
+          if (r < p.di && c < p.dout) f(r, c, S[m][n][e]);
+        }
+  };
+  const auto write_terms = [&]() {
+#pragma unroll
+    for (int m = 0; m < MS; ++m)
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int e2 = 0; e2 < 2; ++e2) {
+          float x = S[m][n][e2 * 2], y = S[m][n][e2 * 2 + 1];
+          unsigned char *at = ss + (d0 + m * 16 + gq + e2 * 8) * VP + (n0 + n * 8 + tq * 2) * 2;
+          *reinterpret_cast<uint32_t *>(at) = term(x, y);
+          *reinterpret_cast<uint32_t *>(at + DI * VP) = term(x, y);
+          if (ts == 3) *reinterpret_cast<uint32_t *>(at + 2 * DI * VP) = term(x, y);
+        }
+  };
+#pragma unroll
+  for (int m = 0; m < MS; ++m)
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) S[m][n][e] = 0.f;
+  const Tile tk = tile_of(p.k, b * p.k_bs + h / p.k_div * p.k_hs, p.k_ls, 0, p.di), tv = tile_of(p.v, b * p.v_bs + h / p.v_div * p.v_hs, p.v_ls, col0, p.dout);
+  const Tile tq_ = tile_of(p.q, b * p.q_bs + h / p.q_div * p.q_hs, p.q_ls, 0, p.di), tx = tile_of(p.x, b * p.x_bs + h / p.x_div * p.x_hs, p.x_ls, col0, p.dout);
+  const auto load_first = [&](int i0) {                  // what is needed first
+    load_tile<64>(p, tv, i0, VP, sv);
+    if (!STATE_ONLY) load_tile<DI>(p, tq_, i0, QP, sq);
+    if (grad) load_tile<64>(p, tx, i0, VP, sx);
+    copies_commit();
+  };
+  const auto load_keys = [&](int i0) {
+    load_tile<DI>(p, tk, i0, QP, sk);
+    copies_commit();
+  };
+  load_first(i_begin);
+  load_keys(i_begin);
+  if (warp == 7) chunk_decays16(p, b, h, i_begin, lane, dd[0]);
+  if (!STATE_ONLY) {
+    if (p.nseg > 1) each([&](int r, int c, float &s) { s = p.seg[(((int64_t)bh * p.nseg + seg) * p.di + r) * p.dout + c]; });
+    else if (p.s0) each([&](int r, int c, float &s) { s = p.s0[b * p.s0_bs + h * p.s0_hs + r * p.s0_is + c * p.s0_os]; });
+    write_terms();
+  }
+  double total = 0.0;
+  for (int i0 = i_begin, it = 0; i0 < i_end; i0 += CH, ++it) {
+    const int chunk = p.rev ? p.chunks - 1 - i0 / CH : i0 / CH;
+    const Decays16 &x16 = dd[it & 1];
+    const Decays &d = x16.d;
+    if (grad && !p.rev && chunk % kSnap == 0)
+      each([&](int r, int c, float &s) { p.snap[(((int64_t)bh * snaps + chunk / kSnap) * p.di + r) * p.dout + c] = s; });
+    copies_wait<1>();
+    __syncthreads();                                     // values and queries have arrived, the state's terms and the decays are written
+    // values as the state takes them up, in terms
+#pragma unroll
+    for (int i = 0; i < CH * DO / 4 / BT; ++i) {
+      const int e = i * BT + tid, r = e / (DO / 4), c = e % (DO / 4) * 8;
+      const uint2 v = *reinterpret_cast<const uint2 *>(sv + r * VP + c);
+      const float w = d.out[r];
+      float y[4] = {__uint_as_float(v.x << 16) * w, __uint_as_float(v.x & 0xffff0000u) * w, __uint_as_float(v.y << 16) * w, __uint_as_float(v.y & 0xffff0000u) * w};
+      unsigned char *at = su + r * VP + c;
+      *reinterpret_cast<uint2 *>(at) = make_uint2(term(y[0], y[1]), term(y[2], y[3]));
+      *reinterpret_cast<uint2 *>(at + CH * VP) = make_uint2(term(y[0], y[1]), term(y[2], y[3]));
+      if (tu == 3) *reinterpret_cast<uint2 *>(at + 2 * CH * VP) = make_uint2(term(y[0], y[1]), term(y[2], y[3]));
+    }
+    if constexpr (!STATE_ONLY) {
+      const uint32_t aq = smem_u32(sq) + (m0 + a_row) * QP + a_col * 2;
+      const int r0 = m0 + gq;
+      float O[4][4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) O[n][e] = 0.f;
+#pragma unroll
+      for (int k0 = 0; k0 < DI; k0 += 16) {
+        uint32_t a[4];
+        ldsm(a, aq + k0 * 2);
+        for (int t = ts - 1; t >= 0; --t) {
+          const uint32_t as = smem_u32(ss) + t * DI * VP + (k0 + a_row) * VP + (n0 + a_col) * 2;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            uint32_t w[4];
+            ldsm_t(w, as + j * 32);
+            mma16(O[2 * j], a, w[0], w[1]);
+            mma16(O[2 * j + 1], a, w[2], w[3]);
+          }
+        }
+      }
+      {
+        const float f0 = d.in[r0] * p.s_inter, f1 = d.in[r0 + 8] * p.s_inter;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          O[n][0] *= f0;
+          O[n][1] *= f0;
+          O[n][2] *= f1;
+          O[n][3] *= f1;
+        }
+      }
+      if (grad) {
+#pragma unroll
+        for (int e2 = 0; e2 < 2; ++e2) {
+          float dot = 0.f;
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const uint32_t w = *reinterpret_cast<const uint32_t *>(sx + (r0 + e2 * 8) * VP + (n0 + n * 8 + tq * 2) * 2);
+            dot = fmaf(O[n][e2 * 2], __uint_as_float(w << 16), fmaf(O[n][e2 * 2 + 1], __uint_as_float(w & 0xffff0000u), dot));
+          }
+          dot += __shfl_xor_sync(0xffffffffu, dot, 1);
+          dot += __shfl_xor_sync(0xffffffffu, dot, 2);
+          if (tq == 0) dots[wc][r0 + e2 * 8] = dot;
+        }
+      }
+      copies_wait<0>();
+      __syncthreads();                                   // the keys have arrived
+      float P[8][4];
+#pragma unroll
+      for (int n = 0; n < 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) P[n][e] = 0.f;
+#pragma unroll
+      for (int k0 = 0; k0 < DI; k0 += 16) {
+        uint32_t a[4];
+        ldsm(a, aq + k0 * 2);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (j <= wr) {                                 // columns of earlier or the same 16 steps
+            uint32_t kb[4];
+            ldsm(kb, smem_u32(sk) + (j * 16 + b_row) * QP + (k0 + b_col) * 2);
+            mma16(P[2 * j], a, kb[0], kb[1]);
+            mma16(P[2 * j + 1], a, kb[2], kb[3]);
+          }
+      }
+      {
+        float f[2];
+#pragma unroll
+        for (int e2 = 0; e2 < 2; ++e2) f[e2] = decay_between(d, r0 + e2 * 8, m0) * p.s_intra;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (j < wr) {
+#pragma unroll
+            for (int n = 2 * j; n < 2 * j + 2; ++n) {
+              const float2 w = *reinterpret_cast<const float2 *>(&x16.back[wr - 1][n * 8 + tq * 2]);
+              P[n][0] *= f[0] * w.x;
+              P[n][1] *= f[0] * w.y;
+              P[n][2] *= f[1] * w.x;
+              P[n][3] *= f[1] * w.y;
+            }
+          } else if (j == wr) {
+#pragma unroll
+            for (int n = 2 * j; n < 2 * j + 2; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int r = r0 + (e >> 1) * 8, c = n * 8 + tq * 2 + (e & 1);
+                P[n][e] = c <= r ? P[n][e] * decay_between(d, r, c) * p.s_intra : 0.f;
+              }
+          }
+        }
+      }
+      if (cross) {                                       // products of a pair's two scores, without the diagonal; every other 16 columns
+        float row[2] = {0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if ((j & 1) == wc) {
+            float X[2][4] = {};
+            if (j <= wr) {
+#pragma unroll
+              for (int k0 = 0; k0 < DO; k0 += 16) {
+                uint32_t a[4], w[4];
+                ldsm(a, smem_u32(sx) + (m0 + a_row) * VP + (k0 + a_col) * 2);
+                ldsm(w, smem_u32(sv) + (j * 16 + b_row) * VP + (k0 + b_col) * 2);
+                mma16(X[0], a, w[0], w[1]);
+                mma16(X[1], a, w[2], w[3]);
+              }
+            }
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+              for (int e1 = 0; e1 < 2; ++e1) {
+                const int c = j * 16 + n * 8 + tq * 2 + e1;
+                float col = 0.f;
+#pragma unroll
+                for (int e2 = 0; e2 < 2; ++e2) {
+                  const float m = c == r0 + e2 * 8 ? 0.f : P[2 * j + n][e2 * 2 + e1] * X[n][e2 * 2 + e1];
+                  row[e2] += m;
+                  col += m;
+                }
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) col += __shfl_xor_sync(0xffffffffu, col, o);
+                if (gq == 0) cols_[wr][c] = col;
+              }
+          }
+#pragma unroll
+        for (int e2 = 0; e2 < 2; ++e2) {
+          row[e2] += __shfl_xor_sync(0xffffffffu, row[e2], 1);
+          row[e2] += __shfl_xor_sync(0xffffffffu, row[e2], 2);
+          if (tq == 0) rows_[wc][r0 + e2 * 8] = row[e2];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j <= wr) {
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float x = P[2 * j + (i >> 1)][(i & 1) * 2], y = P[2 * j + (i >> 1)][(i & 1) * 2 + 1];
+            hi[i] = term(x, y);
+            lo[i] = term(x, y);
+          }
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            uint32_t w[4];
+            ldsm_t(w, smem_u32(sv) + (j * 16 + a_row) * VP + (n0 + n * 16 + a_col) * 2);
+            mma16(O[2 * n], lo, w[0], w[1]);
+            mma16(O[2 * n + 1], lo, w[2], w[3]);
+            mma16(O[2 * n], hi, w[0], w[1]);
+            mma16(O[2 * n + 1], hi, w[2], w[3]);
+          }
+        }
+#pragma unroll
+      for (int e2 = 0; e2 < 2; ++e2) {
+        const int t = time_of(p, i0 + r0 + e2 * 8);
+        if (t >= p.length) continue;
+        const int64_t at = b * p.o_bs + t * p.o_ls + h * p.o_hs + col0;
+        if (p.out_f32) {
+          float *o = reinterpret_cast<float *>(p.out) + at;
+          const bool pair = (reinterpret_cast<uintptr_t>(o) & 7) == 0;
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const int c = n0 + n * 8 + tq * 2;
+            if (pair && col0 + c + 1 < p.dout) *reinterpret_cast<float2 *>(o + c) = make_float2(O[n][e2 * 2], O[n][e2 * 2 + 1]);
+            else {
+              if (col0 + c < p.dout) o[c] = O[n][e2 * 2];
+              if (col0 + c + 1 < p.dout) o[c + 1] = O[n][e2 * 2 + 1];
+            }
+          }
+        } else {
+          __nv_bfloat16 *o = reinterpret_cast<__nv_bfloat16 *>(p.out) + at;
+          const bool pair = (reinterpret_cast<uintptr_t>(o) & 3) == 0;
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const int c = n0 + n * 8 + tq * 2;
+            const __nv_bfloat162 v = __floats2bfloat162_rn(O[n][e2 * 2], O[n][e2 * 2 + 1]);
+            if (pair && col0 + c + 1 < p.dout) *reinterpret_cast<__nv_bfloat162 *>(o + c) = v;
+            else {
+              if (col0 + c < p.dout) o[c] = v.x;
+              if (col0 + c + 1 < p.dout) o[c + 1] = v.y;
+            }
+          }
+        }
+      }
+    } else {
+      copies_wait<0>();
+    }
+    __syncthreads();                                     // queries, values and the state's terms are read, the values' terms written
+    if (i0 + CH < i_end) {
+      load_first(i0 + CH);
+      if (warp == 7) chunk_decays16(p, b, h, i0 + CH, lane, dd[(it + 1) & 1]);
+    }
+    total += d.total;
+    const float keep = d.keep;
+#pragma unroll
+    for (int m = 0; m < MS; ++m)
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) S[m][n][e] *= keep;
+#pragma unroll
+    for (int k0 = 0; k0 < CH; k0 += 16) {
+      uint32_t a[MS][4];
+#pragma unroll
+      for (int m = 0; m < MS; ++m) ldsm_t(a[m], smem_u32(sk) + (k0 + b_row) * QP + (d0 + m * 16 + b_col) * 2);
+      for (int t = tu - 1; t >= 0; --t)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          uint32_t w[4];
+          ldsm_t(w, smem_u32(su) + t * CH * VP + (k0 + a_row) * VP + (n0 + n * 16 + a_col) * 2);
+#pragma unroll
+          for (int m = 0; m < MS; ++m) {
+            mma16(S[m][2 * n], a[m], w[0], w[1]);
+            mma16(S[m][2 * n + 1], a[m], w[2], w[3]);
+          }
+        }
+    }
+    if (grad && warp == 0) {
+      double v[2];
+      float s = 0.f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int i = 2 * lane + j;
+        const float dot = dots[0][i] + dots[1][i];
+        s += dot;
+        v[j] = dot;
+        if (p.rev) v[j] += ((double)rows_[0][i] + rows_[1][i]) - (((double)cols_[0][i] + cols_[1][i]) + ((double)cols_[2][i] + cols_[3][i]));
+      }
+      chunk_runs(p, tile, bh, i0, lane, v[0], v[1], s);
+    }
+    if (cross && chunk % kSnap == 0) {
+      const float f = ex2a((float)log2_of(p, b, h, chunk * CH));
+      each([&](int r, int c, float &s) { p.snap[(((int64_t)bh * snaps + chunk / kSnap) * p.di + r) * p.dout + c] = s * f; });
+    }
+    if (!STATE_ONLY) write_terms();
+    __syncthreads();                                     // the keys and the values' terms are read
+    if (i0 + CH < i_end) load_keys(i0 + CH);
+  }
+  if (STATE_ONLY) {
+    each([&](int r, int c, float &s) { p.seg[(((int64_t)bh * p.nseg + seg) * p.di + r) * p.dout + c] = s; });
+    if (tile == 0 && tid == 0) p.seg_g[(int64_t)bh * p.nseg + seg] = total;
+  } else if (p.last && seg == p.nseg - 1) {
+    const float f = p.last_decay ? ex2a((float)log2_of(p, b, h, 0)) : 1.f;
+    each([&](int r, int c, float &s) { p.last[b * p.last_bs + h * p.last_hs + r * p.last_is + c * p.last_os] = s * f; });
+  }
+}
+
 // Each segment's own state becomes the state before it.
 __global__ void __launch_bounds__(256) linattn_join_kernel(const Walk p) {
   const int64_t per = (int64_t)p.di * p.dout, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -589,28 +1021,36 @@ void cut(Walk &w) {
 }
 int64_t seg_bytes(int64_t bh, int nseg, int di, int dout) { return nseg > 1 ? up(4 * bh * nseg * di * dout, 256) + up(8 * bh * nseg, 256) : 0; }
 
-template <typename T> int walk(Walk &w, unsigned char *work, cudaStream_t st) {
+// the launches of a walk: `own` and `all` are its kernels for a segment's own state and for the results
+template <typename K, typename... More>
+int launch_walk(Walk &w, K own, K all, int threads, int smem_own, int smem_all, unsigned char *work, cudaStream_t st, More... more) {
   const int64_t bh = (int64_t)w.batch * w.heads;
+  cudaError_t e = cudaFuncSetAttribute(all, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_all);
+  if (e == cudaSuccess && w.nseg > 1) e = cudaFuncSetAttribute(own, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_own);
+  if (e != cudaSuccess) { set_error("cudaFuncSetAttribute: %s", cudaGetErrorString(e)); return (int)e; }
   if (w.nseg > 1) {
     w.seg = reinterpret_cast<float *>(work);
     w.seg_g = reinterpret_cast<double *>(work + up(4 * bh * w.nseg * w.di * w.dout, 256));
-    const int sm0 = walk_smem(w.di, true, false);
-    cudaError_t e = cudaFuncSetAttribute(linattn_walk_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, sm0);
-    if (e != cudaSuccess) { set_error("cudaFuncSetAttribute: %s", cudaGetErrorString(e)); return (int)e; }
-    linattn_walk_kernel<T, true><<<(unsigned)(bh * w.tiles * (w.nseg - 1)), WT, sm0, st>>>(w);
+    own<<<(unsigned)(bh * w.tiles * (w.nseg - 1)), threads, smem_own, st>>>(w, more...);
     const int64_t per = (int64_t)w.di * w.dout;
     linattn_join_kernel<<<dim3((unsigned)((per + 255) / 256), (unsigned)bh), 256, 0, st>>>(w);
     if (int r = launch_status()) return r;
   }
-  const int sm1 = walk_smem(w.di, false, w.run != nullptr);
-  cudaError_t e = cudaFuncSetAttribute(linattn_walk_kernel<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, sm1);
-  if (e != cudaSuccess) { set_error("cudaFuncSetAttribute: %s", cudaGetErrorString(e)); return (int)e; }
-  linattn_walk_kernel<T, false><<<(unsigned)(bh * w.tiles * w.nseg), WT, sm1, st>>>(w);
+  all<<<(unsigned)(bh * w.tiles * w.nseg), threads, smem_all, st>>>(w, more...);
   return launch_status();
+}
+template <typename T> int walk(Walk &w, unsigned char *work, cudaStream_t st) {
+  return launch_walk(w, linattn_walk_kernel<T, true>, linattn_walk_kernel<T, false>, WT, walk_smem(w.di, true, false), walk_smem(w.di, false, w.run != nullptr), work, st);
+}
+template <int DI> int walk16(Walk &w, unsigned char *work, cudaStream_t st) {
+  const int ts = w.run ? 3 : 2, tu = w.run || w.last ? 3 : 2, qp = DI * 2 + 16;
+  const int own = CH * qp + (1 + tu) * CH * VP, all = own + CH * qp + ts * DI * VP + (w.run ? CH * VP : 0);
+  return launch_walk(w, linattn_walk16_kernel<DI, true>, linattn_walk16_kernel<DI, false>, BT, own, all, work, st, ts, tu);
 }
 int run_walk(int dtype, Walk &w, unsigned char *work, cudaStream_t st) {
   if (dtype == B200_F32) return walk<float>(w, work, st);
-  return dtype == B200_F16 ? walk<__half>(w, work, st) : walk<__nv_bfloat16>(w, work, st);
+  if (dtype == B200_F16) return walk<__half>(w, work, st);
+  return w.di <= 64 ? walk16<64>(w, work, st) : walk16<128>(w, work, st);
 }
 
 int check_linattn(const b200_linattn_args &a) {
