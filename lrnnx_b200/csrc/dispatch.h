@@ -29,8 +29,9 @@ int selscan_row1_bwd(const b200_selscan_bwd_args &a, cudaStream_t st);
 // status word of the tensor-core projection kernel (cgemm_tc.cu)
 int cgemm_status_read();
 
-// status word of the loss's products (lce.cu)
+// status words of the loss's products (lce.cu) and of linear attention (linattn.cu)
 int lce_status_read();
+int linattn_status_read();
 
 // status word of the decode-step pipeline (ssu.cu): non-zero after an expired bounded wait
 int ssu_status_read();

@@ -76,14 +76,6 @@ __device__ __forceinline__ void tma_st_3d(const CUtensorMap *map, const void *sr
                "r"(y), "r"(z), "r"(smem_u32(src))
                : "memory");
 }
-__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}"
-      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0)
-      : "memory");
-}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -593,10 +585,7 @@ template <int EPI> int launch_gemm(const LceGemm &g, cudaStream_t st) {
   return launch_status();
 }
 
-uint32_t idesc_of(int dtype, bool a_mn, bool b_mn) {
-  const uint32_t f = dtype == B200_F16 ? 0u : 1u;
-  return (1u << 4) | (f << 7) | (f << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((TN >> 3) << 17) | ((TM >> 4) << 24);
-}
+uint32_t idesc_of(int dtype, bool a_mn, bool b_mn) { return idesc_f16(dtype == B200_F16 ? 0u : 1u, a_mn, b_mn, TM, TN); }
 
 struct Operands { const void *h, *w; int64_t h_pitch, w_pitch; };
 

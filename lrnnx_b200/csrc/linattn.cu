@@ -15,24 +15,28 @@
 // before it of (what s puts into the state) . (what r takes from it), decayed from s to r.  Sums of q . dq - k . dk
 // would give it too, but as a small difference of long sums; instead, for a chunk: pairs within it, from the products of their two scores;
 // pairs with one step outside, from the dots of q with the state's part of dq and of k with that of dk; and pairs on
-// both sides of it, from the product of the two walks' states, which they save at every eighth border.
+// both sides of it, from the product of the two walks' states, which they save every 512 steps.
 //
 // One thread block walks 64 output columns of a (batch, head); where these are too few for the GPU the
 // sequence is cut into segments: a first pass forms each segment's own state, a scan joins them, and every segment then
 // starts from the state that the earlier ones lead to.
 #include "common.cuh"
 #include "dispatch.h"
+#include "tc_common.cuh"
 #include <cstring>
 
 namespace b200 {
 namespace {
+
+using namespace tc;
 
 constexpr int CH = 64;                    // steps of a chunk
 constexpr int DO = 64;                    // output columns of a block
 constexpr int WT = 256;
 constexpr int MAX_D = 128;
 constexpr int PP = CH + 4, PV = DO + 8;   // pitches of scores and of values / state (in floats)
-constexpr int kSnap = 8;                  // chunks between the states that the gradient of g is anchored at
+constexpr int kSnapSteps = 512;           // steps between the states that the gradient of g is anchored at
+constexpr int kSnap = kSnapSteps / CH;
 
 struct Walk {
   // operands (batch, length, heads or groups, size), sizes contiguous; strides in elements
@@ -43,7 +47,7 @@ struct Walk {
   int64_t g_bs, g_ls, g_hs;
   int g_dtype;
   int batch, length, heads, di, dout;     // sizes of q, k and of v
-  int chunks, rev;                        // rev: from the last chunk to the first, and backwards within each
+  int ch, chunks, rev;                    // steps of a chunk; rev: from the last chunk to the first, and backwards within each
   float s_inter, s_intra, s_update;
   const float *s0;                        // state at the start: (batch, heads, di, dout) by strides
   int64_t s0_bs, s0_hs, s0_is, s0_os;
@@ -70,7 +74,7 @@ __device__ __forceinline__ float ex2a(float x) {
 __device__ __forceinline__ float load_g(const void *g, int dtype, int64_t i) { return ld_act(g, dtype, i); }
 
 // the time of the walk's step i (past the sequence's end where there is none)
-__device__ __forceinline__ int time_of(const Walk &p, int i) { return p.rev ? p.chunks * CH - 1 - i : i; }
+__device__ __forceinline__ int time_of(const Walk &p, int i) { return p.rev ? p.chunks * p.ch - 1 - i : i; }
 
 // a log decay in units of log2, bounded below; NaN stays
 __device__ __forceinline__ double log2_of(const Walk &p, int b, int h, int t) {
@@ -79,7 +83,7 @@ __device__ __forceinline__ double log2_of(const Walk &p, int b, int h, int t) {
 }
 // the decay before the walk's step i: backwards that of the step after it in time
 __device__ __forceinline__ double log2_decay(const Walk &p, int b, int h, int i) {
-  const int t = p.rev ? p.chunks * CH - i : i;
+  const int t = p.rev ? p.chunks * p.ch - i : i;
   return t < p.length ? log2_of(p, b, h, t) : 0.0;
 }
 
@@ -87,7 +91,7 @@ __device__ __forceinline__ double log2_decay(const Walk &p, int b, int h, int i)
 // exponentials, and what is left of each step at the chunk's end.
 struct Decays {
   float hi[CH], lo[CH], in[CH], out[CH];
-  float keep;
+  float keep, keep_lo;                    // of the state over the chunk, in two floats: it is multiplied up over all chunks
   double total;
 };
 __device__ __forceinline__ void chunk_decays(const Walk &p, int b, int h, int i0, int lane, Decays &d) {
@@ -110,30 +114,39 @@ __device__ __forceinline__ void chunk_decays(const Walk &p, int b, int h, int i0
     d.out[i] = ex2a((float)(end - G[j])) * p.s_update;
   }
   if (lane == 0) {
-    d.keep = ex2a((float)end);
+    const double keep = exp2(end);
+    d.keep = (float)keep;
+    d.keep_lo = end <= 0.0 ? (float)(keep - (double)d.keep) : 0.f;
     d.total = end;
   }
 }
 // exp(G_r - G_c)
 __device__ __forceinline__ float decay_between(const Decays &d, int r, int c) { return ex2a((d.hi[r] - d.hi[c]) + (d.lo[r] - d.lo[c])); }
 
-// The dots of a chunk's steps become what the pairs of steps on both sides of a step give to its decay, by one warp, in 64
-// bits.  Forwards (x . dq, pairs whose earlier step is before the chunk): the sum from the step on.  Backwards (x . dk, pairs whose later step is after
-// the chunk, and pairs within it, by row and column sums without the diagonal): the sum over the steps before it in time.
-__device__ __forceinline__ void chunk_runs(const Walk &p, int tile, int bh, int i0, int lane, double v0, double v1, float dots) {
-  double s = v0 + v1;
+// The dots of a chunk's steps become what the pairs of steps on both sides of a step give to its decay, by one warp, N steps a
+// lane, in 64 bits.  Forwards (x . dq, pairs whose earlier step is before the chunk): the sum from the step on.  Backwards (x . dk,
+// pairs whose later step is after the chunk, and pairs within it, by row and column sums without the diagonal): the sum
+// over the steps before it in time.
+template <int N> __device__ __forceinline__ void chunk_runs(const Walk &p, int tile, int bh, int i0, int lane, const double (&v)[N], float dots) {
+  double own = 0.0;
+#pragma unroll
+  for (int j = 0; j < N; ++j) own += v[j];
+  double s = own;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const double u = __shfl_down_sync(0xffffffffu, s, o);
     if (lane + o < 32) s += u;
   }
   const int64_t row = (int64_t)tile * p.batch * p.heads + bh;
-  const double r0 = p.rev ? s - v0 : s, r1 = p.rev ? s - v0 - v1 : s - v0;
-  const int t0 = time_of(p, i0 + 2 * lane), t1 = time_of(p, i0 + 2 * lane + 1);
-  if (t0 < p.length) p.run[row * p.length + t0] = (float)r0;
-  if (t1 < p.length) p.run[row * p.length + t1] = (float)r1;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int t = time_of(p, i0 + N * lane + j);
+    const double r = p.rev ? s - v[j] : s;
+    if (t < p.length) p.run[row * p.length + t] = (float)r;
+    s -= v[j];
+  }
   dots = warp_sum(dots);
-  if (lane == 0) p.sum[row * p.chunks + (p.rev ? p.chunks - 1 - i0 / CH : i0 / CH)] = dots;
+  if (lane == 0) p.sum[row * p.chunks + (p.rev ? p.chunks - 1 - i0 / p.ch : i0 / p.ch)] = dots;
 }
 
 // One 16 x 8 x 8 product on TF32 operands given as float32 bit patterns.
@@ -357,10 +370,10 @@ template <typename T, bool STATE_ONLY> __global__ void __launch_bounds__(WT) lin
         v[j] = dot;
         if (p.rev) v[j] += ((double)rows_[0][i] + rows_[1][i]) - (((double)cols_[0][i] + cols_[1][i]) + ((double)cols_[2][i] + cols_[3][i]));
       }
-      chunk_runs(p, tile, bh, i0, lane, v[0], v[1], s);
+      chunk_runs(p, tile, bh, i0, lane, v, s);
     }
     total += d.total;
-    const float keep = d.keep;
+    const float keep = d.keep, keep_lo = d.keep_lo;
     for (int u = warp; u < dip / 16 * 2; u += 8) {
       const int r0 = u / 2 * 16, c0 = u % 2 * 32;
       float acc[4][4] = {};
@@ -370,7 +383,7 @@ template <typename T, bool STATE_ONLY> __global__ void __launch_bounds__(WT) lin
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float *s = S + (r0 + gq + (e >> 1) * 8) * PV + c0 + n * 8 + tq * 2 + (e & 1);
-          *s = fmaf(*s, keep, acc[n][e]);
+          *s = fmaf(*s, keep, fmaf(*s, keep_lo, acc[n][e]));
         }
     }
     if (!STATE_ONLY && p.run && p.rev && chunk % kSnap == 0) {
@@ -396,35 +409,30 @@ template <typename T, bool STATE_ONLY> __global__ void __launch_bounds__(WT) lin
 
 // ------------------------------------------------------------------------------------------------ bfloat16
 //
-// The same walk on bfloat16 m16n8k16 products, eight warps a block.  A warp has 16 steps of a chunk and 32 of the 64 columns: scores
-// become the left operand of the product with v without leaving its registers (the two warps of a row each form them).
-// The state lives in the warps' accumulators (a quarter of its rows, half of its columns each) and is scaled and added to
-// there; what is multiplied with q are its bfloat16 terms in shared memory, written once a chunk.  The terms of a float32 number are
-// its bfloat16 rounding, that of the rest, and so on: two keep 2^-17 of it, which a bfloat16 result does not see, three all
-// of it.  Scores are kept in two, the state that q meets in two (three where its dots with x go into the float32 gradient of
-// g), decayed values in two (three where the state is itself a result or goes into such a dot).  float16 stays with the
-// TF32 kernel: its states may exceed what it can hold.
+// The same walk in chunks of 128 steps on the tensor cores' own accumulators (tcgen05 + TMEM).  A chunk is five products, each
+// issued by one thread: scores q k^T (128 x 128), q with the state (128 x 64), scores with v, keys with decayed values (the
+// state's sum of the chunk, a row of TMEM for each of its rows), and for the gradient of g the other scores x v^T.  256 threads do
+// what lies between: a thread has one step (or row of the state) and half of the columns.  The scores are decayed,
+// rounded and put back into TMEM where they were, as the left operand of the product with v; the state stays in the threads'
+// registers in float32.  Two blocks fit an SM (256 columns of TMEM and about 100 KB of shared memory each), and one works
+// while the other waits.
 //
-// Loads are asynchronous copies: queries and values of the next chunk are on their way while the state is brought up to
-// date, its keys while values are decayed and q meets the state.
+// All tiles are 128 rows of 64 columns in the 128-byte swizzle, and serve as K-major and as MN-major operands as they are.
+// Terms of a float32 number are its bfloat16 rounding, that of the rest, and so on: two keep 2^-17 of it, three all of
+// it.  Scores and the state that q meets are rounded once, as the result is (an error of 1.4 times the result's own rounding
+// in all), the state in three terms where its dots with x go into the float32 gradient of g; decayed values, which add up in the state,
+// are kept in two, or in three where the state is itself a result or goes into such a dot.  The small terms' products go into
+// an accumulator first: the tensor core truncates when it adds.  float16 stays with the TF32 kernel: its states may exceed
+// what it can hold.
 
+constexpr int BC = 128;                     // steps of a chunk
 constexpr int BT = 256;                     // threads
-constexpr int VP = DO * 2 + 16;             // bytes: rows of 64 columns, shifted by 16 bytes from row to row
+constexpr int BTILE = BC * 128;             // bytes: 128 rows of 64 columns
+constexpr int kSnapB = kSnapSteps / BC;
+constexpr uint32_t kWaitLimit = 1u << 24;
 
-__device__ __forceinline__ void ldsm(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void ldsm_t(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
-__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
+__device__ int g_linattn_status = 0;
+
 // the next bfloat16 term of two numbers, which keep their rest
 __device__ __forceinline__ uint32_t term(float &a, float &b) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
@@ -433,13 +441,16 @@ __device__ __forceinline__ uint32_t term(float &a, float &b) {
   b -= __uint_as_float(w & 0xffff0000u);
   return w;
 }
+__device__ __forceinline__ float low16(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float high16(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, uint32_t bytes) {      // the rest of 16 bytes is zero
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+// byte offset of 16-byte piece c of row r in a swizzled tile
+__device__ __forceinline__ uint32_t piece_at(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
 
-// An operand's tile: 64 rows of W columns (64 or 128) from step i0 on, zero past the sequence and past its size
+// An operand's tile: 128 rows of W columns (64 or 128, 64 a tile) from step i0 on, zero past the sequence and past its size
 struct Tile {
   const __nv_bfloat16 *src;
   int64_t ls;
@@ -454,15 +465,16 @@ __device__ __forceinline__ Tile tile_of(const void *base, int64_t off, int64_t l
   t.vec = ((reinterpret_cast<uintptr_t>(t.src) | (uintptr_t)(ls * 2)) & 15) == 0;
   return t;
 }
-template <int W> __device__ __forceinline__ void load_tile(const Walk &p, const Tile &o, int i0, int pitch, unsigned char *dst) {
+template <int W> __device__ __forceinline__ void load_tile(const Walk &p, const Tile &o, int i0, unsigned char *dst) {
   constexpr int PER = W / 8, ROWS = BT / PER;            // 16-byte pieces of a row, rows a pass
-  const int r0 = threadIdx.x / PER, c = threadIdx.x % PER * 8, left = o.left - c;
+  const int r0 = threadIdx.x / PER, pc = threadIdx.x % PER, left = o.left - pc * 8;
+  unsigned char *to = dst + (pc >> 3) * BTILE;
 #pragma unroll
-  for (int i = 0; i < CH / ROWS; ++i) {
+  for (int i = 0; i < BC / ROWS; ++i) {
     const int r = r0 + i * ROWS, t = time_of(p, i0 + r);
     const bool in = t < p.length && left > 0;
-    const __nv_bfloat16 *s = o.src + (int64_t)(in ? t : 0) * o.ls + (in ? c : 0);
-    unsigned char *at = dst + r * pitch + c * 2;
+    const __nv_bfloat16 *s = o.src + (in ? (int64_t)t * o.ls + pc * 8 : 0);
+    unsigned char *at = to + piece_at(r, pc & 7);
     if (o.vec) copy16(smem_u32(at), s, in ? (left >= 8 ? 16u : (uint32_t)left * 2) : 0u);
     else {
       uint16_t x[8];
@@ -473,357 +485,386 @@ template <int W> __device__ __forceinline__ void load_tile(const Walk &p, const 
   }
 }
 
-// a chunk's decays, and from each 16 steps' start back to the steps before (what lies between two blocks of 16 steps is
-// the product of two factors of at most one)
-struct Decays16 {
-  Decays d;
-  float back[3][CH];
+// A chunk's decays by one warp, four steps a lane (see Decays), and from each 32 steps' start back to the steps before: what lies
+// between two blocks of 32 steps is the product of two factors of at most one.
+struct DecaysB {
+  float hi[BC], lo[BC], in[BC], out[BC], back[3][BC - 32];
+  float keep, keep_lo;
+  double total;
 };
-__device__ __forceinline__ void chunk_decays16(const Walk &p, int b, int h, int i0, int lane, Decays16 &x) {
-  chunk_decays(p, b, h, i0, lane, x.d);
+__device__ __forceinline__ float between(const DecaysB &d, int r, int c) { return ex2a((d.hi[r] - d.hi[c]) + (d.lo[r] - d.lo[c])); }
+__device__ __forceinline__ void chunk_decays_b(const Walk &p, int b, int h, int i0, int lane, DecaysB &d) {
+  double a[4], s = 0.0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) a[j] = log2_decay(p, b, h, i0 + 4 * lane + j);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) { s += a[j]; a[j] = s; }
+  double inc = s;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double u = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += u;
+  }
+  const double end = __shfl_sync(0xffffffffu, inc, 31);
+  const double before = inc - s;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int i = 4 * lane + j;
+    const double G = before + a[j];
+    const float hi = (float)G;
+    d.hi[i] = hi;
+    d.lo[i] = (float)(G - (double)hi);
+    d.in[i] = ex2a(hi);
+    d.out[i] = ex2a((float)(end - G)) * p.s_update;
+  }
+  if (lane == 0) {
+    const double keep = exp2(end);
+    d.keep = (float)keep;
+    d.keep_lo = end <= 0.0 ? (float)(keep - (double)d.keep) : 0.f;
+    d.total = end;
+  }
   __syncwarp();
 #pragma unroll
   for (int j = 1; j < 4; ++j)
-    for (int c = lane; c < 16 * j; c += 32) x.back[j - 1][c] = decay_between(x.d, 16 * j, c);
+#pragma unroll
+    for (int i = 0; i < j; ++i) d.back[j - 1][i * 32 + lane] = between(d, 32 * j, i * 32 + lane);
 }
 
-template <int DI, bool STATE_ONLY> __global__ void __launch_bounds__(BT, 2) linattn_walk16_kernel(const Walk p, const int ts, const int tu) {
-  constexpr int QP = DI * 2 + 16, MS = DI / 64;          // bytes of a row of q and k; 16-row tiles of the state for each warp
-  extern __shared__ __align__(16) unsigned char sb[];
-  unsigned char *sk = sb, *sv = sk + CH * QP, *su = sv + CH * VP, *ss = su + tu * CH * VP, *sq = ss + ts * DI * VP, *sx = sq + CH * QP;
-  __shared__ Decays16 dd[2];
-  __shared__ float dots[2][CH], rows_[2][CH], cols_[4][CH];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gq = lane >> 2, tq = lane & 3;
+// Sums over the 32 lanes of 16 numbers each: lane l (and l + 16) gets the sum of number l % 16.
+__device__ __forceinline__ float sum_columns(float (&v)[16], int lane) {
+#pragma unroll
+  for (int n = 8; n >= 1; n >>= 1) {
+    const bool up = lane & n;
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const float give = up ? v[i] : v[i + n], keep = up ? v[i + n] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, n);
+    }
+  }
+  return v[0] + __shfl_xor_sync(0xffffffffu, v[0], 16);
+}
+
+// MODE: only a segment's own state; results; results and dots with x, forwards; the same backwards
+enum { OWN_STATE = 0, RESULTS = 1, DOTS = 2, DOTS_REV = 3 };
+
+__host__ __device__ constexpr int up_kb(int n) { return (n + 1023) / 1024 * 1024; }
+// shared memory: q | the state's terms, whose place the values' terms take once both have met; k, v, x
+__host__ __device__ constexpr int terms_bytes(int di, int ts, int tu) {
+  return (di / 64 * BTILE + ts * di * 128) > tu * BTILE ? di / 64 * BTILE + ts * di * 128 : tu * BTILE;
+}
+
+template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && MODE >= DOTS ? 1 : 2) linattn_walk_tc_kernel(const Walk p, const int tu) {
+  constexpr bool STATE_ONLY = MODE == OWN_STATE, grad = MODE >= DOTS, cross = MODE == DOTS_REV;
+  constexpr int ts = grad ? 3 : 1, QB = DI / 64 * BTILE;
+  extern __shared__ __align__(1024) unsigned char raw[];
+  unsigned char *sq = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  unsigned char *ss = sq + QB, *su = sq;
+  unsigned char *sk = sq + (STATE_ONLY ? tu * BTILE : terms_bytes(DI, ts, tu)), *sv = sk + QB, *sx = sv + BTILE;
+  __shared__ DecaysB dd[2];
+  __shared__ float dots[2][BC], rows_[2][BC], cols_[4][BC];
+  __shared__ uint64_t bar;
+  __shared__ uint32_t tmem_base;
+  __shared__ int fail;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int tile = blockIdx.x % p.tiles, bh = blockIdx.x / p.tiles % (p.batch * p.heads), seg = blockIdx.x / p.tiles / (p.batch * p.heads);
   const int b = bh / p.heads, h = bh % p.heads, col0 = tile * DO;
-  const int i_begin = seg * p.seg_chunks * CH, i_end = min(p.chunks, (seg + 1) * p.seg_chunks) * CH;
-  const int snaps = (p.chunks + kSnap - 1) / kSnap;
-  const int wr = warp & 3, wc = warp >> 2;               // this warp's 16 steps (quarter of the state's rows), half of the columns
-  const int d0 = wr * (DI / 4), m0 = wr * 16, n0 = wc * 32;
-  const bool grad = !STATE_ONLY && p.run, cross = grad && p.rev;
-  // ldmatrix addresses of a lane within a 16 x 16 tile: by rows; two 8-row tiles side by side along the rows
-  const int a_row = lane & 15, a_col = (lane >> 4) * 8;
-  const int b_row = (lane & 7) + ((lane >> 4) << 3), b_col = ((lane >> 3) & 1) * 8;
-
-  float S[MS][4][4];
-  const auto each = [&](auto f) {                        // all elements of the state within its size: row, column, value
-#pragma unroll
-    for (int m = 0; m < MS; ++m)
-#pragma unroll
-      for (int n = 0; n < 4; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = d0 + m * 16 + gq + (e >> 1) * 8, c = col0 + n0 + n * 8 + tq * 2 + (e & 1);
-          if (r < p.di && c < p.dout) f(r, c, S[m][n][e]);
-        }
-  };
-  const auto write_terms = [&]() {
-#pragma unroll
-    for (int m = 0; m < MS; ++m)
-#pragma unroll
-      for (int n = 0; n < 4; ++n)
-#pragma unroll
-        for (int e2 = 0; e2 < 2; ++e2) {
-          float x = S[m][n][e2 * 2], y = S[m][n][e2 * 2 + 1];
-          unsigned char *at = ss + (d0 + m * 16 + gq + e2 * 8) * VP + (n0 + n * 8 + tq * 2) * 2;
-          *reinterpret_cast<uint32_t *>(at) = term(x, y);
-          *reinterpret_cast<uint32_t *>(at + DI * VP) = term(x, y);
-          if (ts == 3) *reinterpret_cast<uint32_t *>(at + 2 * DI * VP) = term(x, y);
-        }
-  };
-#pragma unroll
-  for (int m = 0; m < MS; ++m)
-#pragma unroll
-    for (int n = 0; n < 4; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) S[m][n][e] = 0.f;
+  const int i_begin = seg * p.seg_chunks * BC, i_end = min(p.chunks, (seg + 1) * p.seg_chunks) * BC;
+  const int snaps = (p.chunks + kSnapB - 1) / kSnapB;
+  // this thread's TMEM lane (a step of the chunk, a row of the state) and half of the columns
+  const int wr = warp & 3, half = warp >> 2, r = wr * 32 + lane, c0 = half * 32;
+  if (tid == 0) {
+    mbar_init(&bar, 1);
+    fail = 0;
+    mbar_fence_init();
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)), "r"(256) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
   const Tile tk = tile_of(p.k, b * p.k_bs + h / p.k_div * p.k_hs, p.k_ls, 0, p.di), tv = tile_of(p.v, b * p.v_bs + h / p.v_div * p.v_hs, p.v_ls, col0, p.dout);
-  const Tile tq_ = tile_of(p.q, b * p.q_bs + h / p.q_div * p.q_hs, p.q_ls, 0, p.di), tx = tile_of(p.x, b * p.x_bs + h / p.x_div * p.x_hs, p.x_ls, col0, p.dout);
-  const auto load_first = [&](int i0) {                  // what is needed first
-    load_tile<64>(p, tv, i0, VP, sv);
-    if (!STATE_ONLY) load_tile<DI>(p, tq_, i0, QP, sq);
-    if (grad) load_tile<64>(p, tx, i0, VP, sx);
-    copies_commit();
+  const Tile tq = tile_of(p.q, b * p.q_bs + h / p.q_div * p.q_hs, p.q_ls, 0, p.di), tx = tile_of(p.x, b * p.x_bs + h / p.x_div * p.x_hs, p.x_ls, col0, p.dout);
+  const auto load = [&](int i0) {
+    if (!STATE_ONLY) load_tile<DI>(p, tq, i0, sq);
+    load_tile<DI>(p, tk, i0, sk);
+    load_tile<64>(p, tv, i0, sv);
+    if (grad) load_tile<64>(p, tx, i0, sx);
   };
-  const auto load_keys = [&](int i0) {
-    load_tile<DI>(p, tk, i0, QP, sk);
-    copies_commit();
+  load(i_begin);
+  if (warp == 7) chunk_decays_b(p, b, h, i_begin, lane, dd[0]);
+  float S[32];                                           // row r of the state, columns c0 on
+  const bool has_row = r < p.di;
+  const auto each = [&](auto f) {
+    if (has_row)
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (col0 + c0 + j < p.dout) f(col0 + c0 + j, S[j]);
   };
-  load_first(i_begin);
-  load_keys(i_begin);
-  if (warp == 7) chunk_decays16(p, b, h, i_begin, lane, dd[0]);
+  const auto snapshot = [&](int s, float f) { each([&](int c, float &x) { p.snap[(((int64_t)bh * snaps + s) * p.di + r) * p.dout + c] = x * f; }); };
+  const auto write_terms = [&]() {
+    if (r < DI)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = S[j * 8 + e];
+#pragma unroll
+        for (int t = 0; t < ts; ++t)
+          *reinterpret_cast<uint4 *>(ss + t * DI * 128 + piece_at(r, half * 4 + j)) = make_uint4(term(x[0], x[1]), term(x[2], x[3]), term(x[4], x[5]), term(x[6], x[7]));
+      }
+  };
+#pragma unroll
+  for (int j = 0; j < 32; ++j) S[j] = 0.f;
   if (!STATE_ONLY) {
-    if (p.nseg > 1) each([&](int r, int c, float &s) { s = p.seg[(((int64_t)bh * p.nseg + seg) * p.di + r) * p.dout + c]; });
-    else if (p.s0) each([&](int r, int c, float &s) { s = p.s0[b * p.s0_bs + h * p.s0_hs + r * p.s0_is + c * p.s0_os]; });
+    if (p.nseg > 1) each([&](int c, float &x) { x = p.seg[(((int64_t)bh * p.nseg + seg) * p.di + r) * p.dout + c]; });
+    else if (p.s0) each([&](int c, float &x) { x = p.s0[b * p.s0_bs + h * p.s0_hs + r * p.s0_is + c * p.s0_os]; });
     write_terms();
   }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tm = tmem_base, tm_own = tm + ((uint32_t)(wr * 32) << 16);
+  const uint32_t tP = 0, tO = 128, tD = 192;             // columns: scores, result, the state's sum (x v^T takes the place of the last two for a while)
+  constexpr uint32_t kScores = idesc_f16(1, false, false, 128, 128), kState = idesc_f16(1, false, true, 128, 64), kUpdate = idesc_f16(1, true, true, 128, 64);
+  uint32_t phase = 0;
+  const auto wait_products = [&]() {
+    if (!mbar_wait(&bar, phase, kWaitLimit)) *(volatile int *)&fail = 1;
+    phase ^= 1;
+    __syncwarp();
+    tc_fence_after();
+  };
   double total = 0.0;
-  for (int i0 = i_begin, it = 0; i0 < i_end; i0 += CH, ++it) {
-    const int chunk = p.rev ? p.chunks - 1 - i0 / CH : i0 / CH;
-    const Decays16 &x16 = dd[it & 1];
-    const Decays &d = x16.d;
-    if (grad && !p.rev && chunk % kSnap == 0)
-      each([&](int r, int c, float &s) { p.snap[(((int64_t)bh * snaps + chunk / kSnap) * p.di + r) * p.dout + c] = s; });
-    copies_wait<1>();
-    __syncthreads();                                     // values and queries have arrived, the state's terms and the decays are written
-    // values as the state takes them up, in terms
-#pragma unroll
-    for (int i = 0; i < CH * DO / 4 / BT; ++i) {
-      const int e = i * BT + tid, r = e / (DO / 4), c = e % (DO / 4) * 8;
-      const uint2 v = *reinterpret_cast<const uint2 *>(sv + r * VP + c);
-      const float w = d.out[r];
-      float y[4] = {__uint_as_float(v.x << 16) * w, __uint_as_float(v.x & 0xffff0000u) * w, __uint_as_float(v.y << 16) * w, __uint_as_float(v.y & 0xffff0000u) * w};
-      unsigned char *at = su + r * VP + c;
-      *reinterpret_cast<uint2 *>(at) = make_uint2(term(y[0], y[1]), term(y[2], y[3]));
-      *reinterpret_cast<uint2 *>(at + CH * VP) = make_uint2(term(y[0], y[1]), term(y[2], y[3]));
-      if (tu == 3) *reinterpret_cast<uint2 *>(at + 2 * CH * VP) = make_uint2(term(y[0], y[1]), term(y[2], y[3]));
-    }
+  for (int i0 = i_begin, it = 0; i0 < i_end; i0 += BC, ++it) {
+    const int chunk = p.rev ? p.chunks - 1 - i0 / BC : i0 / BC;
+    const DecaysB &d = dd[it & 1];
+    if (grad && !cross && chunk % kSnapB == 0) snapshot(chunk / kSnapB, 1.f);
+    copies_wait();
+    fence_proxy_async();
+    tc_fence_before();
+    __syncthreads();                                     // operands and the state's terms are there, accumulators read
+    if (*(volatile int *)&fail) break;
+    float O[32];
     if constexpr (!STATE_ONLY) {
-      const uint32_t aq = smem_u32(sq) + (m0 + a_row) * QP + a_col * 2;
-      const int r0 = m0 + gq;
-      float O[4][4];
-#pragma unroll
-      for (int n = 0; n < 4; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) O[n][e] = 0.f;
-#pragma unroll
-      for (int k0 = 0; k0 < DI; k0 += 16) {
-        uint32_t a[4];
-        ldsm(a, aq + k0 * 2);
-        for (int t = ts - 1; t >= 0; --t) {
-          const uint32_t as = smem_u32(ss) + t * DI * VP + (k0 + a_row) * VP + (n0 + a_col) * 2;
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            uint32_t w[4];
-            ldsm_t(w, as + j * 32);
-            mma16(O[2 * j], a, w[0], w[1]);
-            mma16(O[2 * j + 1], a, w[2], w[3]);
-          }
-        }
+      if (tid == 0) {
+        tc_fence_after();
+        const uint32_t q = smem_u32(sq), k = smem_u32(sk), s = smem_u32(ss);
+#pragma unroll 1
+        for (int i = 0; i < DI / 16; ++i)
+          mma_f16(tm + tP, smem_desc(q + (i >> 2) * BTILE + (i & 3) * 32, 16, 1024, 2), smem_desc(k + (i >> 2) * BTILE + (i & 3) * 32, 16, 1024, 2), kScores, i > 0);
+#pragma unroll 1
+        for (int t = ts - 1; t >= 0; --t)
+#pragma unroll 1
+          for (int i = 0; i < DI / 16; ++i)
+            mma_f16(tm + tO, smem_desc(q + (i >> 2) * BTILE + (i & 3) * 32, 16, 1024, 2), smem_desc(s + t * DI * 128 + i * 2048, 8192, 1024, 2), kState, t < ts - 1 || i > 0);
+        mma_commit(&bar);
       }
+      __syncwarp();
+      wait_products();
       {
-        const float f0 = d.in[r0] * p.s_inter, f1 = d.in[r0 + 8] * p.s_inter;
+        tmem_ld32(tm_own + tO + c0, O);
+        const float f = d.in[r] * p.s_inter;
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          O[n][0] *= f0;
-          O[n][1] *= f0;
-          O[n][2] *= f1;
-          O[n][3] *= f1;
-        }
+        for (int j = 0; j < 32; ++j) O[j] *= f;
       }
       if (grad) {
-#pragma unroll
-        for (int e2 = 0; e2 < 2; ++e2) {
-          float dot = 0.f;
-#pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            const uint32_t w = *reinterpret_cast<const uint32_t *>(sx + (r0 + e2 * 8) * VP + (n0 + n * 8 + tq * 2) * 2);
-            dot = fmaf(O[n][e2 * 2], __uint_as_float(w << 16), fmaf(O[n][e2 * 2 + 1], __uint_as_float(w & 0xffff0000u), dot));
-          }
-          dot += __shfl_xor_sync(0xffffffffu, dot, 1);
-          dot += __shfl_xor_sync(0xffffffffu, dot, 2);
-          if (tq == 0) dots[wc][r0 + e2 * 8] = dot;
-        }
-      }
-      copies_wait<0>();
-      __syncthreads();                                   // the keys have arrived
-      float P[8][4];
-#pragma unroll
-      for (int n = 0; n < 8; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) P[n][e] = 0.f;
-#pragma unroll
-      for (int k0 = 0; k0 < DI; k0 += 16) {
-        uint32_t a[4];
-        ldsm(a, aq + k0 * 2);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (j <= wr) {                                 // columns of earlier or the same 16 steps
-            uint32_t kb[4];
-            ldsm(kb, smem_u32(sk) + (j * 16 + b_row) * QP + (k0 + b_col) * 2);
-            mma16(P[2 * j], a, kb[0], kb[1]);
-            mma16(P[2 * j + 1], a, kb[2], kb[3]);
-          }
-      }
-      {
-        float f[2];
-#pragma unroll
-        for (int e2 = 0; e2 < 2; ++e2) f[e2] = decay_between(d, r0 + e2 * 8, m0) * p.s_intra;
+        float dot = 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if (j < wr) {
+          const uint4 w = *reinterpret_cast<const uint4 *>(sx + piece_at(r, half * 4 + j));
+          const uint32_t x[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-            for (int n = 2 * j; n < 2 * j + 2; ++n) {
-              const float2 w = *reinterpret_cast<const float2 *>(&x16.back[wr - 1][n * 8 + tq * 2]);
-              P[n][0] *= f[0] * w.x;
-              P[n][1] *= f[0] * w.y;
-              P[n][2] *= f[1] * w.x;
-              P[n][3] *= f[1] * w.y;
-            }
-          } else if (j == wr) {
-#pragma unroll
-            for (int n = 2 * j; n < 2 * j + 2; ++n)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int r = r0 + (e >> 1) * 8, c = n * 8 + tq * 2 + (e & 1);
-                P[n][e] = c <= r ? P[n][e] * decay_between(d, r, c) * p.s_intra : 0.f;
-              }
-          }
+          for (int e = 0; e < 4; ++e) dot = fmaf(O[j * 8 + 2 * e], low16(x[e]), fmaf(O[j * 8 + 2 * e + 1], high16(x[e]), dot));
         }
+        dots[half][r] = dot;
       }
-      if (cross) {                                       // products of a pair's two scores, without the diagonal; every other 16 columns
-        float row[2] = {0.f, 0.f};
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if ((j & 1) == wc) {
-            float X[2][4] = {};
-            if (j <= wr) {
-#pragma unroll
-              for (int k0 = 0; k0 < DO; k0 += 16) {
-                uint32_t a[4], w[4];
-                ldsm(a, smem_u32(sx) + (m0 + a_row) * VP + (k0 + a_col) * 2);
-                ldsm(w, smem_u32(sv) + (j * 16 + b_row) * VP + (k0 + b_col) * 2);
-                mma16(X[0], a, w[0], w[1]);
-                mma16(X[1], a, w[2], w[3]);
-              }
-            }
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-              for (int e1 = 0; e1 < 2; ++e1) {
-                const int c = j * 16 + n * 8 + tq * 2 + e1;
-                float col = 0.f;
-#pragma unroll
-                for (int e2 = 0; e2 < 2; ++e2) {
-                  const float m = c == r0 + e2 * 8 ? 0.f : P[2 * j + n][e2 * 2 + e1] * X[n][e2 * 2 + e1];
-                  row[e2] += m;
-                  col += m;
-                }
-#pragma unroll
-                for (int o = 4; o < 32; o <<= 1) col += __shfl_xor_sync(0xffffffffu, col, o);
-                if (gq == 0) cols_[wr][c] = col;
-              }
-          }
-#pragma unroll
-        for (int e2 = 0; e2 < 2; ++e2) {
-          row[e2] += __shfl_xor_sync(0xffffffffu, row[e2], 1);
-          row[e2] += __shfl_xor_sync(0xffffffffu, row[e2], 2);
-          if (tq == 0) rows_[wc][r0 + e2 * 8] = row[e2];
+      if (cross) {
+        tc_fence_before();
+        __syncthreads();                                 // the result's columns are read
+        if (tid == 0) {
+          tc_fence_after();
+#pragma unroll 1
+          for (int i = 0; i < DO / 16; ++i)
+            mma_f16(tm + tO, smem_desc(smem_u32(sx) + i * 32, 16, 1024, 2), smem_desc(smem_u32(sv) + i * 32, 16, 1024, 2), kScores, i > 0);
+          mma_commit(&bar);
         }
+        __syncwarp();
+      }
+    }
+    // values as the state takes them up, in terms: q and the state's terms have been read
+#pragma unroll 1
+    for (int i = 0; i < BC * 8 / BT; ++i) {
+      const int e = i * BT + tid, row = e >> 3;
+      const uint32_t at = piece_at(row, e & 7);
+      const uint4 w = *reinterpret_cast<const uint4 *>(sv + at);
+      const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+      const float f = d.out[row];
+      float y[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        y[2 * j] = low16(x[j]) * f;
+        y[2 * j + 1] = high16(x[j]) * f;
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (j <= wr) {
-          uint32_t hi[4], lo[4];
+      for (int t = 0; t < 3; ++t)
+        if (t < tu) *reinterpret_cast<uint4 *>(su + t * BTILE + at) = make_uint4(term(y[0], y[1]), term(y[2], y[3]), term(y[4], y[5]), term(y[6], y[7]));
+    }
+    if constexpr (!STATE_ONLY) {
+      if (cross) wait_products();
+      // scores: decayed, zero after the step itself
+      const float f = between(d, r, wr * 32) * p.s_intra;
+      float row = 0.f;
+#pragma unroll 1
+      for (int g = 0; g < 2; ++g) {                      // 32 columns at a time, 16 columns of TMEM as bfloat16
+        const int cb = half * 2 + g;                     // block of 32 columns
+        uint32_t packed[16];
+        if (cb > wr) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float x = P[2 * j + (i >> 1)][(i & 1) * 2], y = P[2 * j + (i >> 1)][(i & 1) * 2 + 1];
-            hi[i] = term(x, y);
-            lo[i] = term(x, y);
-          }
+          for (int j = 0; j < 16; ++j) packed[j] = 0u;
+          if (cross && lane < 16) cols_[wr][cb * 32 + lane] = cols_[wr][cb * 32 + 16 + lane] = 0.f;
+        } else {
 #pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            uint32_t w[4];
-            ldsm_t(w, smem_u32(sv) + (j * 16 + a_row) * VP + (n0 + n * 16 + a_col) * 2);
-            mma16(O[2 * n], lo, w[0], w[1]);
-            mma16(O[2 * n + 1], lo, w[2], w[3]);
-            mma16(O[2 * n], hi, w[0], w[1]);
-            mma16(O[2 * n + 1], hi, w[2], w[3]);
+          for (int q = 0; q < 2; ++q) {
+            const int c = cb * 32 + q * 16;
+            float v[16];
+            tmem_ld16(tm_own + tP + c, v);
+            if (cb < wr) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float4 w = *reinterpret_cast<const float4 *>(&d.back[wr - 1][c + 4 * j]);
+                v[4 * j] *= f * w.x;
+                v[4 * j + 1] *= f * w.y;
+                v[4 * j + 2] *= f * w.z;
+                v[4 * j + 3] *= f * w.w;
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 16; ++j) v[j] = c + j <= r ? v[j] * between(d, r, c + j) * p.s_intra : 0.f;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const __nv_bfloat162 w = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+              packed[q * 8 + j] = *reinterpret_cast<const uint32_t *>(&w);
+            }
+            if (cross) {                                 // products of a pair's two scores, without the diagonal
+              float x[16];
+              tmem_ld16(tm_own + tO + c, x);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                v[j] = c + j == r ? 0.f : v[j] * x[j];
+                row += v[j];
+              }
+              const float col = sum_columns(v, lane);
+              if (lane < 16) cols_[wr][c + lane] = col;
+            }
           }
         }
+        // the columns of 32 scores are free once read; their bfloat16 go into the first half of this half's 64 columns, which
+        // the first of the two rounds has read
+        __syncwarp();
+        tmem_st16(tm_own + tP + half * 64 + g * 16, packed);
+      }
+      if (cross) rows_[half][r] = row;
+      tmem_st_wait();
+    }
+    fence_proxy_async();
+    tc_fence_before();
+    __syncthreads();                                     // scores and the values' terms are written
+    if (tid == 0) {
+      tc_fence_after();
+      const uint32_t k = smem_u32(sk), v = smem_u32(sv), u = smem_u32(su);
+      if constexpr (!STATE_ONLY)
+#pragma unroll 1
+        for (int i = 0; i < BC / 16; ++i)
+          mma_f16_ta(tm + tO, tm + tP + (i >> 2) * 64 + (i & 3) * 8, smem_desc(v + i * 2048, 8192, 1024, 2), kState, i > 0);
+#pragma unroll 1
+      for (int t = tu - 1; t >= 0; --t)
+#pragma unroll 1
+        for (int i = 0; i < BC / 16; ++i)
+          // keys with 64 columns have one tile; what follows it makes up the lanes past 63, which nothing reads
+          mma_f16(tm + tD, smem_desc(k + i * 2048, BTILE, 1024, 2), smem_desc(u + t * BTILE + i * 2048, 8192, 1024, 2), kUpdate, t < tu - 1 || i > 0);
+      mma_commit(&bar);
+    }
+    __syncwarp();
+    wait_products();
+    if (i0 + BC < i_end) {
+      load(i0 + BC);
+      if (warp == 7) chunk_decays_b(p, b, h, i0 + BC, lane, dd[(it + 1) & 1]);
+    }
+    if constexpr (!STATE_ONLY) {
+      float v[32];
+      tmem_ld32(tm_own + tO + c0, v);
 #pragma unroll
-      for (int e2 = 0; e2 < 2; ++e2) {
-        const int t = time_of(p, i0 + r0 + e2 * 8);
-        if (t >= p.length) continue;
-        const int64_t at = b * p.o_bs + t * p.o_ls + h * p.o_hs + col0;
+      for (int j = 0; j < 32; ++j) O[j] += v[j];
+      const int t = time_of(p, i0 + r), left = p.dout - col0 - c0;
+      if (t < p.length && left > 0) {
+        const int64_t at = b * p.o_bs + t * p.o_ls + h * p.o_hs + col0 + c0;
         if (p.out_f32) {
           float *o = reinterpret_cast<float *>(p.out) + at;
-          const bool pair = (reinterpret_cast<uintptr_t>(o) & 7) == 0;
+          if (left >= 32 && (reinterpret_cast<uintptr_t>(o) & 15) == 0) {
 #pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            const int c = n0 + n * 8 + tq * 2;
-            if (pair && col0 + c + 1 < p.dout) *reinterpret_cast<float2 *>(o + c) = make_float2(O[n][e2 * 2], O[n][e2 * 2 + 1]);
-            else {
-              if (col0 + c < p.dout) o[c] = O[n][e2 * 2];
-              if (col0 + c + 1 < p.dout) o[c + 1] = O[n][e2 * 2 + 1];
-            }
+            for (int j = 0; j < 8; ++j) reinterpret_cast<float4 *>(o)[j] = make_float4(O[4 * j], O[4 * j + 1], O[4 * j + 2], O[4 * j + 3]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j < left) o[j] = O[j];
           }
         } else {
           __nv_bfloat16 *o = reinterpret_cast<__nv_bfloat16 *>(p.out) + at;
-          const bool pair = (reinterpret_cast<uintptr_t>(o) & 3) == 0;
+          if (left >= 32 && (reinterpret_cast<uintptr_t>(o) & 15) == 0) {
 #pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            const int c = n0 + n * 8 + tq * 2;
-            const __nv_bfloat162 v = __floats2bfloat162_rn(O[n][e2 * 2], O[n][e2 * 2 + 1]);
-            if (pair && col0 + c + 1 < p.dout) *reinterpret_cast<__nv_bfloat162 *>(o + c) = v;
-            else {
-              if (col0 + c < p.dout) o[c] = v.x;
-              if (col0 + c + 1 < p.dout) o[c + 1] = v.y;
+            for (int j = 0; j < 4; ++j) {
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const __nv_bfloat162 x = __floats2bfloat162_rn(O[j * 8 + 2 * e], O[j * 8 + 2 * e + 1]);
+                w[e] = *reinterpret_cast<const uint32_t *>(&x);
+              }
+              reinterpret_cast<uint4 *>(o)[j] = make_uint4(w[0], w[1], w[2], w[3]);
             }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j < left) o[j] = __float2bfloat16_rn(O[j]);
           }
         }
       }
-    } else {
-      copies_wait<0>();
     }
-    __syncthreads();                                     // queries, values and the state's terms are read, the values' terms written
-    if (i0 + CH < i_end) {
-      load_first(i0 + CH);
-      if (warp == 7) chunk_decays16(p, b, h, i0 + CH, lane, dd[(it + 1) & 1]);
+    {
+      float v[32];
+      tmem_ld32(tm_own + tD + c0, v);
+      const float keep = d.keep, keep_lo = d.keep_lo;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) S[j] = r < DI ? fmaf(S[j], keep, fmaf(S[j], keep_lo, v[j])) : 0.f;
     }
     total += d.total;
-    const float keep = d.keep;
-#pragma unroll
-    for (int m = 0; m < MS; ++m)
-#pragma unroll
-      for (int n = 0; n < 4; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) S[m][n][e] *= keep;
-#pragma unroll
-    for (int k0 = 0; k0 < CH; k0 += 16) {
-      uint32_t a[MS][4];
-#pragma unroll
-      for (int m = 0; m < MS; ++m) ldsm_t(a[m], smem_u32(sk) + (k0 + b_row) * QP + (d0 + m * 16 + b_col) * 2);
-      for (int t = tu - 1; t >= 0; --t)
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          uint32_t w[4];
-          ldsm_t(w, smem_u32(su) + t * CH * VP + (k0 + a_row) * VP + (n0 + n * 16 + a_col) * 2);
-#pragma unroll
-          for (int m = 0; m < MS; ++m) {
-            mma16(S[m][2 * n], a[m], w[0], w[1]);
-            mma16(S[m][2 * n + 1], a[m], w[2], w[3]);
-          }
-        }
-    }
     if (grad && warp == 0) {
-      double v[2];
+      double v[4];
       float s = 0.f;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int i = 2 * lane + j;
+      for (int j = 0; j < 4; ++j) {
+        const int i = 4 * lane + j;
         const float dot = dots[0][i] + dots[1][i];
         s += dot;
         v[j] = dot;
-        if (p.rev) v[j] += ((double)rows_[0][i] + rows_[1][i]) - (((double)cols_[0][i] + cols_[1][i]) + ((double)cols_[2][i] + cols_[3][i]));
+        if (cross) v[j] += ((double)rows_[0][i] + rows_[1][i]) - (((double)cols_[0][i] + cols_[1][i]) + ((double)cols_[2][i] + cols_[3][i]));
       }
-      chunk_runs(p, tile, bh, i0, lane, v[0], v[1], s);
+      chunk_runs(p, tile, bh, i0, lane, v, s);
     }
-    if (cross && chunk % kSnap == 0) {
-      const float f = ex2a((float)log2_of(p, b, h, chunk * CH));
-      each([&](int r, int c, float &s) { p.snap[(((int64_t)bh * snaps + chunk / kSnap) * p.di + r) * p.dout + c] = s * f; });
-    }
+    if (cross && chunk % kSnapB == 0) snapshot(chunk / kSnapB, (float)exp2(log2_of(p, b, h, chunk * BC)));
     if (!STATE_ONLY) write_terms();
-    __syncthreads();                                     // the keys and the values' terms are read
-    if (i0 + CH < i_end) load_keys(i0 + CH);
   }
-  if (STATE_ONLY) {
-    each([&](int r, int c, float &s) { p.seg[(((int64_t)bh * p.nseg + seg) * p.di + r) * p.dout + c] = s; });
+  copies_wait();
+  const bool ok = !*(volatile int *)&fail;
+  if (STATE_ONLY && ok) {
+    each([&](int c, float &x) { p.seg[(((int64_t)bh * p.nseg + seg) * p.di + r) * p.dout + c] = x; });
     if (tile == 0 && tid == 0) p.seg_g[(int64_t)bh * p.nseg + seg] = total;
-  } else if (p.last && seg == p.nseg - 1) {
-    const float f = p.last_decay ? ex2a((float)log2_of(p, b, h, 0)) : 1.f;
-    each([&](int r, int c, float &s) { p.last[b * p.last_bs + h * p.last_hs + r * p.last_is + c * p.last_os] = s * f; });
+  } else if (!STATE_ONLY && ok && p.last && seg == p.nseg - 1) {
+    const float f = p.last_decay ? (float)exp2(log2_of(p, b, h, 0)) : 1.f;
+    each([&](int c, float &x) { p.last[b * p.last_bs + h * p.last_hs + r * p.last_is + c * p.last_os] = x * f; });
   }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(256) : "memory");
+  if (tid == 0 && fail) atomicExch(&g_linattn_status, 9);
 }
 
 // Each segment's own state becomes the state before it.
@@ -837,7 +878,7 @@ __global__ void __launch_bounds__(256) linattn_join_kernel(const Walk p) {
     float *at = p.seg + ((int64_t)bh * p.nseg + n) * per + i;
     const float own = n < p.nseg - 1 ? *at : 0.f;
     *at = s;
-    if (n < p.nseg - 1) s = fmaf(s, ex2a((float)p.seg_g[(int64_t)bh * p.nseg + n]), own);
+    if (n < p.nseg - 1) s = fmaf(s, (float)exp2(p.seg_g[(int64_t)bh * p.nseg + n]), own);
   }
 }
 
@@ -856,10 +897,10 @@ __global__ void __launch_bounds__(256) linattn_fold_kernel(const float *src, int
   }
 }
 
-// What the pairs of steps on both sides of a whole chunk give: at every kSnap-th border all pairs across it are the product of
+// What the pairs of steps on both sides of a whole chunk give: every 512 steps all pairs across a border are the product of
 // the two states there, and from border to border the sums of the chunk's dots are taken off and added on.
 __global__ void __launch_bounds__(256) linattn_across_kernel(const float *snap_q, const float *snap_k, const float *sum_q, const float *sum_k, int tiles, int64_t per,
-                                                            int chunks, int snaps, int bhs, double *across) {
+                                                            int chunks, int snap, int snaps, int bhs, double *across) {
   __shared__ double sh[8];
   const int bh = blockIdx.x / snaps, sn = blockIdx.x % snaps, tid = threadIdx.x;
   const float *a = snap_q + (int64_t)blockIdx.x * per, *c = snap_k + (int64_t)blockIdx.x * per;
@@ -872,7 +913,7 @@ __global__ void __launch_bounds__(256) linattn_across_kernel(const float *snap_q
   if (tid == 0) {
     double x = 0.0;
     for (int i = 0; i < 8; ++i) x += sh[i];
-    for (int n = sn * kSnap; n < min(chunks, (sn + 1) * kSnap); ++n) {
+    for (int n = sn * snap; n < min(chunks, (sn + 1) * snap); ++n) {
       double q = 0.0, k = 0.0;
       for (int t = 0; t < tiles; ++t) {
         q += (double)sum_q[((int64_t)t * bhs + bh) * chunks + n];
@@ -885,32 +926,32 @@ __global__ void __launch_bounds__(256) linattn_across_kernel(const float *snap_q
   }
 }
 
-__device__ __forceinline__ double dg_at(const b200_linattn_args &p, const float *run_q, const float *run_k, int tiles, const double *across, int chunks, int bh, int t) {
+__device__ __forceinline__ double dg_at(const b200_linattn_args &p, const float *run_q, const float *run_k, int tiles, const double *across, int ch, int chunks, int bh, int t) {
   const int b = bh / p.heads, h = bh % p.heads;
   if (load_g(p.g, p.g_dtype, b * p.g_bs + t * p.g_ls + h * p.g_hs) == -INFINITY) return 0.0;      // a decay of nothing has no slope
   const int64_t plane = (int64_t)p.batch * p.heads * p.seqlen, i = (int64_t)bh * p.seqlen + t;
-  double s = across[(int64_t)bh * chunks + t / CH];
+  double s = across[(int64_t)bh * chunks + t / ch];
   for (int n = 0; n < tiles; ++n) s += (double)run_q[n * plane + i] + (double)run_k[n * plane + i];
   return s;
 }
 // 32 steps x 8 heads a block, so that both layouts are read and written in runs
-__global__ void __launch_bounds__(256) linattn_dg_kernel(const b200_linattn_args p, const float *run_q, const float *run_k, int tiles, const double *across, int chunks) {
+__global__ void __launch_bounds__(256) linattn_dg_kernel(const b200_linattn_args p, const float *run_q, const float *run_k, int tiles, const double *across, int ch, int chunks) {
   __shared__ float sh[8][33];
   const int b = blockIdx.z, t0 = blockIdx.x * 32, h0 = blockIdx.y * 8;
   {
     const int t = t0 + (threadIdx.x & 31), h = h0 + (threadIdx.x >> 5);
-    sh[threadIdx.x >> 5][threadIdx.x & 31] = t < p.seqlen && h < p.heads ? (float)dg_at(p, run_q, run_k, tiles, across, chunks, b * p.heads + h, t) : 0.f;
+    sh[threadIdx.x >> 5][threadIdx.x & 31] = t < p.seqlen && h < p.heads ? (float)dg_at(p, run_q, run_k, tiles, across, ch, chunks, b * p.heads + h, t) : 0.f;
   }
   __syncthreads();
   const int t = t0 + (threadIdx.x >> 3), h = h0 + (threadIdx.x & 7);
   if (t < p.seqlen && h < p.heads) st_act(p.dg, p.g_dtype, ((int64_t)b * p.seqlen + t) * p.heads + h, sh[threadIdx.x & 7][threadIdx.x >> 3]);
 }
 // a decay for each head: the sum over a (batch, head), then over the batch
-__global__ void __launch_bounds__(256) linattn_dg_sum_kernel(const b200_linattn_args p, const float *run_q, const float *run_k, int tiles, const double *across, int chunks,
+__global__ void __launch_bounds__(256) linattn_dg_sum_kernel(const b200_linattn_args p, const float *run_q, const float *run_k, int tiles, const double *across, int ch, int chunks,
                                                             double *per_head) {
   __shared__ double sh[8];
   double s = 0.0;
-  for (int t = threadIdx.x; t < p.seqlen; t += 256) s += dg_at(p, run_q, run_k, tiles, across, chunks, blockIdx.x, t);
+  for (int t = threadIdx.x; t < p.seqlen; t += 256) s += dg_at(p, run_q, run_k, tiles, across, ch, chunks, blockIdx.x, t);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = s;
@@ -1042,15 +1083,16 @@ int launch_walk(Walk &w, K own, K all, int threads, int smem_own, int smem_all, 
 template <typename T> int walk(Walk &w, unsigned char *work, cudaStream_t st) {
   return launch_walk(w, linattn_walk_kernel<T, true>, linattn_walk_kernel<T, false>, WT, walk_smem(w.di, true, false), walk_smem(w.di, false, w.run != nullptr), work, st);
 }
-template <int DI> int walk16(Walk &w, unsigned char *work, cudaStream_t st) {
-  const int ts = w.run ? 3 : 2, tu = w.run || w.last ? 3 : 2, qp = DI * 2 + 16;
-  const int own = CH * qp + (1 + tu) * CH * VP, all = own + CH * qp + ts * DI * VP + (w.run ? CH * VP : 0);
-  return launch_walk(w, linattn_walk16_kernel<DI, true>, linattn_walk16_kernel<DI, false>, BT, own, all, work, st, ts, tu);
+template <int DI> int walk_tc(Walk &w, unsigned char *work, cudaStream_t st) {
+  const int ts = w.run ? 3 : 1, tu = w.run || w.last ? 3 : 2, kv = DI / 64 * BTILE + BTILE + 1024;
+  const int own = tu * BTILE + kv, all = terms_bytes(DI, ts, tu) + kv + (w.run ? BTILE : 0);
+  const auto results = !w.run ? linattn_walk_tc_kernel<DI, RESULTS> : w.rev ? linattn_walk_tc_kernel<DI, DOTS_REV> : linattn_walk_tc_kernel<DI, DOTS>;
+  return launch_walk(w, linattn_walk_tc_kernel<DI, OWN_STATE>, results, BT, own, all, work, st, tu);
 }
 int run_walk(int dtype, Walk &w, unsigned char *work, cudaStream_t st) {
   if (dtype == B200_F32) return walk<float>(w, work, st);
   if (dtype == B200_F16) return walk<__half>(w, work, st);
-  return w.di <= 64 ? walk16<64>(w, work, st) : walk16<128>(w, work, st);
+  return w.di <= 64 ? walk_tc<64>(w, work, st) : walk_tc<128>(w, work, st);
 }
 
 int check_linattn(const b200_linattn_args &a) {
@@ -1070,7 +1112,8 @@ Walk base_walk(const b200_linattn_args &a) {
   memset(&w, 0, sizeof(w));
   w.g = a.g; w.g_bs = a.g_bs; w.g_ls = a.g_ls; w.g_hs = a.g_hs; w.g_dtype = a.g_dtype;
   w.batch = a.batch; w.length = a.seqlen; w.heads = a.heads;
-  w.chunks = (a.seqlen + CH - 1) / CH;
+  w.ch = a.dtype == B200_BF16 ? BC : CH;
+  w.chunks = (a.seqlen + w.ch - 1) / w.ch;
   w.q_div = w.k_div = w.v_div = w.x_div = 1;
   return w;
 }
@@ -1151,7 +1194,7 @@ BwdPlan bwd_plan(const b200_linattn_args &a) {
   q.part = a.heads != a.groups ? up(4 * bh * a.seqlen * a.dk, 256) : 0;
   q.run = a.dg ? up(4 * bh * a.seqlen * ws[0].tiles, 256) : 0;
   q.sum = a.dg ? up(4 * bh * chunks * ws[0].tiles, 256) : 0;
-  q.snap = a.dg ? up(4 * bh * ((chunks + kSnap - 1) / kSnap) * a.dk * a.dv, 256) : 0;
+  q.snap = a.dg ? up(4 * bh * ((a.seqlen + kSnapSteps - 1) / kSnapSteps) * a.dk * a.dv, 256) : 0;
   q.across = a.dg ? up(8 * bh * chunks, 256) : 0;
   q.heads = a.dg && a.g_heads ? up(8 * bh, 256) : 0;
   q.total = q.seg + q.part + 2 * (q.run + q.sum + q.snap) + q.across + q.heads;
@@ -1177,6 +1220,13 @@ template <typename TS, typename T> int run_step(const b200_linattn_step_args &a,
 }
 
 }  // namespace
+
+int linattn_status_read() {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_linattn_status, sizeof(int)) != cudaSuccess) return -1;
+  return v;
+}
+
 }  // namespace b200
 
 using namespace b200;
@@ -1208,7 +1258,7 @@ extern "C" int b200_linattn_bwd(const b200_linattn_args *args, void *stream) {
   const b200_linattn_args &a = *args;
   if (int e = check_linattn(a)) return e;
   B200_REQUIRE(a.dout && a.dq && a.dk_out && a.dv_out, B200_ERR_NULL, "linattn_bwd: dout, dq, dk_out and dv_out must be non-null");
-  B200_REQUIRE(!a.dg || (int64_t)a.batch * a.heads * ((a.seqlen + CH * kSnap - 1) / (CH * kSnap)) < (int64_t(1) << 31), B200_ERR_SHAPE, "linattn_bwd: sizes too large");
+  B200_REQUIRE(!a.dg || (int64_t)a.batch * a.heads * ((a.seqlen + kSnapSteps - 1) / kSnapSteps) < (int64_t(1) << 31), B200_ERR_SHAPE, "linattn_bwd: sizes too large");
   const BwdPlan q = bwd_plan(a);
   B200_REQUIRE(a.work_bytes >= q.total && (a.work || !q.total), B200_ERR_TOO_LARGE, "linattn_bwd: work has %lld bytes, %lld are needed", (long long)a.work_bytes,
                (long long)q.total);
@@ -1248,14 +1298,14 @@ extern "C" int b200_linattn_bwd(const b200_linattn_args *args, void *stream) {
   Walk w = walk_dv(a);
   if (int e = run_walk(a.dtype, w, work, st)) return e;
   if (a.dg) {
-    const int bh = a.batch * a.heads, snaps = (chunks + kSnap - 1) / kSnap;
-    linattn_across_kernel<<<(unsigned)((int64_t)bh * snaps), 256, 0, st>>>(snap[0], snap[1], sum[0], sum[1], tiles, (int64_t)a.dk * a.dv, chunks, snaps, bh, across);
+    const int bh = a.batch * a.heads, every = kSnapSteps / w.ch, snaps = (chunks + every - 1) / every;
+    linattn_across_kernel<<<(unsigned)((int64_t)bh * snaps), 256, 0, st>>>(snap[0], snap[1], sum[0], sum[1], tiles, (int64_t)a.dk * a.dv, chunks, every, snaps, bh, across);
     if (a.g_heads) {
-      linattn_dg_sum_kernel<<<(unsigned)bh, 256, 0, st>>>(a, run[0], run[1], tiles, across, chunks, heads);
+      linattn_dg_sum_kernel<<<(unsigned)bh, 256, 0, st>>>(a, run[0], run[1], tiles, across, w.ch, chunks, heads);
       linattn_dg_heads_kernel<<<(unsigned)((a.heads + 127) / 128), 128, 0, st>>>(a, heads);
     } else {
       linattn_dg_kernel<<<dim3((unsigned)((a.seqlen + 31) / 32), (unsigned)((a.heads + 7) / 8), (unsigned)a.batch), 256, 0, st>>>(a, run[0], run[1], tiles, across,
-                                                                                                                             chunks);
+                                                                                                                             w.ch, chunks);
     }
   }
   return launch_status();

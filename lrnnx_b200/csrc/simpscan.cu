@@ -1407,7 +1407,9 @@ int b200_device_status(void) {
   if (g < 0) return -1;
   const int l = lce_status_read();
   if (l < 0) return -1;
-  return v ? v : (w ? w : (g ? g : l));
+  const int a = linattn_status_read();
+  if (a < 0) return -1;
+  return v ? v : (w ? w : (g ? g : (l ? l : a)));
 }
 
 }  // extern "C"
