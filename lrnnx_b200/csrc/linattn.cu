@@ -443,60 +443,74 @@ __device__ __forceinline__ uint32_t term(float &a, float &b) {
 }
 __device__ __forceinline__ float low16(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float high16(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
-__device__ __forceinline__ void copy16(uint32_t dst, const void *src, uint32_t bytes) {      // the rest of 16 bytes is zero
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 // byte offset of 16-byte piece c of row r in a swizzled tile
 __device__ __forceinline__ uint32_t piece_at(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
 
-// An operand's tile: 128 rows of W columns (64 or 128, 64 a tile) from step i0 on, zero past the sequence and past its size
-struct Tile {
-  const __nv_bfloat16 *src;
-  int64_t ls;
-  int left;                                 // columns there are
-  bool vec;
+// The operands as tensors of (size, heads or groups, length, batch), tiles of 64 x 128 steps; `tma` is 0 where an operand's strides or
+// alignment do not allow it, and the blocks load all of them themselves.
+struct Maps {
+  CUtensorMap q, k, v, x;
+  int tma;
 };
-__device__ __forceinline__ Tile tile_of(const void *base, int64_t off, int64_t ls, int col0, int size) {
-  Tile t;
-  t.src = reinterpret_cast<const __nv_bfloat16 *>(base) + off + col0;
-  t.ls = ls;
-  t.left = size - col0;
-  t.vec = ((reinterpret_cast<uintptr_t>(t.src) | (uintptr_t)(ls * 2)) & 15) == 0;
-  return t;
+__device__ __forceinline__ void tma_4d(void *dst, const CUtensorMap *map, int c, int h, int t, int b, uint64_t *bar) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_u32(dst)),
+               "l"(reinterpret_cast<uint64_t>(map)), "r"(c), "r"(h), "r"(t), "r"(b), "r"(smem_u32(bar))
+               : "memory");
 }
-template <int W> __device__ __forceinline__ void load_tile(const Walk &p, const Tile &o, int i0, unsigned char *dst) {
-  constexpr int PER = W / 8, ROWS = BT / PER;            // 16-byte pieces of a row, rows a pass
-  const int r0 = threadIdx.x / PER, pc = threadIdx.x % PER, left = o.left - pc * 8;
-  unsigned char *to = dst + (pc >> 3) * BTILE;
+// 128 steps of W columns (64 a tile) from time t0 on, zero past the sequence and past its size
+template <int W>
+__device__ __forceinline__ void load_tile(const Walk &p, const void *base, int64_t off, int64_t ls, int size, int col0, int t0, unsigned char *dst) {
+  constexpr int PER = W / 8;                             // 16-byte pieces of a row
+  const uint16_t *src = reinterpret_cast<const uint16_t *>(base) + off + col0;
+  for (int e = threadIdx.x; e < BC * PER; e += BT) {
+    const int r = e / PER, pc = e % PER, t = t0 + r, left = size - col0 - pc * 8;
+    const uint16_t *s = src + (int64_t)t * ls + pc * 8;
+    uint32_t x[8];
 #pragma unroll
-  for (int i = 0; i < BC / ROWS; ++i) {
-    const int r = r0 + i * ROWS, t = time_of(p, i0 + r);
-    const bool in = t < p.length && left > 0;
-    const __nv_bfloat16 *s = o.src + (in ? (int64_t)t * o.ls + pc * 8 : 0);
-    unsigned char *at = to + piece_at(r, pc & 7);
-    if (o.vec) copy16(smem_u32(at), s, in ? (left >= 8 ? 16u : (uint32_t)left * 2) : 0u);
-    else {
-      uint16_t x[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = in && j < left ? reinterpret_cast<const uint16_t *>(s)[j] : 0;
-      *reinterpret_cast<uint4 *>(at) = make_uint4(x[0] | (uint32_t)x[1] << 16, x[2] | (uint32_t)x[3] << 16, x[4] | (uint32_t)x[5] << 16, x[6] | (uint32_t)x[7] << 16);
-    }
+    for (int j = 0; j < 8; ++j) x[j] = t < p.length && j < left ? s[j] : 0u;
+    *reinterpret_cast<uint4 *>(dst + (pc >> 3) * BTILE + piece_at(r, pc & 7)) = make_uint4(x[0] | x[1] << 16, x[2] | x[3] << 16, x[4] | x[5] << 16, x[6] | x[7] << 16);
   }
 }
 
-// A chunk's decays by one warp, four steps a lane (see Decays), and from each 32 steps' start back to the steps before: what lies
-// between two blocks of 32 steps is the product of two factors of at most one.
+// A chunk's decays by one warp, four steps a lane (see Decays), by the steps' order in time; G runs in the walk's order.  Between
+// two blocks of 32 steps the decay is the product of two factors of at most one: from a step back to the start of its
+// block (in the walk's order), and from there back to the earlier step (`back`, a row for each block that has earlier ones).
 struct DecaysB {
-  float hi[BC], lo[BC], in[BC], out[BC], back[3][BC - 32];
+  float hi[BC], lo[BC], in[BC], out[BC], back[3][BC];
   float keep, keep_lo;
   double total;
 };
 __device__ __forceinline__ float between(const DecaysB &d, int r, int c) { return ex2a((d.hi[r] - d.hi[c]) + (d.lo[r] - d.lo[c])); }
-__device__ __forceinline__ void chunk_decays_b(const Walk &p, int b, int h, int i0, int lane, DecaysB &d) {
+__device__ __forceinline__ int in_time(const Walk &p, int i) { return p.rev ? BC - 1 - i : i; }
+// the decays before a lane's four steps of the chunk from step i0 on, all four loads in flight at once
+struct Four { float g[4]; };
+__device__ __forceinline__ Four load_decays(const Walk &p, int b, int h, int i0, int lane) {
+  Four f;
+  const int64_t at = b * p.g_bs + h * p.g_hs;
+  int t[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int i = i0 + 4 * lane + j;
+    t[j] = p.rev ? p.chunks * BC - i : i;
+  }
+  if (p.g_dtype == B200_F32) {
+    const float *g = reinterpret_cast<const float *>(p.g) + at;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f.g[j] = __ldg(g + (t[j] < p.length ? t[j] * p.g_ls : 0));
+  } else {
+    const __nv_bfloat16 *g = reinterpret_cast<const __nv_bfloat16 *>(p.g) + at;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f.g[j] = __bfloat162float(g[t[j] < p.length ? t[j] * p.g_ls : 0]);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (t[j] >= p.length) f.g[j] = 0.f;
+  return f;
+}
+__device__ __forceinline__ void chunk_decays_b(const Walk &p, const Four &f, int lane, DecaysB &d) {
   double a[4], s = 0.0;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) a[j] = log2_decay(p, b, h, i0 + 4 * lane + j);
+  for (int j = 0; j < 4; ++j) a[j] = f.g[j] != f.g[j] ? (double)f.g[j] : (double)fmaxf(f.g[j], -300.f) * 1.4426950408889634;
 #pragma unroll
   for (int j = 0; j < 4; ++j) { s += a[j]; a[j] = s; }
   double inc = s;
@@ -509,7 +523,7 @@ __device__ __forceinline__ void chunk_decays_b(const Walk &p, int b, int h, int 
   const double before = inc - s;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int i = 4 * lane + j;
+    const int i = in_time(p, 4 * lane + j);
     const double G = before + a[j];
     const float hi = (float)G;
     d.hi[i] = hi;
@@ -527,7 +541,10 @@ __device__ __forceinline__ void chunk_decays_b(const Walk &p, int b, int h, int 
 #pragma unroll
   for (int j = 1; j < 4; ++j)
 #pragma unroll
-    for (int i = 0; i < j; ++i) d.back[j - 1][i * 32 + lane] = between(d, 32 * j, i * 32 + lane);
+    for (int i = 0; i < j; ++i) {
+      const int c = in_time(p, i * 32 + lane);
+      d.back[j - 1][c] = between(d, in_time(p, 32 * j), c);
+    }
 }
 
 // Sums over the 32 lanes of 16 numbers each: lane l (and l + 16) gets the sum of number l % 16.
@@ -547,13 +564,12 @@ __device__ __forceinline__ float sum_columns(float (&v)[16], int lane) {
 // MODE: only a segment's own state; results; results and dots with x, forwards; the same backwards
 enum { OWN_STATE = 0, RESULTS = 1, DOTS = 2, DOTS_REV = 3 };
 
-__host__ __device__ constexpr int up_kb(int n) { return (n + 1023) / 1024 * 1024; }
 // shared memory: q | the state's terms, whose place the values' terms take once both have met; k, v, x
 __host__ __device__ constexpr int terms_bytes(int di, int ts, int tu) {
   return (di / 64 * BTILE + ts * di * 128) > tu * BTILE ? di / 64 * BTILE + ts * di * 128 : tu * BTILE;
 }
 
-template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && MODE >= DOTS ? 1 : 2) linattn_walk_tc_kernel(const Walk p, const int tu) {
+template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && MODE >= DOTS ? 1 : 2) linattn_walk_tc_kernel(const Walk p, const __grid_constant__ Maps maps, const int tu) {
   constexpr bool STATE_ONLY = MODE == OWN_STATE, grad = MODE >= DOTS, cross = MODE == DOTS_REV;
   constexpr int ts = grad ? 3 : 1, QB = DI / 64 * BTILE;
   extern __shared__ __align__(1024) unsigned char raw[];
@@ -562,7 +578,7 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
   unsigned char *sk = sq + (STATE_ONLY ? tu * BTILE : terms_bytes(DI, ts, tu)), *sv = sk + QB, *sx = sv + BTILE;
   __shared__ DecaysB dd[2];
   __shared__ float dots[2][BC], rows_[2][BC], cols_[4][BC];
-  __shared__ uint64_t bar;
+  __shared__ uint64_t bar, bar_d, loaded_qk, loaded_v;
   __shared__ uint32_t tmem_base;
   __shared__ int fail;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -574,6 +590,9 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
   const int wr = warp & 3, half = warp >> 2, r = wr * 32 + lane, c0 = half * 32;
   if (tid == 0) {
     mbar_init(&bar, 1);
+    mbar_init(&bar_d, 1);
+    mbar_init(&loaded_qk, 1);
+    mbar_init(&loaded_v, 1);
     fail = 0;
     mbar_fence_init();
   }
@@ -581,16 +600,33 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)), "r"(256) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  const Tile tk = tile_of(p.k, b * p.k_bs + h / p.k_div * p.k_hs, p.k_ls, 0, p.di), tv = tile_of(p.v, b * p.v_bs + h / p.v_div * p.v_hs, p.v_ls, col0, p.dout);
-  const Tile tq = tile_of(p.q, b * p.q_bs + h / p.q_div * p.q_hs, p.q_ls, 0, p.di), tx = tile_of(p.x, b * p.x_bs + h / p.x_div * p.x_hs, p.x_ls, col0, p.dout);
-  const auto load = [&](int i0) {
-    if (!STATE_ONLY) load_tile<DI>(p, tq, i0, sq);
-    load_tile<DI>(p, tk, i0, sk);
-    load_tile<64>(p, tv, i0, sv);
-    if (grad) load_tile<64>(p, tx, i0, sx);
+  const auto time0 = [&](int i0) { return p.rev ? (p.chunks - 1) * BC - i0 : i0; };      // of the chunk's first step in time
+  // The first and the last warp of the diagonal have no scores of their own off it: one of them forms the next chunk's
+  // decays, the other's neighbour issues copies and products.
+  const int decay_warp = p.rev ? 3 : 4, issue_warp = p.rev ? 2 : 5;
+  const bool issuer = warp == issue_warp && lane == 0;
+  const int hq = h / p.q_div, hk = h / p.k_div, hv = h / p.v_div, hx = h / p.x_div;
+  const auto copy_qk = [&](int i0) {                     // by the issuer
+    const int t0 = time0(i0);
+    mbar_expect_tx(&loaded_qk, (STATE_ONLY ? 1 : 2) * QB);
+#pragma unroll
+    for (int j = 0; j < DI / 64; ++j) {
+      if (!STATE_ONLY) tma_4d(sq + j * BTILE, &maps.q, j * 64, hq, t0, b, &loaded_qk);
+      tma_4d(sk + j * BTILE, &maps.k, j * 64, hk, t0, b, &loaded_qk);
+    }
   };
-  load(i_begin);
-  if (warp == 7) chunk_decays_b(p, b, h, i_begin, lane, dd[0]);
+  const auto copy_v = [&](int i0) {
+    mbar_expect_tx(&loaded_v, (grad ? 2 : 1) * BTILE);
+    tma_4d(sv, &maps.v, col0, hv, time0(i0), b, &loaded_v);
+    if (grad) tma_4d(sx, &maps.x, col0, hx, time0(i0), b, &loaded_v);
+  };
+  const auto load_all = [&](int i0) {                    // by all threads, where the operands cannot be copied
+    const int t0 = time0(i0);
+    if (!STATE_ONLY) load_tile<DI>(p, p.q, b * p.q_bs + hq * p.q_hs, p.q_ls, p.di, 0, t0, sq);
+    load_tile<DI>(p, p.k, b * p.k_bs + hk * p.k_hs, p.k_ls, p.di, 0, t0, sk);
+    load_tile<64>(p, p.v, b * p.v_bs + hv * p.v_hs, p.v_ls, p.dout, col0, t0, sv);
+    if (grad) load_tile<64>(p, p.x, b * p.x_bs + hx * p.x_hs, p.x_ls, p.dout, col0, t0, sx);
+  };
   float S[32];                                           // row r of the state, columns c0 on
   const bool has_row = r < p.di;
   const auto each = [&](auto f) {
@@ -619,52 +655,69 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
     else if (p.s0) each([&](int c, float &x) { x = p.s0[b * p.s0_bs + h * p.s0_hs + r * p.s0_is + c * p.s0_os]; });
     write_terms();
   }
+  if (warp == 7) chunk_decays_b(p, load_decays(p, b, h, i_begin, lane), lane, dd[0]);
+  fence_proxy_async();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (!maps.tma) load_all(i_begin);
+  else if (issuer) {
+    copy_qk(i_begin);
+    copy_v(i_begin);
+  }
   const uint32_t tm = tmem_base, tm_own = tm + ((uint32_t)(wr * 32) << 16);
   const uint32_t tP = 0, tO = 128, tD = 192;             // columns: scores, result, the state's sum (x v^T takes the place of the last two for a while)
   constexpr uint32_t kScores = idesc_f16(1, false, false, 128, 128), kState = idesc_f16(1, false, true, 128, 64), kUpdate = idesc_f16(1, true, true, 128, 64);
+  const auto kmajor = [](int i) { return (uint64_t)(((i >> 2) * BTILE + (i & 3) * 32) / 16); };      // to the i-th 16 columns of a K-major operand
   uint32_t phase = 0;
-  const auto wait_products = [&]() {
-    if (!mbar_wait(&bar, phase, kWaitLimit)) *(volatile int *)&fail = 1;
-    phase ^= 1;
+  const auto wait_products = [&](uint64_t &on, uint32_t parity) {
+    if (!mbar_wait(&on, parity, kWaitLimit)) *(volatile int *)&fail = 1;
     __syncwarp();
     tc_fence_after();
+  };
+  // the state's sum of the chunk: keys with 64 columns have one tile; what follows it makes up the lanes past 63, which nothing reads
+  const auto issue_update = [&]() {
+    const uint64_t k = smem_desc(smem_u32(sk), BTILE, 1024, 2), u = smem_desc(smem_u32(su), 8192, 1024, 2);
+#pragma unroll 1
+    for (int t = tu - 1; t >= 0; --t)
+#pragma unroll
+      for (int i = 0; i < BC / 16; ++i) mma_f16(tm + tD, k + i * 128, u + t * (BTILE / 16) + i * 128, kUpdate, t < tu - 1 || i > 0);
   };
   double total = 0.0;
   for (int i0 = i_begin, it = 0; i0 < i_end; i0 += BC, ++it) {
     const int chunk = p.rev ? p.chunks - 1 - i0 / BC : i0 / BC;
     const DecaysB &d = dd[it & 1];
     if (grad && !cross && chunk % kSnapB == 0) snapshot(chunk / kSnapB, 1.f);
-    copies_wait();
     fence_proxy_async();
     tc_fence_before();
-    __syncthreads();                                     // operands and the state's terms are there, accumulators read
+    __syncthreads();                                     // the state's terms are written, accumulators read
     if (*(volatile int *)&fail) break;
+    Four next = {};
+    if (warp == decay_warp && i0 + BC < i_end) next = load_decays(p, b, h, i0 + BC, lane);
+    if (issuer && maps.tma && !mbar_wait(&loaded_qk, it & 1, kWaitLimit)) *(volatile int *)&fail = 1;
     float O[32];
     if constexpr (!STATE_ONLY) {
-      if (tid == 0) {
+      if (issuer) {
         tc_fence_after();
-        const uint32_t q = smem_u32(sq), k = smem_u32(sk), s = smem_u32(ss);
-#pragma unroll 1
-        for (int i = 0; i < DI / 16; ++i)
-          mma_f16(tm + tP, smem_desc(q + (i >> 2) * BTILE + (i & 3) * 32, 16, 1024, 2), smem_desc(k + (i >> 2) * BTILE + (i & 3) * 32, 16, 1024, 2), kScores, i > 0);
-#pragma unroll 1
+        const uint64_t q = smem_desc(smem_u32(sq), 16, 1024, 2), k = smem_desc(smem_u32(sk), 16, 1024, 2), st = smem_desc(smem_u32(ss), 8192, 1024, 2);
+#pragma unroll
+        for (int i = 0; i < DI / 16; ++i) mma_f16(tm + tP, q + kmajor(i), k + kmajor(i), kScores, i > 0);
+#pragma unroll
         for (int t = ts - 1; t >= 0; --t)
-#pragma unroll 1
-          for (int i = 0; i < DI / 16; ++i)
-            mma_f16(tm + tO, smem_desc(q + (i >> 2) * BTILE + (i & 3) * 32, 16, 1024, 2), smem_desc(s + t * DI * 128 + i * 2048, 8192, 1024, 2), kState, t < ts - 1 || i > 0);
+#pragma unroll
+          for (int i = 0; i < DI / 16; ++i) mma_f16(tm + tO, q + kmajor(i), st + (t * DI * 128 + i * 2048) / 16, kState, t < ts - 1 || i > 0);
         mma_commit(&bar);
       }
       __syncwarp();
-      wait_products();
+      wait_products(bar, phase);
+      phase ^= 1;
       {
         tmem_ld32(tm_own + tO + c0, O);
         const float f = d.in[r] * p.s_inter;
 #pragma unroll
         for (int j = 0; j < 32; ++j) O[j] *= f;
       }
+      if (maps.tma && !mbar_wait(&loaded_v, it & 1, kWaitLimit)) *(volatile int *)&fail = 1;
       if (grad) {
         float dot = 0.f;
 #pragma unroll
@@ -679,16 +732,17 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
       if (cross) {
         tc_fence_before();
         __syncthreads();                                 // the result's columns are read
-        if (tid == 0) {
+        if (issuer) {
           tc_fence_after();
-#pragma unroll 1
-          for (int i = 0; i < DO / 16; ++i)
-            mma_f16(tm + tO, smem_desc(smem_u32(sx) + i * 32, 16, 1024, 2), smem_desc(smem_u32(sv) + i * 32, 16, 1024, 2), kScores, i > 0);
+          const uint64_t x = smem_desc(smem_u32(sx), 16, 1024, 2), v = smem_desc(smem_u32(sv), 16, 1024, 2);
+#pragma unroll
+          for (int i = 0; i < DO / 16; ++i) mma_f16(tm + tO, x + kmajor(i), v + kmajor(i), kScores, i > 0);
           mma_commit(&bar);
         }
         __syncwarp();
       }
     }
+    if (STATE_ONLY && maps.tma && !mbar_wait(&loaded_v, it & 1, kWaitLimit)) *(volatile int *)&fail = 1;
     // values as the state takes them up, in terms: q and the state's terms have been read
 #pragma unroll 1
     for (int i = 0; i < BC * 8 / BT; ++i) {
@@ -707,29 +761,45 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
       for (int t = 0; t < 3; ++t)
         if (t < tu) *reinterpret_cast<uint4 *>(su + t * BTILE + at) = make_uint4(term(y[0], y[1]), term(y[2], y[3]), term(y[4], y[5]), term(y[6], y[7]));
     }
+    if constexpr (!cross) {                              // the state's sum of the chunk, while scores are decayed
+      fence_proxy_async();
+      tc_fence_before();
+      __syncthreads();
+      if (issuer) {
+        tc_fence_after();
+        issue_update();
+        mma_commit(&bar_d);
+      }
+      __syncwarp();
+    }
     if constexpr (!STATE_ONLY) {
-      if (cross) wait_products();
-      // scores: decayed, zero after the step itself
-      const float f = between(d, r, wr * 32) * p.s_intra;
+      if (cross) {
+        wait_products(bar, phase);
+        phase ^= 1;
+      }
+      // scores: decayed, zero after the step itself (in the walk's order)
+      const int start = p.rev ? wr * 32 + 31 : wr * 32;
+      const float hr = d.hi[r], lr = d.lo[r], f = between(d, r, start) * p.s_intra;
+      const float *back = d.back[p.rev ? max(0, 2 - wr) : max(0, wr - 1)];
       float row = 0.f;
 #pragma unroll 1
       for (int g = 0; g < 2; ++g) {                      // 32 columns at a time, 16 columns of TMEM as bfloat16
         const int cb = half * 2 + g;                     // block of 32 columns
         uint32_t packed[16];
-        if (cb > wr) {
+        if (p.rev ? cb < wr : cb > wr) {
 #pragma unroll
           for (int j = 0; j < 16; ++j) packed[j] = 0u;
-          if (cross && lane < 16) cols_[wr][cb * 32 + lane] = cols_[wr][cb * 32 + 16 + lane] = 0.f;
+          if (cross) cols_[wr][cb * 32 + lane] = 0.f;
         } else {
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
             const int c = cb * 32 + q * 16;
             float v[16];
             tmem_ld16(tm_own + tP + c, v);
-            if (cb < wr) {
+            if (cb != wr) {
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
-                const float4 w = *reinterpret_cast<const float4 *>(&d.back[wr - 1][c + 4 * j]);
+                const float4 w = *reinterpret_cast<const float4 *>(&back[c + 4 * j]);
                 v[4 * j] *= f * w.x;
                 v[4 * j + 1] *= f * w.y;
                 v[4 * j + 2] *= f * w.z;
@@ -737,7 +807,16 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
               }
             } else {
 #pragma unroll
-              for (int j = 0; j < 16; ++j) v[j] = c + j <= r ? v[j] * between(d, r, c + j) * p.s_intra : 0.f;
+              for (int j = 0; j < 4; ++j) {
+                const float4 hi = *reinterpret_cast<const float4 *>(&d.hi[c + 4 * j]), lo = *reinterpret_cast<const float4 *>(&d.lo[c + 4 * j]);
+                const float x[4] = {(hr - hi.x) + (lr - lo.x), (hr - hi.y) + (lr - lo.y), (hr - hi.z) + (lr - lo.z), (hr - hi.w) + (lr - lo.w)};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const bool on = p.rev ? c + 4 * j + e >= r : c + 4 * j + e <= r;
+                  const float w = ex2a(on ? x[e] : 0.f) * p.s_intra;
+                  v[4 * j + e] = on ? v[4 * j + e] * w : 0.f;
+                }
+              }
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -765,36 +844,57 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
       if (cross) rows_[half][r] = row;
       tmem_st_wait();
     }
-    fence_proxy_async();
-    tc_fence_before();
-    __syncthreads();                                     // scores and the values' terms are written
-    if (tid == 0) {
-      tc_fence_after();
-      const uint32_t k = smem_u32(sk), v = smem_u32(sv), u = smem_u32(su);
-      if constexpr (!STATE_ONLY)
-#pragma unroll 1
-        for (int i = 0; i < BC / 16; ++i)
-          mma_f16_ta(tm + tO, tm + tP + (i >> 2) * 64 + (i & 3) * 8, smem_desc(v + i * 2048, 8192, 1024, 2), kState, i > 0);
-#pragma unroll 1
-      for (int t = tu - 1; t >= 0; --t)
-#pragma unroll 1
-        for (int i = 0; i < BC / 16; ++i)
-          // keys with 64 columns have one tile; what follows it makes up the lanes past 63, which nothing reads
-          mma_f16(tm + tD, smem_desc(k + i * 2048, BTILE, 1024, 2), smem_desc(u + t * BTILE + i * 2048, 8192, 1024, 2), kUpdate, t < tu - 1 || i > 0);
-      mma_commit(&bar);
+    // the next chunk's decays, by a warp whose scores are all zero
+    if (warp == decay_warp && i0 + BC < i_end) chunk_decays_b(p, next, lane, dd[(it + 1) & 1]);
+    if (!cross && issuer) {                              // keys and q are free once the sum is there
+      if (!mbar_wait(&bar_d, it & 1, kWaitLimit)) *(volatile int *)&fail = 1;
+      if (maps.tma && i0 + BC < i_end) copy_qk(i0 + BC);
     }
     __syncwarp();
-    wait_products();
+    fence_proxy_async();
+    tc_fence_before();
+    __syncthreads();                                     // scores (and backwards the values' terms) are written
+    if (!STATE_ONLY && issuer) {
+      tc_fence_after();
+      const uint64_t v = smem_desc(smem_u32(sv), 8192, 1024, 2);
+#pragma unroll
+      for (int i = 0; i < BC / 16; ++i) mma_f16_ta(tm + tO, tm + tP + (i >> 2) * 64 + (i & 3) * 8, v + i * 128, kState, i > 0);
+      if (cross) issue_update();
+      mma_commit(&bar);
+    }
+    if (grad && warp == decay_warp) {
+      double v[4];
+      float s = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = in_time(p, 4 * lane + j);
+        const float dot = dots[0][i] + dots[1][i];
+        s += dot;
+        v[j] = dot;
+        if (cross) v[j] += ((double)rows_[0][i] + rows_[1][i]) - (((double)cols_[0][i] + cols_[1][i]) + ((double)cols_[2][i] + cols_[3][i]));
+      }
+      chunk_runs(p, tile, bh, i0, lane, v, s);
+    }
+    __syncwarp();
+    if (!cross) wait_products(bar_d, it & 1);
+    if (!STATE_ONLY) {
+      wait_products(bar, phase);
+      phase ^= 1;
+    }
     if (i0 + BC < i_end) {
-      load(i0 + BC);
-      if (warp == 7) chunk_decays_b(p, b, h, i0 + BC, lane, dd[(it + 1) & 1]);
+      if (!maps.tma) load_all(i0 + BC);
+      else if (issuer) {
+        if (cross) copy_qk(i0 + BC);
+        copy_v(i0 + BC);
+      }
+      __syncwarp();
     }
     if constexpr (!STATE_ONLY) {
       float v[32];
       tmem_ld32(tm_own + tO + c0, v);
 #pragma unroll
       for (int j = 0; j < 32; ++j) O[j] += v[j];
-      const int t = time_of(p, i0 + r), left = p.dout - col0 - c0;
+      const int t = time0(i0) + r, left = p.dout - col0 - c0;
       if (t < p.length && left > 0) {
         const int64_t at = b * p.o_bs + t * p.o_ls + h * p.o_hs + col0 + c0;
         if (p.out_f32) {
@@ -836,23 +936,9 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
       for (int j = 0; j < 32; ++j) S[j] = r < DI ? fmaf(S[j], keep, fmaf(S[j], keep_lo, v[j])) : 0.f;
     }
     total += d.total;
-    if (grad && warp == 0) {
-      double v[4];
-      float s = 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int i = 4 * lane + j;
-        const float dot = dots[0][i] + dots[1][i];
-        s += dot;
-        v[j] = dot;
-        if (cross) v[j] += ((double)rows_[0][i] + rows_[1][i]) - (((double)cols_[0][i] + cols_[1][i]) + ((double)cols_[2][i] + cols_[3][i]));
-      }
-      chunk_runs(p, tile, bh, i0, lane, v, s);
-    }
     if (cross && chunk % kSnapB == 0) snapshot(chunk / kSnapB, (float)exp2(log2_of(p, b, h, chunk * BC)));
     if (!STATE_ONLY) write_terms();
   }
-  copies_wait();
   const bool ok = !*(volatile int *)&fail;
   if (STATE_ONLY && ok) {
     each([&](int c, float &x) { p.seg[(((int64_t)bh * p.nseg + seg) * p.di + r) * p.dout + c] = x; });
@@ -1083,11 +1169,29 @@ int launch_walk(Walk &w, K own, K all, int threads, int smem_own, int smem_all, 
 template <typename T> int walk(Walk &w, unsigned char *work, cudaStream_t st) {
   return launch_walk(w, linattn_walk_kernel<T, true>, linattn_walk_kernel<T, false>, WT, walk_smem(w.di, true, false), walk_smem(w.di, false, w.run != nullptr), work, st);
 }
+bool map_of(CUtensorMap *m, const void *base, int size, int heads, int length, int batch, int64_t hs, int64_t ls, int64_t bs) {
+  EncodeTiledFn enc = encoder();
+  if (!enc || (reinterpret_cast<uintptr_t>(base) & 15)) return false;
+  const cuuint64_t dims[4] = {(cuuint64_t)size, (cuuint64_t)heads, (cuuint64_t)length, (cuuint64_t)batch};
+  int64_t st[3] = {heads > 1 ? hs : 8, length > 1 ? ls : 8, batch > 1 ? bs : 8};
+  for (int64_t x : st)
+    if (x <= 0 || x % 8 || x >= (int64_t(1) << 38)) return false;
+  const cuuint64_t strides[3] = {(cuuint64_t)st[0] * 2, (cuuint64_t)st[1] * 2, (cuuint64_t)st[2] * 2};
+  const cuuint32_t box[4] = {64, 1, BC, 1}, one[4] = {1, 1, 1, 1};
+  return enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 template <int DI> int walk_tc(Walk &w, unsigned char *work, cudaStream_t st) {
   const int ts = w.run ? 3 : 1, tu = w.run || w.last ? 3 : 2, kv = DI / 64 * BTILE + BTILE + 1024;
   const int own = tu * BTILE + kv, all = terms_bytes(DI, ts, tu) + kv + (w.run ? BTILE : 0);
   const auto results = !w.run ? linattn_walk_tc_kernel<DI, RESULTS> : w.rev ? linattn_walk_tc_kernel<DI, DOTS_REV> : linattn_walk_tc_kernel<DI, DOTS>;
-  return launch_walk(w, linattn_walk_tc_kernel<DI, OWN_STATE>, results, BT, own, all, work, st, tu);
+  Maps m;
+  memset(&m, 0, sizeof(m));
+  m.tma = map_of(&m.q, w.q, w.di, w.heads / w.q_div, w.length, w.batch, w.q_hs, w.q_ls, w.q_bs) &&
+          map_of(&m.k, w.k, w.di, w.heads / w.k_div, w.length, w.batch, w.k_hs, w.k_ls, w.k_bs) &&
+          map_of(&m.v, w.v, w.dout, w.heads / w.v_div, w.length, w.batch, w.v_hs, w.v_ls, w.v_bs) &&
+          (!w.run || map_of(&m.x, w.x, w.dout, w.heads / w.x_div, w.length, w.batch, w.x_hs, w.x_ls, w.x_bs));
+  return launch_walk(w, linattn_walk_tc_kernel<DI, OWN_STATE>, results, BT, own, all, work, st, m, tu);
 }
 int run_walk(int dtype, Walk &w, unsigned char *work, cudaStream_t st) {
   if (dtype == B200_F32) return walk<float>(w, work, st);
