@@ -37,6 +37,7 @@ constexpr int MAX_D = 128;
 constexpr int PP = CH + 4, PV = DO + 8;   // pitches of scores and of values / state (in floats)
 constexpr int kSnapSteps = 512;           // steps between the states that the gradient of g is anchored at
 constexpr int kSnap = kSnapSteps / CH;
+constexpr int kMaxSeg = 64;               // segments of a sequence
 
 struct Walk {
   // operands (batch, length, heads or groups, size), sizes contiguous; strides in elements
@@ -449,12 +450,17 @@ __device__ __forceinline__ uint32_t piece_at(int r, int c) { return (uint32_t)(r
 // The operands as tensors of (size, heads or groups, length, batch), tiles of 64 x 128 steps; `tma` is 0 where an operand's strides or
 // alignment do not allow it, and the blocks load all of them themselves.
 struct Maps {
-  CUtensorMap q, k, v, x;
-  int tma;
+  CUtensorMap q, k, v, x, out;
+  int tma, tma_out;
 };
 __device__ __forceinline__ void tma_4d(void *dst, const CUtensorMap *map, int c, int h, int t, int b, uint64_t *bar) {
   asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_u32(dst)),
                "l"(reinterpret_cast<uint64_t>(map)), "r"(c), "r"(h), "r"(t), "r"(b), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void tma_st_4d(const CUtensorMap *map, const void *src, int c, int h, int t, int b) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(c), "r"(h),
+               "r"(t), "r"(b), "r"(smem_u32(src))
                : "memory");
 }
 // 128 steps of W columns (64 a tile) from time t0 on, zero past the sequence and past its size
@@ -627,32 +633,35 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
     load_tile<64>(p, p.v, b * p.v_bs + hv * p.v_hs, p.v_ls, p.dout, col0, t0, sv);
     if (grad) load_tile<64>(p, p.x, b * p.x_bs + hx * p.x_hs, p.x_ls, p.dout, col0, t0, sx);
   };
-  float S[32];                                           // row r of the state, columns c0 on
-  const bool has_row = r < p.di;
+  // This thread's part of the state: a row and NS columns.  With 64 rows TMEM's upper 64 lanes hold them once more, and the
+  // warps there take half of the columns.
+  constexpr int NS = DI == 64 ? 16 : 32;
+  const int rs = r & (DI - 1), cs = half * 32 + (DI == 64 ? (wr >> 1) * 16 : 0);
+  float S[NS];
+  const bool has_row = rs < p.di;
   const auto each = [&](auto f) {
     if (has_row)
 #pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (col0 + c0 + j < p.dout) f(col0 + c0 + j, S[j]);
+      for (int j = 0; j < NS; ++j)
+        if (col0 + cs + j < p.dout) f(col0 + cs + j, S[j]);
   };
-  const auto snapshot = [&](int s, float f) { each([&](int c, float &x) { p.snap[(((int64_t)bh * snaps + s) * p.di + r) * p.dout + c] = x * f; }); };
+  const auto snapshot = [&](int s, float f) { each([&](int c, float &x) { p.snap[(((int64_t)bh * snaps + s) * p.di + rs) * p.dout + c] = x * f; }); };
   const auto write_terms = [&]() {
-    if (r < DI)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float x[8];
+    for (int j = 0; j < NS / 8; ++j) {
+      float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = S[j * 8 + e];
+      for (int e = 0; e < 8; ++e) x[e] = S[j * 8 + e];
 #pragma unroll
-        for (int t = 0; t < ts; ++t)
-          *reinterpret_cast<uint4 *>(ss + t * DI * 128 + piece_at(r, half * 4 + j)) = make_uint4(term(x[0], x[1]), term(x[2], x[3]), term(x[4], x[5]), term(x[6], x[7]));
-      }
+      for (int t = 0; t < ts; ++t)
+        *reinterpret_cast<uint4 *>(ss + t * DI * 128 + piece_at(rs, cs / 8 + j)) = make_uint4(term(x[0], x[1]), term(x[2], x[3]), term(x[4], x[5]), term(x[6], x[7]));
+    }
   };
 #pragma unroll
-  for (int j = 0; j < 32; ++j) S[j] = 0.f;
+  for (int j = 0; j < NS; ++j) S[j] = 0.f;
   if (!STATE_ONLY) {
-    if (p.nseg > 1) each([&](int c, float &x) { x = p.seg[(((int64_t)bh * p.nseg + seg) * p.di + r) * p.dout + c]; });
-    else if (p.s0) each([&](int c, float &x) { x = p.s0[b * p.s0_bs + h * p.s0_hs + r * p.s0_is + c * p.s0_os]; });
+    if (p.nseg > 1) each([&](int c, float &x) { x = p.seg[(((int64_t)bh * p.nseg + seg) * p.di + rs) * p.dout + c]; });
+    else if (p.s0) each([&](int c, float &x) { x = p.s0[b * p.s0_bs + h * p.s0_hs + rs * p.s0_is + c * p.s0_os]; });
     write_terms();
   }
   if (warp == 7) chunk_decays_b(p, load_decays(p, b, h, i_begin, lane), lane, dd[0]);
@@ -675,14 +684,20 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
     __syncwarp();
     tc_fence_after();
   };
-  // the state's sum of the chunk: keys with 64 columns have one tile; what follows it makes up the lanes past 63, which nothing reads
+  // the state's sum of the chunk; keys of 64 columns are both halves of the 128 rows
   const auto issue_update = [&]() {
-    const uint64_t k = smem_desc(smem_u32(sk), BTILE, 1024, 2), u = smem_desc(smem_u32(su), 8192, 1024, 2);
+    const uint64_t k = smem_desc(smem_u32(sk), DI == 64 ? 0 : BTILE, 1024, 2), u = smem_desc(smem_u32(su), 8192, 1024, 2);
 #pragma unroll 1
     for (int t = tu - 1; t >= 0; --t)
 #pragma unroll
       for (int i = 0; i < BC / 16; ++i) mma_f16(tm + tD, k + i * 128, u + t * (BTILE / 16) + i * 128, kUpdate, t < tu - 1 || i > 0);
   };
+  const auto issue_scores = [&]() {
+    const uint64_t q = smem_desc(smem_u32(sq), 16, 1024, 2), k = smem_desc(smem_u32(sk), 16, 1024, 2);
+#pragma unroll
+    for (int i = 0; i < DI / 16; ++i) mma_f16(tm + tP, q + kmajor(i), k + kmajor(i), kScores, i > 0);
+  };
+  bool scores_on = false;                                // the issuer's: this chunk's are on their way since the last one
   double total = 0.0;
   for (int i0 = i_begin, it = 0; i0 < i_end; i0 += BC, ++it) {
     const int chunk = p.rev ? p.chunks - 1 - i0 / BC : i0 / BC;
@@ -694,14 +709,14 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
     if (*(volatile int *)&fail) break;
     Four next = {};
     if (warp == decay_warp && i0 + BC < i_end) next = load_decays(p, b, h, i0 + BC, lane);
-    if (issuer && maps.tma && !mbar_wait(&loaded_qk, it & 1, kWaitLimit)) *(volatile int *)&fail = 1;
+    if (issuer && maps.tma && !scores_on && !mbar_wait(&loaded_qk, it & 1, kWaitLimit)) *(volatile int *)&fail = 1;
     float O[32];
     if constexpr (!STATE_ONLY) {
       if (issuer) {
         tc_fence_after();
-        const uint64_t q = smem_desc(smem_u32(sq), 16, 1024, 2), k = smem_desc(smem_u32(sk), 16, 1024, 2), st = smem_desc(smem_u32(ss), 8192, 1024, 2);
-#pragma unroll
-        for (int i = 0; i < DI / 16; ++i) mma_f16(tm + tP, q + kmajor(i), k + kmajor(i), kScores, i > 0);
+        const uint64_t q = smem_desc(smem_u32(sq), 16, 1024, 2), st = smem_desc(smem_u32(ss), 8192, 1024, 2);
+        if (!scores_on) issue_scores();
+        scores_on = false;
 #pragma unroll
         for (int t = ts - 1; t >= 0; --t)
 #pragma unroll
@@ -881,11 +896,19 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
       wait_products(bar, phase);
       phase ^= 1;
     }
-    if (i0 + BC < i_end) {
-      if (!maps.tma) load_all(i0 + BC);
-      else if (issuer) {
+    const bool more = i0 + BC < i_end, staged = !STATE_ONLY && maps.tma_out;
+    if (more) {
+      if (!maps.tma) {
+        if (!staged) load_all(i0 + BC);                  // else once the results have left
+      } else if (issuer) {
         if (cross) copy_qk(i0 + BC);
-        copy_v(i0 + BC);
+        else if (!STATE_ONLY) {
+          if (!mbar_wait(&loaded_qk, (it + 1) & 1, kWaitLimit)) *(volatile int *)&fail = 1;
+          tc_fence_after();
+          issue_scores();
+          scores_on = true;
+        }
+        if (!staged) copy_v(i0 + BC);
       }
       __syncwarp();
     }
@@ -895,7 +918,32 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
 #pragma unroll
       for (int j = 0; j < 32; ++j) O[j] += v[j];
       const int t = time0(i0) + r, left = p.dout - col0 - c0;
-      if (t < p.length && left > 0) {
+      if (staged) {                                      // by way of shared memory, where v (and x) were
+        if (p.out_f32) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<float4 *>(sv + half * BTILE + piece_at(r, j)) = make_float4(O[4 * j], O[4 * j + 1], O[4 * j + 2], O[4 * j + 3]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const __nv_bfloat162 x = __floats2bfloat162_rn(O[j * 8 + 2 * e], O[j * 8 + 2 * e + 1]);
+              w[e] = *reinterpret_cast<const uint32_t *>(&x);
+            }
+            *reinterpret_cast<uint4 *>(sv + piece_at(r, half * 4 + j)) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+        fence_proxy_async();
+        __syncthreads();
+        if (issuer) {
+          tma_st_4d(&maps.out, sv, col0, h, time0(i0), b);
+          if (p.out_f32 && col0 + 32 < p.dout) tma_st_4d(&maps.out, sv + BTILE, col0 + 32, h, time0(i0), b);
+          bulk_commit();
+        }
+        __syncwarp();
+      } else if (t < p.length && left > 0) {
         const int64_t at = b * p.o_bs + t * p.o_ls + h * p.o_hs + col0 + c0;
         if (p.out_f32) {
           float *o = reinterpret_cast<float *>(p.out) + at;
@@ -929,23 +977,37 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
       }
     }
     {
-      float v[32];
-      tmem_ld32(tm_own + tD + c0, v);
+      float v[NS];
+      if constexpr (NS == 32) tmem_ld32(tm_own + tD + cs, v);
+      else tmem_ld16(tm_own + tD + cs, v);
       const float keep = d.keep, keep_lo = d.keep_lo;
 #pragma unroll
-      for (int j = 0; j < 32; ++j) S[j] = r < DI ? fmaf(S[j], keep, fmaf(S[j], keep_lo, v[j])) : 0.f;
+      for (int j = 0; j < NS; ++j) S[j] = fmaf(S[j], keep, fmaf(S[j], keep_lo, v[j]));
     }
     total += d.total;
     if (cross && chunk % kSnapB == 0) snapshot(chunk / kSnapB, (float)exp2(log2_of(p, b, h, chunk * BC)));
     if (!STATE_ONLY) write_terms();
+    if (staged && more) {
+      if (issuer) {
+        bulk_wait_read<0>();
+        if (maps.tma) copy_v(i0 + BC);
+      }
+      __syncwarp();
+      if (!maps.tma) {
+        __syncthreads();                                 // the results have left
+        load_all(i0 + BC);
+      }
+    }
   }
+  if (!STATE_ONLY && issuer) bulk_wait<0>();
+  __syncwarp();
   const bool ok = !*(volatile int *)&fail;
   if (STATE_ONLY && ok) {
-    each([&](int c, float &x) { p.seg[(((int64_t)bh * p.nseg + seg) * p.di + r) * p.dout + c] = x; });
+    each([&](int c, float &x) { p.seg[(((int64_t)bh * p.nseg + seg) * p.di + rs) * p.dout + c] = x; });
     if (tile == 0 && tid == 0) p.seg_g[(int64_t)bh * p.nseg + seg] = total;
   } else if (!STATE_ONLY && ok && p.last && seg == p.nseg - 1) {
     const float f = p.last_decay ? (float)exp2(log2_of(p, b, h, 0)) : 1.f;
-    each([&](int c, float &x) { p.last[b * p.last_bs + h * p.last_hs + r * p.last_is + c * p.last_os] = x * f; });
+    each([&](int c, float &x) { p.last[b * p.last_bs + h * p.last_hs + rs * p.last_is + c * p.last_os] = x * f; });
   }
   tc_fence_before();
   __syncthreads();
@@ -955,16 +1017,25 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
 
 // Each segment's own state becomes the state before it.
 __global__ void __launch_bounds__(256) linattn_join_kernel(const Walk p) {
+  __shared__ float keep[kMaxSeg];
   const int64_t per = (int64_t)p.di * p.dout, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int bh = blockIdx.y, b = bh / p.heads, h = bh % p.heads;
+  if (threadIdx.x < p.nseg - 1) keep[threadIdx.x] = (float)exp2(p.seg_g[(int64_t)bh * p.nseg + threadIdx.x]);
+  __syncthreads();
   if (i >= per) return;
   float s = 0.f;
   if (p.s0) s = p.s0[b * p.s0_bs + h * p.s0_hs + i / p.dout * p.s0_is + i % p.dout * p.s0_os];
-  for (int n = 0; n < p.nseg; ++n) {
-    float *at = p.seg + ((int64_t)bh * p.nseg + n) * per + i;
-    const float own = n < p.nseg - 1 ? *at : 0.f;
-    *at = s;
-    if (n < p.nseg - 1) s = fmaf(s, (float)exp2(p.seg_g[(int64_t)bh * p.nseg + n]), own);
+  float *at = p.seg + (int64_t)bh * p.nseg * per + i;
+  for (int n0 = 0; n0 < p.nseg; n0 += 8) {              // eight segments' loads in flight
+    float own[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) own[j] = n0 + j < p.nseg - 1 ? at[(n0 + j) * per] : 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (n0 + j < p.nseg) {
+        at[(n0 + j) * per] = s;
+        if (n0 + j < p.nseg - 1) s = fmaf(s, keep[n0 + j], own[j]);
+      }
   }
 }
 
@@ -1124,16 +1195,19 @@ int walk_smem(int di, bool state_only, bool with_x) {
   return 4 * (CH * (dip + 4) + CH * PV + dip * PV + (state_only ? 0 : CH * (dip + 4) + (with_x ? 2 : 1) * CH * PP));
 }
 
-// Segments: as many as make the walk shortest, counted in chunks that one SM goes through, a first pass over segments at 0.45 of a walk.
-int segments(int64_t blocks, int chunks) {
-  const int sms = sm_count_current();
+// Segments: as many as make the walk shortest.  Counted in chunks that an SM goes through with as many blocks as fit it
+// (`resident`; a last round that leaves the SMs one block each takes 0.6 of one), one more for a block's start; the first pass over
+// the segments takes 0.7 of the second.  A prompt of 16384 steps x 16 heads of 128 x 128: 9 segments.
+int segments(int64_t blocks, int chunks, int resident) {
+  const int64_t sms = sm_count_current(), slots = sms * resident;
   int best = 1;
   double cost = 1e30;
-  for (int n = 1; n <= 64 && n <= chunks; ++n) {
+  for (int n = 1; n <= kMaxSeg && n <= chunks; ++n) {
     const int per = (chunks + n - 1) / n;
     if ((int64_t)(n - 1) * per >= chunks) continue;
-    const double waves = (double)((blocks * n + sms - 1) / sms);
-    const double c = waves * per * (n > 1 ? 1.45 : 1.0) + (n > 1 ? 2 : 0);
+    const int64_t left = blocks * n % slots;
+    const double rounds = (double)(blocks * n / slots) + (left == 0 ? 0.0 : left <= sms && resident > 1 ? 0.6 : 1.0);
+    const double c = rounds * (per + 1) * (n > 1 ? 1.7 : 1.0) + (n > 1 ? 1 : 0);
     if (c < cost * 0.97) { cost = c; best = n; }
   }
   return best;
@@ -1142,7 +1216,7 @@ int segments(int64_t blocks, int chunks) {
 void cut(Walk &w) {
   const int chunks = w.chunks;
   w.tiles = (w.dout + DO - 1) / DO;
-  const int n = segments((int64_t)w.batch * w.heads * w.tiles, chunks);
+  const int n = segments((int64_t)w.batch * w.heads * w.tiles, chunks, w.ch == BC ? 2 : 1);
   w.seg_chunks = (chunks + n - 1) / n;
   w.nseg = (chunks + w.seg_chunks - 1) / w.seg_chunks;
 }
@@ -1169,16 +1243,17 @@ int launch_walk(Walk &w, K own, K all, int threads, int smem_own, int smem_all, 
 template <typename T> int walk(Walk &w, unsigned char *work, cudaStream_t st) {
   return launch_walk(w, linattn_walk_kernel<T, true>, linattn_walk_kernel<T, false>, WT, walk_smem(w.di, true, false), walk_smem(w.di, false, w.run != nullptr), work, st);
 }
-bool map_of(CUtensorMap *m, const void *base, int size, int heads, int length, int batch, int64_t hs, int64_t ls, int64_t bs) {
+bool map_of(CUtensorMap *m, const void *base, int size, int heads, int length, int batch, int64_t hs, int64_t ls, int64_t bs, bool f32 = false) {
   EncodeTiledFn enc = encoder();
   if (!enc || (reinterpret_cast<uintptr_t>(base) & 15)) return false;
   const cuuint64_t dims[4] = {(cuuint64_t)size, (cuuint64_t)heads, (cuuint64_t)length, (cuuint64_t)batch};
+  const int unit = f32 ? 4 : 2;
   int64_t st[3] = {heads > 1 ? hs : 8, length > 1 ? ls : 8, batch > 1 ? bs : 8};
   for (int64_t x : st)
-    if (x <= 0 || x % 8 || x >= (int64_t(1) << 38)) return false;
-  const cuuint64_t strides[3] = {(cuuint64_t)st[0] * 2, (cuuint64_t)st[1] * 2, (cuuint64_t)st[2] * 2};
-  const cuuint32_t box[4] = {64, 1, BC, 1}, one[4] = {1, 1, 1, 1};
-  return enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+    if (x <= 0 || x * unit % 16 || x >= (int64_t(1) << 37)) return false;
+  const cuuint64_t strides[3] = {(cuuint64_t)st[0] * unit, (cuuint64_t)st[1] * unit, (cuuint64_t)st[2] * unit};
+  const cuuint32_t box[4] = {(cuuint32_t)(128 / unit), 1, BC, 1}, one[4] = {1, 1, 1, 1};
+  return enc(m, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 template <int DI> int walk_tc(Walk &w, unsigned char *work, cudaStream_t st) {
@@ -1191,6 +1266,8 @@ template <int DI> int walk_tc(Walk &w, unsigned char *work, cudaStream_t st) {
           map_of(&m.k, w.k, w.di, w.heads / w.k_div, w.length, w.batch, w.k_hs, w.k_ls, w.k_bs) &&
           map_of(&m.v, w.v, w.dout, w.heads / w.v_div, w.length, w.batch, w.v_hs, w.v_ls, w.v_bs) &&
           (!w.run || map_of(&m.x, w.x, w.dout, w.heads / w.x_div, w.length, w.batch, w.x_hs, w.x_ls, w.x_bs));
+  // float32 results take the room of v and x
+  m.tma_out = (!w.out_f32 || w.run) && map_of(&m.out, w.out, w.dout, w.heads, w.length, w.batch, w.o_hs, w.o_ls, w.o_bs, w.out_f32);
   return launch_walk(w, linattn_walk_tc_kernel<DI, OWN_STATE>, results, BT, own, all, work, st, m, tu);
 }
 int run_walk(int dtype, Walk &w, unsigned char *work, cudaStream_t st) {
