@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import re
+import struct as _struct
 from functools import lru_cache
 from pathlib import Path
 
@@ -95,6 +96,18 @@ def struct(name: str) -> type:
     return parse_header()[0][name]
 
 
+@lru_cache(maxsize=None)
+def packer(name: str):
+    """``pack(*values)`` -> bytes of an argument block, all its fields in the header's order (null pointers as 0).  For calls
+    whose time is a few microseconds: filling a ctypes structure costs as much as the kernel."""
+    code = {ctypes.c_int32: "i", ctypes.c_int64: "q", ctypes.c_uint32: "I", ctypes.c_float: "f", ctypes.c_void_p: "P"}
+    st = struct(name)
+    s = _struct.Struct("@" + "".join(code[t] for _, t in st._fields_) + "0q")
+    if s.size != ctypes.sizeof(st):
+        raise RuntimeError(f"{name}: packed size {s.size}, structure {ctypes.sizeof(st)}")
+    return s.pack
+
+
 def enum(name: str) -> int:
     return parse_header()[1][name]
 
@@ -169,9 +182,10 @@ def stream_of(t) -> int:
     return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
-def call(fn_name: str, args: ctypes.Structure, stream: int) -> None:
-    """Invoke an entry point; raise RuntimeError carrying the library's message on failure."""
-    rc = getattr(lib(), fn_name)(ctypes.byref(args), ctypes.c_void_p(stream))
+def call(fn_name: str, args, stream: int) -> None:
+    """Invoke an entry point with a structure or a packed block; raise RuntimeError carrying the library's message on failure."""
+    fn = getattr(_lib or lib(), fn_name)
+    rc = fn(args, stream) if type(args) is bytes else fn(ctypes.byref(args), ctypes.c_void_p(stream))
     if rc != 0:
         msg = lib().b200_last_error().decode(errors="replace")
         raise RuntimeError(f"{fn_name} failed (status {rc}): {msg}")

@@ -6,38 +6,40 @@ the order of their positions, so it is the same at every call, and rounds once.
 """
 from __future__ import annotations
 
-import ctypes
+import functools
 
 import torch
 
 from .. import _lib
-from .mamba_block import _DT, _stream
+from .mamba_block import _DT
 
 
-def _args(ids, features, classes, dtype, scale, padding_idx):
-    a = _lib.struct("b200_embed_args")()
-    a.tokens, a.features, a.classes = ids.numel(), features, classes
-    a.dtype, a.ids_wide = _lib.enum(_DT[dtype]), int(ids.dtype == torch.int64)
-    a.scale, a.padding_idx = scale, padding_idx
-    a.ids = ids.data_ptr()
-    return a
+@functools.lru_cache(maxsize=None)
+def _setup():
+    return _lib.packer("b200_embed_args"), {t: _lib.enum(n) for t, n in _DT.items()}
+
+
+def _lookup(ids, weight, scale, padding_idx):
+    """out, and the ids in a row"""
+    if weight.stride(1) != 1 or weight.stride(0) < weight.shape[1]:
+        weight = weight.contiguous()
+    flat = ids if ids.is_contiguous() else ids.contiguous()
+    classes, features = weight.shape
+    pack, codes = _setup()
+    with _lib.on_device(weight):
+        out = torch.empty(ids.shape + (features,), dtype=weight.dtype, device=weight.device)
+        _lib.call("b200_embed_fwd", pack(flat.numel(), padding_idx, classes, features, codes[weight.dtype], flat.dtype == torch.int64, scale, 0,
+                                         flat.data_ptr(), weight.data_ptr(), 0, out.data_ptr(), 0, weight.stride(0), features, 0, 0, 0, 0),
+                  _lib.stream_of(weight))
+    return out, flat
 
 
 class TokenEmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, weight, scale, padding_idx):
-        if weight.stride(1) != 1 or weight.stride(0) < weight.shape[1]:
-            weight = weight.contiguous()
-        flat = ids.reshape(-1).contiguous()
-        classes, features = weight.shape
-        with _lib.on_device(weight):
-            out = torch.empty(*ids.shape, features, dtype=weight.dtype, device=weight.device)
-            a = _args(flat, features, classes, weight.dtype, scale, padding_idx)
-            a.weight, a.out = weight.data_ptr(), out.data_ptr()
-            a.weight_rs, a.out_rs = weight.stride(0), features
-            _lib.call("b200_embed_fwd", a, _stream(weight))
+        out, flat = _lookup(ids, weight, scale, padding_idx)
         ctx.save_for_backward(flat)
-        ctx.meta = classes, scale, padding_idx
+        ctx.meta = weight.shape[0], scale, padding_idx
         return out
 
     @staticmethod
@@ -48,15 +50,14 @@ class TokenEmbeddingFn(torch.autograd.Function):
         dout = dout.reshape(-1, features)
         if dout.stride(1) != 1 and features > 1:
             dout = dout.contiguous()
+        pack, codes = _setup()
         with _lib.on_device(dout):
             dweight = torch.empty(classes, features, dtype=dout.dtype, device=dout.device)
-            a = _args(flat, features, classes, dout.dtype, scale, padding_idx)
-            a.dout, a.dweight = dout.data_ptr(), dweight.data_ptr()
-            a.dout_rs, a.dweight_rs = dout.stride(0), features
-            a.work_bytes = _lib.lib().b200_embed_bwd_work_bytes(ctypes.byref(a))
-            work = torch.empty(max(a.work_bytes, 1), dtype=torch.uint8, device=dout.device)
-            a.work = work.data_ptr()
-            _lib.call("b200_embed_bwd", a, _stream(dout))
+            head = (flat.numel(), padding_idx, classes, features, codes[dout.dtype], flat.dtype == torch.int64, scale, 0, flat.data_ptr(), 0, dout.data_ptr(), 0,
+                    dweight.data_ptr(), 0, 0, dout.stride(0), features)
+            work_bytes = _lib.lib().b200_embed_bwd_work_bytes(pack(*head, 0, 0))
+            work = torch.empty(max(work_bytes, 1), dtype=torch.uint8, device=dout.device)
+            _lib.call("b200_embed_bwd", pack(*head, work.data_ptr(), work_bytes), _lib.stream_of(dout))
             del work
         return None, dweight, None, None
 
@@ -79,4 +80,7 @@ def token_embedding(ids, weight, scale=1.0, padding_idx=None):
         padding_idx %= weight.shape[0]
     if ids.numel() == 0:
         return weight[:0].sum() + torch.empty(*ids.shape, weight.shape[1], dtype=weight.dtype, device=weight.device)
-    return TokenEmbeddingFn.apply(ids, weight, float(scale), -1 if padding_idx is None else padding_idx)
+    padding_idx = -1 if padding_idx is None else padding_idx
+    if weight.requires_grad and torch.is_grad_enabled():
+        return TokenEmbeddingFn.apply(ids, weight, float(scale), padding_idx)
+    return _lookup(ids, weight, scale, padding_idx)[0]

@@ -10,6 +10,7 @@ token in place, as ``selective_state_update`` does.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -49,6 +50,11 @@ def _work(a, name, like):
     work = torch.empty(a.work_bytes, dtype=torch.uint8, device=like.device)
     a.work = work.data_ptr()
     return work
+
+
+@functools.lru_cache(maxsize=None)
+def _step_setup():
+    return _lib.packer("b200_linattn_step_args"), {t: _lib.enum(n) for t, n in _DT.items()}
 
 
 class LinearAttentionFn(torch.autograd.Function):
@@ -158,25 +164,15 @@ def linear_attention_step(state, q, k, v, g, scale=1.0, state_batch_indices=None
           or state_batch_indices.device != q.device):
         raise RuntimeError("linear_attention_step: state_batch_indices must be a contiguous int32 tensor (batch,) on the device of q")
     q, k, v = _inner(q), _inner(k), _inner(v)
-    a = _lib.struct("b200_linattn_step_args")()
-    a.batch, a.groups, a.dk = q.shape
-    a.heads, a.dv, a.slots, a.scale = heads, dv, state.shape[0], scale
-    a.dtype, a.g_dtype, a.state_dtype = (_lib.enum(_DT[t.dtype]) for t in (q, g, state))
+    pack, codes = _step_setup()
+    sq, sk, sv, sg, ss = q.stride(), k.stride(), v.stride(), g.stride(), state.stride()
     with _lib.on_device(q):
         out = torch.empty(batch, heads, dv, dtype=v.dtype, device=v.device)
         if batch == 0:
             return out
-        a.state, a.q, a.k, a.v, a.g, a.out = (t.data_ptr() for t in (state, q, k, v, g, out))
-        if state_batch_indices is not None:
-            a.state_batch_indices = state_batch_indices.data_ptr()
-        a.state_bs, a.state_hs, a.state_ks, _ = state.stride()
-        a.q_bs, a.q_gs, _ = q.stride()
-        a.k_bs, a.k_gs, _ = k.stride()
-        a.v_bs, a.v_hs, _ = v.stride()
-        if g.dim() == 1:
-            a.g_hs = g.stride(0)
-        else:
-            a.g_bs, a.g_hs = g.stride()
-        a.out_bs, a.out_hs, _ = out.stride()
-        _lib.call("b200_linattn_step", a, _stream(q))
+        _lib.call("b200_linattn_step",
+                  pack(batch, heads, q.shape[1], q.shape[2], dv, codes[q.dtype], codes[g.dtype], codes[state.dtype], scale, state.shape[0], state.data_ptr(),
+                       q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), 0 if state_batch_indices is None else state_batch_indices.data_ptr(),
+                       out.data_ptr(), ss[0], ss[1], ss[2], sq[0], sq[1], sk[0], sk[1], sv[0], sv[1], sg[0] if g.dim() == 2 else 0, sg[-1], heads * dv, dv),
+                  _lib.stream_of(q))
     return out
