@@ -4,11 +4,12 @@
 //
 // Forward: a copy of rows, 16 bytes a thread; bound by HBM, and by the launch for the few tokens of a decoding step.
 // Backward: the (id, position) pairs are sorted by id, stably (least significant digit first, up to 9 bits a pass), so
-// that rows of one id are added in the order of their positions: no atomics, the same bits every time.  Every 32 sorted
-// pairs are a piece, whatever ids they hold, so a frequent token does not make one block slow: a thread block adds up the
-// runs of equal ids in its piece in float32 and writes a run that lies inside it; what a run crossing borders has in a piece goes to
-// the workspace and is joined by the piece where the run begins.  Each row is rounded once.  Ids outside [0, classes) and the padding id
-// sort behind all others and are not summed.
+// that rows of one id are added in the order of their positions: no atomics, the same bits every time.  One cluster of eight
+// thread blocks sorts, with its digit counts in distributed shared memory; the other SMs clear the gradient meanwhile.
+// Every 16 sorted pairs are a piece, whatever ids they hold, so a frequent token does not make one block slow: a thread
+// block adds up the runs of equal ids in its piece in float32 and writes a run that lies inside it; what a run crossing
+// borders has in a piece goes to the workspace and is joined by the piece where the run begins.  Each row is rounded
+// once.  Ids outside [0, classes) and the padding id sort behind all others and are not summed.
 #include "common.cuh"
 #include "dispatch.h"
 #include <cstring>
@@ -16,8 +17,8 @@
 namespace b200 {
 namespace {
 
-constexpr int PIECE = 32;             // sorted pairs a piece
-constexpr int SORT_T = 256, SORT_TILE = 2048, SORT_PER = SORT_TILE / SORT_T;
+constexpr int PIECE = 16;             // sorted pairs a piece
+constexpr int SORT_T = 1024, SORT_WARPS = SORT_T / 32, CLUSTER = 8;
 constexpr int MAX_BITS = 9, MAX_BINS = 1 << MAX_BITS;
 constexpr int ROW_T = 128;
 
@@ -75,33 +76,78 @@ __device__ __forceinline__ uint32_t key_of(const b200_embed_args &p, int64_t t) 
   return id >= 0 && id < p.classes && id != p.padding_idx ? (uint32_t)id : (uint32_t)p.classes;
 }
 
-// Digit counts of a tile, digit-major (the scan over all of them gives each tile's place for each digit).
-__global__ void __launch_bounds__(SORT_T) embed_count_kernel(const b200_embed_args p, const uint32_t *keys, int shift, int bits, uint32_t *hist) {
-  __shared__ uint32_t h[MAX_BINS];
-  const int bins = 1 << bits;
-  for (int i = threadIdx.x; i < bins; i += SORT_T) h[i] = 0;
-  __syncthreads();
-  const int64_t t0 = (int64_t)blockIdx.x * SORT_TILE;
-#pragma unroll
-  for (int i = 0; i < SORT_PER; ++i) {
-    const int64_t t = t0 + i * SORT_T + threadIdx.x;
-    if (t < p.tokens) atomicAdd(&h[((keys ? keys[t] : key_of(p, t)) >> shift) & (bins - 1)], 1u);
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < bins; i += SORT_T) hist[(int64_t)i * gridDim.x + blockIdx.x] = h[i];
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// a word of another block's shared memory, at the place of `p` in this one's
+__device__ __forceinline__ uint32_t peer_word(const uint32_t *p, int rank) {
+  uint32_t at, v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+  return v;
 }
 
-// Exclusive sums of n counts by one block.
-__global__ void __launch_bounds__(1024) embed_scan_kernel(uint32_t *x, int64_t n) {
-  __shared__ uint32_t ws[32];
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  uint32_t carry = 0;
-  for (int64_t i0 = 0; i0 < n; i0 += 4096) {
-    const int64_t i = i0 + threadIdx.x * 4;
-    uint32_t v[4], s = 0;
+struct SortArgs {
+  uint32_t *keys[2], *pos[2];
+  int passes, bits;
+};
+
+// The first cluster sorts: each warp has a run of the pairs, counts the digits of 32 at a time by comparing lanes, and places
+// them by the same comparison once it knows where each of its digits begins (pairs are read twice, and nothing is kept, so
+// that any number of them will do).  The blocks of the other clusters clear the gradient.
+__global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(SORT_T) embed_sort_kernel(const b200_embed_args p, const SortArgs q, int esz) {
+  extern __shared__ uint32_t cnt[];                              // (warps, bins)
+  __shared__ uint32_t total[MAX_BINS], base[MAX_BINS], ws[32];
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, bins = 1 << q.bits;
+  if (blockIdx.x >= CLUSTER) {
+    const int64_t bytes = (int64_t)p.classes * p.features * esz, words = bytes / 16;
+    uint4 *dw = reinterpret_cast<uint4 *>(p.dweight);            // as torch allocates: 16-byte aligned (checked)
+    const int64_t step = (int64_t)(gridDim.x - CLUSTER) * SORT_T;
+    const int64_t first = (int64_t)(blockIdx.x - CLUSTER) * SORT_T + tid;
+    for (int64_t i = first; i < words; i += step) dw[i] = make_uint4(0, 0, 0, 0);
+    for (int64_t i = words * 16 + first; i < bytes; i += step) reinterpret_cast<unsigned char *>(p.dweight)[i] = 0;
+    return;
+  }
+  const int rank = blockIdx.x;
+  const int64_t per = (p.tokens + CLUSTER * SORT_WARPS * 32 - 1) / (CLUSTER * SORT_WARPS * 32) * 32;     // pairs a warp
+  const int64_t t0 = ((int64_t)rank * SORT_WARPS + w) * per, t1 = min(p.tokens, t0 + per);
+  for (int pass = 0; pass < q.passes; ++pass) {
+    const uint32_t *keys = pass ? q.keys[(pass - 1) & 1] : nullptr, *pos = pass ? q.pos[(pass - 1) & 1] : nullptr;
+    uint32_t *keys_out = q.keys[pass & 1], *pos_out = q.pos[pass & 1];
+    const int shift = pass * q.bits;
+    uint32_t *mine = cnt + w * bins;
+    for (int i = lane; i < bins; i += 32) mine[i] = 0;
+    __syncwarp();
+    const auto key_at = [&](int64_t t) { return t < t1 ? (keys ? __ldcg(keys + t) : key_of(p, t)) : 0u; };
+    for (int64_t i = t0; i < t1; i += 32) {
+      const int64_t t = i + lane;
+      const uint32_t d = t < t1 ? (key_at(t) >> shift) & (bins - 1) : 0xffffffffu;
+      const uint32_t peers = __match_any_sync(0xffffffffu, d);
+      if (t < t1 && (peers >> lane) == 1u) mine[d] += __popc(peers);      // the last of the equal lanes
+      __syncwarp();
+    }
+    __syncthreads();
+    if (tid < bins) {
+      uint32_t s = 0;
+#pragma unroll 8
+      for (int j = 0; j < SORT_WARPS; ++j) {
+        const uint32_t c = cnt[j * bins + tid];
+        cnt[j * bins + tid] = s;
+        s += c;
+      }
+      total[tid] = s;
+    }
+    cluster_sync();
+    uint32_t before = 0, all = 0;
+    if (tid < bins) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) { v[j] = i + j < n ? x[i + j] : 0; s += v[j]; }
-    uint32_t inc = s;
+      for (int j = 0; j < CLUSTER; ++j) {
+        const uint32_t c = peer_word(&total[tid], j);
+        before += j < rank ? c : 0;
+        all += c;
+      }
+    }
+    uint32_t inc = all;                                          // exclusive sums over the bins
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const uint32_t u = __shfl_up_sync(0xffffffffu, inc, o);
@@ -109,52 +155,25 @@ __global__ void __launch_bounds__(1024) embed_scan_kernel(uint32_t *x, int64_t n
     }
     if (lane == 31) ws[w] = inc;
     __syncthreads();
-    uint32_t before = 0, all = 0;
-    for (int j = 0; j < 32; ++j) { const uint32_t u = ws[j]; before += j < w ? u : 0; all += u; }
-    uint32_t e = carry + before + inc - s;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) { if (i + j < n) x[i + j] = e; e += v[j]; }
-    carry += all;
-    __syncthreads();
-  }
-}
-
-// Stable placement: a warp takes 256 consecutive pairs, 32 at a time, and counts what it has placed of each digit.
-__global__ void __launch_bounds__(SORT_T) embed_place_kernel(const b200_embed_args p, const uint32_t *keys, const uint32_t *pos, int shift, int bits,
-                                                            const uint32_t *hist, uint32_t *keys_out, uint32_t *pos_out) {
-  __shared__ uint32_t cnt[SORT_T / 32][MAX_BINS];
-  const int bins = 1 << bits, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  for (int i = threadIdx.x; i < bins * (SORT_T / 32); i += SORT_T) cnt[i >> bits][i & (bins - 1)] = 0;
-  __syncthreads();
-  const int64_t t0 = (int64_t)blockIdx.x * SORT_TILE + w * (SORT_PER * 32);
-  uint32_t k[SORT_PER], at[SORT_PER];
-#pragma unroll
-  for (int i = 0; i < SORT_PER; ++i) {
-    const int64_t t = t0 + i * 32 + lane;
-    const bool in = t < p.tokens;
-    k[i] = in ? (keys ? keys[t] : key_of(p, t)) : 0;
-    const uint32_t d = in ? (k[i] >> shift) & (bins - 1) : 0xffffffffu;
-    const uint32_t peers = __match_any_sync(0xffffffffu, d);
-    const uint32_t before = in ? cnt[w][d] : 0;
-    __syncwarp();
-    if (in && (peers >> lane) == 1u) cnt[w][d] = before + __popc(peers);        // the last of the equal lanes
-    __syncwarp();
-    at[i] = before + __popc(peers & ((1u << lane) - 1));
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < bins; i += SORT_T) {
-    uint32_t s = hist[(int64_t)i * gridDim.x + blockIdx.x];
-    for (int j = 0; j < SORT_T / 32; ++j) { const uint32_t c = cnt[j][i]; cnt[j][i] = s; s += c; }
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < SORT_PER; ++i) {
-    const int64_t t = t0 + i * 32 + lane;
-    if (t < p.tokens) {
-      const uint32_t o = cnt[w][(k[i] >> shift) & (bins - 1)] + at[i];
-      keys_out[o] = k[i];
-      pos_out[o] = pos ? pos[t] : (uint32_t)t;
+    uint32_t lower = 0;
+    for (int j = 0; j < w; ++j) lower += ws[j];
+    if (tid < bins) base[tid] = lower + inc - all + before;
+    cluster_sync();                                              // counts have been read
+    for (int64_t i = t0; i < t1; i += 32) {
+      const int64_t t = i + lane;
+      const uint32_t key = key_at(t);
+      const uint32_t d = t < t1 ? (key >> shift) & (bins - 1) : 0xffffffffu;
+      const uint32_t peers = __match_any_sync(0xffffffffu, d);
+      if (t < t1) {
+        const uint32_t o = base[d] + mine[d] + __popc(peers & ((1u << lane) - 1));
+        keys_out[o] = key;
+        pos_out[o] = pos ? __ldcg(pos + t) : (uint32_t)t;
+      }
+      __syncwarp();
+      if (t < t1 && (peers >> lane) == 1u) mine[d] += __popc(peers);
+      __syncwarp();
     }
+    cluster_sync();                                              // places are written, and visible to the cluster
   }
 }
 
@@ -212,9 +231,10 @@ __global__ void __launch_bounds__(ROW_T) embed_sum_kernel(const b200_embed_args 
 }
 
 // The runs that cross borders: the piece where one begins adds up its parts, eight interleaved shares of them.
+constexpr int JOIN_C = 128;                 // columns a block
 template <typename T>
 __global__ void __launch_bounds__(256) embed_join_kernel(const b200_embed_args p, const uint32_t *keys, const float *head, const float *tail, int pieces) {
-  __shared__ float sh[8][32];
+  __shared__ float sh[8][JOIN_C];
   __shared__ int ends;
   const int piece = blockIdx.x;
   const int64_t last = (int64_t)piece * PIECE + PIECE - 1;              // of this piece
@@ -222,10 +242,11 @@ __global__ void __launch_bounds__(256) embed_join_kernel(const b200_embed_args p
   const uint32_t key = keys[last];
   if (key >= (uint32_t)p.classes || keys[last + 1] != key) return;      // nothing goes on
   const int64_t first = (int64_t)piece * PIECE;
-  if (first > 0 && keys[first - 1] == key) return;                      // it began earlier
+  if (first > 0 && keys[first - 1] == key && keys[first] == key) return;      // it began earlier
   // the piece that the run ends in: the last whose entry border still has the key
   if (threadIdx.x == 0) {
     int lo = piece + 1, hi = pieces - 1;                                // keys are sorted
+    if (lo < hi && keys[(int64_t)(lo + 1) * PIECE] != key) hi = lo;
     while (lo < hi) {
       const int mid = (lo + hi + 1) / 2;
       if (keys[(int64_t)mid * PIECE] == key) lo = mid;
@@ -234,23 +255,29 @@ __global__ void __launch_bounds__(256) embed_join_kernel(const b200_embed_args p
     ends = lo;
   }
   __syncthreads();
-  const int to = ends, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  for (int c0 = 0; c0 < p.features; c0 += 32) {
-    const int c = c0 + lane;
-    float s = 0.f;
-    if (c < p.features) {
-      if (w == 0) s = tail[(int64_t)piece * p.features + c];
-#pragma unroll 4
-      for (int i = piece + 1 + w; i <= to; i += 8) s += head[(int64_t)i * p.features + c];
-    }
-    sh[w][lane] = s;
-    __syncthreads();
-    if (w == 0 && c < p.features) {
+  const int to = ends, lane = threadIdx.x & 31, w = threadIdx.x >> 5, c0 = blockIdx.y * JOIN_C;
+  float s[JOIN_C / 32];
 #pragma unroll
-      for (int i = 1; i < 8; ++i) s += sh[i][lane];
-      reinterpret_cast<T *>(p.dweight)[(int64_t)key * p.dweight_rs + c] = T(s * p.scale);
+  for (int j = 0; j < JOIN_C / 32; ++j) {
+    const int c = c0 + j * 32 + lane;
+    s[j] = w == 0 && c < p.features ? tail[(int64_t)piece * p.features + c] : 0.f;
+  }
+#pragma unroll 4
+  for (int i = piece + 1 + w; i <= to; i += 8)
+#pragma unroll
+    for (int j = 0; j < JOIN_C / 32; ++j) {
+      const int c = c0 + j * 32 + lane;
+      if (c < p.features) s[j] += head[(int64_t)i * p.features + c];
     }
-    __syncthreads();
+#pragma unroll
+  for (int j = 0; j < JOIN_C / 32; ++j) sh[w][j * 32 + lane] = s[j];
+  __syncthreads();
+  const int c = c0 + threadIdx.x;
+  if (threadIdx.x < JOIN_C && c < p.features) {
+    float x = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x += sh[i][threadIdx.x];
+    reinterpret_cast<T *>(p.dweight)[(int64_t)key * p.dweight_rs + c] = T(x * p.scale);
   }
 }
 
@@ -258,7 +285,7 @@ __global__ void __launch_bounds__(256) embed_join_kernel(const b200_embed_args p
 
 int64_t up(int64_t n, int64_t unit) { return (n + unit - 1) / unit * unit; }
 
-struct Sort { int passes, bits; int64_t tiles, pieces; };
+struct Sort { int passes, bits; int64_t pieces; };
 
 Sort sort_of(const b200_embed_args &a) {
   Sort s;
@@ -266,15 +293,14 @@ Sort sort_of(const b200_embed_args &a) {
   while ((int64_t(1) << width) <= a.classes) ++width;           // keys reach classes
   s.passes = (width + MAX_BITS - 1) / MAX_BITS;
   s.bits = (width + s.passes - 1) / s.passes;
-  s.tiles = (a.tokens + SORT_TILE - 1) / SORT_TILE;
   s.pieces = (a.tokens + PIECE - 1) / PIECE;
   return s;
 }
 
 int check_embed(const b200_embed_args &a, bool bwd) {
   B200_REQUIRE(a.ids && (bwd ? a.dout && a.dweight : a.weight && a.out), B200_ERR_NULL, "embed: null operand");
-  B200_REQUIRE(a.tokens > 0 && a.classes > 0 && a.features > 0 && a.tokens < (int64_t(1) << 31) - SORT_TILE && a.classes < (1 << 30), B200_ERR_SHAPE,
-               "embed: sizes must be positive and tokens below 2^31 (tokens %lld, classes %d, features %d)", (long long)a.tokens, a.classes, a.features);
+  B200_REQUIRE(a.tokens > 0 && a.classes > 0 && a.features > 0 && a.tokens < (int64_t(1) << 30) && a.classes < (1 << 30), B200_ERR_SHAPE,
+               "embed: sizes must be positive and tokens below 2^30 (tokens %lld, classes %d, features %d)", (long long)a.tokens, a.classes, a.features);
   B200_REQUIRE(a.dtype == B200_F32 || a.dtype == B200_F16 || a.dtype == B200_BF16, B200_ERR_DTYPE, "embed: unknown dtype %d", a.dtype);
   return 0;
 }
@@ -298,7 +324,7 @@ template <typename T> int run_sums(const b200_embed_args &a, const Sort &s, cons
   if (vec) embed_sum_kernel<T, V><<<grid, ROW_T, 0, st>>>(a, keys, pos, head, tail);
   else embed_sum_kernel<T, 1><<<grid, ROW_T, 0, st>>>(a, keys, pos, head, tail);
   if (int e = launch_status()) return e;
-  if (s.pieces > 1) embed_join_kernel<T><<<(unsigned)s.pieces, 256, 0, st>>>(a, keys, head, tail, (int)s.pieces);
+  if (s.pieces > 1) embed_join_kernel<T><<<dim3((unsigned)s.pieces, (unsigned)((a.features + JOIN_C - 1) / JOIN_C)), 256, 0, st>>>(a, keys, head, tail, (int)s.pieces);
   return launch_status();
 }
 
@@ -318,7 +344,7 @@ extern "C" int b200_embed_fwd(const b200_embed_args *args, void *stream) {
 extern "C" int64_t b200_embed_bwd_work_bytes(const b200_embed_args *args) {
   if (!args || check_embed(*args, true)) return 0;
   const Sort s = sort_of(*args);
-  return 4 * up(4 * args->tokens, 256) + up(4 * (s.tiles << s.bits), 256) + 2 * up(4 * s.pieces * args->features, 256);
+  return 4 * up(4 * args->tokens, 256) + 2 * up(4 * s.pieces * args->features, 256);
 }
 
 extern "C" int b200_embed_bwd(const b200_embed_args *args, void *stream) {
@@ -330,26 +356,29 @@ extern "C" int b200_embed_bwd(const b200_embed_args *args, void *stream) {
   B200_REQUIRE(a.work_bytes >= b200_embed_bwd_work_bytes(args), B200_ERR_TOO_LARGE, "embed_bwd: work has %lld bytes, %lld are needed", (long long)a.work_bytes,
                (long long)b200_embed_bwd_work_bytes(args));
   B200_REQUIRE(a.dweight_rs == a.features, B200_ERR_SHAPE, "embed_bwd: dweight must be dense");
+  B200_REQUIRE((reinterpret_cast<uintptr_t>(a.dweight) & 15) == 0, B200_ERR_ALIGN, "embed_bwd: dweight must be 16-byte aligned");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const Sort s = sort_of(a);
   unsigned char *w = reinterpret_cast<unsigned char *>(a.work);
   const int64_t arr = up(4 * a.tokens, 256);
-  uint32_t *keys[2] = {reinterpret_cast<uint32_t *>(w), reinterpret_cast<uint32_t *>(w + arr)};
-  uint32_t *pos[2] = {reinterpret_cast<uint32_t *>(w + 2 * arr), reinterpret_cast<uint32_t *>(w + 3 * arr)};
-  uint32_t *hist = reinterpret_cast<uint32_t *>(w + 4 * arr);
-  float *head = reinterpret_cast<float *>(w + 4 * arr + up(4 * (s.tiles << s.bits), 256));
-  float *tail = head + up(4 * s.pieces * a.features, 256) / 4;
-  cudaError_t ce = cudaMemsetAsync(a.dweight, 0, (size_t)a.classes * a.features * act_size(a.dtype), st);
-  if (ce != cudaSuccess) { set_error("cudaMemsetAsync: %s", cudaGetErrorString(ce)); return (int)ce; }
-  const uint32_t *k = nullptr, *q = nullptr;
-  for (int i = 0; i < s.passes; ++i) {
-    embed_count_kernel<<<(unsigned)s.tiles, SORT_T, 0, st>>>(a, k, i * s.bits, s.bits, hist);
-    embed_scan_kernel<<<1, 1024, 0, st>>>(hist, s.tiles << s.bits);
-    embed_place_kernel<<<(unsigned)s.tiles, SORT_T, 0, st>>>(a, k, q, i * s.bits, s.bits, hist, keys[i & 1], pos[i & 1]);
-    if (int e = launch_status()) return e;
-    k = keys[i & 1];
-    q = pos[i & 1];
+  SortArgs q;
+  for (int i = 0; i < 2; ++i) {
+    q.keys[i] = reinterpret_cast<uint32_t *>(w + i * arr);
+    q.pos[i] = reinterpret_cast<uint32_t *>(w + (2 + i) * arr);
   }
-  if (a.dtype == B200_F32) return run_sums<float>(a, s, k, q, head, tail, st);
-  return a.dtype == B200_F16 ? run_sums<__half>(a, s, k, q, head, tail, st) : run_sums<__nv_bfloat16>(a, s, k, q, head, tail, st);
+  q.passes = s.passes;
+  q.bits = s.bits;
+  float *head = reinterpret_cast<float *>(w + 4 * arr);
+  float *tail = head + up(4 * s.pieces * a.features, 256) / 4;
+  const int smem = 4 * SORT_WARPS << s.bits, esz = act_size(a.dtype);
+  cudaError_t ce = cudaFuncSetAttribute(embed_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (ce != cudaSuccess) { set_error("cudaFuncSetAttribute: %s", cudaGetErrorString(ce)); return (int)ce; }
+  // a cluster to sort, and clusters that clear: about one a GPC's worth of SMs, fewer where there is little to clear
+  int64_t clear = ((int64_t)a.classes * a.features * esz / 16 + SORT_T * CLUSTER - 1) / (SORT_T * CLUSTER), most = sm_count_current() / CLUSTER - 1;
+  clear = clear < most ? clear : most;
+  embed_sort_kernel<<<(unsigned)(CLUSTER * (1 + (clear > 0 ? clear : 1))), SORT_T, smem, st>>>(a, q, esz);
+  if (int e = launch_status()) return e;
+  const uint32_t *k = q.keys[(s.passes - 1) & 1], *at = q.pos[(s.passes - 1) & 1];
+  if (a.dtype == B200_F32) return run_sums<float>(a, s, k, at, head, tail, st);
+  return a.dtype == B200_F16 ? run_sums<__half>(a, s, k, at, head, tail, st) : run_sums<__nv_bfloat16>(a, s, k, at, head, tail, st);
 }
