@@ -42,7 +42,8 @@ constexpr int LCE_THREADS = 384;                 // 4 warps that issue, 8 that e
 constexpr int LCE_SMEM = NST * ST_BYTES + 8 * STAGING + 1024;
 constexpr uint32_t LCE_WAIT = 1u << 24;
 constexpr int64_t kPieceBytes = int64_t(1) << 30;
-constexpr int kSegSteps = 16;                    // float32 only: stages (of 64) in one accumulation chain's leading product
+constexpr int kSegSteps = 8;              // float32 only: stages (of 64) in one accumulation chain of the leading product
+constexpr int kMaxSplits = 32;            // blocks that share the contraction of a tile
 
 enum { EPI_LSE = 0, EPI_DZ = 1, EPI_OUT = 2 };
 
@@ -69,6 +70,7 @@ struct LceGemm {
   void *dst;
   int64_t dst_rs;
   int add, last;               // OUT: acc holds earlier pieces; this is the last one
+  int splits, per;             // OUT: blocks that share a tile's contraction, and their stages; each has its sums at acc + split rows acc_rs
 };
 
 __device__ __forceinline__ void tma_st_3d(const CUtensorMap *map, const void *src, int x, int y, int z) {
@@ -163,7 +165,7 @@ __global__ void __launch_bounds__(LCE_THREADS, 1) lce_gemm_kernel(const __grid_c
   unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ LcePipe pipe;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int tiles = p.mt * p.nt;
+  const int tiles = p.mt * p.nt * (EPI == EPI_OUT ? p.splits : 1);
   if (tid == 0) {
     for (int s = 0; s < NST; ++s) {
       mbar_init(&pipe.full[s], 1);
@@ -186,8 +188,11 @@ __global__ void __launch_bounds__(LCE_THREADS, 1) lce_gemm_kernel(const __grid_c
   tc_fence_after();
   const uint32_t tmem = pipe.tmem_base;
   // z and dz: neighbouring blocks share W's tile; products of dz: they share dz's
-  const auto m_of = [&](int t) { return EPI == EPI_OUT ? t / p.nt : t % p.mt; };
+  const auto m_of = [&](int t) { return EPI == EPI_OUT ? t / p.nt % p.mt : t % p.mt; };
   const auto n_of = [&](int t) { return EPI == EPI_OUT ? t % p.nt : t / p.mt; };
+  // the stages of a block's part of the contraction
+  const auto k_from = [&](int t) { return EPI == EPI_OUT ? t / (p.nt * p.mt) * p.per : 0; };
+  const auto k_to = [&](int t) { return EPI == EPI_OUT ? min(p.nk, k_from(t) + p.per) : p.nk; };
 
   if (warp == 0 && lane == 0) {
     // ------------------------------------------------------------------ loads
@@ -195,8 +200,9 @@ __global__ void __launch_bounds__(LCE_THREADS, 1) lce_gemm_kernel(const __grid_c
     bool ok = true;
     for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
       const int m0 = m_of(t) * TM, n0 = n_of(t) * TN;
-      for (int k0 = 0; k0 < p.nk && ok; k0 += p.seg) {
-        const int k1 = min(p.nk, k0 + p.seg);
+      const int ke = k_to(t);
+      for (int k0 = k_from(t); k0 < ke && ok; k0 += p.seg) {
+        const int k1 = min(ke, k0 + p.seg);
         for (int ps = 0; ps < p.passes && ok; ++ps) {
           const int pa = plane_a(p.passes, ps), pb = plane_b(p.passes, ps);
           for (int k = k0; k < k1; ++k, ++g) {
@@ -231,8 +237,9 @@ __global__ void __launch_bounds__(LCE_THREADS, 1) lce_gemm_kernel(const __grid_c
     const uint32_t a_lbo = p.a_mn ? 8192 : 16, b_lbo = p.b_mn ? 8192 : 16;
     const uint32_t a_step = p.a_mn ? 2048 : 32, b_step = p.b_mn ? 2048 : 32;      // bytes to the next 16 of the contraction
     for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-      for (int k0 = 0; k0 < p.nk && ok; k0 += p.seg, ++ch) {
-        const int n = (min(p.nk, k0 + p.seg) - k0) * p.passes;
+      const int ke = k_to(t);
+      for (int k0 = k_from(t); k0 < ke && ok; k0 += p.seg, ++ch) {
+        const int n = (min(ke, k0 + p.seg) - k0) * p.passes;
         const uint32_t d = tmem + (ch & 1) * TN;
         if (ch >= 2 && !mbar_wait(&pipe.acc_empty[ch & 1], ((ch >> 1) - 1) & 1, LCE_WAIT)) { ok = false; break; }
         tc_fence_after();
@@ -260,7 +267,8 @@ __global__ void __launch_bounds__(LCE_THREADS, 1) lce_gemm_kernel(const __grid_c
       const int m0 = m_of(t) * TM, n0 = n_of(t) * TN;
       const int row = m0 + q * 32 + lane, c0 = n0 + half * (TN / 2);      // this thread's row and 128 columns
       const bool in = row < p.rows;
-      for (int k0 = 0; k0 < p.nk; k0 += p.seg, ++ch) {
+      const int kb = k_from(t), ke = k_to(t);
+      for (int k0 = kb; k0 < ke; k0 += p.seg, ++ch) {
         // what the epilogue needs besides is loaded before the wait
         float lse2 = 0.f, sc = 0.f;
         int at = -1;                                                     // the label's column within this thread's columns
@@ -291,8 +299,9 @@ __global__ void __launch_bounds__(LCE_THREADS, 1) lce_gemm_kernel(const __grid_c
               for (int j = 0; j < 32; ++j) v[j] = j < left ? v[j] : -INFINITY;
             }
             if ((at >> 5) == c) {
+              const uint32_t one = 1u << (at & 31);                       // (an index into v would put all of it into memory)
 #pragma unroll
-              for (int j = 0; j < 32; ++j) target = j == (at & 31) ? v[j] : target;
+              for (int j = 0; j < 32; ++j) target = one & (1u << j) ? v[j] : target;
             }
             float vm = v[0];
 #pragma unroll
@@ -345,7 +354,8 @@ __global__ void __launch_bounds__(LCE_THREADS, 1) lce_gemm_kernel(const __grid_c
           __syncwarp();
           if (lane == 0) mbar_arrive(&pipe.acc_empty[ch & 1]);
         } else {
-          const bool first = k0 == 0 && !p.add, last = k0 + p.seg >= p.nk && p.last;
+          const bool first = k0 == kb && !p.add, last = k0 + p.seg >= ke && p.last;
+          float *acc = p.acc + (int64_t)(t / (p.nt * p.mt)) * p.rows * p.acc_rs;
           const float unit = unit_of(p.common);
           const bool vec = (p.dst_rs * (p.dtype == B200_F32 ? 4 : 2)) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.dst) & 15) == 0;
 #pragma unroll 1
@@ -356,7 +366,7 @@ __global__ void __launch_bounds__(LCE_THREADS, 1) lce_gemm_kernel(const __grid_c
             const int col = c0 + c * 32, n = min(32, p.cols - col);
             if (!in || n <= 0) continue;
             if (!first) {
-              const float4 *o = reinterpret_cast<const float4 *>(p.acc + (int64_t)row * p.acc_rs + col);
+              const float4 *o = reinterpret_cast<const float4 *>(acc + (int64_t)row * p.acc_rs + col);
 #pragma unroll
               for (int j = 0; j < 8; ++j)
                 if (4 * j < n) {
@@ -368,7 +378,7 @@ __global__ void __launch_bounds__(LCE_THREADS, 1) lce_gemm_kernel(const __grid_c
                 }
             }
             if (!last) {
-              float4 *o = reinterpret_cast<float4 *>(p.acc + (int64_t)row * p.acc_rs + col);
+              float4 *o = reinterpret_cast<float4 *>(acc + (int64_t)row * p.acc_rs + col);
 #pragma unroll
               for (int j = 0; j < 8; ++j)
                 if (4 * j < n) o[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
@@ -500,6 +510,31 @@ __global__ void __launch_bounds__(256) lce_scale_kernel(const float *dloss, int 
   if ((threadIdx.x & 31) == 0 && m) atomicMax(common, m);
 }
 
+// The blocks' parts of a product, added up in their order, scaled and rounded.
+__global__ void __launch_bounds__(256) lce_fold_kernel(const float *acc, int splits, int64_t rows, int cols, int64_t acc_rs, const float *common, int dtype, void *dst,
+                                                      int64_t dst_rs) {
+  const int64_t n = rows * (acc_rs / 4), plane = rows * acc_rs;
+  const float unit = unit_of(common);
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / (acc_rs / 4);
+    const int c = (int)(i - r * (acc_rs / 4)) * 4;
+    const float *a = acc + r * acc_rs + c;
+    float4 s = *reinterpret_cast<const float4 *>(a);
+#pragma unroll 4
+    for (int k = 1; k < splits; ++k) {
+      const float4 w = *reinterpret_cast<const float4 *>(a + k * plane);
+      s.x += w.x;
+      s.y += w.y;
+      s.z += w.z;
+      s.w += w.w;
+    }
+    const float v[4] = {s.x * unit, s.y * unit, s.z * unit, s.w * unit};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (c + j < cols) st_act(dst, dtype, r * dst_rs + c + j, v[j]);
+  }
+}
+
 // ------------------------------------------------------------------------------------------------ host
 
 int64_t up(int64_t n, int64_t unit) { return (n + unit - 1) / unit * unit; }
@@ -524,7 +559,23 @@ struct Plan {
   int64_t dz_pitch, dz_bytes, acc_h_bytes, acc_w_bytes;
   int64_t Da;                     // pitch of the float32 sums
   int seg;
+  int splits_h, per_h, splits_w, per_w;
 };
+
+// How many blocks share the contraction of `stages` for each of `tiles` tiles: as few as fill the SMs (at least 8 stages
+// each, to be worth 128 KB of sums).
+void split_of(int64_t tiles, int stages, int &splits, int &per) {
+  const int64_t sms = sm_count_current();
+  splits = 1;
+  per = stages;
+  int64_t best = (tiles + sms - 1) / sms * stages;
+  for (int s = 2; s <= kMaxSplits && stages / s >= 8 && tiles * (s - 1) < sms; ++s) {
+    const int p = (stages + s - 1) / s;
+    if ((int64_t)(s - 1) * p >= stages) continue;
+    const int64_t cost = (tiles * s + sms - 1) / sms * p;
+    if (cost * 100 < best * 90) { best = cost; splits = s; per = p; }
+  }
+}
 
 bool in_place(const void *p, int64_t rs, int cols) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && rs % 8 == 0 && rs >= cols && rs < (int64_t(1) << 36);
@@ -548,9 +599,12 @@ Plan plan_of(const b200_lce_args &a) {
   q.n_pieces = (a.classes + q.piece - 1) / q.piece;
   q.dz_pitch = q.piece;
   q.dz_bytes = up(2 * q.planes * a.rows * q.dz_pitch, 256);
-  // float32 sums: of dH over the pieces and the chains, of dW over the chains
-  q.acc_h_bytes = f32 || q.n_pieces > 1 ? up(4 * a.rows * q.Da, 256) : 0;
-  q.acc_w_bytes = f32 && (a.rows + TK - 1) / TK > q.seg ? up(4 * (int64_t)q.piece * q.Da, 256) : 0;
+  const int64_t dt = (a.features + TN - 1) / TN;
+  split_of((a.rows + TM - 1) / TM * dt, (q.piece + TK - 1) / TK, q.splits_h, q.per_h);
+  split_of((q.piece + TM - 1) / TM * dt, (int)((a.rows + TK - 1) / TK), q.splits_w, q.per_w);
+  // float32 sums: of dH over the pieces, the chains and the blocks that share a tile, of dW over the chains and blocks
+  q.acc_h_bytes = f32 || q.n_pieces > 1 || q.splits_h > 1 ? up(4 * q.splits_h * a.rows * q.Da, 256) : 0;
+  q.acc_w_bytes = q.splits_w > 1 || (f32 && (a.rows + TK - 1) / TK > q.seg) ? up(4 * q.splits_w * (int64_t)q.piece * q.Da, 256) : 0;
   return q;
 }
 
@@ -580,12 +634,18 @@ int pack(const void *src, int64_t rs, int64_t rows, const b200_lce_args &a, cons
 template <int EPI> int launch_gemm(const LceGemm &g, cudaStream_t st) {
   cudaError_t e = cudaFuncSetAttribute(lce_gemm_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, LCE_SMEM);
   if (e != cudaSuccess) { set_error("cudaFuncSetAttribute: %s", cudaGetErrorString(e)); return (int)e; }
-  const int tiles = g.mt * g.nt, sms = sm_count_current();
+  const int tiles = g.mt * g.nt * (EPI == EPI_OUT ? g.splits : 1), sms = sm_count_current();
   lce_gemm_kernel<EPI><<<(unsigned)(tiles < sms ? tiles : sms), LCE_THREADS, LCE_SMEM, st>>>(g);
   return launch_status();
 }
 
 uint32_t idesc_of(int dtype, bool a_mn, bool b_mn) { return idesc_f16(dtype == B200_F16 ? 0u : 1u, a_mn, b_mn, TM, TN); }
+
+int fold(const LceGemm &g, cudaStream_t st) {
+  const int64_t n = (int64_t)g.rows * (g.acc_rs / 4), most = (int64_t)sm_count_current() * 16, blocks = (n + 255) / 256;
+  lce_fold_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, st>>>(g.acc, g.splits, g.rows, g.cols, g.acc_rs, g.common, g.dtype, g.dst, g.dst_rs);
+  return launch_status();
+}
 
 struct Operands { const void *h, *w; int64_t h_pitch, w_pitch; };
 
@@ -723,6 +783,8 @@ extern "C" int b200_lce_bwd(const b200_lce_args *args, void *stream) {
       B200_REQUIRE(map16(&g.a, a.dtype, dz, cols, a.rows, q.dz_pitch, q.planes, TM) && map16(&g.b, a.dtype, o.w, a.features, a.classes, o.w_pitch, q.planes, 64),
                    B200_ERR_UNSUPPORTED, "lce: tensor-map encoding failed");
       g.nk = (cols + TK - 1) / TK;
+      g.splits = q.splits_h;                                     // of a shorter last piece some blocks have no part; their sums stay
+      g.per = q.per_h;
       if (g.seg > g.nk) g.seg = g.nk;
       g.a_mn = 0;
       g.bk_row0 = c0;
@@ -731,8 +793,10 @@ extern "C" int b200_lce_bwd(const b200_lce_args *args, void *stream) {
       g.dst = a.dhidden;
       g.dst_rs = a.dhidden_rs;
       g.add = pc > 0;
-      g.last = pc == q.n_pieces - 1;
+      g.last = pc == q.n_pieces - 1 && g.splits == 1;
       if (int e = launch_gemm<EPI_OUT>(g, st)) return e;
+      if (g.splits > 1 && pc == q.n_pieces - 1)
+        if (int e = fold(g, st)) return e;
     }
     if (a.dweight) {                                             // dz^T H: contraction over the rows
       B200_REQUIRE(map16(&g.a, a.dtype, dz, cols, a.rows, q.dz_pitch, q.planes, 64) && map16(&g.b, a.dtype, o.h, a.features, a.rows, o.h_pitch, q.planes, 64),
@@ -748,8 +812,12 @@ extern "C" int b200_lce_bwd(const b200_lce_args *args, void *stream) {
       g.dst = reinterpret_cast<unsigned char *>(a.dweight) + (int64_t)c0 * a.dweight_rs * esz;
       g.dst_rs = a.dweight_rs;
       g.add = 0;
-      g.last = 1;
+      g.splits = q.splits_w;
+      g.per = q.per_w;
+      g.last = g.splits == 1;
       if (int e = launch_gemm<EPI_OUT>(g, st)) return e;
+      if (g.splits > 1)
+        if (int e = fold(g, st)) return e;
     }
   }
   return 0;
