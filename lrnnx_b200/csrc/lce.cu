@@ -11,10 +11,13 @@
 // float16 dz neither overflows under a scaled loss nor vanishes under a mean over many rows; the products are scaled back
 // in 32 bits.  s_r = 0 (ignored labels) makes an exact zero row.
 //
-// The products run on tcgen05 with accumulators in TMEM, one kernel with three epilogues.  Persistent thread blocks take
-// tiles in turn: warp 0 issues TMA loads into a 4-stage ring (64 of the contraction a stage), warp 1 issues the MMAs,
-// warps 4-11 empty one of two 256-column accumulators while the other is filled.  Either operand may have the contraction
-// along its rows (z) or across them (dz W, dz^T H): both are 128-byte swizzled tiles, of K-major or of MN-major layout.
+// The products run on tcgen05 with accumulators in TMEM, one kernel with three epilogues.  Pairs of thread blocks
+// (cta_group::2) take tiles of 256 x 256 in turn, each block with its 128 rows of both operands: in each, warp 0 issues TMA
+// loads into a 6-stage ring (64 of the contraction a stage) and warps 4-11 empty one of two 256-column accumulators while
+// the other is filled; warp 1 of the first block issues the MMAs for both.  A single block's tile of 128 x 256 takes 96 bytes
+// a clock from L2 where a pair takes 64, and its MMAs waited for loads a quarter of the time (16384 x 50280 x 768: the
+// product with W 488 -> 456 us, 90 % of the tensor pipe's cycles; the forward 849 -> 844 us, 1.5 PFLOP/s).  Either operand may have the contraction along its rows (z) or across them (dz W, dz^T H): both are 128-byte
+// swizzled tiles, of K-major or of MN-major layout.
 //
 // float32 operands are split into three bfloat16 (8 bits of mantissa each) and multiplied as six products of the
 // planes, the small ones first; what is left out is below 2^-24.  The tensor core truncates when it adds into its
@@ -33,10 +36,10 @@ using namespace tc;
 
 __device__ int g_lce_status = 0;
 
-constexpr int TM = 128, TN = 256, TK = 64;       // tile of the result, contraction of a stage
-constexpr int NST = 4;
-constexpr int A_BYTES = TM * TK * 2, B_BYTES = TN * TK * 2;
-constexpr int ST_BYTES = A_BYTES + B_BYTES;      // 48 KB
+constexpr int TM = 128, TN = 256, TK = 64;       // a block's rows of the result, columns, contraction of a stage
+constexpr int NST = 6;
+constexpr int A_BYTES = TM * TK * 2, B_BYTES = TN / 2 * TK * 2;      // a block's half of the pair's operands
+constexpr int ST_BYTES = A_BYTES + B_BYTES;      // 32 KB
 constexpr int STAGING = 32 * 128;                // a warp's 32 rows x 64 columns of dz on their way out
 constexpr int LCE_THREADS = 384;                 // 4 warps that issue, 8 that empty accumulators
 constexpr int LCE_SMEM = NST * ST_BYTES + 8 * STAGING + 1024;
@@ -77,6 +80,39 @@ __device__ __forceinline__ void tma_st_3d(const CUtensorMap *map, const void *sr
   asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x),
                "r"(y), "r"(z), "r"(smem_u32(src))
                : "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// the first block's barrier at the place of `bar` in this one's shared memory
+__device__ __forceinline__ uint32_t of_first(const uint64_t *bar) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(bar)));
+  return a;
+}
+__device__ __forceinline__ void arrive_at(uint32_t bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+// a load into this block's shared memory that counts on a barrier of the pair
+__device__ __forceinline__ void tma_3d_pair(void *dst, const CUtensorMap *map, int x, int y, int z, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
+               "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// arrives at both blocks' barrier once the products issued so far are done
+__device__ __forceinline__ void commit_pair(uint64_t *bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
 }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -160,12 +196,13 @@ template <typename T> __device__ __forceinline__ void store_row16(T *dst, const 
 }
 
 template <int EPI>
-__global__ void __launch_bounds__(LCE_THREADS, 1) lce_gemm_kernel(const __grid_constant__ LceGemm p) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LCE_THREADS, 1) lce_gemm_kernel(const __grid_constant__ LceGemm p) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ LcePipe pipe;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int tiles = p.mt * p.nt * (EPI == EPI_OUT ? p.splits : 1);
+  const int tiles = p.mt * p.nt * (EPI == EPI_OUT ? p.splits : 1), pairs = gridDim.x >> 1, pair = blockIdx.x >> 1;
+  const int rank = (int)cluster_rank();
   if (tid == 0) {
     for (int s = 0; s < NST; ++s) {
       mbar_init(&pipe.full[s], 1);
@@ -173,18 +210,19 @@ __global__ void __launch_bounds__(LCE_THREADS, 1) lce_gemm_kernel(const __grid_c
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&pipe.acc_full[s], 1);
-      mbar_init(&pipe.acc_empty[s], 8);
+      mbar_init(&pipe.acc_empty[s], 16);               // the epilogue warps of both blocks
     }
     pipe.fail = 0;
     mbar_fence_init();
     fence_proxy_async();
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&pipe.tmem_base)), "r"(2 * TN) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&pipe.tmem_base)), "r"(2 * TN) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();
+  cluster_sync();                                      // the other block's barriers are set up
   tc_fence_after();
   const uint32_t tmem = pipe.tmem_base;
   // z and dz: neighbouring blocks share W's tile; products of dz: they share dz's
@@ -198,8 +236,8 @@ __global__ void __launch_bounds__(LCE_THREADS, 1) lce_gemm_kernel(const __grid_c
     // ------------------------------------------------------------------ loads
     int g = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-      const int m0 = m_of(t) * TM, n0 = n_of(t) * TN;
+    for (int t = pair; t < tiles && ok; t += pairs) {
+      const int m0 = (m_of(t) * 2 + rank) * TM, n0 = n_of(t) * TN + rank * (TN / 2);      // this block's halves
       const int ke = k_to(t);
       for (int k0 = k_from(t); k0 < ke && ok; k0 += p.seg) {
         const int k1 = min(ke, k0 + p.seg);
@@ -209,18 +247,19 @@ __global__ void __launch_bounds__(LCE_THREADS, 1) lce_gemm_kernel(const __grid_c
             const int s = g % NST;
             if (g >= NST && !mbar_wait(&pipe.empty[s], ((g / NST) - 1) & 1, LCE_WAIT)) { ok = false; break; }
             unsigned char *st = smem + (size_t)s * ST_BYTES;
-            mbar_expect_tx(&pipe.full[s], ST_BYTES);
+            const uint32_t full = of_first(&pipe.full[s]);
+            if (rank == 0) mbar_expect_tx(&pipe.full[s], 2 * ST_BYTES);      // of both blocks
             if (p.a_mn) {
 #pragma unroll
-              for (int j = 0; j < TM / 64; ++j) tma_3d(st + j * 8192, &p.a, m0 + 64 * j, k * TK, pa, &pipe.full[s]);
+              for (int j = 0; j < TM / 64; ++j) tma_3d_pair(st + j * 8192, &p.a, m0 + 64 * j, k * TK, pa, full);
             } else {
-              tma_3d(st, &p.a, k * TK, m0, pa, &pipe.full[s]);
+              tma_3d_pair(st, &p.a, k * TK, m0, pa, full);
             }
             if (p.b_mn) {
 #pragma unroll
-              for (int j = 0; j < TN / 64; ++j) tma_3d(st + A_BYTES + j * 8192, &p.b, n0 + 64 * j, p.bk_row0 + k * TK, pb, &pipe.full[s]);
+              for (int j = 0; j < TN / 128; ++j) tma_3d_pair(st + A_BYTES + j * 8192, &p.b, n0 + 64 * j, p.bk_row0 + k * TK, pb, full);
             } else {
-              tma_3d(st + A_BYTES, &p.b, k * TK, p.b_row0 + n0, pb, &pipe.full[s]);
+              tma_3d_pair(st + A_BYTES, &p.b, k * TK, p.b_row0 + n0, pb, full);
             }
           }
         }
@@ -228,15 +267,15 @@ __global__ void __launch_bounds__(LCE_THREADS, 1) lce_gemm_kernel(const __grid_c
     }
     if (!ok) {
       atomicExch(&pipe.fail, 1);
-      for (int i = max(0, g - NST); i < g; ++i) mbar_wait(&pipe.full[i % NST], (i / NST) & 1, 1u << 16);     // copies in flight
+      for (int i = 0; i < 1 << 12; ++i) __nanosleep(256);        // copies in flight: a millisecond, many times what they take
     }
-  } else if (warp == 1 && lane == 0) {
+  } else if (warp == 1 && lane == 0 && rank == 0) {
     // ------------------------------------------------------------------ products
     int g = 0, ch = 0;
     bool ok = true;
     const uint32_t a_lbo = p.a_mn ? 8192 : 16, b_lbo = p.b_mn ? 8192 : 16;
     const uint32_t a_step = p.a_mn ? 2048 : 32, b_step = p.b_mn ? 2048 : 32;      // bytes to the next 16 of the contraction
-    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+    for (int t = pair; t < tiles && ok; t += pairs) {
       const int ke = k_to(t);
       for (int k0 = k_from(t); k0 < ke && ok; k0 += p.seg, ++ch) {
         const int n = (min(ke, k0 + p.seg) - k0) * p.passes;
@@ -250,10 +289,10 @@ __global__ void __launch_bounds__(LCE_THREADS, 1) lce_gemm_kernel(const __grid_c
           const uint32_t st = smem_u32(smem + (size_t)s * ST_BYTES);
 #pragma unroll
           for (int kk = 0; kk < TK / 16; ++kk)
-            mma_f16(d, smem_desc(st + kk * a_step, a_lbo, 1024, 2), smem_desc(st + A_BYTES + kk * b_step, b_lbo, 1024, 2), p.idesc, i > 0 || kk > 0 ? 1u : 0u);
-          mma_commit(&pipe.empty[s]);
+            mma_pair(d, smem_desc(st + kk * a_step, a_lbo, 1024, 2), smem_desc(st + A_BYTES + kk * b_step, b_lbo, 1024, 2), p.idesc, i > 0 || kk > 0 ? 1u : 0u);
+          commit_pair(&pipe.empty[s]);
         }
-        if (ok) mma_commit(&pipe.acc_full[ch & 1]);
+        if (ok) commit_pair(&pipe.acc_full[ch & 1]);
       }
     }
     if (!ok) atomicExch(&pipe.fail, 1);
@@ -263,8 +302,8 @@ __global__ void __launch_bounds__(LCE_THREADS, 1) lce_gemm_kernel(const __grid_c
     unsigned char *staging = smem + NST * ST_BYTES + (warp - 4) * STAGING;
     int ch = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-      const int m0 = m_of(t) * TM, n0 = n_of(t) * TN;
+    for (int t = pair; t < tiles && ok; t += pairs) {
+      const int m0 = (m_of(t) * 2 + rank) * TM, n0 = n_of(t) * TN;
       const int row = m0 + q * 32 + lane, c0 = n0 + half * (TN / 2);      // this thread's row and 128 columns
       const bool in = row < p.rows;
       const int kb = k_from(t), ke = k_to(t);
@@ -318,7 +357,7 @@ __global__ void __launch_bounds__(LCE_THREADS, 1) lce_gemm_kernel(const __grid_c
           }
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&pipe.acc_empty[ch & 1]);
+          if (lane == 0) arrive_at(of_first(&pipe.acc_empty[ch & 1]));
           if (in) {
             p.part[(int64_t)(n_of(t) * 2 + half) * p.rows + row] = make_float2(m, sum);
             if (at >= 0) p.target[row] = target;
@@ -352,7 +391,7 @@ __global__ void __launch_bounds__(LCE_THREADS, 1) lce_gemm_kernel(const __grid_c
           }
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&pipe.acc_empty[ch & 1]);
+          if (lane == 0) arrive_at(of_first(&pipe.acc_empty[ch & 1]));
         } else {
           const bool first = k0 == kb && !p.add, last = k0 + p.seg >= ke && p.last;
           float *acc = p.acc + (int64_t)(t / (p.nt * p.mt)) * p.rows * p.acc_rs;
@@ -393,7 +432,7 @@ __global__ void __launch_bounds__(LCE_THREADS, 1) lce_gemm_kernel(const __grid_c
           }
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&pipe.acc_empty[ch & 1]);
+          if (lane == 0) arrive_at(of_first(&pipe.acc_empty[ch & 1]));
         }
       }
     }
@@ -402,7 +441,8 @@ __global__ void __launch_bounds__(LCE_THREADS, 1) lce_gemm_kernel(const __grid_c
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * TN) : "memory");
+  cluster_sync();                                      // neither block leaves while the other uses its memory
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * TN) : "memory");
   if (tid == 0 && pipe.fail) atomicExch(&g_lce_status, 7);
 }
 
@@ -433,32 +473,33 @@ __global__ void __launch_bounds__(256) lce_pack_kernel(const void *src, int64_t 
 __device__ __forceinline__ bool is_target(int64_t label, int64_t ignore, int classes) { return label != ignore && label >= 0 && label < classes; }
 
 // Joins the partial maxima and sums of 32 rows: a warp reads the same slot of 32 rows.
-__global__ void __launch_bounds__(256) lce_join_kernel(const float2 *part, const float *target, const int64_t *labels, int64_t ignore, int classes, int rows,
-                                                      int slots, float *lse, float *loss) {
-  __shared__ float2 sh[8][32];
+constexpr int JOIN_WARPS = 32;
+__global__ void __launch_bounds__(JOIN_WARPS * 32) lce_join_kernel(const float2 *part, const float *target, const int64_t *labels, int64_t ignore, int classes, int rows,
+                                                                  int slots, float *lse, float *loss) {
+  __shared__ float2 sh[JOIN_WARPS][33];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, row = blockIdx.x * 32 + lane;
   float m = -INFINITY, s = 0.f;
+  const auto join = [&](float2 v) {
+    const float nm = fmaxf(m, v.x), off = nm == -INFINITY ? 0.f : nm;
+    s = s * ex2(m - off) + v.y * ex2(v.x - off);
+    m = nm;
+  };
   if (row < rows) {
-#pragma unroll 4
-    for (int i = w; i < slots; i += 8) {
-      const float2 v = part[(int64_t)i * rows + row];
-      const float nm = fmaxf(m, v.x), off = nm == -INFINITY ? 0.f : nm;
-      s = s * ex2(m - off) + v.y * ex2(v.x - off);
-      m = nm;
-    }
+#pragma unroll 8
+    for (int i = w; i < slots; i += JOIN_WARPS) join(part[(int64_t)i * rows + row]);
   }
   sh[w][lane] = make_float2(m, s);
   __syncthreads();
-  if (w == 0 && row < rows) {
-    for (int i = 1; i < 8; ++i) {
-      const float2 v = sh[i][lane];
-      const float nm = fmaxf(m, v.x), off = nm == -INFINITY ? 0.f : nm;
-      s = s * ex2(m - off) + v.y * ex2(v.x - off);
-      m = nm;
-    }
+  const int r = blockIdx.x * 32 + w;                   // a warp a row
+  const float2 v = sh[lane][w];
+  m = v.x;
+  s = v.y;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) join(make_float2(__shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o)));
+  if (lane == 0 && r < rows) {
     const float l = m / kLog2e + logf(s);
-    lse[row] = l;
-    loss[row] = is_target(labels[row], ignore, classes) ? l - target[row] : 0.f;
+    lse[r] = l;
+    loss[r] = is_target(labels[r], ignore, classes) ? l - target[r] : 0.f;
   }
 }
 
@@ -565,14 +606,14 @@ struct Plan {
 // How many blocks share the contraction of `stages` for each of `tiles` tiles: as few as fill the SMs (at least 8 stages
 // each, to be worth 128 KB of sums).
 void split_of(int64_t tiles, int stages, int &splits, int &per) {
-  const int64_t sms = sm_count_current();
+  const int64_t pairs = sm_count_current() / 2;
   splits = 1;
   per = stages;
-  int64_t best = (tiles + sms - 1) / sms * stages;
-  for (int s = 2; s <= kMaxSplits && stages / s >= 8 && tiles * (s - 1) < sms; ++s) {
+  int64_t best = (tiles + pairs - 1) / pairs * stages;
+  for (int s = 2; s <= kMaxSplits && stages / s >= 8 && tiles * (s - 1) < pairs; ++s) {
     const int p = (stages + s - 1) / s;
     if ((int64_t)(s - 1) * p >= stages) continue;
-    const int64_t cost = (tiles * s + sms - 1) / sms * p;
+    const int64_t cost = (tiles * s + pairs - 1) / pairs * p;
     if (cost * 100 < best * 90) { best = cost; splits = s; per = p; }
   }
 }
@@ -600,8 +641,8 @@ Plan plan_of(const b200_lce_args &a) {
   q.dz_pitch = q.piece;
   q.dz_bytes = up(2 * q.planes * a.rows * q.dz_pitch, 256);
   const int64_t dt = (a.features + TN - 1) / TN;
-  split_of((a.rows + TM - 1) / TM * dt, (q.piece + TK - 1) / TK, q.splits_h, q.per_h);
-  split_of((q.piece + TM - 1) / TM * dt, (int)((a.rows + TK - 1) / TK), q.splits_w, q.per_w);
+  split_of((a.rows + 2 * TM - 1) / (2 * TM) * dt, (q.piece + TK - 1) / TK, q.splits_h, q.per_h);
+  split_of((q.piece + 2 * TM - 1) / (2 * TM) * dt, (int)((a.rows + TK - 1) / TK), q.splits_w, q.per_w);
   // float32 sums: of dH over the pieces, the chains and the blocks that share a tile, of dW over the chains and blocks
   q.acc_h_bytes = f32 || q.n_pieces > 1 || q.splits_h > 1 ? up(4 * q.splits_h * a.rows * q.Da, 256) : 0;
   q.acc_w_bytes = q.splits_w > 1 || (f32 && (a.rows + TK - 1) / TK > q.seg) ? up(4 * q.splits_w * (int64_t)q.piece * q.Da, 256) : 0;
@@ -635,11 +676,11 @@ template <int EPI> int launch_gemm(const LceGemm &g, cudaStream_t st) {
   cudaError_t e = cudaFuncSetAttribute(lce_gemm_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, LCE_SMEM);
   if (e != cudaSuccess) { set_error("cudaFuncSetAttribute: %s", cudaGetErrorString(e)); return (int)e; }
   const int tiles = g.mt * g.nt * (EPI == EPI_OUT ? g.splits : 1), sms = sm_count_current();
-  lce_gemm_kernel<EPI><<<(unsigned)(tiles < sms ? tiles : sms), LCE_THREADS, LCE_SMEM, st>>>(g);
+  lce_gemm_kernel<EPI><<<(unsigned)(2 * (tiles < sms / 2 ? tiles : sms / 2)), LCE_THREADS, LCE_SMEM, st>>>(g);
   return launch_status();
 }
 
-uint32_t idesc_of(int dtype, bool a_mn, bool b_mn) { return idesc_f16(dtype == B200_F16 ? 0u : 1u, a_mn, b_mn, TM, TN); }
+uint32_t idesc_of(int dtype, bool a_mn, bool b_mn) { return idesc_f16(dtype == B200_F16 ? 0u : 1u, a_mn, b_mn, 2 * TM, TN); }
 
 int fold(const LceGemm &g, cudaStream_t st) {
   const int64_t n = (int64_t)g.rows * (g.acc_rs / 4), most = (int64_t)sm_count_current() * 16, blocks = (n + 255) / 256;
@@ -652,9 +693,9 @@ struct Operands { const void *h, *w; int64_t h_pitch, w_pitch; };
 // z = H W^T for classes c0 .. c0 + cols
 int gemm_z(LceGemm &g, const b200_lce_args &a, const Plan &q, const Operands &o, int c0, int cols) {
   memset(&g, 0, sizeof(g));
-  B200_REQUIRE(map16(&g.a, a.dtype, o.h, a.features, a.rows, o.h_pitch, q.planes, TM) && map16(&g.b, a.dtype, o.w, a.features, a.classes, o.w_pitch, q.planes, TN),
+  B200_REQUIRE(map16(&g.a, a.dtype, o.h, a.features, a.rows, o.h_pitch, q.planes, TM) && map16(&g.b, a.dtype, o.w, a.features, a.classes, o.w_pitch, q.planes, TN / 2),
                B200_ERR_UNSUPPORTED, "lce: tensor-map encoding failed");
-  g.mt = (int)((a.rows + TM - 1) / TM);
+  g.mt = (int)((a.rows + 2 * TM - 1) / (2 * TM));
   g.nt = (cols + TN - 1) / TN;
   g.nk = (a.features + TK - 1) / TK;
   g.seg = g.nk;
@@ -720,7 +761,7 @@ extern "C" int b200_lce_fwd(const b200_lce_args *args, void *stream) {
   w += up(4 * a.rows, 256);
   float *row_loss = a.reduction == 0 ? reinterpret_cast<float *>(a.loss) : reinterpret_cast<float *>(w);
   if (int e = launch_gemm<EPI_LSE>(g, st)) return e;
-  lce_join_kernel<<<(unsigned)((a.rows + 31) / 32), 256, 0, st>>>(g.part, g.target, g.labels, a.ignore_index, a.classes, (int)a.rows, slots_of(a),
+  lce_join_kernel<<<(unsigned)((a.rows + 31) / 32), JOIN_WARPS * 32, 0, st>>>(g.part, g.target, g.labels, a.ignore_index, a.classes, (int)a.rows, slots_of(a),
                                                                 reinterpret_cast<float *>(a.lse), row_loss);
   if (int e = launch_status()) return e;
   if (a.reduction != 0)
@@ -801,7 +842,7 @@ extern "C" int b200_lce_bwd(const b200_lce_args *args, void *stream) {
     if (a.dweight) {                                             // dz^T H: contraction over the rows
       B200_REQUIRE(map16(&g.a, a.dtype, dz, cols, a.rows, q.dz_pitch, q.planes, 64) && map16(&g.b, a.dtype, o.h, a.features, a.rows, o.h_pitch, q.planes, 64),
                    B200_ERR_UNSUPPORTED, "lce: tensor-map encoding failed");
-      g.mt = (cols + TM - 1) / TM;
+      g.mt = (cols + 2 * TM - 1) / (2 * TM);
       g.nk = (int)((a.rows + TK - 1) / TK);
       g.seg = q.seg < g.nk ? q.seg : g.nk;
       g.a_mn = 1;
