@@ -167,6 +167,7 @@ __device__ __forceinline__ uint32_t tf32(float x) {
 template <bool SPLIT_A, bool SPLIT_B>
 __device__ __forceinline__ void product(float (&acc)[4][4], const float *a, int am, int ak, const float *wk, const float *b, int bk, int bn, int K, int lane) {
   const int g = lane >> 2, t = lane & 3;
+#pragma unroll 4
   for (int k0 = 0; k0 < K; k0 += 8) {
     float av[4];
     av[0] = a[g * am + (k0 + t) * ak];
@@ -184,7 +185,7 @@ __device__ __forceinline__ void product(float (&acc)[4][4], const float *a, int 
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       ah[i] = SPLIT_A ? tf32(av[i]) : __float_as_uint(av[i]);
-      al[i] = SPLIT_A ? __float_as_uint(av[i] - __uint_as_float(ah[i])) : 0u;
+      al[i] = SPLIT_A ? tf32(av[i] - __uint_as_float(ah[i])) : 0u;
     }
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
@@ -195,53 +196,62 @@ __device__ __forceinline__ void product(float (&acc)[4][4], const float *a, int 
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         bh[i] = SPLIT_B ? tf32(bv[i]) : __float_as_uint(bv[i]);
-        bl[i] = SPLIT_B ? __float_as_uint(bv[i] - __uint_as_float(bh[i])) : 0u;
+        bl[i] = SPLIT_B ? tf32(bv[i] - __uint_as_float(bh[i])) : 0u;
       }
-      if (SPLIT_A) mma8(acc[n], al, bh);
-      if (SPLIT_B) mma8(acc[n], ah, bl);
-      mma8(acc[n], ah, bh);
+      // the unit truncates when it adds: each step's products start from zero, the small ones first, and are added rounded
+      float c[4] = {0.f, 0.f, 0.f, 0.f};
+      if (SPLIT_A) mma8(c, al, bh);
+      if (SPLIT_B) mma8(c, ah, bl);
+      mma8(c, ah, bh);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[n][i] += c[i];
     }
   }
 }
 
-// 64 rows of an operand from step i0 on into shared memory as float32, zero past the sequence and past its size.
+// 64 rows of an operand from step i0 on into shared memory as float32, zero past the sequence and past its size: 16 threads a
+// row, 4 columns each, four rows in flight.
 template <typename T>
 __device__ __forceinline__ void load_rows(const Walk &p, const void *base, int64_t off, int64_t ls, int i0, int col0, int size, int width, int pitch, float *dst) {
-  const T *src = reinterpret_cast<const T *>(base) + off;
-  const bool vec = ((reinterpret_cast<uintptr_t>(src + col0) | (uintptr_t)(ls * sizeof(T))) & (4 * sizeof(T) - 1)) == 0;
-  const int per = width / 4;
-  for (int e = threadIdx.x; e < CH * per; e += WT) {
-    const int r = e / per, c = e % per * 4, i = time_of(p, i0 + r);
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    if (i < p.length) {
-      const T *s = src + (int64_t)i * ls + col0 + c;
-      const int left = size - col0 - c;
+  const T *src = reinterpret_cast<const T *>(base) + off + col0;
+  const bool vec = ((reinterpret_cast<uintptr_t>(src) | (uintptr_t)(ls * sizeof(T))) & (4 * sizeof(T) - 1)) == 0;
+  const int r0 = threadIdx.x >> 4;
+  for (int c = (threadIdx.x & 15) * 4; c < width; c += 64) {
+    const int left = size - col0 - c;
+    float4 v[CH / 16];
+#pragma unroll
+    for (int i = 0; i < CH / 16; ++i) {
+      const int t = time_of(p, i0 + r0 + i * 16);
+      const T *s = src + (int64_t)t * ls + c;
+      const bool in = t < p.length;
+      v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (vec && left >= 4) {
-        if constexpr (sizeof(T) == 4) {
-          const float4 w = *reinterpret_cast<const float4 *>(s);
-          v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
-        } else {
-          const uint2 w = *reinterpret_cast<const uint2 *>(s);
-          const T *x = reinterpret_cast<const T *>(&w);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) v[j] = (float)x[j];
+        if (in) {
+          if constexpr (sizeof(T) == 4) v[i] = __ldg(reinterpret_cast<const float4 *>(s));
+          else {
+            const uint2 w = __ldg(reinterpret_cast<const uint2 *>(s));
+            const T *x = reinterpret_cast<const T *>(&w);
+            v[i] = make_float4((float)x[0], (float)x[1], (float)x[2], (float)x[3]);
+          }
         }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (j < left) v[j] = (float)s[j];
+      } else if (in) {
+        if (left > 0) v[i].x = (float)s[0];
+        if (left > 1) v[i].y = (float)s[1];
+        if (left > 2) v[i].z = (float)s[2];
+        if (left > 3) v[i].w = (float)s[3];
       }
     }
-    *reinterpret_cast<float4 *>(dst + r * pitch + c) = make_float4(v[0], v[1], v[2], v[3]);
+#pragma unroll
+    for (int i = 0; i < CH / 16; ++i) *reinterpret_cast<float4 *>(dst + (r0 + i * 16) * pitch + c) = v[i];
   }
 }
 
-template <typename T, bool STATE_ONLY> __global__ void __launch_bounds__(WT) linattn_walk_kernel(const Walk p) {
+template <typename T, bool STATE_ONLY> __global__ void __launch_bounds__(WT, 1) linattn_walk_kernel(const Walk p) {
   constexpr bool F32 = sizeof(T) == 4;
   extern __shared__ __align__(16) float sm[];
   const int dip = (p.di + 15) / 16 * 16, PQ = dip + 4;
   float *sk = sm, *sv = sk + CH * PQ, *S = sv + CH * PV, *sq = S + dip * PV, *sp = sq + CH * PQ, *sx = sp + CH * PP;
-  __shared__ Decays d;
+  __shared__ Decays dd[2];
   __shared__ float dots[2][CH], rows_[2][CH], cols_[4][CH];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gq = lane >> 2, tq = lane & 3;
   const int tile = blockIdx.x % p.tiles, bh = blockIdx.x / p.tiles % (p.batch * p.heads), seg = blockIdx.x / p.tiles / (p.batch * p.heads);
@@ -265,11 +275,12 @@ template <typename T, bool STATE_ONLY> __global__ void __launch_bounds__(WT) lin
     S[r * PV + c] = s;
   }
   double total = 0.0;
-  for (int i0 = i_begin; i0 < i_end; i0 += CH) {
+  if (warp == 4) chunk_decays(p, b, h, i_begin, lane, dd[0]);
+  for (int i0 = i_begin, it = 0; i0 < i_end; i0 += CH, ++it) {
     __syncthreads();                                 // the last chunk's reads and writes are done
     const int chunk = p.rev ? p.chunks - 1 - i0 / CH : i0 / CH;
+    const Decays &d = dd[it & 1];
     if (!STATE_ONLY && p.run && !p.rev && chunk % kSnap == 0) snapshot(chunk, 1.f);
-    if (warp == 0) chunk_decays(p, b, h, i0, lane, d);
     load_rows<T>(p, p.k, b * p.k_bs + h / p.k_div * p.k_hs, p.k_ls, i0, 0, p.di, dip, PQ, sk);
     load_rows<T>(p, p.v, b * p.v_bs + h / p.v_div * p.v_hs, p.v_ls, i0, col0, p.dout, DO, PV, sv);
     if (!STATE_ONLY) {
@@ -278,6 +289,8 @@ template <typename T, bool STATE_ONLY> __global__ void __launch_bounds__(WT) lin
     }
     __syncthreads();
     const int m0 = (warp & 3) * 16, n0 = (warp >> 2) * 32;      // this warp's 16 x 32 of scores and of results
+    // the next chunk's decays, by the warp whose scores are all zero
+    if (warp == 4 && i0 + CH < i_end) chunk_decays(p, b, h, i0 + CH, lane, dd[(it + 1) & 1]);
     if (!STATE_ONLY) {
       float acc[4][4] = {};
       const bool any = n0 <= m0 + 15;
