@@ -9,7 +9,6 @@ token in place, as ``selective_state_update`` does.
 """
 from __future__ import annotations
 
-import ctypes
 import functools
 
 import torch
@@ -25,31 +24,24 @@ def _inner(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def _fill(a, q, k, v, g, scale, s0):
-    a.batch, a.seqlen, a.groups, a.dk = q.shape
-    a.heads, a.dv = v.shape[2:]
-    a.dtype, a.g_dtype = _lib.enum(_DT[q.dtype]), _lib.enum(_DT[g.dtype])
-    a.scale = scale
-    a.q, a.k, a.v, a.g = q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr()
-    a.q_bs, a.q_ls, a.q_hs, _ = q.stride()
-    a.k_bs, a.k_ls, a.k_hs, _ = k.stride()
-    a.v_bs, a.v_ls, a.v_hs, _ = v.stride()
-    if g.dim() == 1:
-        a.g_heads, a.g_hs = 1, g.stride(0)
-    else:
-        a.g_bs, a.g_ls, a.g_hs = g.stride()
-    if s0 is not None:
-        a.s0 = s0.data_ptr()
-        a.s0_bs, a.s0_hs, a.s0_ks, _ = s0.stride()
+@functools.lru_cache(maxsize=None)
+def _setup():
+    return _lib.packer("b200_linattn_args"), {t: _lib.enum(n) for t, n in _DT.items()}
 
 
-def _work(a, name, like):
-    a.work_bytes = getattr(_lib.lib(), name)(ctypes.byref(a))
-    if not a.work_bytes:
-        return None
-    work = torch.empty(a.work_bytes, dtype=torch.uint8, device=like.device)
-    a.work = work.data_ptr()
-    return work
+def _call(name, q, k, v, g, scale, s0, out, last, back):
+    """Runs b200_linattn_fwd or _bwd; ``back`` is the tail of the argument block that only the backward has."""
+    pack, codes = _setup()
+    batch, length, groups, dk = q.shape
+    heads, dv = v.shape[2:]
+    by_head = g.dim() == 1
+    head = (batch, length, heads, groups, dk, dv, codes[q.dtype], codes[g.dtype], scale, by_head, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(),
+            0 if s0 is None else s0.data_ptr(), out, last, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
+            *((0, 0, g.stride(0)) if by_head else g.stride()), *((0, 0, 0) if s0 is None else s0.stride()[:3]), length * heads * dv, heads * dv, dv, *back)
+    lib = _lib.lib()
+    work_bytes = getattr(lib, name + "_work_bytes")(pack(*head, 0, 0))
+    work = torch.empty(work_bytes, dtype=torch.uint8, device=q.device) if work_bytes else None
+    _lib.call(name, pack(*head, work.data_ptr() if work_bytes else 0, work_bytes), _lib.stream_of(q))
 
 
 @functools.lru_cache(maxsize=None)
@@ -57,24 +49,20 @@ def _step_setup():
     return _lib.packer("b200_linattn_step_args"), {t: _lib.enum(n) for t, n in _DT.items()}
 
 
+def _forward(q, k, v, g, scale, s0, return_last_state):
+    with _lib.on_device(q):
+        out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+        last = torch.empty((v.shape[0], v.shape[2], q.shape[3], v.shape[3]), dtype=torch.float32, device=v.device) if return_last_state else None
+        _call("b200_linattn_fwd", q, k, v, g, scale, s0, out.data_ptr(), last.data_ptr() if return_last_state else 0, (0,) * 10)
+    return out, last
+
+
 class LinearAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, g, scale, initial_state, return_last_state):
         q, k, v = _inner(q), _inner(k), _inner(v)
         s0 = None if initial_state is None else _inner(initial_state)
-        a = _lib.struct("b200_linattn_args")()
-        _fill(a, q, k, v, g, scale, s0)
-        last = None
-        with _lib.on_device(q):
-            out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
-            a.out = out.data_ptr()
-            a.out_bs, a.out_ls, a.out_hs, _ = out.stride()
-            if return_last_state:
-                last = torch.empty(a.batch, a.heads, a.dk, a.dv, dtype=torch.float32, device=v.device)
-                a.last = last.data_ptr()
-            work = _work(a, "b200_linattn_fwd_work_bytes", q)
-            _lib.call("b200_linattn_fwd", a, _stream(q))
-            del work
+        out, last = _forward(q, k, v, g, scale, s0, return_last_state)
         ctx.save_for_backward(q, k, v, g, s0)
         ctx.scale = scale
         ctx.set_materialize_grads(False)
@@ -85,27 +73,16 @@ class LinearAttentionFn(torch.autograd.Function):
         q, k, v, g, s0 = ctx.saved_tensors
         if dout is None and dlast is None:
             return None, None, None, None, None, None, None
-        a = _lib.struct("b200_linattn_args")()
-        _fill(a, q, k, v, g, ctx.scale, s0)
+        new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
         with _lib.on_device(q):
             dout = torch.zeros(v.shape, dtype=v.dtype, device=v.device) if dout is None else _inner(dout)
-            a.dout = dout.data_ptr()
-            a.dout_bs, a.dout_ls, a.dout_hs, _ = dout.stride()
-            if dlast is not None:
-                dlast = dlast.contiguous()
-                a.dlast = dlast.data_ptr()
-            new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
+            dlast = None if dlast is None else dlast.contiguous()
             dq, dk, dv = new(q), new(k), new(v)
-            a.dq, a.dk_out, a.dv_out = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
             dg = new(g) if ctx.needs_input_grad[3] else None
             ds0 = new(s0) if ctx.needs_input_grad[5] else None
-            if dg is not None:
-                a.dg = dg.data_ptr()
-            if ds0 is not None:
-                a.ds0 = ds0.data_ptr()
-            work = _work(a, "b200_linattn_bwd_work_bytes", q)
-            _lib.call("b200_linattn_bwd", a, _stream(q))
-            del work
+            at = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+            _call("b200_linattn_bwd", q, k, v, g, ctx.scale, s0, 0, 0,
+                  (dout.data_ptr(), at(dlast), *dout.stride()[:3], dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), at(dg), at(ds0)))
         return dq, dk, dv, dg, None, ds0, None
 
 
@@ -143,7 +120,11 @@ def linear_attention_fn(q, k, v, g, scale=1.0, initial_state=None, return_last_s
         if not return_last_state:
             return out
         return out, initial_state.clone() if initial_state is not None else torch.zeros(batch, heads, q.shape[-1], dv, device=v.device)
-    return LinearAttentionFn.apply(q, k, v, g, float(scale), initial_state, return_last_state)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad
+                                    or initial_state is not None and initial_state.requires_grad):
+        return LinearAttentionFn.apply(q, k, v, g, float(scale), initial_state, return_last_state)
+    out, last = _forward(_inner(q), _inner(k), _inner(v), g, scale, None if initial_state is None else _inner(initial_state), return_last_state)
+    return (out, last) if return_last_state else out
 
 
 def linear_attention_step(state, q, k, v, g, scale=1.0, state_batch_indices=None):

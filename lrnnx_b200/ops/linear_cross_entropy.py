@@ -9,12 +9,12 @@ classes the logits of 16384 tokens are the largest tensor of a training step.
 """
 from __future__ import annotations
 
-import ctypes
+import functools
 
 import torch
 
 from .. import _lib
-from .mamba_block import _DT, _stream
+from .mamba_block import _DT
 
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
@@ -24,61 +24,53 @@ def _rows(t):
     return t if (t.stride(-1) == 1 or t.shape[-1] == 1) and t.stride(0) >= t.shape[-1] else t.contiguous()
 
 
-def _work(a, name, like):
-    a.work_bytes = getattr(_lib.lib(), name)(ctypes.byref(a))
-    work = torch.empty(max(a.work_bytes, 1), dtype=torch.uint8, device=like.device)
-    a.work = work.data_ptr()
-    return work
+@functools.lru_cache(maxsize=None)
+def _setup():
+    return _lib.packer("b200_lce_args"), {t: _lib.enum(n) for t, n in _DT.items()}
+
+
+def _call(name, hidden, weight, labels, ignore_index, reduction, lse, loss, count, dloss, dh, dw):
+    pack, codes = _setup()
+    rows, features = hidden.shape
+    at = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    head = (rows, ignore_index, weight.shape[0], features, codes[hidden.dtype], reduction, hidden.data_ptr(), weight.data_ptr(), labels.data_ptr(),
+            hidden.stride(0), weight.stride(0), lse.data_ptr(), at(loss), at(count), at(dloss), at(dh), at(dw), features, features)
+    work_bytes = getattr(_lib.lib(), name + "_work_bytes")(pack(*head, 0, 0))
+    work = torch.empty(max(work_bytes, 1), dtype=torch.uint8, device=hidden.device)
+    _lib.call(name, pack(*head, work.data_ptr(), work_bytes), _lib.stream_of(hidden))
+
+
+def _forward(hidden, weight, labels, ignore_index, reduction, shape):
+    with _lib.on_device(hidden):
+        lse = torch.empty(hidden.shape[0], dtype=torch.float32, device=hidden.device)
+        loss = torch.empty(shape if reduction == 0 else (), dtype=torch.float32, device=hidden.device)
+        count = torch.empty((), dtype=torch.float32, device=hidden.device) if reduction == 1 else None
+        _call("b200_lce_fwd", hidden, weight, labels, ignore_index, reduction, lse, loss, count, None, None, None)
+    return loss, lse, count
 
 
 class LinearCrossEntropyFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, labels, ignore_index, reduction):
-        ctx.shapes = hidden.shape, weight.shape
-        labels_shape = labels.shape
-        hidden, weight = _rows(hidden.reshape(-1, hidden.shape[-1])), _rows(weight)
-        labels = labels.reshape(-1).to(torch.int64).contiguous()
-        a = _lib.struct("b200_lce_args")()
-        a.rows, a.features = hidden.shape
-        a.classes, a.ignore_index, a.reduction = weight.shape[0], ignore_index, reduction
-        a.dtype = _lib.enum(_DT[hidden.dtype])
-        with _lib.on_device(hidden):
-            lse = torch.empty(a.rows, dtype=torch.float32, device=hidden.device)
-            loss = torch.empty(labels_shape if reduction == 0 else (), dtype=torch.float32, device=hidden.device)
-            count = torch.empty((), dtype=torch.float32, device=hidden.device)
-            a.hidden, a.weight, a.labels = hidden.data_ptr(), weight.data_ptr(), labels.data_ptr()
-            a.hidden_rs, a.weight_rs = hidden.stride(0), weight.stride(0)
-            a.lse, a.loss, a.count = lse.data_ptr(), loss.data_ptr(), count.data_ptr()
-            work = _work(a, "b200_lce_fwd_work_bytes", hidden)
-            _lib.call("b200_lce_fwd", a, _stream(hidden))
-            del work
-        ctx.save_for_backward(hidden, weight, labels, lse, count)
-        ctx.ignore_index, ctx.reduction = ignore_index, reduction
+        ctx.shape = hidden.shape
+        hidden = _rows(hidden.reshape(-1, hidden.shape[-1]))
+        weight = _rows(weight)
+        flat = labels.reshape(-1).to(torch.int64).contiguous()
+        loss, lse, count = _forward(hidden, weight, flat, ignore_index, reduction, labels.shape)
+        ctx.save_for_backward(hidden, weight, flat, lse, count)
+        ctx.meta = ignore_index, reduction
         return loss
 
     @staticmethod
     def backward(ctx, grad):
         hidden, weight, labels, lse, count = ctx.saved_tensors
         need_h, need_w = ctx.needs_input_grad[:2]
-        a = _lib.struct("b200_lce_args")()
-        a.rows, a.features = hidden.shape
-        a.classes, a.ignore_index, a.reduction = weight.shape[0], ctx.ignore_index, ctx.reduction
-        a.dtype = _lib.enum(_DT[hidden.dtype])
         with _lib.on_device(hidden):
             grad = grad.to(torch.float32).contiguous()
             dh = torch.empty(hidden.shape, dtype=hidden.dtype, device=hidden.device) if need_h else None
             dw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device) if need_w else None
-            a.hidden, a.weight, a.labels = hidden.data_ptr(), weight.data_ptr(), labels.data_ptr()
-            a.hidden_rs, a.weight_rs = hidden.stride(0), weight.stride(0)
-            a.lse, a.count, a.dloss = lse.data_ptr(), count.data_ptr(), grad.data_ptr()
-            if need_h:
-                a.dhidden, a.dhidden_rs = dh.data_ptr(), dh.stride(0)
-            if need_w:
-                a.dweight, a.dweight_rs = dw.data_ptr(), dw.stride(0)
-            work = _work(a, "b200_lce_bwd_work_bytes", hidden)
-            _lib.call("b200_lce_bwd", a, _stream(hidden))
-            del work
-        return dh.view(ctx.shapes[0]) if need_h else None, dw, None, None, None
+            _call("b200_lce_bwd", hidden, weight, labels, *ctx.meta, lse, None, count, grad, dh, dw)
+        return dh.view(ctx.shape) if need_h else None, dw, None, None, None
 
 
 def linear_cross_entropy(hidden, weight, labels, ignore_index=-100, reduction="mean"):
@@ -102,4 +94,7 @@ def linear_cross_entropy(hidden, weight, labels, ignore_index=-100, reduction="m
     if labels.numel() == 0:                        # no rows: a sum over nothing, with gradients of zero
         zero = (hidden.sum() + weight[:0].sum()).float()
         return zero.expand(labels.shape) if reduction == "none" else zero
-    return LinearCrossEntropyFn.apply(hidden, weight, labels, ignore_index, _REDUCTIONS[reduction])
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        return LinearCrossEntropyFn.apply(hidden, weight, labels, ignore_index, _REDUCTIONS[reduction])
+    return _forward(_rows(hidden.reshape(-1, hidden.shape[-1])), _rows(weight), labels.reshape(-1).to(torch.int64).contiguous(), ignore_index,
+                    _REDUCTIONS[reduction], labels.shape)[0]
