@@ -19,16 +19,16 @@ def _setup():
     return _lib.packer("b200_embed_args"), {t: _lib.enum(n) for t, n in _DT.items()}
 
 
-def _lookup(ids, weight, scale, padding_idx):
+def _lookup(ids, weight, classes, features, scale, padding_idx):
     """out, and the ids in a row"""
-    if weight.stride(1) != 1 or weight.stride(0) < weight.shape[1]:
+    if weight.stride(1) != 1 or weight.stride(0) < features:
         weight = weight.contiguous()
     flat = ids if ids.is_contiguous() else ids.contiguous()
-    classes, features = weight.shape
     pack, codes = _setup()
+    dtype = weight.dtype
     with _lib.on_device(weight):
-        out = torch.empty(ids.shape + (features,), dtype=weight.dtype, device=weight.device)
-        _lib.call("b200_embed_fwd", pack(flat.numel(), padding_idx, classes, features, codes[weight.dtype], flat.dtype == torch.int64, scale, 0,
+        out = weight.new_empty(ids.shape + (features,))
+        _lib.call("b200_embed_fwd", pack(flat.numel(), padding_idx, classes, features, codes[dtype], flat.dtype == torch.int64, scale, 0,
                                          flat.data_ptr(), weight.data_ptr(), 0, out.data_ptr(), 0, weight.stride(0), features, 0, 0, 0, 0),
                   _lib.stream_of(weight))
     return out, flat
@@ -37,7 +37,7 @@ def _lookup(ids, weight, scale, padding_idx):
 class TokenEmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, weight, scale, padding_idx):
-        out, flat = _lookup(ids, weight, scale, padding_idx)
+        out, flat = _lookup(ids, weight, *weight.shape, scale, padding_idx)
         ctx.save_for_backward(flat)
         ctx.meta = weight.shape[0], scale, padding_idx
         return out
@@ -66,21 +66,23 @@ def token_embedding(ids, weight, scale=1.0, padding_idx=None):
     """``scale * weight[ids]``: ids (...) int32 or int64, weight (classes, features) float32, float16 or
     bfloat16 -> (..., features).  The gradient of row ``padding_idx`` is zero.  An id outside
     [0, classes) reads nothing: its row is NaN, and it adds to no gradient."""
-    if weight.dim() != 2 or weight.shape[0] == 0 or weight.shape[1] == 0:
+    shape = weight.shape
+    if len(shape) != 2 or 0 in shape:
         raise RuntimeError("token_embedding: weight (classes, features) expected")
     if weight.dtype not in _DT or not weight.is_cuda:
         raise RuntimeError("token_embedding: weight must be a float32 / float16 / bfloat16 CUDA tensor")
-    if ids.dtype not in (torch.int32, torch.int64):
+    if ids.dtype is not torch.int64 and ids.dtype is not torch.int32:
         raise RuntimeError("token_embedding: ids must be int32 or int64")
-    if ids.device != weight.device:
+    if ids.get_device() != weight.get_device():
         raise RuntimeError("token_embedding: ids and weight must be on one device")
-    if padding_idx is not None:
-        if not -weight.shape[0] <= padding_idx < weight.shape[0]:
-            raise RuntimeError("token_embedding: padding_idx must be a row of weight")
-        padding_idx %= weight.shape[0]
+    if padding_idx is None:
+        padding_idx = -1
+    elif -shape[0] <= padding_idx < shape[0]:
+        padding_idx %= shape[0]
+    else:
+        raise RuntimeError("token_embedding: padding_idx must be a row of weight")
     if ids.numel() == 0:
-        return weight[:0].sum() + torch.empty(*ids.shape, weight.shape[1], dtype=weight.dtype, device=weight.device)
-    padding_idx = -1 if padding_idx is None else padding_idx
-    if weight.requires_grad and torch.is_grad_enabled():
+        return weight[:0].sum() + weight.new_empty(ids.shape + (shape[1],))
+    if torch.is_grad_enabled() and weight.requires_grad:
         return TokenEmbeddingFn.apply(ids, weight, float(scale), padding_idx)
-    return _lookup(ids, weight, scale, padding_idx)[0]
+    return _lookup(ids, weight, *shape, scale, padding_idx)[0]

@@ -87,20 +87,22 @@ class LinearAttentionFn(torch.autograd.Function):
 
 
 def _check(name, dims, q, k, v, g, state):
-    batch, heads, dv = v.shape[0], v.shape[-2], v.shape[-1]
-    if q.shape != k.shape or q.dim() != dims or v.dim() != dims or q.shape[:dims - 2] != v.shape[:dims - 2]:
+    qs, vs, gs = q.shape, v.shape, g.shape
+    if len(qs) != dims or qs != k.shape or len(vs) != dims or qs[:dims - 2] != vs[:dims - 2]:
         raise RuntimeError(f"{name}: q and k of one shape, v with the same batch{' and length' if dims == 4 else ''} expected")
-    if q.shape[-2] == 0 or heads % q.shape[-2] != 0:
+    heads, dv = vs[-2:]
+    if qs[-2] == 0 or heads % qs[-2] != 0:
         raise RuntimeError(f"{name}: the heads of v must be a multiple of the groups of q and k")
-    if not (1 <= q.shape[-1] <= MAX_SIZE and 1 <= dv <= MAX_SIZE):
+    if not (1 <= qs[-1] <= MAX_SIZE and 1 <= dv <= MAX_SIZE):
         raise RuntimeError(f"{name}: head sizes must be 1 to {MAX_SIZE}")
-    if tuple(g.shape) not in ((heads,), tuple(v.shape[:-1])):
+    if gs != vs[:-1] and (len(gs) != 1 or gs[0] != heads):
         raise RuntimeError(f"{name}: g must be ({'batch, length, ' if dims == 4 else 'batch, '}heads) or (heads,)")
-    if q.dtype not in _DT or k.dtype != q.dtype or v.dtype != q.dtype or g.dtype not in (torch.float32, q.dtype):
+    dtype = q.dtype
+    if dtype not in _DT or k.dtype != dtype or v.dtype != dtype or g.dtype != dtype and g.dtype != torch.float32:
         raise RuntimeError(f"{name}: q, k and v must be float32 / float16 / bfloat16 of one dtype, g float32 or of that dtype")
-    for t in (q, k, v, g, state):
-        if t is not None and (not t.is_cuda or t.device != q.device):
-            raise RuntimeError(f"{name}: all operands must be CUDA tensors on one device")
+    device = q.get_device()
+    if device < 0 or k.get_device() != device or v.get_device() != device or g.get_device() != device or state is not None and state.get_device() != device:
+        raise RuntimeError(f"{name}: all operands must be CUDA tensors on one device")
 
 
 def linear_attention_fn(q, k, v, g, scale=1.0, initial_state=None, return_last_state=False):
@@ -134,26 +136,28 @@ def linear_attention_step(state, q, k, v, g, scale=1.0, state_batch_indices=None
     state and gives zeros.  Returns out (batch, heads, dv).  No gradient; legal inside CUDA-graph capture."""
     _check("linear_attention_step", 3, q, k, v, g, state)
     batch, heads, dv = v.shape
-    if state.dim() != 4 or tuple(state.shape[1:]) != (heads, q.shape[-1], dv) or state.stride(-1) != 1 and dv > 1:
+    _, groups, dk = q.shape
+    slots, ss = state.shape[0], state.stride()
+    if state.shape[1:] != (heads, dk, dv) or ss[3] != 1 and dv > 1:
         raise RuntimeError("linear_attention_step: state must be (batch, heads, dk, dv) with dv contiguous")
-    if state.dtype not in (torch.float32, q.dtype):
+    if state.dtype != q.dtype and state.dtype != torch.float32:
         raise RuntimeError("linear_attention_step: the state must be float32 or of the dtype of q")
     if state_batch_indices is None:
-        if state.shape[0] != batch:
+        if slots != batch:
             raise RuntimeError("linear_attention_step: state and q must have the same batch")
-    elif (tuple(state_batch_indices.shape) != (batch,) or state_batch_indices.dtype != torch.int32 or not state_batch_indices.is_contiguous()
-          or state_batch_indices.device != q.device):
+    elif (state_batch_indices.shape != (batch,) or state_batch_indices.dtype != torch.int32 or not state_batch_indices.is_contiguous()
+          or state_batch_indices.get_device() != q.get_device()):
         raise RuntimeError("linear_attention_step: state_batch_indices must be a contiguous int32 tensor (batch,) on the device of q")
     q, k, v = _inner(q), _inner(k), _inner(v)
     pack, codes = _step_setup()
-    sq, sk, sv, sg, ss = q.stride(), k.stride(), v.stride(), g.stride(), state.stride()
+    sq, sk, sv, sg = q.stride(), k.stride(), v.stride(), g.stride()
     with _lib.on_device(q):
-        out = torch.empty(batch, heads, dv, dtype=v.dtype, device=v.device)
+        out = v.new_empty((batch, heads, dv))
         if batch == 0:
             return out
         _lib.call("b200_linattn_step",
-                  pack(batch, heads, q.shape[1], q.shape[2], dv, codes[q.dtype], codes[g.dtype], codes[state.dtype], scale, state.shape[0], state.data_ptr(),
+                  pack(batch, heads, groups, dk, dv, codes[q.dtype], codes[g.dtype], codes[state.dtype], scale, slots, state.data_ptr(),
                        q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), 0 if state_batch_indices is None else state_batch_indices.data_ptr(),
-                       out.data_ptr(), ss[0], ss[1], ss[2], sq[0], sq[1], sk[0], sk[1], sv[0], sv[1], sg[0] if g.dim() == 2 else 0, sg[-1], heads * dv, dv),
+                       out.data_ptr(), ss[0], ss[1], ss[2], sq[0], sq[1], sk[0], sk[1], sv[0], sv[1], sg[0] if len(sg) == 2 else 0, sg[-1], heads * dv, dv),
                   _lib.stream_of(q))
     return out
