@@ -13,6 +13,7 @@
 #include "common.cuh"
 #include "dispatch.h"
 #include <cstring>
+#include <type_traits>
 
 namespace b200 {
 namespace {
@@ -22,26 +23,26 @@ constexpr int SORT_T = 1024, SORT_WARPS = SORT_T / 32, CLUSTER = 8;
 constexpr int MAX_BITS = 9, MAX_BINS = 1 << MAX_BITS;
 constexpr int ROW_T = 128;
 
+// VEC consecutive elements as floats, by one access of up to 16 bytes
+template <int BYTES> struct Word;
+template <> struct Word<2> { typedef uint16_t type; };
+template <> struct Word<4> { typedef uint32_t type; };
+template <> struct Word<8> { typedef uint2 type; };
+template <> struct Word<16> { typedef uint4 type; };
 template <typename T, int VEC> struct Row {
-  // VEC consecutive elements as floats, by one access of 16 bytes where VEC > 1
-  static __device__ __forceinline__ void load(const T *p, float (&v)[VEC]) {
-    if constexpr (VEC == 1) v[0] = (float)*p;
-    else {
-      const uint4 w = __ldg(reinterpret_cast<const uint4 *>(p));
-      const T *e = reinterpret_cast<const T *>(&w);
+  typedef typename Word<VEC * sizeof(T)>::type W;
+  static __device__ __forceinline__ W raw(const T *p) { return __ldg(reinterpret_cast<const W *>(p)); }
+  static __device__ __forceinline__ void open(const W &w, float (&v)[VEC]) {
+    const T *e = reinterpret_cast<const T *>(&w);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) v[i] = (float)e[i];
-    }
+    for (int i = 0; i < VEC; ++i) v[i] = (float)e[i];
   }
   static __device__ __forceinline__ void store(T *p, const float (&v)[VEC]) {
-    if constexpr (VEC == 1) *p = T(v[0]);
-    else {
-      uint4 w;
-      T *e = reinterpret_cast<T *>(&w);
+    W w;
+    T *e = reinterpret_cast<T *>(&w);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) e[i] = T(v[i]);
-      *reinterpret_cast<uint4 *>(p) = w;
-    }
+    for (int i = 0; i < VEC; ++i) e[i] = T(v[i]);
+    *reinterpret_cast<W *>(p) = w;
   }
 };
 
@@ -49,23 +50,38 @@ __device__ __forceinline__ int64_t id_at(const void *ids, int wide, int64_t t) {
   return wide ? reinterpret_cast<const int64_t *>(ids)[t] : reinterpret_cast<const int32_t *>(ids)[t];
 }
 
-template <typename T, int VEC> __global__ void __launch_bounds__(256) embed_fwd_kernel(const b200_embed_args p) {
-  const int per = (p.features + VEC - 1) / VEC;
-  const int64_t n = p.tokens * per;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const int64_t t = n <= 0xffffffffll ? (int64_t)((uint32_t)i / (uint32_t)per) : i / per;
-    const int c = (int)(i - t * per) * VEC;
+// A warp takes up to FWD_PER accesses a lane of one row.
+constexpr int FWD_PER = 4;
+template <typename T, int VEC> __global__ void __launch_bounds__(256) embed_fwd_kernel(const b200_embed_args p, int parts) {
+  const int lane = threadIdx.x & 31, per = p.features / VEC;
+  const int64_t n = p.tokens * parts, step = (int64_t)gridDim.x * 8;
+  for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < n; i += step) {
+    const int64_t t = parts == 1 ? i : i / parts;
+    const int c0 = (int)(i - t * parts) * (FWD_PER * 32) + lane;
     const int64_t id = id_at(p.ids, p.ids_wide, t);
-    float v[VEC];
+    T *out = reinterpret_cast<T *>(p.out) + t * p.out_rs;
     if (id >= 0 && id < p.classes) {
-      Row<T, VEC>::load(reinterpret_cast<const T *>(p.weight) + id * p.weight_rs + c, v);
+      const T *row = reinterpret_cast<const T *>(p.weight) + id * p.weight_rs;
+      typename Row<T, VEC>::W w[FWD_PER];
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) v[j] *= p.scale;
+      for (int j = 0; j < FWD_PER; ++j)
+        if (c0 + j * 32 < per) w[j] = Row<T, VEC>::raw(row + (c0 + j * 32) * VEC);
+#pragma unroll
+      for (int j = 0; j < FWD_PER; ++j)
+        if (c0 + j * 32 < per) {
+          float v[VEC];
+          Row<T, VEC>::open(w[j], v);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) v[e] *= p.scale;
+          Row<T, VEC>::store(out + (c0 + j * 32) * VEC, v);
+        }
     } else {
+      float v[VEC];
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) v[j] = __int_as_float(0x7fffffff);      // no such row: NaN
+      for (int e = 0; e < VEC; ++e) v[e] = __int_as_float(0x7fffffff);      // no such row: NaN
+      for (int j = 0; j < FWD_PER; ++j)
+        if (c0 + j * 32 < per) Row<T, VEC>::store(out + (c0 + j * 32) * VEC, v);
     }
-    Row<T, VEC>::store(reinterpret_cast<T *>(p.out) + t * p.out_rs + c, v);
   }
 }
 
@@ -155,8 +171,8 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(SORT_T) embed_
     }
     if (lane == 31) ws[w] = inc;
     __syncthreads();
-    uint32_t lower = 0;
-    for (int j = 0; j < w; ++j) lower += ws[j];
+    uint32_t lower = lane < w ? ws[lane] : 0;                    // of the warps before
+    lower = __reduce_add_sync(0xffffffffu, lower);
     if (tid < bins) base[tid] = lower + inc - all + before;
     cluster_sync();                                              // counts have been read
     for (int64_t i = t0; i < t1; i += 32) {
@@ -173,7 +189,7 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(SORT_T) embed_
       if (t < t1 && (peers >> lane) == 1u) mine[d] += __popc(peers);
       __syncwarp();
     }
-    cluster_sync();                                              // places are written, and visible to the cluster
+    if (pass + 1 < q.passes) cluster_sync();                     // places are written, and visible to the cluster
   }
 }
 
@@ -200,33 +216,33 @@ __global__ void __launch_bounds__(ROW_T) embed_sum_kernel(const b200_embed_args 
 #pragma unroll
   for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
   bool came_in = k[0] == k[1];
-  for (int i0 = 0; i0 < n; i0 += 8) {
-    float v[8][VEC];
+  typename Row<T, VEC>::W w[PIECE];                            // all rows of the piece in flight
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i0 + i < n && k[i0 + i + 1] < (uint32_t)p.classes) Row<T, VEC>::load(dout + (int64_t)at[i0 + i] * p.dout_rs, v[i]);
+  for (int i = 0; i < PIECE; ++i)
+    if (i < n && k[i + 1] < (uint32_t)p.classes) w[i] = Row<T, VEC>::raw(dout + (int64_t)at[i] * p.dout_rs);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (i0 + i >= n) break;
-      const uint32_t key = k[i0 + i + 1];
-      if (key >= (uint32_t)p.classes) return;                 // these sort behind all others
+  for (int i = 0; i < PIECE; ++i) {
+    if (i >= n) break;
+    const uint32_t key = k[i + 1];
+    if (key >= (uint32_t)p.classes) return;                    // these sort behind all others
+    float v[VEC];
+    Row<T, VEC>::open(w[i], v);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) acc[j] += v[i][j];
-      const bool ends = k[i0 + i + 2] != key;
-      if (!ends && i0 + i + 1 < n) continue;
-      if (ends && !came_in) {
+    for (int j = 0; j < VEC; ++j) acc[j] += v[j];
+    const bool ends = k[i + 2] != key;
+    if (!ends && i + 1 < n) continue;
+    if (ends && !came_in) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) acc[j] *= p.scale;
-        Row<T, VEC>::store(dw + (int64_t)key * p.dweight_rs, acc);
-      } else {
-        float *o = (came_in ? head : tail) + (int64_t)blockIdx.x * p.features + c;
+      for (int j = 0; j < VEC; ++j) acc[j] *= p.scale;
+      Row<T, VEC>::store(dw + (int64_t)key * p.dweight_rs, acc);
+    } else {
+      float *o = (came_in ? head : tail) + (int64_t)blockIdx.x * p.features + c;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) o[j] = acc[j];
-      }
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
-      came_in = false;
+      for (int j = 0; j < VEC; ++j) o[j] = acc[j];
     }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
+    came_in = false;
   }
 }
 
@@ -305,24 +321,33 @@ int check_embed(const b200_embed_args &a, bool bwd) {
   return 0;
 }
 
-bool al16(const void *p, int64_t rs, int esz) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && rs * esz % 16 == 0; }
+// The widest access, in elements, that rows of two tensors allow.
+template <typename T> int widest(int features, const void *p, int64_t p_rs, const void *q, int64_t q_rs) {
+  const uint64_t all = (uint64_t)features * sizeof(T) | reinterpret_cast<uintptr_t>(p) | (uint64_t)p_rs * sizeof(T) | reinterpret_cast<uintptr_t>(q) | (uint64_t)q_rs * sizeof(T);
+  int bytes = 16;
+  while (bytes > (int)sizeof(T) && all % bytes) bytes >>= 1;
+  return bytes / (int)sizeof(T);
+}
+// f of that width as a constant
+template <typename T, typename F> void with_width(int vec, F f) {
+  if (vec == 1) f(std::integral_constant<int, 1>());
+  else if (vec == 2) f(std::integral_constant<int, 2>());
+  else if (vec == 4) f(std::integral_constant<int, 4>());
+  else if constexpr (sizeof(T) == 2) f(std::integral_constant<int, 8>());
+}
 
 template <typename T> int run_fwd(const b200_embed_args &a, cudaStream_t st) {
-  constexpr int V = 16 / sizeof(T);
-  const bool vec = a.features % V == 0 && al16(a.weight, a.weight_rs, sizeof(T)) && al16(a.out, a.out_rs, sizeof(T));
-  const int64_t n = a.tokens * (vec ? a.features / V : a.features), blocks = (n + 255) / 256, most = int64_t(1) << 22;
-  if (vec) embed_fwd_kernel<T, V><<<(unsigned)(blocks < most ? blocks : most), 256, 0, st>>>(a);
-  else embed_fwd_kernel<T, 1><<<(unsigned)(blocks < most ? blocks : most), 256, 0, st>>>(a);
+  const int vec = widest<T>(a.features, a.weight, a.weight_rs, a.out, a.out_rs);
+  const int parts = (a.features / vec + FWD_PER * 32 - 1) / (FWD_PER * 32);
+  const int64_t blocks = (a.tokens * parts + 7) / 8, most = int64_t(1) << 20;
+  with_width<T>(vec, [&](auto v) { embed_fwd_kernel<T, decltype(v)::value><<<(unsigned)(blocks < most ? blocks : most), 256, 0, st>>>(a, parts); });
   return launch_status();
 }
 
 template <typename T> int run_sums(const b200_embed_args &a, const Sort &s, const uint32_t *keys, const uint32_t *pos, float *head, float *tail, cudaStream_t st) {
-  constexpr int V = 16 / sizeof(T);
-  const bool vec = a.features % V == 0 && al16(a.dout, a.dout_rs, sizeof(T)) && al16(a.dweight, a.dweight_rs, sizeof(T));
-  const int cols = ROW_T * (vec ? V : 1);
-  const dim3 grid((unsigned)s.pieces, (unsigned)((a.features + cols - 1) / cols));
-  if (vec) embed_sum_kernel<T, V><<<grid, ROW_T, 0, st>>>(a, keys, pos, head, tail);
-  else embed_sum_kernel<T, 1><<<grid, ROW_T, 0, st>>>(a, keys, pos, head, tail);
+  const int vec = widest<T>(a.features, a.dout, a.dout_rs, a.dweight, a.dweight_rs);
+  const dim3 grid((unsigned)s.pieces, (unsigned)((a.features / vec + ROW_T - 1) / ROW_T));
+  with_width<T>(vec, [&](auto v) { embed_sum_kernel<T, decltype(v)::value><<<grid, ROW_T, 0, st>>>(a, keys, pos, head, tail); });
   if (int e = launch_status()) return e;
   if (s.pieces > 1) embed_join_kernel<T><<<dim3((unsigned)s.pieces, (unsigned)((a.features + JOIN_C - 1) / JOIN_C)), 256, 0, st>>>(a, keys, head, tail, (int)s.pieces);
   return launch_status();
