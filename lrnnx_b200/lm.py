@@ -6,8 +6,9 @@ use: Mamba mixers, RMSNorm, tied embeddings, no MLP (lrnnx/architectures/languag
 parameters carry lrnnx's names, so a state dict of the reference model loads unchanged
 (``dtA_proj``, which only the event mode reads, is accepted and ignored).
 
-What runs where: embedding, the four projections of a block and the LM head are library GEMMs
-(torch / cuBLAS: plumbing around the path); residual add + RMSNorm, the causal convolution and
+What runs where: the four projections of a block and the LM head's logits are library GEMMs
+(torch / cuBLAS: plumbing around the path); the embedding and its gradient, the loss without logits
+(``loss``), residual add + RMSNorm, the causal convolution and
 the selective scan (training / prefill) and the convolution update and selective state update
 (decoding) are this package's CUDA kernels.  lrnnx has no LM-level generation loop (its
 ``generate`` drives single mixer layers from a float buffer, lrnnx/utils/generation.py:26-162);
@@ -22,6 +23,8 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .ops.embedding import token_embedding
+from .ops.linear_cross_entropy import linear_cross_entropy
 from .ops.linear_step import linear_step
 from .ops.mamba_block import causal_conv1d_fn, causal_conv1d_update, rms_norm_fn
 from .ops.mamba_inner import mamba_inner_fn
@@ -157,7 +160,7 @@ class Backbone(nn.Module):
         self.norm_f = RMSNorm(d_model, eps, device=device, dtype=dtype)
 
     def forward(self, input_ids, caches=None):
-        hidden = self.embedding(input_ids)
+        hidden = token_embedding(input_ids, self.embedding.weight)
         residual = None
         for i, layer in enumerate(self.layers):
             normed, residual = layer.norm(hidden, residual, prenorm=True, residual_in_fp32=self.residual_in_fp32)
@@ -165,7 +168,7 @@ class Backbone(nn.Module):
         return self.norm_f(hidden, residual)
 
     def step(self, token_ids, caches):
-        hidden = self.embedding(token_ids)
+        hidden = token_embedding(token_ids, self.embedding.weight)
         residual = None
         for i, layer in enumerate(self.layers):
             normed, residual = layer.norm(hidden, residual, prenorm=True, residual_in_fp32=self.residual_in_fp32)
@@ -204,6 +207,12 @@ class MambaLMHeadModel(nn.Module):
         if num_last_tokens > 0:
             hidden = hidden[:, -num_last_tokens:]
         return self.lm_head(hidden)
+
+    def loss(self, input_ids, labels, ignore_index=-100, reduction="mean"):
+        """``cross_entropy(self(input_ids), labels)`` without the logits: labels (batch, L) are the tokens
+        that follow, ``ignore_index`` where none counts; the mean (``reduction``: "mean", "sum", "none") in
+        float32."""
+        return linear_cross_entropy(self.backbone(input_ids), self.lm_head.weight, labels, ignore_index, reduction)
 
     def step(self, token_ids, caches):
         """token_ids (batch,) -> logits (batch, vocab); caches advance in place."""
