@@ -32,7 +32,6 @@ using namespace tc;
 
 constexpr int CH = 64;                    // steps of a chunk
 constexpr int DO = 64;                    // output columns of a block
-constexpr int WT = 512;                   // threads of a block: 16 warps of 16 x 16 scores and results each
 constexpr int MAX_D = 128;
 constexpr int PP = CH + 4, PV = DO + 8;   // pitches of scores and of values / state (in floats)
 constexpr int kSnapSteps = 512;           // steps between the states that the gradient of g is anchored at
@@ -162,10 +161,10 @@ __device__ __forceinline__ uint32_t tf32(float x) {
   return y;
 }
 
-// acc (16 x 16 of a warp, two 8-column tiles) += A (16 x K) B (K x 16).  A(m, k) = a[m * AM + k * AK] * wk[k] (wk nullable), B(k, n) = b[k * BK + n * BN].
+// acc (16 x 8 NT of a warp) += A (16 x K) B (K x 8 NT).  A(m, k) = a[m * AM + k * AK] * wk[k] (wk nullable), B(k, n) = b[k * BK + n * BN].
 // An operand whose values have at most 11 bits (16-bit inputs) is exact in TF32; others are split in two: a b ~ a_hi b_hi + a_lo b_hi + a_hi b_lo.
-template <bool SPLIT_A, bool SPLIT_B, int AM, int AK, int BK, int BN>
-__device__ __forceinline__ void product(float (&acc)[2][4], const float *a, const float *wk, const float *b, int K, int lane) {
+template <bool SPLIT_A, bool SPLIT_B, int AM, int AK, int BK, int BN, int NT>
+__device__ __forceinline__ void product(float (&acc)[NT][4], const float *a, const float *wk, const float *b, int K, int lane) {
   const int g = lane >> 2, t = lane & 3;
   a += g * AM + t * AK;
   b += t * BK + g * BN;
@@ -186,7 +185,7 @@ __device__ __forceinline__ void product(float (&acc)[2][4], const float *a, cons
       al[i] = SPLIT_A ? tf32(av[i] - __uint_as_float(ah[i])) : 0u;
     }
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
+    for (int n = 0; n < NT; ++n) {
       const float bv[2] = {b[n * 8 * BN], b[n * 8 * BN + 4 * BK]};
       uint32_t bh[2], bl[2];
 #pragma unroll
@@ -207,7 +206,7 @@ __device__ __forceinline__ void product(float (&acc)[2][4], const float *a, cons
 
 // 64 rows of an operand from step i0 on into shared memory as float32, zero past the sequence and past its size: 16 threads a
 // row, 4 columns each.
-template <typename T>
+template <typename T, int WT>
 __device__ __forceinline__ void load_rows(const Walk &p, const void *base, int64_t off, int64_t ls, int i0, int col0, int size, int width, int pitch, float *dst) {
   const T *src = reinterpret_cast<const T *>(base) + off + col0;
   const bool vec = ((reinterpret_cast<uintptr_t>(src) | (uintptr_t)(ls * sizeof(T))) & (4 * sizeof(T) - 1)) == 0;
@@ -242,22 +241,26 @@ __device__ __forceinline__ void load_rows(const Walk &p, const void *base, int64
   }
 }
 
-// eight threads a row, 16 columns each, of at most 64 (128) columns
+// the cache lines of the rows: four threads a row, 32 columns apart
 template <typename T>
 __device__ __forceinline__ void prefetch_rows(const Walk &p, const void *base, int64_t off, int64_t ls, int i0, int col0, int size) {
-  const int t = time_of(p, i0 + (threadIdx.x >> 3)), c = (threadIdx.x & 7) * 16;
-  if (t < p.length && c < min(size - col0, MAX_D))
+  const int t = time_of(p, i0 + (threadIdx.x >> 2)), c = (threadIdx.x & 3) * 32;
+  if (threadIdx.x < CH * 4 && t < p.length && c < min(size - col0, MAX_D))
     asm volatile("prefetch.global.L1 [%0];" ::"l"(reinterpret_cast<const T *>(base) + off + (int64_t)t * ls + col0 + c));
 }
 
-template <typename T, int DI, bool STATE_ONLY> __global__ void __launch_bounds__(WT, 1) linattn_walk_kernel(const Walk p) {
+// WT threads: a warp has 16 x 8 NT scores and results.  With 512 a block is done with a chunk sooner; where there are
+// more blocks than SMs and two fit (up to 64 rows of state), two of 256 get through more (2 x 640 steps x 128 heads of 64 x
+// 64, float16, with gradients: 966 -> 720 us; 2 x 100 steps x 8 heads 102 -> 117 us).
+template <typename T, int DI, int WT, bool STATE_ONLY> __global__ void __launch_bounds__(WT, WT == 256 ? 2 : 1) linattn_walk_kernel(const Walk p) {
+  constexpr int NT = 1024 / WT, NW = 8 / NT;             // NW: warps along 64 columns
   constexpr bool F32 = sizeof(T) == 4;
   extern __shared__ __align__(16) float sm[];
   constexpr int PQ = DI + 4;
   const int dip = (p.di + 15) / 16 * 16;                // rows and columns in use, of DI
   float *sk = sm, *sv = sk + CH * PQ, *S = sv + CH * PV, *sq = S + DI * PV, *sp = sq + CH * PQ, *sx = sp + CH * PP;
   __shared__ Decays dd[2];
-  __shared__ float dots[4][CH], rows_[4][CH], cols_[4][CH];
+  __shared__ float dots[NW][CH], rows_[NW][CH], cols_[4][CH];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gq = lane >> 2, tq = lane & 3;
   const int tile = blockIdx.x % p.tiles, bh = blockIdx.x / p.tiles % (p.batch * p.heads), seg = blockIdx.x / p.tiles / (p.batch * p.heads);
   const int b = bh / p.heads, h = bh % p.heads, col0 = tile * DO;
@@ -286,14 +289,14 @@ template <typename T, int DI, bool STATE_ONLY> __global__ void __launch_bounds__
     const int chunk = p.rev ? p.chunks - 1 - i0 / CH : i0 / CH;
     const Decays &d = dd[it & 1];
     if (!STATE_ONLY && p.run && !p.rev && chunk % kSnap == 0) snapshot(chunk, 1.f);
-    load_rows<T>(p, p.k, b * p.k_bs + h / p.k_div * p.k_hs, p.k_ls, i0, 0, p.di, dip, PQ, sk);
-    load_rows<T>(p, p.v, b * p.v_bs + h / p.v_div * p.v_hs, p.v_ls, i0, col0, p.dout, DO, PV, sv);
+    load_rows<T, WT>(p, p.k, b * p.k_bs + h / p.k_div * p.k_hs, p.k_ls, i0, 0, p.di, dip, PQ, sk);
+    load_rows<T, WT>(p, p.v, b * p.v_bs + h / p.v_div * p.v_hs, p.v_ls, i0, col0, p.dout, DO, PV, sv);
     if (!STATE_ONLY) {
-      load_rows<T>(p, p.q, b * p.q_bs + h / p.q_div * p.q_hs, p.q_ls, i0, 0, p.di, dip, PQ, sq);
-      if (p.run) load_rows<T>(p, p.x, b * p.x_bs + h / p.x_div * p.x_hs, p.x_ls, i0, col0, p.dout, DO, PP, sx);
+      load_rows<T, WT>(p, p.q, b * p.q_bs + h / p.q_div * p.q_hs, p.q_ls, i0, 0, p.di, dip, PQ, sq);
+      if (p.run) load_rows<T, WT>(p, p.x, b * p.x_bs + h / p.x_div * p.x_hs, p.x_ls, i0, col0, p.dout, DO, PP, sx);
     }
     __syncthreads();
-    const int m0 = (warp & 3) * 16, n0 = (warp >> 2) * 16;      // this warp's 16 x 16 of scores and of results
+    const int m0 = (warp & 3) * 16, n0 = (warp >> 2) * 8 * NT;  // this warp's scores and results
     if (i0 + CH < i_end) {                           // the next chunk's rows into the first-level cache
       prefetch_rows<T>(p, p.k, b * p.k_bs + h / p.k_div * p.k_hs, p.k_ls, i0 + CH, 0, p.di);
       prefetch_rows<T>(p, p.v, b * p.v_bs + h / p.v_div * p.v_hs, p.v_ls, i0 + CH, col0, p.dout);
@@ -305,11 +308,11 @@ template <typename T, int DI, bool STATE_ONLY> __global__ void __launch_bounds__
     // the next chunk's decays, by a warp whose scores are all zero
     if (warp == 4 && i0 + CH < i_end) chunk_decays(p, b, h, i0 + CH, lane, dd[(it + 1) & 1]);
     if (!STATE_ONLY) {
-      float acc[2][4] = {};
+      float acc[NT][4] = {};
       const bool any = n0 <= m0 + 15;
-      if (any) product<F32, F32, PQ, 1, 1, PQ>(acc, sq + m0 * PQ, nullptr, sk + n0 * PQ, dip, lane);
+      if (any) product<F32, F32, PQ, 1, 1, PQ, NT>(acc, sq + m0 * PQ, nullptr, sk + n0 * PQ, dip, lane);
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int r = m0 + gq + (e >> 1) * 8, c = n0 + n * 8 + tq * 2 + (e & 1);
@@ -317,11 +320,11 @@ template <typename T, int DI, bool STATE_ONLY> __global__ void __launch_bounds__
           sp[r * PP + c] = acc[n][e];
         }
       if (p.run && p.rev) {                          // products of a pair's two scores, without the diagonal
-        float x[2][4] = {};
-        if (any) product<F32, F32, PP, 1, 1, PV>(x, sx + m0 * PP, nullptr, sv + n0 * PV, DO, lane);
+        float x[NT][4] = {};
+        if (any) product<F32, F32, PP, 1, 1, PV, NT>(x, sx + m0 * PP, nullptr, sv + n0 * PV, DO, lane);
         float row[2] = {0.f, 0.f};
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int e1 = 0; e1 < 2; ++e1) {
             const int c = n0 + n * 8 + tq * 2 + e1;
@@ -345,12 +348,12 @@ template <typename T, int DI, bool STATE_ONLY> __global__ void __launch_bounds__
       }
       __syncthreads();
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
-      product<F32, true, PQ, 1, PV, 1>(acc, sq + m0 * PQ, nullptr, S + n0, dip, lane);
+      product<F32, true, PQ, 1, PV, 1, NT>(acc, sq + m0 * PQ, nullptr, S + n0, dip, lane);
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[n][e] *= d.in[m0 + gq + (e >> 1) * 8] * p.s_inter;
       if (p.run) {
@@ -359,7 +362,7 @@ template <typename T, int DI, bool STATE_ONLY> __global__ void __launch_bounds__
           const int r = m0 + gq + e2 * 8;
           float s = 0.f;
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e1 = 0; e1 < 2; ++e1) s = fmaf(acc[n][e2 * 2 + e1], sx[r * PP + n0 + n * 8 + tq * 2 + e1], s);
           s += __shfl_xor_sync(0xffffffffu, s, 1);
@@ -367,14 +370,14 @@ template <typename T, int DI, bool STATE_ONLY> __global__ void __launch_bounds__
           if (tq == 0) dots[warp >> 2][r] = s;
         }
       }
-      product<true, F32, PP, 1, PV, 1>(acc, sp + m0 * PP, nullptr, sv + n0, min(CH, m0 + 16), lane);
+      product<true, F32, PP, 1, PV, 1, NT>(acc, sp + m0 * PP, nullptr, sv + n0, min(CH, m0 + 16), lane);
 #pragma unroll
       for (int e2 = 0; e2 < 2; ++e2) {
         const int t = time_of(p, i0 + m0 + gq + e2 * 8);
         if (t >= p.length) continue;
         const int64_t o = b * p.o_bs + t * p.o_ls + h * p.o_hs;
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int e1 = 0; e1 < 2; ++e1) {
             const int c = col0 + n0 + n * 8 + tq * 2 + e1;
@@ -392,21 +395,27 @@ template <typename T, int DI, bool STATE_ONLY> __global__ void __launch_bounds__
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int i = 2 * lane + j;
-        const float dot = (dots[0][i] + dots[1][i]) + (dots[2][i] + dots[3][i]);
+        float dot = 0.f;
+        double row = 0.0;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+          dot += dots[w][i];
+          if (p.rev) row += (double)rows_[w][i];
+        }
         s += dot;
         v[j] = dot;
-        if (p.rev) v[j] += (((double)rows_[0][i] + rows_[1][i]) + ((double)rows_[2][i] + rows_[3][i])) - (((double)cols_[0][i] + cols_[1][i]) + ((double)cols_[2][i] + cols_[3][i]));
+        if (p.rev) v[j] += row - (((double)cols_[0][i] + cols_[1][i]) + ((double)cols_[2][i] + cols_[3][i]));
       }
       chunk_runs(p, tile, bh, i0, lane, v, s);
     }
     total += d.total;
     const float keep = d.keep, keep_lo = d.keep_lo;
-    for (int u = warp; u < dip / 16 * 4; u += WT / 32) {
-      const int r0 = u / 4 * 16, c0 = u % 4 * 16;
-      float acc[2][4] = {};
-      product<true, F32, 1, PQ, PV, 1>(acc, sk + r0, d.out, sv + c0, CH, lane);
+    for (int u = warp; u < dip / 16 * NW; u += WT / 32) {
+      const int r0 = u / NW * 16, c0 = u % NW * (8 * NT);
+      float acc[NT][4] = {};
+      product<true, F32, 1, PQ, PV, 1, NT>(acc, sk + r0, d.out, sv + c0, CH, lane);
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float *s = S + (r0 + gq + (e >> 1) * 8) * PV + c0 + n * 8 + tq * 2 + (e & 1);
@@ -1241,7 +1250,7 @@ int segments(int64_t blocks, int chunks, int resident) {
 void cut(Walk &w) {
   const int chunks = w.chunks;
   w.tiles = (w.dout + DO - 1) / DO;
-  const int n = segments((int64_t)w.batch * w.heads * w.tiles, chunks, w.ch == BC ? 2 : 1);
+  const int n = segments((int64_t)w.batch * w.heads * w.tiles, chunks, w.ch == BC || w.di <= 64 ? 2 : 1);
   w.seg_chunks = (chunks + n - 1) / n;
   w.nseg = (chunks + w.seg_chunks - 1) / w.seg_chunks;
 }
@@ -1265,9 +1274,14 @@ int launch_walk(Walk &w, K own, K all, int threads, int smem_own, int smem_all, 
   all<<<(unsigned)(bh * w.tiles * w.nseg), threads, smem_all, st>>>(w, more...);
   return launch_status();
 }
-template <typename T, int DI> int walk(Walk &w, unsigned char *work, cudaStream_t st) {
-  return launch_walk(w, linattn_walk_kernel<T, DI, true>, linattn_walk_kernel<T, DI, false>, WT, walk_smem(DI, true, false), walk_smem(DI, false, w.run != nullptr), work,
-                     st);
+template <typename T, int DI, int WT> int walk(Walk &w, unsigned char *work, cudaStream_t st) {
+  return launch_walk(w, linattn_walk_kernel<T, DI, WT, true>, linattn_walk_kernel<T, DI, WT, false>, WT, walk_smem(DI, true, false),
+                     walk_smem(DI, false, w.run != nullptr), work, st);
+}
+template <typename T> int walk(Walk &w, unsigned char *work, cudaStream_t st) {
+  if (w.di > 64) return walk<T, 128, 512>(w, work, st);
+  const int64_t blocks = (int64_t)w.batch * w.heads * w.tiles * w.nseg;
+  return blocks > sm_count_current() ? walk<T, 64, 256>(w, work, st) : walk<T, 64, 512>(w, work, st);
 }
 bool map_of(CUtensorMap *m, const void *base, int size, int heads, int length, int batch, int64_t hs, int64_t ls, int64_t bs, bool f32 = false) {
   EncodeTiledFn enc = encoder();
@@ -1297,8 +1311,8 @@ template <int DI> int walk_tc(Walk &w, unsigned char *work, cudaStream_t st) {
   return launch_walk(w, linattn_walk_tc_kernel<DI, OWN_STATE>, results, BT, own, all, work, st, m, tu);
 }
 int run_walk(int dtype, Walk &w, unsigned char *work, cudaStream_t st) {
-  if (dtype == B200_F32) return w.di <= 64 ? walk<float, 64>(w, work, st) : walk<float, 128>(w, work, st);
-  if (dtype == B200_F16) return w.di <= 64 ? walk<__half, 64>(w, work, st) : walk<__half, 128>(w, work, st);
+  if (dtype == B200_F32) return walk<float>(w, work, st);
+  if (dtype == B200_F16) return walk<__half>(w, work, st);
   return w.di <= 64 ? walk_tc<64>(w, work, st) : walk_tc<128>(w, work, st);
 }
 
