@@ -642,9 +642,9 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   const auto time0 = [&](int i0) { return p.rev ? (p.chunks - 1) * BC - i0 : i0; };      // of the chunk's first step in time
-  // The first and the last warp of the diagonal have no scores of their own off it: one of them forms the next chunk's
-  // decays, the other's neighbour issues copies and products.
-  const int decay_warp = p.rev ? 3 : 4, issue_warp = p.rev ? 2 : 5;
+  // Two of the warps without scores (their blocks lie after the steps themselves): one forms the next chunk's decays while all
+  // wait for the first products, the other issues copies and products.  A third sums up the last chunk's dots meanwhile.
+  const int decay_warp = p.rev ? 3 : 4, issue_warp = p.rev ? 2 : 5, sum_warp = p.rev ? 7 : 0;
   const bool issuer = warp == issue_warp && lane == 0;
   const int hq = h / p.q_div, hk = h / p.k_div, hv = h / p.v_div, hx = h / p.x_div;
   const auto copy_qk = [&](int i0) {                     // by the issuer
@@ -680,7 +680,15 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
       for (int j = 0; j < NS; ++j)
         if (col0 + cs + j < p.dout) f(col0 + cs + j, S[j]);
   };
-  const auto snapshot = [&](int s, float f) { each([&](int c, float &x) { p.snap[(((int64_t)bh * snaps + s) * p.di + rs) * p.dout + c] = x * f; }); };
+  const auto snapshot = [&](int s, float f) {
+    float *at = p.snap + (((int64_t)bh * snaps + s) * p.di + rs) * p.dout;
+    if (p.dout % 4 == 0 && has_row && col0 + cs + NS <= p.dout) {
+#pragma unroll
+      for (int j = 0; j < NS; j += 4) *reinterpret_cast<float4 *>(at + col0 + cs + j) = make_float4(S[j] * f, S[j + 1] * f, S[j + 2] * f, S[j + 3] * f);
+    } else {
+      each([&](int c, float &x) { at[c] = x * f; });
+    }
+  };
   const auto write_terms = [&]() {
 #pragma unroll
     for (int j = 0; j < NS / 8; ++j) {
@@ -732,6 +740,10 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
 #pragma unroll
     for (int i = 0; i < DI / 16; ++i) mma_f16(tm + tP, q + kmajor(i), k + kmajor(i), kScores, i > 0);
   };
+  Four next = {};                                        // the decay warp's: logarithms of the next chunk's decays
+  if (warp == decay_warp && i_begin + BC < i_end) next = load_decays(p, b, h, i_begin + BC, lane);
+  double pairs[4] = {};                                  // the sum warp's: of the last chunk, four steps a lane
+  float dot_sum = 0.f;
   bool scores_on = false;                                // the issuer's: this chunk's are on their way since the last one
   double total = 0.0;
   for (int i0 = i_begin, it = 0; i0 < i_end; i0 += BC, ++it) {
@@ -742,9 +754,15 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
     tc_fence_before();
     __syncthreads();                                     // the state's terms are written, accumulators read
     if (*(volatile int *)&fail) break;
-    Four next = {};
-    if (warp == decay_warp && i0 + BC < i_end) next = load_decays(p, b, h, i0 + BC, lane);
     if (issuer && maps.tma && !scores_on && !mbar_wait(&loaded_qk, it & 1, kWaitLimit)) *(volatile int *)&fail = 1;
+    const auto meanwhile = [&]() {
+      if (warp == decay_warp && i0 + BC < i_end) {
+        chunk_decays_b(p, next, lane, dd[(it + 1) & 1]);
+        if (i0 + 2 * BC < i_end) next = load_decays(p, b, h, i0 + 2 * BC, lane);
+      }
+      if (grad && warp == sum_warp && it > 0) chunk_runs(p, tile, bh, i0 - BC, lane, pairs, dot_sum);
+    };
+    if (STATE_ONLY) meanwhile();
     float O[32];
     if constexpr (!STATE_ONLY) {
       if (issuer) {
@@ -759,6 +777,7 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
         mma_commit(&bar);
       }
       __syncwarp();
+      meanwhile();
       wait_products(bar, phase);
       phase ^= 1;
       {
@@ -844,8 +863,9 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
             const int c = cb * 32 + q * 16;
-            float v[16];
-            tmem_ld16(tm_own + tP + c, v);
+            float v[16], x2[16];
+            if constexpr (cross) tmem_ld16x2(tm_own + tP + c, tm_own + tO + c, v, x2);
+            else tmem_ld16(tm_own + tP + c, v);
             if (cb != wr) {
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
@@ -874,11 +894,9 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
               packed[q * 8 + j] = *reinterpret_cast<const uint32_t *>(&w);
             }
             if (cross) {                                 // products of a pair's two scores, without the diagonal
-              float x[16];
-              tmem_ld16(tm_own + tO + c, x);
 #pragma unroll
               for (int j = 0; j < 16; ++j) {
-                v[j] = c + j == r ? 0.f : v[j] * x[j];
+                v[j] = c + j == r ? 0.f : v[j] * x2[j];
                 row += v[j];
               }
               const float col = sum_columns(v, lane);
@@ -894,8 +912,6 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
       if (cross) rows_[half][r] = row;
       tmem_st_wait();
     }
-    // the next chunk's decays, by a warp whose scores are all zero
-    if (warp == decay_warp && i0 + BC < i_end) chunk_decays_b(p, next, lane, dd[(it + 1) & 1]);
     if (!cross && issuer) {                              // keys and q are free once the sum is there
       if (!mbar_wait(&bar_d, it & 1, kWaitLimit)) *(volatile int *)&fail = 1;
       if (maps.tma && i0 + BC < i_end) copy_qk(i0 + BC);
@@ -912,18 +928,16 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
       if (cross) issue_update();
       mma_commit(&bar);
     }
-    if (grad && warp == decay_warp) {
-      double v[4];
-      float s = 0.f;
+    if (grad && warp == sum_warp) {                      // before the next chunk's take their place
+      dot_sum = 0.f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int i = in_time(p, 4 * lane + j);
         const float dot = dots[0][i] + dots[1][i];
-        s += dot;
-        v[j] = dot;
-        if (cross) v[j] += ((double)rows_[0][i] + rows_[1][i]) - (((double)cols_[0][i] + cols_[1][i]) + ((double)cols_[2][i] + cols_[3][i]));
+        dot_sum += dot;
+        pairs[j] = dot;
+        if (cross) pairs[j] += ((double)rows_[0][i] + rows_[1][i]) - (((double)cols_[0][i] + cols_[1][i]) + ((double)cols_[2][i] + cols_[3][i]));
       }
-      chunk_runs(p, tile, bh, i0, lane, v, s);
     }
     __syncwarp();
     if (!cross) wait_products(bar_d, it & 1);
@@ -937,12 +951,6 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
         if (!staged) load_all(i0 + BC);                  // else once the results have left
       } else if (issuer) {
         if (cross) copy_qk(i0 + BC);
-        else if (!STATE_ONLY) {
-          if (!mbar_wait(&loaded_qk, (it + 1) & 1, kWaitLimit)) *(volatile int *)&fail = 1;
-          tc_fence_after();
-          issue_scores();
-          scores_on = true;
-        }
         if (!staged) copy_v(i0 + BC);
       }
       __syncwarp();
@@ -1026,6 +1034,11 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
       if (issuer) {
         bulk_wait_read<0>();
         if (maps.tma) copy_v(i0 + BC);
+        if (maps.tma && !cross && mbar_wait(&loaded_qk, (it + 1) & 1, 1)) {      // where they have arrived, the next scores start now
+          tc_fence_after();
+          issue_scores();
+          scores_on = true;
+        }
       }
       __syncwarp();
       if (!maps.tma) {
@@ -1034,6 +1047,7 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
       }
     }
   }
+  if (grad && warp == sum_warp && i_end > i_begin && !*(volatile int *)&fail) chunk_runs(p, tile, bh, i_end - BC, lane, pairs, dot_sum);
   if (!STATE_ONLY && issuer) bulk_wait<0>();
   __syncwarp();
   const bool ok = !*(volatile int *)&fail;
