@@ -71,20 +71,49 @@ __device__ __forceinline__ float ex2a(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// A sum in two floats (the second what the first leaves out): 48 bits, at a tenth of the latency of 64-bit arithmetic in a
+// chain that a whole block waits for.
+struct Two { float h, l; };
+__device__ __forceinline__ Two two(float x) { return Two{x, 0.f}; }
+__device__ __forceinline__ Two operator+(Two a, Two b) {
+  const float s = a.h + b.h, t = s - a.h;
+  const float e = ((a.h - (s - t)) + (b.h - t)) + (a.l + b.l);
+  const float h = s + e;
+  return Two{h, e - (h - s)};
+}
+__device__ __forceinline__ Two operator-(Two a) { return Two{-a.h, -a.l}; }
+__device__ __forceinline__ Two shfl_up2(Two a, int d) { return Two{__shfl_up_sync(0xffffffffu, a.h, d), __shfl_up_sync(0xffffffffu, a.l, d)}; }
+__device__ __forceinline__ Two shfl_down2(Two a, int d) { return Two{__shfl_down_sync(0xffffffffu, a.h, d), __shfl_down_sync(0xffffffffu, a.l, d)}; }
+__device__ __forceinline__ float minus(Two a, Two b) { return (a.h - b.h) + (a.l - b.l); }
+// 2^x in 64 bits: the series of 2^f for the fraction f, |f| <= 1/2, to 2^-38
+__device__ __forceinline__ double exp2_two(Two x) {
+  if (!(x.h > -1000.f && x.h < 1000.f)) return exp2((double)x.h);
+  const float n = rintf(x.h);
+  const double f = ((double)(x.h - n) + (double)x.l) * 0.6931471805599453;
+  double y = 1.0 / 3628800;
+#pragma unroll
+  for (int k = 9; k >= 0; --k) {
+    constexpr double inv[10] = {1.0, 1.0, 1.0 / 2, 1.0 / 6, 1.0 / 24, 1.0 / 120, 1.0 / 720, 1.0 / 5040, 1.0 / 40320, 1.0 / 362880};
+    y = fma(y, f, inv[k]);
+  }
+  return ldexp(y, (int)n);
+}
+
 __device__ __forceinline__ float load_g(const void *g, int dtype, int64_t i) { return ld_act(g, dtype, i); }
 
 // the time of the walk's step i (past the sequence's end where there is none)
 __device__ __forceinline__ int time_of(const Walk &p, int i) { return p.rev ? p.chunks * p.ch - 1 - i : i; }
 
 // a log decay in units of log2, bounded below; NaN stays
-__device__ __forceinline__ double log2_of(const Walk &p, int b, int h, int t) {
-  const float g = load_g(p.g, p.g_dtype, b * p.g_bs + t * p.g_ls + h * p.g_hs);
-  return g != g ? (double)g : (double)fmaxf(g, -300.f) * 1.4426950408889634;
+__device__ __forceinline__ Two to_log2(float g) {
+  const float x = g != g ? g : fmaxf(g, -300.f), y = x * 1.44269504f;      // log2 e in two floats
+  return Two{y, fmaf(x, 1.92596303e-8f, fmaf(x, 1.44269504f, -y))};
 }
+__device__ __forceinline__ Two log2_of(const Walk &p, int b, int h, int t) { return to_log2(load_g(p.g, p.g_dtype, b * p.g_bs + t * p.g_ls + h * p.g_hs)); }
 // the decay before the walk's step i: backwards that of the step after it in time
-__device__ __forceinline__ double log2_decay(const Walk &p, int b, int h, int i) {
+__device__ __forceinline__ Two log2_decay(const Walk &p, int b, int h, int i) {
   const int t = p.rev ? p.chunks * p.ch - i : i;
-  return t < p.length ? log2_of(p, b, h, t) : 0.0;
+  return t < p.length ? log2_of(p, b, h, t) : two(0.f);
 }
 
 // What the chunk's decays come to, by one warp, two steps a lane: sums from the chunk's start in two floats, their
@@ -92,33 +121,36 @@ __device__ __forceinline__ double log2_decay(const Walk &p, int b, int h, int i)
 struct Decays {
   float hi[CH], lo[CH], in[CH], out[CH];
   float keep, keep_lo;                    // of the state over the chunk, in two floats: it is multiplied up over all chunks
-  double total;
+  Two total;
 };
-__device__ __forceinline__ void chunk_decays(const Walk &p, int b, int h, int i0, int lane, Decays &d) {
-  const double a0 = log2_decay(p, b, h, i0 + 2 * lane), a1 = log2_decay(p, b, h, i0 + 2 * lane + 1);
-  double s = a0 + a1;
+template <typename D> __device__ __forceinline__ void keep_of(D &d, Two end) {
+  const double keep = exp2_two(end);
+  d.keep = (float)keep;
+  d.keep_lo = end.h <= 0.f ? (float)(keep - (double)d.keep) : 0.f;
+  d.total = end;
+}
+__device__ __forceinline__ Two inclusive(Two s, int lane) {
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const double u = __shfl_up_sync(0xffffffffu, s, o);
-    if (lane >= o) s += u;
+    const Two u = shfl_up2(s, o);
+    if (lane >= o) s = s + u;
   }
-  const double end = __shfl_sync(0xffffffffu, s, 31);
-  const double G[2] = {s - a1, s};
+  return s;
+}
+__device__ __forceinline__ Two from_lane(Two s, int lane) { return Two{__shfl_sync(0xffffffffu, s.h, lane), __shfl_sync(0xffffffffu, s.l, lane)}; }
+__device__ __forceinline__ void chunk_decays(const Walk &p, int b, int h, int i0, int lane, Decays &d) {
+  const Two a0 = log2_decay(p, b, h, i0 + 2 * lane), a1 = log2_decay(p, b, h, i0 + 2 * lane + 1);
+  const Two s = inclusive(a0 + a1, lane), end = from_lane(s, 31);
+  const Two G[2] = {s + -a1, s};
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const int i = 2 * lane + j;
-    const float hi = (float)G[j];
-    d.hi[i] = hi;
-    d.lo[i] = (float)(G[j] - (double)hi);
-    d.in[i] = ex2a(hi);
-    d.out[i] = ex2a((float)(end - G[j])) * p.s_update;
+    d.hi[i] = G[j].h;
+    d.lo[i] = G[j].l;
+    d.in[i] = ex2a(G[j].h);
+    d.out[i] = ex2a(minus(end, G[j])) * p.s_update;
   }
-  if (lane == 0) {
-    const double keep = exp2(end);
-    d.keep = (float)keep;
-    d.keep_lo = end <= 0.0 ? (float)(keep - (double)d.keep) : 0.f;
-    d.total = end;
-  }
+  if (lane == 0) keep_of(d, end);
 }
 // exp(G_r - G_c)
 __device__ __forceinline__ float decay_between(const Decays &d, int r, int c) { return ex2a((d.hi[r] - d.hi[c]) + (d.lo[r] - d.lo[c])); }
@@ -127,23 +159,22 @@ __device__ __forceinline__ float decay_between(const Decays &d, int r, int c) { 
 // lane, in 64 bits.  Forwards (x . dq, pairs whose earlier step is before the chunk): the sum from the step on.  Backwards (x . dk,
 // pairs whose later step is after the chunk, and pairs within it, by row and column sums without the diagonal): the sum
 // over the steps before it in time.
-template <int N> __device__ __forceinline__ void chunk_runs(const Walk &p, int tile, int bh, int i0, int lane, const double (&v)[N], float dots) {
-  double own = 0.0;
+template <int N> __device__ __forceinline__ void chunk_runs(const Walk &p, int tile, int bh, int i0, int lane, const Two (&v)[N], float dots) {
+  Two s = v[N - 1];
 #pragma unroll
-  for (int j = 0; j < N; ++j) own += v[j];
-  double s = own;
+  for (int j = N - 2; j >= 0; --j) s = s + v[j];
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const double u = __shfl_down_sync(0xffffffffu, s, o);
-    if (lane + o < 32) s += u;
+    const Two u = shfl_down2(s, o);
+    if (lane + o < 32) s = s + u;
   }
   const int64_t row = (int64_t)tile * p.batch * p.heads + bh;
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     const int t = time_of(p, i0 + N * lane + j);
-    const double r = p.rev ? s - v[j] : s;
-    if (t < p.length) p.run[row * p.length + t] = (float)r;
-    s -= v[j];
+    const Two next = s + -v[j], r = p.rev ? next : s;
+    if (t < p.length) p.run[row * p.length + t] = r.h;
+    s = next;
   }
   dots = warp_sum(dots);
   if (lane == 0) p.sum[row * p.chunks + (p.rev ? p.chunks - 1 - i0 / p.ch : i0 / p.ch)] = dots;
@@ -390,25 +421,25 @@ template <typename T, int DI, int WT, bool STATE_ONLY> __global__ void __launch_
     }
     __syncthreads();                                 // all have read the state
     if (!STATE_ONLY && p.run && warp == 0) {
-      double v[2];
+      Two v[2];
       float s = 0.f;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int i = 2 * lane + j;
         float dot = 0.f;
-        double row = 0.0;
+        Two row = two(0.f);
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
           dot += dots[w][i];
-          if (p.rev) row += (double)rows_[w][i];
+          if (p.rev) row = row + two(rows_[w][i]);
         }
         s += dot;
-        v[j] = dot;
-        if (p.rev) v[j] += row - (((double)cols_[0][i] + cols_[1][i]) + ((double)cols_[2][i] + cols_[3][i]));
+        v[j] = two(dot);
+        if (p.rev) v[j] = (v[j] + row) + -((two(cols_[0][i]) + two(cols_[1][i])) + (two(cols_[2][i]) + two(cols_[3][i])));
       }
       chunk_runs(p, tile, bh, i0, lane, v, s);
     }
-    total += d.total;
+    if (STATE_ONLY) total += (double)d.total.h + (double)d.total.l;
     const float keep = d.keep, keep_lo = d.keep_lo;
     for (int u = warp; u < dip / 16 * NW; u += WT / 32) {
       const int r0 = u / NW * 16, c0 = u % NW * (8 * NT);
@@ -424,7 +455,7 @@ template <typename T, int DI, int WT, bool STATE_ONLY> __global__ void __launch_
     }
     if (!STATE_ONLY && p.run && p.rev && chunk % kSnap == 0) {
       __syncthreads();
-      snapshot(chunk, ex2a((float)log2_of(p, b, h, chunk * CH)));
+      snapshot(chunk, (float)exp2_two(log2_of(p, b, h, chunk * CH)));
     }
   }
   __syncthreads();
@@ -435,7 +466,7 @@ template <typename T, int DI, int WT, bool STATE_ONLY> __global__ void __launch_
     }
     if (tile == 0 && tid == 0) p.seg_g[(int64_t)bh * p.nseg + seg] = total;
   } else if (p.last && seg == p.nseg - 1) {
-    const float f = p.last_decay ? ex2a((float)log2_of(p, b, h, 0)) : 1.f;
+    const float f = p.last_decay ? (float)exp2_two(log2_of(p, b, h, 0)) : 1.f;
     for (int e = tid; e < p.di * DO; e += WT) {
       const int r = e / DO, c = e % DO;
       if (col0 + c < p.dout) p.last[b * p.last_bs + h * p.last_hs + r * p.last_is + (col0 + c) * p.last_os] = S[r * PV + c] * f;
@@ -519,7 +550,7 @@ __device__ __forceinline__ void load_tile(const Walk &p, const void *base, int64
 struct DecaysB {
   float hi[BC], lo[BC], in[BC], out[BC], back[3][BC];
   float keep, keep_lo;
-  double total;
+  Two total;
 };
 __device__ __forceinline__ float between(const DecaysB &d, int r, int c) { return ex2a((d.hi[r] - d.hi[c]) + (d.lo[r] - d.lo[c])); }
 __device__ __forceinline__ int in_time(const Walk &p, int i) { return p.rev ? BC - 1 - i : i; }
@@ -549,35 +580,24 @@ __device__ __forceinline__ Four load_decays(const Walk &p, int b, int h, int i0,
   return f;
 }
 __device__ __forceinline__ void chunk_decays_b(const Walk &p, const Four &f, int lane, DecaysB &d) {
-  double a[4], s = 0.0;
+  Two a[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) a[j] = f.g[j] != f.g[j] ? (double)f.g[j] : (double)fmaxf(f.g[j], -300.f) * 1.4426950408889634;
+  for (int j = 0; j < 4; ++j) a[j] = to_log2(f.g[j]);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) { s += a[j]; a[j] = s; }
-  double inc = s;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const double u = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += u;
-  }
-  const double end = __shfl_sync(0xffffffffu, inc, 31);
-  const double before = inc - s;
+  for (int j = 1; j < 4; ++j) a[j] = a[j] + a[j - 1];
+  const Two inc = inclusive(a[3], lane), end = from_lane(inc, 31);
+  Two before = shfl_up2(inc, 1);
+  if (lane == 0) before = two(0.f);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int i = in_time(p, 4 * lane + j);
-    const double G = before + a[j];
-    const float hi = (float)G;
-    d.hi[i] = hi;
-    d.lo[i] = (float)(G - (double)hi);
-    d.in[i] = ex2a(hi);
-    d.out[i] = ex2a((float)(end - G)) * p.s_update;
+    const Two G = before + a[j];
+    d.hi[i] = G.h;
+    d.lo[i] = G.l;
+    d.in[i] = ex2a(G.h);
+    d.out[i] = ex2a(minus(end, G)) * p.s_update;
   }
-  if (lane == 0) {
-    const double keep = exp2(end);
-    d.keep = (float)keep;
-    d.keep_lo = end <= 0.0 ? (float)(keep - (double)d.keep) : 0.f;
-    d.total = end;
-  }
+  if (lane == 0) keep_of(d, end);
   __syncwarp();
 #pragma unroll
   for (int j = 1; j < 4; ++j)
@@ -742,7 +762,7 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
   };
   Four next = {};                                        // the decay warp's: logarithms of the next chunk's decays
   if (warp == decay_warp && i_begin + BC < i_end) next = load_decays(p, b, h, i_begin + BC, lane);
-  double pairs[4] = {};                                  // the sum warp's: of the last chunk, four steps a lane
+  Two pairs[4] = {};                                     // the sum warp's: of the last chunk, four steps a lane
   float dot_sum = 0.f;
   bool scores_on = false;                                // the issuer's: this chunk's are on their way since the last one
   double total = 0.0;
@@ -935,8 +955,8 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
         const int i = in_time(p, 4 * lane + j);
         const float dot = dots[0][i] + dots[1][i];
         dot_sum += dot;
-        pairs[j] = dot;
-        if (cross) pairs[j] += ((double)rows_[0][i] + rows_[1][i]) - (((double)cols_[0][i] + cols_[1][i]) + ((double)cols_[2][i] + cols_[3][i]));
+        pairs[j] = two(dot);
+        if (cross) pairs[j] = (pairs[j] + (two(rows_[0][i]) + two(rows_[1][i]))) + -((two(cols_[0][i]) + two(cols_[1][i])) + (two(cols_[2][i]) + two(cols_[3][i])));
       }
     }
     __syncwarp();
@@ -1027,8 +1047,8 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
 #pragma unroll
       for (int j = 0; j < NS; ++j) S[j] = fmaf(S[j], keep, fmaf(S[j], keep_lo, v[j]));
     }
-    total += d.total;
-    if (cross && chunk % kSnapB == 0) snapshot(chunk / kSnapB, (float)exp2(log2_of(p, b, h, chunk * BC)));
+    if (STATE_ONLY) total += (double)d.total.h + (double)d.total.l;
+    if (cross && chunk % kSnapB == 0) snapshot(chunk / kSnapB, (float)exp2_two(log2_of(p, b, h, chunk * BC)));
     if (!STATE_ONLY) write_terms();
     if (staged && more) {
       if (issuer) {
@@ -1055,7 +1075,7 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
     each([&](int c, float &x) { p.seg[(((int64_t)bh * p.nseg + seg) * p.di + rs) * p.dout + c] = x; });
     if (tile == 0 && tid == 0) p.seg_g[(int64_t)bh * p.nseg + seg] = total;
   } else if (!STATE_ONLY && ok && p.last && seg == p.nseg - 1) {
-    const float f = p.last_decay ? (float)exp2(log2_of(p, b, h, 0)) : 1.f;
+    const float f = p.last_decay ? (float)exp2_two(log2_of(p, b, h, 0)) : 1.f;
     each([&](int c, float &x) { p.last[b * p.last_bs + h * p.last_hs + rs * p.last_is + c * p.last_os] = x * f; });
   }
   tc_fence_before();
