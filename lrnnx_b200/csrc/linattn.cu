@@ -1200,6 +1200,8 @@ __global__ void linattn_dg_heads_kernel(const b200_linattn_args p, const double 
 
 // A block takes a (batch entry, head): the state is read and written once, 16 bytes an access where its rows allow it.  Threads
 // along the state's rows of dv, and groups of them along dk whose sums are joined in shared memory.
+template <typename TS, int VEC> struct Piece { typedef uint4 type; };
+template <typename TS> struct Piece<TS, 1> { typedef TS type; };
 template <typename TS, typename T, int VEC> __global__ void __launch_bounds__(128) linattn_step_kernel(const b200_linattn_step_args p) {
   __shared__ float sh[128 * VEC], sq[MAX_D], sk[MAX_D];
   const int b = blockIdx.x / p.heads, h = blockIdx.x % p.heads, grp = h / (p.heads / p.groups), tid = threadIdx.x;
@@ -1213,14 +1215,26 @@ template <typename TS, typename T, int VEC> __global__ void __launch_bounds__(12
       return;
     }
   }
+  const int across = (p.dv + VEC - 1) / VEC, along = 128 / across;           // threads along dv (at most 128) and along dk
+  const int cx = tid % across, ry = tid / across, c0 = cx * VEC;
+  typename Piece<TS, VEC>::type *S = reinterpret_cast<typename Piece<TS, VEC>::type *>(reinterpret_cast<TS *>(p.state) + slot * p.state_bs + h * p.state_hs + c0);
+  const int64_t row = p.state_ks / VEC;
+  // the state's rows are on their way before anything else is
+  constexpr int AHEAD = 8;
+  typename Piece<TS, VEC>::type e[AHEAD];
+  const auto load = [&](int r0) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int r = r0 + i * along;
+      if (ry < along && r < p.dk) e[i] = S[r * row];
+    }
+  };
+  load(ry);
   for (int i = tid; i < p.dk; i += 128) {
     sq[i] = (float)reinterpret_cast<const T *>(p.q)[b * p.q_bs + grp * p.q_gs + i] * p.scale;
     sk[i] = (float)reinterpret_cast<const T *>(p.k)[b * p.k_bs + grp * p.k_gs + i];
   }
   const float a = expf(load_g(p.g, p.g_dtype, b * p.g_bs + h * p.g_hs));
-  const int across = (p.dv + VEC - 1) / VEC, along = 128 / across;           // threads along dv (at most 128) and along dk
-  const int cx = tid % across, ry = tid / across, c0 = cx * VEC;
-  TS *S = reinterpret_cast<TS *>(p.state) + slot * p.state_bs + h * p.state_hs + c0;
   __syncthreads();
   float acc[VEC], vv[VEC];
 #pragma unroll
@@ -1229,20 +1243,21 @@ template <typename TS, typename T, int VEC> __global__ void __launch_bounds__(12
     vv[j] = (float)v[c0 + j];
   }
   if (ry < along) {
-#pragma unroll 4
-    for (int r = ry; r < p.dk; r += along) {
-      TS *s = S + (int64_t)r * p.state_ks;
-      TS e[VEC];
-      if constexpr (VEC > 1) *reinterpret_cast<uint4 *>(e) = *reinterpret_cast<const uint4 *>(s);
-      else e[0] = *s;
+    for (int r0 = ry; r0 < p.dk; r0 += AHEAD * along) {
+      if (r0 > ry) load(r0);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float x = fmaf(a, (float)e[j], sk[r] * vv[j]);
-        acc[j] = fmaf(sq[r], x, acc[j]);
-        e[j] = TS(x);
+      for (int i = 0; i < AHEAD; ++i) {
+        const int r = r0 + i * along;
+        if (r >= p.dk) break;
+        TS *x = reinterpret_cast<TS *>(&e[i]);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const float y = fmaf(a, (float)x[j], sk[r] * vv[j]);
+          acc[j] = fmaf(sq[r], y, acc[j]);
+          x[j] = TS(y);
+        }
+        S[r * row] = e[i];
       }
-      if constexpr (VEC > 1) *reinterpret_cast<uint4 *>(s) = *reinterpret_cast<const uint4 *>(e);
-      else *s = e[0];
     }
   }
 #pragma unroll
