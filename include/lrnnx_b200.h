@@ -552,7 +552,7 @@ int b200_lce_bwd(const b200_lce_args *args, void *stream);
 
 /* ------------------------------------------------------------------------
  * Embedding lookup with a scale, and its gradient by sorted tokens; replaces nn.Embedding in
- * lrnnx's backbone (lrnnx/architectures/language_model.py:198-240) and the scatter of its backward.
+ * lrnnx's backbone (lrnnx/architectures/language_model.py:198-511) and the scatter of its backward.
  *   out[t] = scale weight[ids[t]];  an id outside [0, classes) reads nothing and gives NaN
  *   dweight[v] = scale sum_{t: ids[t] = v} dout[t], float32 sums in the order of t; zero for other
  *   rows and for padding_idx (-1: none)

@@ -5,7 +5,8 @@ The package provides, behind lrnnx's own call surface,
     modules with the ``fwd`` / ``bwd`` functions lrnnx's compiled extensions export,
   * ``lrnnx_b200.ops``: the autograd wrappers (``selective_scan_fn``,
     ``simplified_scan_fn``, ``s5_inner_fn``, ``rglru_scan_fn``, ``s7_scan_fn``,
-    ``selective_state_update``, ``cauchy_mult``, ``log_vandermonde_cuda``),
+    ``selective_state_update``, ``cauchy_mult``, ``log_vandermonde_cuda``) and, beyond lrnnx's own,
+    ``linear_cross_entropy``, ``token_embedding``, ``linear_attention_fn`` and ``linear_attention_step``,
   * ``install()``: registers the three extension modules in ``sys.modules`` under
     the names lrnnx imports, so unmodified lrnnx Python runs on these kernels.
 

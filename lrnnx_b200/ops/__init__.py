@@ -1,5 +1,6 @@
 """Autograd wrappers with the names and signatures of ``lrnnx.ops``
-(lrnnx/ops/__init__.py:1-25)."""
+(lrnnx/ops/__init__.py:1-25), and the operators beside them that lrnnx does not have: the loss
+without logits, the embedding, linear attention."""
 from .embedding import TokenEmbeddingFn, token_embedding
 from .linear_attention import LinearAttentionFn, linear_attention_fn, linear_attention_step
 from .linear_cross_entropy import LinearCrossEntropyFn, linear_cross_entropy

@@ -1,7 +1,7 @@
 """Embedding lookup with a scale, and its gradient by sorted tokens (``b200_embed_fwd / bwd``).
 
 ``token_embedding(ids, weight)`` takes the place of nn.Embedding in the language model
-(lrnnx/architectures/language_model.py:198-240).  Its gradient adds the rows of each token in float32 in
+(lrnnx/architectures/language_model.py:198-511).  Its gradient adds the rows of each token in float32 in
 the order of their positions, so it is the same at every call, and rounds once.
 """
 from __future__ import annotations
