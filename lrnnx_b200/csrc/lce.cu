@@ -451,19 +451,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LCE_THREADS, 1) lce_
   if (tid == 0 && pipe.fail) atomicExch(&g_lce_status, 7);
 }
 
-// Rows of 16-byte pitch from rows of any: a copy for 16-bit types, three bfloat16 planes for float32.
-__global__ void __launch_bounds__(256) lce_pack_kernel(const void *src, int64_t rs, int64_t rows, int cols, int pitch, int split, uint16_t *dst) {
-  const int64_t n = rows * (pitch / 2);
+__device__ __forceinline__ bool is_target(int64_t label, int64_t ignore, int classes) { return label != ignore && label >= 0 && label < classes; }
+
+// Rows of 16-byte pitch from rows of any: a copy for 16-bit types, three bfloat16 planes for float32.  With labels, rows without a
+// target become zeros: whatever they hold (NaN in the padding of a batch) is then in no product.
+__global__ void __launch_bounds__(256) lce_pack_kernel(const void *src, int64_t rs, int64_t rows, int cols, int pitch, int split, int wide, const int64_t *labels,
+                                                      int64_t ignore, int classes, uint16_t *dst) {
+  const int per = pitch / (wide ? 8 : 2);
+  const int64_t n = rows * per;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / (pitch / 2);
-    const int c = (int)(i - r * (pitch / 2)) * 2;
-    if (!split) {
+    const int64_t r = i / per;
+    const int c = (int)(i - r * per) * (wide ? 8 : 2);
+    const bool on = !labels || is_target(labels[r], ignore, classes);
+    if (wide) {                                          // 16-bit rows of 16-byte pitch
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (on) {
+        w = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(src) + r * rs + c));
+        uint32_t *x = reinterpret_cast<uint32_t *>(&w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (c + j >= cols) x[j >> 1] &= j & 1 ? 0x0000ffffu : 0xffff0000u;
+      }
+      *reinterpret_cast<uint4 *>(dst + r * pitch + c) = w;
+    } else if (!split) {
       const uint16_t *s = reinterpret_cast<const uint16_t *>(src) + r * rs;
-      const uint32_t lo = c < cols ? s[c] : 0, hi = c + 1 < cols ? s[c + 1] : 0;
+      const uint32_t lo = on && c < cols ? s[c] : 0, hi = on && c + 1 < cols ? s[c + 1] : 0;
       *reinterpret_cast<uint32_t *>(dst + r * pitch + c) = lo | hi << 16;
     } else {
       const float *s = reinterpret_cast<const float *>(src) + r * rs;
-      float a = c < cols ? s[c] : 0.f, b = c + 1 < cols ? s[c + 1] : 0.f;
+      float a = on && c < cols ? s[c] : 0.f, b = on && c + 1 < cols ? s[c + 1] : 0.f;
 #pragma unroll
       for (int pl = 0; pl < 3; ++pl) {
         const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
@@ -474,8 +490,6 @@ __global__ void __launch_bounds__(256) lce_pack_kernel(const void *src, int64_t 
     }
   }
 }
-
-__device__ __forceinline__ bool is_target(int64_t label, int64_t ignore, int classes) { return label != ignore && label >= 0 && label < classes; }
 
 // Joins the partial maxima and sums of 32 rows: a warp reads the same slot of 32 rows.
 constexpr int JOIN_WARPS = 32;
@@ -627,12 +641,12 @@ bool in_place(const void *p, int64_t rs, int cols) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && rs % 8 == 0 && rs >= cols && rs < (int64_t(1) << 36);
 }
 
-Plan plan_of(const b200_lce_args &a) {
+Plan plan_of(const b200_lce_args &a, bool bwd) {
   Plan q;
   const bool f32 = a.dtype == B200_F32;
   q.planes = f32 ? 3 : 1;
   q.Dp = (int)up(a.features, 8);
-  q.pack_h = f32 || !in_place(a.hidden, a.hidden_rs, a.features);
+  q.pack_h = f32 || bwd || !in_place(a.hidden, a.hidden_rs, a.features);      // backwards: a copy without the rows that have no target
   q.pack_w = f32 || !in_place(a.weight, a.weight_rs, a.features);
   q.pack_bytes_h = q.pack_h ? up(2 * q.planes * a.rows * q.Dp, 256) : 0;
   q.pack_bytes_w = q.pack_w ? up(2 * q.planes * (int64_t)a.classes * q.Dp, 256) : 0;
@@ -669,10 +683,12 @@ int check_lce(const b200_lce_args &a) {
   return 0;
 }
 
-int pack(const void *src, int64_t rs, int64_t rows, const b200_lce_args &a, const Plan &q, void *dst, cudaStream_t st) {
-  const int64_t n = rows * (q.Dp / 2);
+int pack(const void *src, int64_t rs, int64_t rows, const b200_lce_args &a, const Plan &q, bool masked, void *dst, cudaStream_t st) {
+  const bool wide = a.dtype != B200_F32 && in_place(src, rs, a.features) && rs >= q.Dp;
+  const int64_t n = rows * (q.Dp / (wide ? 8 : 2));
   const int64_t blocks = (n + 255) / 256, most = (int64_t)sm_count_current() * 32;
-  lce_pack_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, st>>>(src, rs, rows, a.features, q.Dp, a.dtype == B200_F32,
+  lce_pack_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, st>>>(src, rs, rows, a.features, q.Dp, a.dtype == B200_F32, wide,
+                                                                            masked ? reinterpret_cast<const int64_t *>(a.labels) : nullptr, a.ignore_index, a.classes,
                                                                             reinterpret_cast<uint16_t *>(dst));
   return launch_status();
 }
@@ -732,14 +748,14 @@ using namespace b200;
 extern "C" int64_t b200_lce_fwd_work_bytes(const b200_lce_args *args) {
   if (!args || check_lce(*args)) return 0;
   const b200_lce_args &a = *args;
-  const Plan q = plan_of(a);
+  const Plan q = plan_of(a, false);
   return q.pack_bytes_h + q.pack_bytes_w + up(8 * a.rows * slots_of(a), 256) + 2 * up(4 * a.rows, 256);
 }
 
 extern "C" int64_t b200_lce_bwd_work_bytes(const b200_lce_args *args) {
   if (!args || check_lce(*args)) return 0;
   const b200_lce_args &a = *args;
-  const Plan q = plan_of(a);
+  const Plan q = plan_of(a, true);
   return q.pack_bytes_h + q.pack_bytes_w + q.dz_bytes + (a.dhidden ? q.acc_h_bytes : 0) + (a.dweight ? q.acc_w_bytes : 0) + up(4 * a.rows, 256) + 256;
 }
 
@@ -748,15 +764,15 @@ extern "C" int b200_lce_fwd(const b200_lce_args *args, void *stream) {
   const b200_lce_args &a = *args;
   if (int e = check_lce(a)) return e;
   B200_REQUIRE(a.lse && a.loss && a.work && (a.reduction != 1 || a.count), B200_ERR_NULL, "lce_fwd: lse, loss, work and (for a mean) count must be non-null");
-  const Plan q = plan_of(a);
+  const Plan q = plan_of(a, false);
   B200_REQUIRE(a.work_bytes >= b200_lce_fwd_work_bytes(args), B200_ERR_TOO_LARGE, "lce_fwd: work has %lld bytes, %lld are needed", (long long)a.work_bytes,
                (long long)b200_lce_fwd_work_bytes(args));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   unsigned char *w = reinterpret_cast<unsigned char *>(a.work);
   Operands o = {a.hidden, a.weight, a.hidden_rs, a.weight_rs};
-  if (q.pack_h) { o.h = w; o.h_pitch = q.Dp; if (int e = pack(a.hidden, a.hidden_rs, a.rows, a, q, w, st)) return e; }
+  if (q.pack_h) { o.h = w; o.h_pitch = q.Dp; if (int e = pack(a.hidden, a.hidden_rs, a.rows, a, q, false, w, st)) return e; }
   w += q.pack_bytes_h;
-  if (q.pack_w) { o.w = w; o.w_pitch = q.Dp; if (int e = pack(a.weight, a.weight_rs, a.classes, a, q, w, st)) return e; }
+  if (q.pack_w) { o.w = w; o.w_pitch = q.Dp; if (int e = pack(a.weight, a.weight_rs, a.classes, a, q, false, w, st)) return e; }
   w += q.pack_bytes_w;
   LceGemm g;
   if (int e = gemm_z(g, a, q, o, 0, a.classes)) return e;
@@ -783,15 +799,17 @@ extern "C" int b200_lce_bwd(const b200_lce_args *args, void *stream) {
   B200_REQUIRE(a.dhidden || a.dweight, B200_ERR_NULL, "lce_bwd: dhidden or dweight must be non-null");
   B200_REQUIRE((!a.dhidden || a.dhidden_rs >= a.features) && (!a.dweight || a.dweight_rs >= a.features), B200_ERR_SHAPE,
                "lce_bwd: row pitches must be at least the features");
-  const Plan q = plan_of(a);
+  const Plan q = plan_of(a, true);
   B200_REQUIRE(a.work_bytes >= b200_lce_bwd_work_bytes(args), B200_ERR_TOO_LARGE, "lce_bwd: work has %lld bytes, %lld are needed", (long long)a.work_bytes,
                (long long)b200_lce_bwd_work_bytes(args));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   unsigned char *w = reinterpret_cast<unsigned char *>(a.work);
   Operands o = {a.hidden, a.weight, a.hidden_rs, a.weight_rs};
-  if (q.pack_h) { o.h = w; o.h_pitch = q.Dp; if (int e = pack(a.hidden, a.hidden_rs, a.rows, a, q, w, st)) return e; }
+  o.h = w;
+  o.h_pitch = q.Dp;
+  if (int e = pack(a.hidden, a.hidden_rs, a.rows, a, q, true, w, st)) return e;
   w += q.pack_bytes_h;
-  if (q.pack_w) { o.w = w; o.w_pitch = q.Dp; if (int e = pack(a.weight, a.weight_rs, a.classes, a, q, w, st)) return e; }
+  if (q.pack_w) { o.w = w; o.w_pitch = q.Dp; if (int e = pack(a.weight, a.weight_rs, a.classes, a, q, false, w, st)) return e; }
   w += q.pack_bytes_w;
   void *dz = w;
   w += q.dz_bytes;

@@ -247,12 +247,13 @@ __device__ __forceinline__ void product(float (&acc)[NT][4], const float *a, con
 }
 
 // 64 rows of an operand from step i0 on into shared memory as float32, zero past the sequence and past its size: 16 threads a
-// row, 4 columns each.
+// row, 4 columns each.  Returns whether one of them is infinite or NaN.
 template <typename T, int WT>
-__device__ __forceinline__ void load_rows(const Walk &p, const void *base, int64_t off, int64_t ls, int i0, int col0, int size, int width, int pitch, float *dst) {
+__device__ __forceinline__ bool load_rows(const Walk &p, const void *base, int64_t off, int64_t ls, int i0, int col0, int size, int width, int pitch, float *dst) {
   const T *src = reinterpret_cast<const T *>(base) + off + col0;
   const bool vec = ((reinterpret_cast<uintptr_t>(src) | (uintptr_t)(ls * sizeof(T))) & (4 * sizeof(T) - 1)) == 0;
   const int r0 = threadIdx.x >> 4;
+  float zero = 0.f;
   for (int c = (threadIdx.x & 15) * 4; c < width; c += 64) {
     const int left = size - col0 - c;
     float4 v[CH / (WT / 16)];
@@ -279,8 +280,12 @@ __device__ __forceinline__ void load_rows(const Walk &p, const void *base, int64
       }
     }
 #pragma unroll
-    for (int i = 0; i < CH / (WT / 16); ++i) *reinterpret_cast<float4 *>(dst + (r0 + i * (WT / 16)) * pitch + c) = v[i];
+    for (int i = 0; i < CH / (WT / 16); ++i) {
+      *reinterpret_cast<float4 *>(dst + (r0 + i * (WT / 16)) * pitch + c) = v[i];
+      zero = fmaf(v[i].x, 0.f, fmaf(v[i].y, 0.f, fmaf(v[i].z, 0.f, fmaf(v[i].w, 0.f, zero))));
+    }
   }
+  return zero != 0.f;
 }
 
 // the cache lines of the rows: four threads a row, 32 columns apart
@@ -332,12 +337,12 @@ template <typename T, int DI, int WT, bool STATE_ONLY> __global__ void __launch_
     const Decays &d = dd[it & 1];
     if (!STATE_ONLY && p.run && !p.rev && chunk % kSnap == 0) snapshot(chunk, 1.f);
     load_rows<T, WT>(p, p.k, b * p.k_bs + h / p.k_div * p.k_hs, p.k_ls, i0, 0, p.di, dip, PQ, sk);
-    load_rows<T, WT>(p, p.v, b * p.v_bs + h / p.v_div * p.v_hs, p.v_ls, i0, col0, p.dout, DO, PV, sv);
+    bool odd = load_rows<T, WT>(p, p.v, b * p.v_bs + h / p.v_div * p.v_hs, p.v_ls, i0, col0, p.dout, DO, PV, sv);
     if (!STATE_ONLY) {
       load_rows<T, WT>(p, p.q, b * p.q_bs + h / p.q_div * p.q_hs, p.q_ls, i0, 0, p.di, dip, PQ, sq);
       if (p.run) load_rows<T, WT>(p, p.x, b * p.x_bs + h / p.x_div * p.x_hs, p.x_ls, i0, col0, p.dout, DO, PP, sx);
     }
-    __syncthreads();
+    odd = __syncthreads_or(odd);                     // some value is infinite or NaN
     const int m0 = (warp & 3) * 16, n0 = (warp >> 2) * 8 * NT;  // this warp's scores and results
     if (i0 + CH < i_end) {                           // the next chunk's rows into the first-level cache
       prefetch_rows<T>(p, p.k, b * p.k_bs + h / p.k_div * p.k_hs, p.k_ls, i0 + CH, 0, p.di);
@@ -412,7 +417,18 @@ template <typename T, int DI, int WT, bool STATE_ONLY> __global__ void __launch_
           if (tq == 0) dots[warp >> 2][r] = s;
         }
       }
-      product<true, F32, PP, 1, PV, 1, NT>(acc, sp + m0 * PP, nullptr, sv + n0, min(CH, m0 + 16), lane);
+      if (!odd) product<true, F32, PP, 1, PV, 1, NT>(acc, sp + m0 * PP, nullptr, sv + n0, min(CH, m0 + 16), lane);
+      else                                           // one by one: a zero score of a later step would carry it to earlier ones
+        for (int e2 = 0; e2 < 2; ++e2) {
+          const int r = m0 + gq + e2 * 8;
+          for (int j = 0; j <= r; ++j)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int e1 = 0; e1 < 2; ++e1)
+                if (e2 == 0) acc[n][e1] = fmaf(sp[r * PP + j], sv[j * PV + n0 + n * 8 + tq * 2 + e1], acc[n][e1]);
+                else acc[n][2 + e1] = fmaf(sp[r * PP + j], sv[j * PV + n0 + n * 8 + tq * 2 + e1], acc[n][2 + e1]);
+        }
 #pragma unroll
       for (int e2 = 0; e2 < 2; ++e2) {
         const int t = time_of(p, i0 + m0 + gq + e2 * 8);
@@ -633,6 +649,14 @@ __device__ __forceinline__ float sum_columns(float (&v)[16], int lane) {
   return v[0] + __shfl_xor_sync(0xffffffffu, v[0], 16);
 }
 
+// Whether one of eight bfloat16 is infinite or NaN: it times zero is NaN.
+__device__ __forceinline__ bool not_finite(const uint32_t (&x)[4]) {
+  __nv_bfloat162 t = __float2bfloat162_rn(0.f);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) t = __hfma2(*reinterpret_cast<const __nv_bfloat162 *>(&x[j]), __float2bfloat162_rn(0.f), t);
+  return (*reinterpret_cast<const uint32_t *>(&t) & 0x7fff7fffu) != 0u;
+}
+
 // MODE: only a segment's own state; results; results and dots with x, forwards; the same backwards
 enum { OWN_STATE = 0, RESULTS = 1, DOTS = 2, DOTS_REV = 3 };
 
@@ -652,7 +676,7 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
   __shared__ float dots[2][BC], rows_[2][BC], cols_[4][BC];
   __shared__ uint64_t bar, bar_d, loaded_qk, loaded_v;
   __shared__ uint32_t tmem_base;
-  __shared__ int fail;
+  __shared__ int fail, odd[2], odd_from[2][DO];               // odd: a value of the chunk is infinite or NaN, from which step on in each column
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int tile = blockIdx.x % p.tiles, bh = blockIdx.x / p.tiles % (p.batch * p.heads), seg = blockIdx.x / p.tiles / (p.batch * p.heads);
   const int b = bh / p.heads, h = bh % p.heads, col0 = tile * DO;
@@ -660,6 +684,10 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
   const int snaps = (p.chunks + kSnapB - 1) / kSnapB;
   // this thread's TMEM lane (a step of the chunk, a row of the state) and half of the columns
   const int wr = warp & 3, half = warp >> 2, r = wr * 32 + lane, c0 = half * 32;
+  if (tid < DO) {
+    odd[0] = 0;
+    odd_from[0][tid] = BC;
+  }
   if (tid == 0) {
     mbar_init(&bar, 1);
     mbar_init(&bar_d, 1);
@@ -785,6 +813,10 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
     tc_fence_before();
     __syncthreads();                                     // the state's terms are written, accumulators read
     if (*(volatile int *)&fail) break;
+    if (!STATE_ONLY && tid < DO) {                       // the next chunk's
+      odd[(it + 1) & 1] = 0;
+      odd_from[(it + 1) & 1][tid] = BC;
+    }
     if (issuer && maps.tma && !scores_on && !mbar_wait(&loaded_qk, it & 1, kWaitLimit)) *(volatile int *)&fail = 1;
     const auto meanwhile = [&]() {
       if (warp == decay_warp && i0 + BC < i_end) {
@@ -856,6 +888,18 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
       for (int j = 0; j < 4; ++j) {
         y[2 * j] = low16(x[j]) * f;
         y[2 * j + 1] = high16(x[j]) * f;
+      }
+      if (!STATE_ONLY && not_finite(x)) {
+        // The zeros that stand for the scores of later steps would carry an infinite or NaN value to earlier results: the product
+        // with the scores takes a zero for it, and the results from its step on become NaN in its column.
+        if (cross && !mbar_wait(&bar, phase, kWaitLimit)) *(volatile int *)&fail = 1;      // x v^T has read it
+        odd[it & 1] = 1;
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t half_of = j & 1 ? x[j >> 1] >> 16 : x[j >> 1] & 0xffffu;
+          if ((half_of & 0x7f80u) != 0x7f80u) continue;
+          atomicMin(&odd_from[it & 1][(e & 7) * 8 + j], p.rev ? BC - 1 - row : row);
+          *reinterpret_cast<uint16_t *>(sv + at + j * 2) = 0;
+        }
       }
 #pragma unroll
       for (int t = 0; t < 3; ++t)
@@ -991,6 +1035,12 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
       tmem_ld32(tm_own + tO + c0, v);
 #pragma unroll
       for (int j = 0; j < 32; ++j) O[j] += v[j];
+      if (odd[it & 1]) {
+        const int i = p.rev ? BC - 1 - r : r;
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (i >= odd_from[it & 1][c0 + j]) O[j] = __int_as_float(0x7fffffff);
+      }
       const int t = time0(i0) + r, left = p.dout - col0 - c0;
       if (staged) {                                      // by way of shared memory, where v (and x) were
         if (p.out_f32) {

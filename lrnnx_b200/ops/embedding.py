@@ -85,4 +85,4 @@ def token_embedding(ids, weight, scale=1.0, padding_idx=None):
         return weight[:0].sum() + weight.new_empty(ids.shape + (shape[1],))
     if torch.is_grad_enabled() and weight.requires_grad:
         return TokenEmbeddingFn.apply(ids, weight, float(scale), padding_idx)
-    return _lookup(ids, weight, *shape, scale, padding_idx)[0]
+    return _lookup(ids, weight, *shape, float(scale), padding_idx)[0]

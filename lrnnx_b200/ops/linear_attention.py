@@ -125,7 +125,7 @@ def linear_attention_fn(q, k, v, g, scale=1.0, initial_state=None, return_last_s
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad
                                     or initial_state is not None and initial_state.requires_grad):
         return LinearAttentionFn.apply(q, k, v, g, float(scale), initial_state, return_last_state)
-    out, last = _forward(_inner(q), _inner(k), _inner(v), g, scale, None if initial_state is None else _inner(initial_state), return_last_state)
+    out, last = _forward(_inner(q), _inner(k), _inner(v), g, float(scale), None if initial_state is None else _inner(initial_state), return_last_state)
     return (out, last) if return_last_state else out
 
 
@@ -156,7 +156,7 @@ def linear_attention_step(state, q, k, v, g, scale=1.0, state_batch_indices=None
         if batch == 0:
             return out
         _lib.call("b200_linattn_step",
-                  pack(batch, heads, groups, dk, dv, codes[q.dtype], codes[g.dtype], codes[state.dtype], scale, slots, state.data_ptr(),
+                  pack(batch, heads, groups, dk, dv, codes[q.dtype], codes[g.dtype], codes[state.dtype], float(scale), slots, state.data_ptr(),
                        q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), 0 if state_batch_indices is None else state_batch_indices.data_ptr(),
                        out.data_ptr(), ss[0], ss[1], ss[2], sq[0], sq[1], sk[0], sk[1], sv[0], sv[1], sg[0] if len(sg) == 2 else 0, sg[-1], heads * dv, dv),
                   _lib.stream_of(q))

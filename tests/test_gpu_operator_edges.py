@@ -385,3 +385,58 @@ def test_embedding_mixer_and_loss_together():
     assert abs(float(a.detach()) - float(b.detach())) <= 200 * 2.0 ** -23 * (1 + float(b.detach()))
     for x, y in zip(torch.autograd.grad(a, ours), torch.autograd.grad(b, exact)):
         assert float((x.double() - y).norm()) <= 3 * 200 * 2.0 ** -23 * float(y.norm())
+
+
+# ------------------------------------------------------------------------------------------------ what is masked stays out
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_ignored_rows_may_hold_anything(dtype):
+    """NaN and infinities in the hidden states of rows without a label (the padding of a batch) are in no result."""
+    from lrnnx_b200.ops import linear_cross_entropy
+    for pad in (None, 3):
+        h, w, labels = loss_operands(140, 500, 72, dtype)
+        labels[5], labels[6], labels[139] = -100, 500, -100
+        bad = h.clone()
+        bad[labels == -100], bad[6] = float("nan"), float("inf")
+        zero = h.clone()
+        zero[labels == -100], zero[6] = 0, 0
+        res = []
+        for x in (bad, zero):
+            x = (x if pad is None else moat(x, pad)).requires_grad_()
+            ww = w.clone().requires_grad_()
+            loss = linear_cross_entropy(x, ww, labels)
+            res.append([loss.detach(), *torch.autograd.grad(loss, (x, ww))])
+        assert bool(torch.isfinite(res[0][2]).all()) and torch.count_nonzero(res[0][1][labels == -100]) == 0
+        assert all(torch.equal(a, b) for a, b in zip(*res))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_attention_is_causal_whatever_comes_later(dtype, value):
+    """Values, keys and queries that are infinite or NaN at a step reach no earlier step, and a value only its own column."""
+    from lrnnx_b200.ops import linear_attention_fn
+    (q, k, v, g, _), _, _ = attn_operands(2, 200, 4, 2, 48, 64, dtype, "token", seed=14)
+    clean = linear_attention_fn(q, k, v, g)
+    mag, _ = recurrence(*(t.double().abs() for t in (q, k, v)), g.double(), 1.0, torch.zeros(2, 4, 48, 64, dtype=torch.float64, device="cuda"))
+    bound = 2 * ((200 / 16 + 200) * 2.0 ** -23 + 3 * ATTN_HALF[dtype]) * mag + 2 * TINY[dtype]
+    for t in (0, 37, 150, 199):
+        x = v.clone()
+        x[0, t, 1, 5] = value
+        o = linear_attention_fn(q, k, x, g)
+        hit = torch.zeros_like(o, dtype=torch.bool)
+        hit[0, t:, 1, 5] = True
+        assert not bool(torch.isfinite(o[0, t, 1, 5]))
+        within("values", o[~hit], clean[~hit].double(), bound[~hit])
+        x = k.clone()
+        x[0, t, 1, 5] = value
+        o = linear_attention_fn(q, x, v, g)
+        hit = torch.zeros_like(o, dtype=torch.bool)
+        hit[0, t:, 2:] = True
+        within("keys", o[~hit], clean[~hit].double(), bound[~hit])
+        x = q.clone()
+        x[0, t, 1, 5] = value
+        o = linear_attention_fn(x, k, v, g)
+        hit = torch.zeros_like(o, dtype=torch.bool)
+        hit[0, t, 2:] = True
+        within("queries", o[~hit], clean[~hit].double(), bound[~hit])
