@@ -558,7 +558,7 @@ __device__ __forceinline__ void tma_st_4d(const CUtensorMap *map, const void *sr
 }
 // 128 steps of W columns (64 a tile) from time t0 on, zero past the sequence and past its size
 template <int W>
-__device__ __forceinline__ void load_tile(const Walk &p, const void *base, int64_t off, int64_t ls, int size, int col0, int t0, unsigned char *dst) {
+__device__ __noinline__ void load_tile(const Walk &p, const void *base, int64_t off, int64_t ls, int size, int col0, int t0, unsigned char *dst) {
   constexpr int PER = W / 8;                             // 16-byte pieces of a row
   const uint16_t *src = reinterpret_cast<const uint16_t *>(base) + off + col0;
   for (int e = threadIdx.x; e < BC * PER; e += BT) {
