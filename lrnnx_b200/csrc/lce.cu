@@ -11,7 +11,7 @@
 // float16 dz neither overflows under a scaled loss nor vanishes under a mean over many rows; the products are scaled back
 // in 32 bits.  s_r = 0 (ignored labels) makes an exact zero row.
 //
-// The products run on tcgen05 with accumulators in TMEM, one kernel with three epilogues.  Pairs of thread blocks
+// The products run on tcgen05 with accumulators in TMEM, one kernel with four epilogues.  Pairs of thread blocks
 // (cta_group::2) take tiles of 256 x 256 in turn, each block with its 128 rows of both operands: in each, warp 0 issues TMA
 // loads into a 6-stage ring (64 of the contraction a stage) and warps 4-11 empty one of two 256-column accumulators while
 // the other is filled; warp 1 of the first block issues the MMAs for both.  A single block's tile of 128 x 256 takes 96 bytes
@@ -22,13 +22,14 @@
 // float32 operands are split into three bfloat16 (8 bits of mantissa each) and multiplied as six products of the
 // planes, the small ones first; what is left out is below 2^-24.  The tensor core truncates when it adds into its
 // accumulator, an error to one side that grows with the length of the chain, so that long contractions are cut into
-// chains of kSegSteps whose sums are added up in float32, rounded to nearest.  (An infinite float32 operand gives NaN
+// chains of kSegSteps whose sums are added up in float32, rounded to nearest: for the gradients in the epilogue's registers
+// (through memory a chain's sums cost 40 us of the 205 of dz W at 2031 x 16411 x 509).  (An infinite float32 operand gives NaN
 // where its product with the rest of a split is none.)
 //
 // Measured (one B200, 16384 x 50280 x 768 bfloat16, forward and backward 4.34 ms, 1.17 PFLOP/s over the four products, under the power
 // limit as a library product would be): z and its log-sum-exp 827-844 us (tensor pipe 82 %), the two pieces of dz 479 us each
 // (74 %: the epilogue's stores), dz W 439-456 us each (90 %), dz^T H 510 and 438 us (80 %: 297 tiles on 74 pairs).  float32,
-// 2031 x 16411 x 509: 0.89 ms, six times the products.
+// 2031 x 16411 x 509: 0.84 ms, six times the products.
 #include "common.cuh"
 #include "dispatch.h"
 #include "tc_common.cuh"
@@ -53,7 +54,8 @@ constexpr int64_t kPieceBytes = int64_t(1) << 30;
 constexpr int kSegSteps = 8;              // float32 only: stages (of 64) in one accumulation chain of the leading product
 constexpr int kMaxSplits = 32;            // blocks that share the contraction of a tile
 
-enum { EPI_LSE = 0, EPI_DZ = 1, EPI_OUT = 2 };
+// EPI_SUM: as EPI_OUT, the sums of a tile's chains kept in registers
+enum { EPI_LSE = 0, EPI_DZ = 1, EPI_OUT = 2, EPI_SUM = 3 };
 
 struct LceGemm {
   CUtensorMap a, b, out;       // (inner, rows, plane); out: dz
@@ -173,18 +175,7 @@ __device__ __forceinline__ void store_dz(const LceGemm &p, unsigned char *stagin
   }
 }
 
-template <typename T> __device__ __forceinline__ void store_row(T *dst, const float (&v)[32], int n, bool vec);
-template <> __device__ __forceinline__ void store_row<float>(float *dst, const float (&v)[32], int n, bool vec) {
-  if (vec && n >= 32) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) reinterpret_cast<float4 *>(dst)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (j < n) dst[j] = v[j];
-  }
-}
-template <typename T> __device__ __forceinline__ void store_row16(T *dst, const float (&v)[32], int n, bool vec) {
+template <typename T> __device__ __forceinline__ void store_row(T *dst, const float (&v)[32], int n, bool vec) {
   if (vec && n >= 32) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -206,7 +197,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LCE_THREADS, 1) lce_
   unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ LcePipe pipe;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int tiles = p.mt * p.nt * (EPI == EPI_OUT ? p.splits : 1), pairs = gridDim.x >> 1, pair = blockIdx.x >> 1;
+  const int tiles = p.mt * p.nt * (EPI >= EPI_OUT ? p.splits : 1), pairs = gridDim.x >> 1, pair = blockIdx.x >> 1;
   const int rank = (int)cluster_rank();
   if (tid == 0) {
     for (int s = 0; s < NST; ++s) {
@@ -231,11 +222,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LCE_THREADS, 1) lce_
   tc_fence_after();
   const uint32_t tmem = pipe.tmem_base;
   // z and dz: neighbouring blocks share W's tile; products of dz: they share dz's
-  const auto m_of = [&](int t) { return EPI == EPI_OUT ? t / p.nt % p.mt : t % p.mt; };
-  const auto n_of = [&](int t) { return EPI == EPI_OUT ? t % p.nt : t / p.mt; };
+  const auto m_of = [&](int t) { return EPI >= EPI_OUT ? t / p.nt % p.mt : t % p.mt; };
+  const auto n_of = [&](int t) { return EPI >= EPI_OUT ? t % p.nt : t / p.mt; };
   // the stages of a block's part of the contraction
-  const auto k_from = [&](int t) { return EPI == EPI_OUT ? t / (p.nt * p.mt) * p.per : 0; };
-  const auto k_to = [&](int t) { return EPI == EPI_OUT ? min(p.nk, k_from(t) + p.per) : p.nk; };
+  const auto k_from = [&](int t) { return EPI >= EPI_OUT ? t / (p.nt * p.mt) * p.per : 0; };
+  const auto k_to = [&](int t) { return EPI >= EPI_OUT ? min(p.nk, k_from(t) + p.per) : p.nk; };
 
   if (warp == 0 && lane == 0) {
     // ------------------------------------------------------------------ loads
@@ -312,11 +303,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LCE_THREADS, 1) lce_
       const int row = m0 + q * 32 + lane, c0 = n0 + half * (TN / 2);      // this thread's row and 128 columns
       const bool in = row < p.rows;
       const int kb = k_from(t), ke = k_to(t);
+      float sums[EPI == EPI_SUM ? TN / 64 : 1][32];
       for (int k0 = kb; k0 < ke; k0 += p.seg, ++ch) {
         // what the epilogue needs besides is loaded before the wait
         float lse2 = 0.f, sc = 0.f;
         int at = -1;                                                     // the label's column within this thread's columns
-        if (EPI != EPI_OUT && in) {
+        if (EPI < EPI_OUT && in) {
           const int64_t label = p.labels[row];
           if (label != p.ignore_index && label >= 0 && label < p.classes) {
             const int64_t c = label - p.col0 - c0;
@@ -398,46 +390,78 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LCE_THREADS, 1) lce_
           __syncwarp();
           if (lane == 0) arrive_at(of_first(&pipe.acc_empty[ch & 1]));
         } else {
-          const bool first = k0 == kb && !p.add, last = k0 + p.seg >= ke && p.last;
           float *acc = p.acc + (int64_t)(t / (p.nt * p.mt)) * p.rows * p.acc_rs;
           const float unit = unit_of(p.common);
-          const bool vec = (p.dst_rs * (p.dtype == B200_F32 ? 4 : 2)) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.dst) & 15) == 0;
-#pragma unroll 1
-          for (int c = 0; c < TN / 64; ++c) {
-            float v[32];
+          if constexpr (EPI == EPI_SUM) {
+#pragma unroll
+            for (int c = 0; c < TN / 64; ++c) {
+              float v[32];
+              tmem_ld32(ta + c * 32, v);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) sums[c][j] = k0 == kb ? v[j] : sums[c][j] + v[j];
+            }
+            tc_fence_before();
             __syncwarp();
-            tmem_ld32(ta + c * 32, v);
-            const int col = c0 + c * 32, n = min(32, p.cols - col);
-            if (!in || n <= 0) continue;
-            if (!first) {
-              const float4 *o = reinterpret_cast<const float4 *>(acc + (int64_t)row * p.acc_rs + col);
+            if (lane == 0) arrive_at(of_first(&pipe.acc_empty[ch & 1]));
+            if (k0 + p.seg < ke) continue;
+            // 32 x 32 of them, a row a lane, are turned over in shared memory, so that a row leaves as one line
+            float *turn = reinterpret_cast<float *>(staging);
+            const int r0 = m0 + q * 32, n = min(32, p.rows - r0);
 #pragma unroll
-              for (int j = 0; j < 8; ++j)
-                if (4 * j < n) {
-                  const float4 w = o[j];
-                  v[4 * j] += w.x;
-                  v[4 * j + 1] += w.y;
-                  v[4 * j + 2] += w.z;
-                  v[4 * j + 3] += w.w;
-                }
+            for (int c = 0; c < TN / 64; ++c) {
+              const int col = c0 + c * 32 + lane;
+              __syncwarp();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) turn[lane * 32 + (j ^ lane)] = sums[c][j];
+              __syncwarp();
+              if (col >= p.cols) continue;
+              float *sum = acc + (int64_t)r0 * p.acc_rs + col, *dst = reinterpret_cast<float *>(p.dst) + (int64_t)r0 * p.dst_rs + col;
+#pragma unroll 8
+              for (int i = 0; i < n; ++i) {
+                float x = turn[i * 32 + (lane ^ i)];
+                if (p.add) x += sum[i * p.acc_rs];
+                if (p.last) dst[i * p.dst_rs] = x * unit;
+                else sum[i * p.acc_rs] = x;
+              }
             }
-            if (!last) {
+          } else {
+            // one chain: a row a lane, which writes the whole line of a bfloat16 or float16 row by itself
+            const bool vec = (p.dst_rs * 2) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.dst) & 15) == 0;
+#pragma unroll 1
+            for (int c = 0; c < TN / 64; ++c) {
+              float v[32];
+              __syncwarp();
+              tmem_ld32(ta + c * 32, v);
+              const int col = c0 + c * 32, n = min(32, p.cols - col);
+              if (!in || n <= 0) continue;
               float4 *o = reinterpret_cast<float4 *>(acc + (int64_t)row * p.acc_rs + col);
+              if (p.add) {
 #pragma unroll
-              for (int j = 0; j < 8; ++j)
-                if (4 * j < n) o[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-            } else {
+                for (int j = 0; j < 8; ++j)
+                  if (4 * j < n) {
+                    const float4 w = o[j];
+                    v[4 * j] += w.x;
+                    v[4 * j + 1] += w.y;
+                    v[4 * j + 2] += w.z;
+                    v[4 * j + 3] += w.w;
+                  }
+              }
+              if (!p.last) {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] *= unit;
-              const int64_t i = (int64_t)row * p.dst_rs + col;
-              if (p.dtype == B200_F32) store_row<float>(reinterpret_cast<float *>(p.dst) + i, v, n, vec);
-              else if (p.dtype == B200_BF16) store_row16<__nv_bfloat16>(reinterpret_cast<__nv_bfloat16 *>(p.dst) + i, v, n, vec);
-              else store_row16<__half>(reinterpret_cast<__half *>(p.dst) + i, v, n, vec);
+                for (int j = 0; j < 8; ++j)
+                  if (4 * j < n) o[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+              } else {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] *= unit;
+                const int64_t i = (int64_t)row * p.dst_rs + col;
+                if (p.dtype == B200_BF16) store_row<__nv_bfloat16>(reinterpret_cast<__nv_bfloat16 *>(p.dst) + i, v, n, vec);
+                else store_row<__half>(reinterpret_cast<__half *>(p.dst) + i, v, n, vec);
+              }
             }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive_at(of_first(&pipe.acc_empty[ch & 1]));
           }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) arrive_at(of_first(&pipe.acc_empty[ch & 1]));
         }
       }
     }
@@ -662,9 +686,9 @@ Plan plan_of(const b200_lce_args &a, bool bwd) {
   const int64_t dt = (a.features + TN - 1) / TN;
   split_of((a.rows + 2 * TM - 1) / (2 * TM) * dt, (q.piece + TK - 1) / TK, q.splits_h, q.per_h);
   split_of((q.piece + 2 * TM - 1) / (2 * TM) * dt, (int)((a.rows + TK - 1) / TK), q.splits_w, q.per_w);
-  // float32 sums: of dH over the pieces, the chains and the blocks that share a tile, of dW over the chains and blocks
-  q.acc_h_bytes = f32 || q.n_pieces > 1 || q.splits_h > 1 ? up(4 * q.splits_h * a.rows * q.Da, 256) : 0;
-  q.acc_w_bytes = q.splits_w > 1 || (f32 && (a.rows + TK - 1) / TK > q.seg) ? up(4 * q.splits_w * (int64_t)q.piece * q.Da, 256) : 0;
+  // float32 sums: of dH over the pieces and the blocks that share a tile, of dW over the blocks
+  q.acc_h_bytes = q.n_pieces > 1 || q.splits_h > 1 ? up(4 * q.splits_h * a.rows * q.Da, 256) : 0;
+  q.acc_w_bytes = q.splits_w > 1 ? up(4 * q.splits_w * (int64_t)q.piece * q.Da, 256) : 0;
   return q;
 }
 
@@ -696,7 +720,7 @@ int pack(const void *src, int64_t rs, int64_t rows, const b200_lce_args &a, cons
 template <int EPI> int launch_gemm(const LceGemm &g, cudaStream_t st) {
   cudaError_t e = cudaFuncSetAttribute(lce_gemm_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, LCE_SMEM);
   if (e != cudaSuccess) { set_error("cudaFuncSetAttribute: %s", cudaGetErrorString(e)); return (int)e; }
-  const int tiles = g.mt * g.nt * (EPI == EPI_OUT ? g.splits : 1), sms = sm_count_current();
+  const int tiles = g.mt * g.nt * (EPI >= EPI_OUT ? g.splits : 1), sms = sm_count_current();
   lce_gemm_kernel<EPI><<<(unsigned)(2 * (tiles < sms / 2 ? tiles : sms / 2)), LCE_THREADS, LCE_SMEM, st>>>(g);
   return launch_status();
 }
@@ -858,7 +882,7 @@ extern "C" int b200_lce_bwd(const b200_lce_args *args, void *stream) {
       g.dst_rs = a.dhidden_rs;
       g.add = pc > 0;
       g.last = pc == q.n_pieces - 1 && g.splits == 1;
-      if (int e = launch_gemm<EPI_OUT>(g, st)) return e;
+      if (int e = a.dtype == B200_F32 ? launch_gemm<EPI_SUM>(g, st) : launch_gemm<EPI_OUT>(g, st)) return e;
       if (g.splits > 1 && pc == q.n_pieces - 1)
         if (int e = fold(g, st)) return e;
     }
@@ -879,7 +903,7 @@ extern "C" int b200_lce_bwd(const b200_lce_args *args, void *stream) {
       g.splits = q.splits_w;
       g.per = q.per_w;
       g.last = g.splits == 1;
-      if (int e = launch_gemm<EPI_OUT>(g, st)) return e;
+      if (int e = a.dtype == B200_F32 ? launch_gemm<EPI_SUM>(g, st) : launch_gemm<EPI_OUT>(g, st)) return e;
       if (g.splits > 1)
         if (int e = fold(g, st)) return e;
     }
