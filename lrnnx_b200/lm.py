@@ -43,6 +43,16 @@ class RMSNorm(nn.Module):
                            residual_in_fp32=residual_in_fp32)
 
 
+class TokenEmbedding(nn.Embedding):
+    """nn.Embedding whose lookup and gradient are this package's kernels (``token_embedding``)."""
+
+    def __init__(self, num_embeddings, embedding_dim, padding_idx=None, device=None, dtype=None):
+        super().__init__(num_embeddings, embedding_dim, padding_idx=padding_idx, device=device, dtype=dtype)
+
+    def forward(self, ids):
+        return token_embedding(ids, self.weight, padding_idx=self.padding_idx)
+
+
 class _InProjFn(torch.autograd.Function):
     """xz = W hidden^T per batch row, produced directly in the (batch, channel, L) layout the scan
     kernels read.  A plain bmm would do the forward; its autograd hands the input gradient back as
@@ -154,13 +164,13 @@ class Backbone(nn.Module):
     def __init__(self, d_model, d_state, n_layer, vocab_size, eps, residual_in_fp32, device=None, dtype=None, **mixer_kw):
         super().__init__()
         self.residual_in_fp32 = residual_in_fp32
-        self.embedding = nn.Embedding(vocab_size, d_model, device=device, dtype=dtype)
+        self.embedding = TokenEmbedding(vocab_size, d_model, device=device, dtype=dtype)
         self.layers = nn.ModuleList([Block(d_model, d_state, eps, device=device, dtype=dtype, **mixer_kw)
                                      for _ in range(n_layer)])
         self.norm_f = RMSNorm(d_model, eps, device=device, dtype=dtype)
 
     def forward(self, input_ids, caches=None):
-        hidden = token_embedding(input_ids, self.embedding.weight)
+        hidden = self.embedding(input_ids)
         residual = None
         for i, layer in enumerate(self.layers):
             normed, residual = layer.norm(hidden, residual, prenorm=True, residual_in_fp32=self.residual_in_fp32)
@@ -168,7 +178,7 @@ class Backbone(nn.Module):
         return self.norm_f(hidden, residual)
 
     def step(self, token_ids, caches):
-        hidden = token_embedding(token_ids, self.embedding.weight)
+        hidden = self.embedding(token_ids)
         residual = None
         for i, layer in enumerate(self.layers):
             normed, residual = layer.norm(hidden, residual, prenorm=True, residual_in_fp32=self.residual_in_fp32)

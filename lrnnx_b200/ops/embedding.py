@@ -12,6 +12,7 @@ import torch
 
 from .. import _lib
 from .mamba_block import _DT
+from .once import once
 
 
 @functools.lru_cache(maxsize=None)
@@ -47,7 +48,7 @@ class TokenEmbeddingFn(torch.autograd.Function):
         flat, = ctx.saved_tensors
         classes, scale, padding_idx = ctx.meta
         features = dout.shape[-1]
-        dout = dout.reshape(-1, features)
+        given, dout = dout, dout.reshape(-1, features)
         if dout.stride(1) != 1 and features > 1:
             dout = dout.contiguous()
         pack, codes = _setup()
@@ -59,7 +60,7 @@ class TokenEmbeddingFn(torch.autograd.Function):
             work = torch.empty(max(work_bytes, 1), dtype=torch.uint8, device=dout.device)
             _lib.call("b200_embed_bwd", pack(*head, work.data_ptr(), work_bytes), _lib.stream_of(dout))
             del work
-        return None, dweight, None, None
+        return None, *once((given,), (dweight,)), None, None
 
 
 def token_embedding(ids, weight, scale=1.0, padding_idx=None):

@@ -14,7 +14,8 @@ import functools
 import torch
 
 from .. import _lib
-from .mamba_block import _DT, _stream
+from .mamba_block import _DT
+from .once import once
 
 MAX_SIZE = 128            # of dk and dv
 
@@ -73,6 +74,7 @@ class LinearAttentionFn(torch.autograd.Function):
         q, k, v, g, s0 = ctx.saved_tensors
         if dout is None and dlast is None:
             return None, None, None, None, None, None, None
+        given = [t for t in (q, k, v, g, s0, dout, dlast) if t is not None]
         new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
         with _lib.on_device(q):
             dout = torch.zeros(v.shape, dtype=v.dtype, device=v.device) if dout is None else _inner(dout)
@@ -83,6 +85,7 @@ class LinearAttentionFn(torch.autograd.Function):
             at = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
             _call("b200_linattn_bwd", q, k, v, g, ctx.scale, s0, 0, 0,
                   (dout.data_ptr(), at(dlast), *dout.stride()[:3], dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), at(dg), at(ds0)))
+        dq, dk, dv, dg, ds0 = once(given, (dq, dk, dv, dg, ds0))
         return dq, dk, dv, dg, None, ds0, None
 
 

@@ -15,13 +15,16 @@ import torch
 
 from .. import _lib
 from .mamba_block import _DT
+from .once import once
 
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 
 def _rows(t):
     """t with its last dimension contiguous and rows that do not overlap."""
-    return t if (t.stride(-1) == 1 or t.shape[-1] == 1) and t.stride(0) >= t.shape[-1] else t.contiguous()
+    if (t.stride(-1) == 1 or t.shape[-1] == 1) and t.stride(0) >= t.shape[-1]:
+        return t
+    return t.clone(memory_format=torch.contiguous_format) if t.shape[0] == 1 else t.contiguous()      # a single row of any pitch counts as contiguous
 
 
 @functools.lru_cache(maxsize=None)
@@ -66,11 +69,11 @@ class LinearCrossEntropyFn(torch.autograd.Function):
         hidden, weight, labels, lse, count = ctx.saved_tensors
         need_h, need_w = ctx.needs_input_grad[:2]
         with _lib.on_device(hidden):
-            grad = grad.to(torch.float32).contiguous()
+            given, grad = grad, grad.to(torch.float32).contiguous()
             dh = torch.empty(hidden.shape, dtype=hidden.dtype, device=hidden.device) if need_h else None
             dw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device) if need_w else None
             _call("b200_lce_bwd", hidden, weight, labels, *ctx.meta, lse, None, count, grad, dh, dw)
-        return dh.view(ctx.shape) if need_h else None, dw, None, None, None
+        return *once((hidden, weight, given), (dh.view(ctx.shape) if need_h else None, dw)), None, None, None
 
 
 def linear_cross_entropy(hidden, weight, labels, ignore_index=-100, reduction="mean"):

@@ -440,3 +440,55 @@ def test_attention_is_causal_whatever_comes_later(dtype, value):
         hit = torch.zeros_like(o, dtype=torch.bool)
         hit[0, t, 2:] = True
         within("queries", o[~hit], clean[~hit].double(), bound[~hit])
+
+
+# ------------------------------------------------------------------------------------------------ calls that were answered wrongly
+
+
+def test_model_embedding_is_a_module():
+    """The model calls its embedding as a module: hooks on it run, and a module put in its place is the one that is called."""
+    from lrnnx_b200.lm import MambaLMHeadModel
+    torch.manual_seed(0)
+    m = MambaLMHeadModel(32, 1, 100, device="cuda")
+    ids = torch.randint(0, 100, (2, 9), device="cuda")
+    seen = []
+    handle = m.backbone.embedding.register_forward_hook(lambda module, args, out: seen.append(out.shape))
+    want = m(ids)
+    handle.remove()
+    assert seen == [(2, 9, 32)] and isinstance(m.backbone.embedding, torch.nn.Embedding)
+    plain = torch.nn.Embedding(100, 32, device="cuda")
+    plain.weight = m.backbone.embedding.weight
+    m.backbone.embedding = torch.nn.Sequential(plain, torch.nn.Identity())
+    assert torch.equal(m(ids), want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_one_row_with_any_stride(dtype):
+    """The pitch of a single row, or of a single class, means nothing and may be zero."""
+    from lrnnx_b200.ops import linear_cross_entropy, token_embedding
+    h, w, labels = loss_operands(6, 40, 24, dtype)
+    one = h[0].expand(6, 24)[:1]
+    assert one.stride(0) == 0
+    want = linear_cross_entropy(h[:1], w, labels[:1], reduction="none")
+    assert torch.equal(linear_cross_entropy(one, w, labels[:1], reduction="none"), want)
+    hg, wg = h[:1].clone().requires_grad_(), w[0].expand(5, 24)[:1].requires_grad_()
+    loss = linear_cross_entropy(hg, wg, torch.zeros_like(labels[:1]))
+    a = torch.autograd.grad(loss, (hg, wg))
+    # the softmax of one class is one: three roundings of log-sums up to 8 in the loss, times values up to 4 in the gradients
+    assert abs(float(loss.detach())) <= 3 * 2.0 ** -21 and all(float(x.float().abs().max()) <= 3 * 2.0 ** -19 for x in a)
+    assert torch.equal(token_embedding(torch.zeros(3, dtype=torch.int64, device="cuda"), one.detach()), h[:1].expand(3, 24))
+
+
+def test_second_derivatives_are_refused():
+    """The gradients have no gradients of their own: asking for them is an error and not a silent zero."""
+    from lrnnx_b200.ops import linear_attention_fn, linear_cross_entropy, token_embedding
+    h, w, labels = loss_operands(6, 40, 24, torch.float32)
+    q, k, v, g, _ = attn_operands(1, 5, 1, 1, 8, 8, torch.float32, "step")[0]
+    ids = labels.clamp(0, 39)
+    for make, x in ((lambda x: linear_cross_entropy(x, w, labels), h), (lambda x: token_embedding(ids, x).square().sum(), w),
+                    (lambda x: linear_attention_fn(x, k, v, g).square().sum(), q)):
+        x = x.detach().clone().requires_grad_()
+        dx, = torch.autograd.grad(make(x), x, create_graph=True)
+        assert torch.equal(dx, torch.autograd.grad(make(x), x)[0])
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            (dx.sum() + x.sum()).backward()
