@@ -33,6 +33,7 @@
 #include "common.cuh"
 #include "dispatch.h"
 #include "tc_common.cuh"
+#include <algorithm>
 #include <cstring>
 
 namespace b200 {
@@ -52,6 +53,7 @@ constexpr int LCE_SMEM = NST * ST_BYTES + 8 * STAGING + 1024;
 constexpr uint32_t LCE_WAIT = 1u << 24;
 constexpr int64_t kPieceBytes = int64_t(1) << 30;
 constexpr int kSegSteps = 8;              // float32 only: stages (of 64) in one accumulation chain of the leading product
+constexpr int kPieceStages = 64;           // what a piece costs besides, in stages: launches, the sums of dH read and written
 constexpr int kMaxSplits = 32;            // blocks that share the contraction of a tile
 
 // EPI_SUM: as EPI_OUT, the sums of a tile's chains kept in registers
@@ -648,7 +650,8 @@ struct Plan {
 
 // How many blocks share the contraction of `stages` for each of `tiles` tiles: as few as fill the SMs (at least 8 stages
 // each, to be worth 128 KB of sums).
-void split_of(int64_t tiles, int stages, int &splits, int &per) {
+// Returns the stages that pass until all is done.
+int64_t split_of(int64_t tiles, int stages, int &splits, int &per) {
   const int64_t pairs = sm_count_current() / 2;
   splits = 1;
   per = stages;
@@ -659,6 +662,28 @@ void split_of(int64_t tiles, int stages, int &splits, int &per) {
     const int64_t cost = (tiles * s + pairs - 1) / pairs * p;
     if (cost * 100 < best * 90) { best = cost; splits = s; per = p; }
   }
+  return best;
+}
+
+// The classes of a piece, in tiles of 256, where dz has to be made in pieces of at most `most`: the number for which the
+// products with dz, taken a wave of tiles after the other, take the fewest stages (16384 x 50280 x 768 on 74 pairs: pieces
+// of 99 and 98 leave dz^T H one tile for a fifth wave, 510 + 438 us; 123 and 74 fill five and three, see the figures above).
+int64_t piece_of(const b200_lce_args &a, int64_t total, int64_t most) {
+  if (total <= most) return total;
+  const int64_t least = (total + (total + most - 1) / most) / ((total + most - 1) / most + 1), step = most / 256 + 1;
+  const int64_t dt = (a.features + TN - 1) / TN, mt = (a.rows + 2 * TM - 1) / (2 * TM), pairs = sm_count_current() / 2;
+  int64_t best = most, cost = INT64_MAX;
+  for (int64_t p = most; p >= least; p -= step) {
+    const int64_t full = total / p, rest = total % p;
+    int s, per;
+    int64_t c = (mt * total / pairs + full + 1) * ((a.features + TK - 1) / TK) + (full + (rest > 0)) * kPieceStages;
+    c += full * split_of(mt * dt, (int)(p * (TN / TK)), s, per);
+    if (rest) c += (mt * dt * s + pairs - 1) / pairs * std::min<int64_t>(per, rest * (TN / TK));
+    c += full * split_of(p * dt, (int)((a.rows + TK - 1) / TK), s, per);
+    if (rest) c += (rest * dt * s + pairs - 1) / pairs * per;                      // a last, smaller piece is split as the others
+    if (c < cost) { cost = c; best = p; }
+  }
+  return best;
 }
 
 bool in_place(const void *p, int64_t rs, int cols) {
@@ -676,10 +701,8 @@ Plan plan_of(const b200_lce_args &a, bool bwd) {
   q.pack_bytes_w = q.pack_w ? up(2 * q.planes * (int64_t)a.classes * q.Dp, 256) : 0;
   q.seg = f32 ? kSegSteps : 1 << 30;
   q.Da = up(a.features, 4);
-  int64_t most = kPieceBytes / (2 * q.planes * a.rows) / TN * TN;
-  if (most < TN) most = TN;
-  q.n_pieces = (int)((a.classes + most - 1) / most);
-  q.piece = (int)up((a.classes + q.n_pieces - 1) / q.n_pieces, TN);
+  const int64_t most = kPieceBytes / (2 * q.planes * a.rows) / TN;
+  q.piece = bwd ? (int)piece_of(a, (a.classes + TN - 1) / TN, most < 1 ? 1 : most) * TN : TN;
   q.n_pieces = (a.classes + q.piece - 1) / q.piece;
   q.dz_pitch = q.piece;
   q.dz_bytes = up(2 * q.planes * a.rows * q.dz_pitch, 256);
