@@ -75,7 +75,13 @@ struct Walk {
   int tiles, nseg, seg_chunks;            // blocks for a sequence's columns; segments and their chunks
   float *seg;                             // (batch heads, nseg, di, dout): states
   double *seg_g;                          // (batch heads, nseg): sums of g
+  int beside;                             // host: needs nothing of the walk launched before it
 };
+
+// The walks of a backward pass need nothing of one another: the next one's blocks take the places that the last blocks of
+// this one leave free.  Every block waits for the walk before at its end, so that what follows the last walk follows all.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_last() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 __device__ __forceinline__ float ex2a(float x) {
   float y;
@@ -319,6 +325,7 @@ template <typename T, int DI, int WT, bool STATE_ONLY> __global__ void __launch_
       if (col0 + col < p.dout) p.snap[(((int64_t)bh * snaps + c / kSnap) * p.di + r) * p.dout + col0 + col] = S[r * PV + col] * f;
     }
   };
+  let_next_start();
   // the state before the first step
   for (int e = tid; e < dip * DO; e += WT) {
     const int r = e / DO, c = e % DO;
@@ -499,6 +506,7 @@ template <typename T, int DI, int WT, bool STATE_ONLY> __global__ void __launch_
       if (col0 + c < p.dout) p.last[b * p.last_bs + h * p.last_hs + r * p.last_is + (col0 + c) * p.last_os] = S[r * PV + c] * f;
     }
   }
+  wait_for_last();
 }
 
 // ------------------------------------------------------------------------------------------------ bfloat16
@@ -696,6 +704,7 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
     fail = 0;
     mbar_fence_init();
   }
+  let_next_start();
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)), "r"(256) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -1143,6 +1152,7 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
   __syncthreads();
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(256) : "memory");
   if (tid == 0 && fail) atomicExch(&g_linattn_status, 9);
+  wait_for_last();
 }
 
 // Each segment's own state becomes the state before it.
@@ -1383,7 +1393,18 @@ int launch_walk(Walk &w, K own, K all, int threads, int smem_own, int smem_all, 
     linattn_join_kernel<<<dim3((unsigned)((per + 255) / 256), (unsigned)bh), 256, 0, st>>>(w);
     if (int r = launch_status()) return r;
   }
-  all<<<(unsigned)(bh * w.tiles * w.nseg), threads, smem_all, st>>>(w, more...);
+  cudaLaunchAttribute beside = {};
+  beside.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  beside.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(bh * w.tiles * w.nseg));
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem_all;
+  cfg.stream = st;
+  cfg.attrs = &beside;
+  cfg.numAttrs = w.beside && w.nseg == 1 ? 1 : 0;          // segments' states lie in the workspace that the walks share
+  e = cudaLaunchKernelEx(&cfg, all, (const Walk)w, more...);
+  if (e != cudaSuccess) { set_error("CUDA launch failed: %s", cudaGetErrorString(e)); return (int)e; }
   return launch_status();
 }
 template <typename T, int DI, int WT> int walk(Walk &w, unsigned char *work, cudaStream_t st) {
@@ -1524,13 +1545,13 @@ BwdPlan bwd_plan(const b200_linattn_args &a) {
     if (s > q.seg) q.seg = s;
   }
   const int64_t chunks = ws[0].chunks;
-  q.part = a.heads != a.groups ? up(4 * bh * a.seqlen * a.dk, 256) : 0;
+  q.part = a.heads != a.groups ? up(4 * bh * a.seqlen * a.dk, 256) : 0;          // of each of dq and dk
   q.run = a.dg ? up(4 * bh * a.seqlen * ws[0].tiles, 256) : 0;
   q.sum = a.dg ? up(4 * bh * chunks * ws[0].tiles, 256) : 0;
   q.snap = a.dg ? up(4 * bh * ((a.seqlen + kSnapSteps - 1) / kSnapSteps) * a.dk * a.dv, 256) : 0;
   q.across = a.dg ? up(8 * bh * chunks, 256) : 0;
   q.heads = a.dg && a.g_heads ? up(8 * bh, 256) : 0;
-  q.total = q.seg + q.part + 2 * (q.run + q.sum + q.snap) + q.across + q.heads;
+  q.total = q.seg + 2 * (q.part + q.run + q.sum + q.snap) + q.across + q.heads;
   return q;
 }
 
@@ -1599,9 +1620,9 @@ extern "C" int b200_linattn_bwd(const b200_linattn_args *args, void *stream) {
   unsigned char *work = reinterpret_cast<unsigned char *>(a.work);
   unsigned char *at = work + q.seg;
   const auto take = [&](int64_t bytes) { unsigned char *r = at; at += bytes; return r; };
-  float *part = reinterpret_cast<float *>(take(q.part));
-  float *run[2], *sum[2], *snap[2];
+  float *part[2], *run[2], *sum[2], *snap[2];
   for (int i = 0; i < 2; ++i) {
+    part[i] = reinterpret_cast<float *>(take(q.part));
     run[i] = reinterpret_cast<float *>(take(q.run));
     sum[i] = reinterpret_cast<float *>(take(q.sum));
     snap[i] = reinterpret_cast<float *>(take(q.snap));
@@ -1609,10 +1630,12 @@ extern "C" int b200_linattn_bwd(const b200_linattn_args *args, void *stream) {
   double *across = reinterpret_cast<double *>(take(q.across)), *heads = reinterpret_cast<double *>(take(q.heads));
   const bool shared = a.heads != a.groups;
   int tiles = 0, chunks = 0;
+  Walk w = walk_dv(a);                                   // from the shortest blocks to the longest: none waits long for the walk before
+  if (int e = run_walk(a.dtype, w, work, st)) return e;
   for (int i = 0; i < 2; ++i) {
-    Walk w = i == 0 ? walk_dq(a) : walk_dk(a);
-    void *dst = i == 0 ? a.dq : a.dk_out;
-    w.out = shared ? part : dst;
+    w = i == 0 ? walk_dq(a) : walk_dk(a);
+    w.beside = 1;
+    w.out = shared ? part[i] : i == 0 ? a.dq : a.dk_out;
     w.out_f32 = shared;
     w.o_bs = (int64_t)a.seqlen * a.heads * a.dk;
     w.o_ls = (int64_t)a.heads * a.dk;
@@ -1625,11 +1648,11 @@ extern "C" int b200_linattn_bwd(const b200_linattn_args *args, void *stream) {
     tiles = w.tiles;
     chunks = w.chunks;
     if (int e = run_walk(a.dtype, w, work, st)) return e;
-    if (shared)
-      if (int e = fold(a, part, dst, st)) return e;
   }
-  Walk w = walk_dv(a);
-  if (int e = run_walk(a.dtype, w, work, st)) return e;
+  if (shared) {
+    if (int e = fold(a, part[0], a.dq, st)) return e;
+    if (int e = fold(a, part[1], a.dk_out, st)) return e;
+  }
   if (a.dg) {
     const int bh = a.batch * a.heads, every = kSnapSteps / w.ch, snaps = (chunks + every - 1) / every;
     linattn_across_kernel<<<(unsigned)((int64_t)bh * snaps), 256, 0, st>>>(snap[0], snap[1], sum[0], sum[1], tiles, (int64_t)a.dk * a.dv, chunks, every, snaps, bh, across);
