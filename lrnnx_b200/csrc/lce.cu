@@ -16,19 +16,21 @@
 // loads into a 6-stage ring (64 of the contraction a stage) and warps 4-11 empty one of two 256-column accumulators while
 // the other is filled; warp 1 of the first block issues the MMAs for both.  A single block's tile of 128 x 256 takes 96 bytes
 // a clock from L2 where a pair takes 64, and its MMAs waited for loads a quarter of the time (16384 x 50280 x 768: the
-// product with W 488 -> 456 us, 90 % of the tensor pipe's cycles; the forward 849 -> 844 us, 1.5 PFLOP/s).  Either operand may have the contraction along its rows (z) or across them (dz W, dz^T H): both are 128-byte
+// product with W 488 -> 456 us, 90 % of the tensor pipe's cycles; the forward 849 -> 844 us, 1.5 PFLOP/s).
+// Either operand may have the contraction along its rows (z) or across them (dz W, dz^T H): both are 128-byte
 // swizzled tiles, of K-major or of MN-major layout.
 //
 // float32 operands are split into three bfloat16 (8 bits of mantissa each) and multiplied as six products of the
 // planes, the small ones first; what is left out is below 2^-24.  The tensor core truncates when it adds into its
 // accumulator, an error to one side that grows with the length of the chain, so that long contractions are cut into
 // chains of kSegSteps whose sums are added up in float32, rounded to nearest: for the gradients in the epilogue's registers
-// (through memory a chain's sums cost 40 us of the 205 of dz W at 2031 x 16411 x 509).  (An infinite float32 operand gives NaN
+// (through memory they cost dz W 32 us of 204 at 2031 x 16411 x 509).  (An infinite float32 operand gives NaN
 // where its product with the rest of a split is none.)
 //
 // Measured (one B200, 16384 x 50280 x 768 bfloat16, forward and backward 4.34 ms, 1.17 PFLOP/s over the four products, under the power
 // limit as a library product would be): z and its log-sum-exp 827-844 us (tensor pipe 82 %), the two pieces of dz 479 us each
-// (74 %: the epilogue's stores), dz W 439-456 us each (90 %), dz^T H 510 and 438 us (80 %: 297 tiles on 74 pairs).  float32,
+// (74 %: the epilogue's stores), dz W 439-456 us each (90 %), dz^T H 510 and 438 us (80 %: 297
+// tiles on 74 pairs), with pieces of equal size; cut as piece_of does, 65 us less for the whole.  float32,
 // 2031 x 16411 x 509: 0.84 ms, six times the products.
 #include "common.cuh"
 #include "dispatch.h"

@@ -113,7 +113,8 @@ def linear_attention_fn(q, k, v, g, scale=1.0, initial_state=None, return_last_s
     multiple of groups, dk and dv up to 128.  g: log decays, (batch, length, heads) or (heads,), float32 or the dtype of
     q; -inf starts from an empty state at that step (a new document).  ``initial_state`` float32 (batch, heads, dk, dv)
     is the state before the first step.  Returns out (batch, length, heads, dv), and with ``return_last_state`` the float32
-    state after the last step.  Gradients for q, k, v, g and initial_state."""
+    state after the last step.  An infinite or NaN value reaches its own step and later ones, no earlier result.  Gradients for q, k, v, g and
+    initial_state."""
     _check("linear_attention_fn", 4, q, k, v, g, initial_state)
     batch, length, heads, dv = v.shape
     if initial_state is not None and (tuple(initial_state.shape) != (batch, heads, q.shape[-1], dv) or initial_state.dtype != torch.float32):
