@@ -709,7 +709,8 @@ Plan plan_of(const b200_lce_args &a, bool bwd) {
   q.dz_pitch = q.piece;
   q.dz_bytes = up(2 * q.planes * a.rows * q.dz_pitch, 256);
   const int64_t dt = (a.features + TN - 1) / TN;
-  split_of((a.rows + 2 * TM - 1) / (2 * TM) * dt, (q.piece + TK - 1) / TK, q.splits_h, q.per_h);
+  // by the stages of the first piece, which has all the classes where it is the only one: each of its blocks has a part then, and writes its sums
+  split_of((a.rows + 2 * TM - 1) / (2 * TM) * dt, (std::min(q.piece, a.classes) + TK - 1) / TK, q.splits_h, q.per_h);
   split_of((q.piece + 2 * TM - 1) / (2 * TM) * dt, (int)((a.rows + TK - 1) / TK), q.splits_w, q.per_w);
   // float32 sums: of dH over the pieces and the blocks that share a tile, of dW over the blocks
   q.acc_h_bytes = q.n_pieces > 1 || q.splits_h > 1 ? up(4 * q.splits_h * a.rows * q.Da, 256) : 0;
@@ -896,7 +897,7 @@ extern "C" int b200_lce_bwd(const b200_lce_args *args, void *stream) {
       B200_REQUIRE(map16(&g.a, a.dtype, dz, cols, a.rows, q.dz_pitch, q.planes, TM) && map16(&g.b, a.dtype, o.w, a.features, a.classes, o.w_pitch, q.planes, 64),
                    B200_ERR_UNSUPPORTED, "lce: tensor-map encoding failed");
       g.nk = (cols + TK - 1) / TK;
-      g.splits = q.splits_h;                                     // of a shorter last piece some blocks have no part; their sums stay
+      g.splits = q.splits_h;                                     // of a shorter piece after the first some blocks have no part; their sums stay
       g.per = q.per_h;
       if (g.seg > g.nk) g.seg = g.nk;
       g.a_mn = 0;
