@@ -161,7 +161,9 @@ __device__ __forceinline__ Two from_lane(Two s, int lane) { return Two{__shfl_sy
 __device__ __forceinline__ void chunk_decays(const Walk &p, int b, int h, int i0, int lane, Decays &d) {
   const Two a0 = log2_decay(p, b, h, i0 + 2 * lane), a1 = log2_decay(p, b, h, i0 + 2 * lane + 1);
   const Two s = inclusive(a0 + a1, lane), end = from_lane(s, 31);
-  const Two G[2] = {s + -a1, s};
+  Two before = shfl_up2(s, 1);
+  if (lane == 0) before = two(0.f);
+  const Two G[2] = {before + a0, s};                 // (s less a1 would be NaN where a1 is infinite or NaN, a step before it)
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const int i = 2 * lane + j;
