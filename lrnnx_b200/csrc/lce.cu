@@ -7,8 +7,9 @@
 // The forward is one product whose tiles never leave the SM: each 128 x 256 tile of z is reduced to a running maximum
 // and sum of a row's half (float32, natural units scaled by log2 e), a second kernel joins them.  The backward makes z
 // again in pieces of the vocabulary, writes a piece of dz in the operands' type and multiplies it from both sides; the
-// piece's columns are chosen so that dz stays below kPieceBytes.  dz is kept in units of the largest |s_r|, so that a
-// float16 dz neither overflows under a scaled loss nor vanishes under a mean over many rows; the products are scaled back
+// piece's columns are chosen so that dz stays below kPieceBytes.  dz is kept in units of the largest |s_r|, float16 in a
+// 2^15th of it, so that a float16 dz neither overflows under a scaled loss nor vanishes under a mean over many rows or where
+// probabilities are small: below 2^-29 of the largest weight it loses bits, below 2^-40 it is zero.  The products are scaled back
 // in 32 bits.  s_r = 0 (ignored labels) makes an exact zero row.
 //
 // The products run on tcgen05 with accumulators in TMEM, one kernel with four epilogues.  Pairs of thread blocks
@@ -141,11 +142,16 @@ struct LcePipe {
 __device__ __forceinline__ int plane_a(int passes, int p) { return passes == 1 ? 0 : (0x021010 >> (4 * (5 - p))) & 15; }
 __device__ __forceinline__ int plane_b(int passes, int p) { return passes == 1 ? 0 : (0x201100 >> (4 * (5 - p))) & 15; }
 
-// The largest |s_r|, which dz is kept in units of; 1 where there is none to divide by.
+// The largest finite |s_r|, which dz is kept in units of; 1 where there is none to divide by.
 __device__ __forceinline__ float unit_of(const float *common) {
   const float c = *common;
-  return c > 0.f && c < INFINITY ? c : 1.f;
+  return c > 0.f ? c : 1.f;
 }
+// A float16 dz, at most 1 in that unit, is kept 2^15 times as large, near the top of the type's range (65504): its probabilities would
+// otherwise lie in the lower half of the range, and at 50280 classes the mean one below the smallest normal number, 2^-14.
+__host__ __device__ constexpr float dz_up(int dtype) { return dtype == B200_F16 ? 32768.f : 1.f; }
+// what a sum over dz is multiplied by
+__device__ __forceinline__ float unit_back(const float *common, int dtype) { return unit_of(common) / dz_up(dtype); }
 
 template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
 template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
@@ -320,7 +326,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LCE_THREADS, 1) lce_
           }
           if (EPI == EPI_DZ) {
             lse2 = p.lse[row] * kLog2e;
-            sc = p.rs[row] / unit_of(p.common);
+            sc = p.rs[row] / unit_of(p.common) * dz_up(p.dtype);
           }
         }
         if (!mbar_wait(&pipe.acc_full[ch & 1], (ch >> 1) & 1, LCE_WAIT)) { ok = false; break; }
@@ -395,7 +401,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LCE_THREADS, 1) lce_
           if (lane == 0) arrive_at(of_first(&pipe.acc_empty[ch & 1]));
         } else {
           float *acc = p.acc + (int64_t)(t / (p.nt * p.mt)) * p.rows * p.acc_rs;
-          const float unit = unit_of(p.common);
+          const float unit = unit_back(p.common, p.dtype);
           if constexpr (EPI == EPI_SUM) {
 #pragma unroll
             for (int c = 0; c < TN / 64; ++c) {
@@ -585,7 +591,7 @@ __global__ void __launch_bounds__(1024) lce_sum_kernel(const float *loss, const 
   }
 }
 
-// s_r, and the largest |s_r| by an atomic maximum of its bits (any order gives the same; the word was cleared).
+// s_r, and the largest finite |s_r| by an atomic maximum of its bits (any order gives the same; the word was cleared).
 __global__ void __launch_bounds__(256) lce_scale_kernel(const float *dloss, int per_row, const float *count, const int64_t *labels, int64_t ignore, int classes,
                                                        int rows, float *rs, unsigned *common) {
   const int r = blockIdx.x * 256 + threadIdx.x;
@@ -594,7 +600,7 @@ __global__ void __launch_bounds__(256) lce_scale_kernel(const float *dloss, int 
     if (is_target(labels[r], ignore, classes)) s = dloss[per_row ? r : 0] / (count ? *count : 1.f);
     rs[r] = s;
   }
-  const unsigned m = __reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(s)));
+  const unsigned m = __reduce_max_sync(0xffffffffu, isfinite(s) ? __float_as_uint(fabsf(s)) : 0u);
   if ((threadIdx.x & 31) == 0 && m) atomicMax(common, m);
 }
 
@@ -602,7 +608,7 @@ __global__ void __launch_bounds__(256) lce_scale_kernel(const float *dloss, int 
 __global__ void __launch_bounds__(256) lce_fold_kernel(const float *acc, int splits, int64_t rows, int cols, int64_t acc_rs, const float *common, int dtype, void *dst,
                                                       int64_t dst_rs) {
   const int64_t n = rows * (acc_rs / 4), plane = rows * acc_rs;
-  const float unit = unit_of(common);
+  const float unit = unit_back(common, dtype);
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
     const int64_t r = i / (acc_rs / 4);
     const int c = (int)(i - r * (acc_rs / 4)) * 4;

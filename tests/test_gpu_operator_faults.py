@@ -40,6 +40,57 @@ def test_shared_contractions_add_up_what_was_written(rows, classes, features, dt
     check(got, ref, h, w, dtype)
 
 
+@pytest.mark.parametrize("spread,classes,features", [(1.0, 50280, 64), (4.0, 50280, 48), (2.0, 131072, 16), (0.5, 300, 64)])
+def test_float16_gradients_keep_small_probabilities(spread, classes, features):
+    """Row weights from 1e-4 to 1 of the largest and probabilities around 1 / classes.  dz is rounded to half a step of itself, at
+    least 2^-25 in units of a 2^15th of the largest row weight: 2^-40 of it, where a row's own weight is 1e-4 = 2^-13.3 of it.  The
+    other terms are those of any gradient; weights are positive on average, so that the softmax's part of a row's gradient does not cancel."""
+    from lrnnx_b200.ops import linear_cross_entropy
+    rows, u = 96, 2.0 ** -11
+    h, w, labels = loss_operands(rows, classes, features, torch.float16, spread=spread)
+    w = (w.float() + 0.25).to(torch.float16)
+    up = 1024 * 10.0 ** -torch.linspace(0, 4, rows, device="cuda")
+    hh, ww = h.detach().requires_grad_(), w.detach().requires_grad_()
+    got = torch.autograd.grad(linear_cross_entropy(hh, ww, labels, reduction="none"), (hh, ww), up)
+    ref = reference(h, w, labels, up)
+    e = ref["p_err"] + u * ref["dz"].abs() + 2.0 ** -40 * ref["unit"]
+    for name, x, err, mag, n in (("dh", got[0], e @ w.double().abs(), ref["dz"].abs() @ w.double().abs(), classes),
+                                 ("dw", got[1], e.t() @ h.double().abs(), ref["dz"].abs().t() @ h.double().abs(), rows)):
+        within(name, x, ref[name], err + (n / 16 + 8) * 2.0 ** -23 * mag + u * ref[name].abs() + 2.0 ** -25)
+
+
+def test_float16_gradients_at_the_largest_scale():
+    """A certain row's dz is at most 2 float16 steps over its weight, 2^15 units: no overflow, and none where the upstream gradient is huge."""
+    from lrnnx_b200.ops import linear_cross_entropy
+    h, w = torch.full((4, 8), 8.0, dtype=torch.float16, device="cuda"), torch.zeros(5, 8, dtype=torch.float16, device="cuda")
+    w[0], w[1] = 8.0, -8.0                               # logits 512 and -512: the first class for certain
+    labels = torch.tensor([0, 1, 2, 0], device="cuda")
+    for up in (1.0, 2.0 ** 12, 2.0 ** -12):
+        hh, ww = h.clone().requires_grad_(), w.clone().requires_grad_()
+        dh, dw = torch.autograd.grad(linear_cross_entropy(hh, ww, labels, reduction="none"), (hh, ww), torch.full((4,), up, device="cuda"))
+        want = torch.zeros(4, 8, device="cuda")
+        want[1], want[2] = 16.0 * up, 8.0 * up           # W[0] - W[label]
+        assert torch.equal(dh.float(), want.half().float())
+        want = torch.zeros(5, 8, device="cuda")
+        want[0], want[1], want[2] = 16.0 * up, -8.0 * up, -8.0 * up
+        assert torch.equal(dw.float(), want.half().float())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+def test_a_row_weight_that_is_not_finite_stays_in_its_row(value, dtype):
+    """An upstream gradient that overflowed in one row leaves the other rows' hidden gradients as they are."""
+    from lrnnx_b200.ops import linear_cross_entropy
+    h, w, labels = loss_operands(40, 500, 64, dtype)
+    labels[7] = 3
+    up = 64 * (1 + torch.arange(40, device="cuda") % 7).float()
+    rows = torch.arange(40, device="cuda") != 7
+    clean, = torch.autograd.grad(linear_cross_entropy(h.requires_grad_(), w, labels, reduction="none"), h, up)
+    up[7] = value
+    got, = torch.autograd.grad(linear_cross_entropy(h, w, labels, reduction="none"), h, up)
+    assert torch.equal(got[rows], clean[rows]) and not bool(torch.isfinite(got[7]).any())
+
+
 # ------------------------------------------------------------------------------------------------ linear attention
 
 
