@@ -406,6 +406,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LCE_THREADS, 1) lce_
 #pragma unroll
             for (int c = 0; c < TN / 64; ++c) {
               float v[32];
+              __syncwarp();                              // lanes come from their own waits, and from the last tile's stores
               tmem_ld32(ta + c * 32, v);
 #pragma unroll
               for (int j = 0; j < 32; ++j) sums[c][j] = k0 == kb ? v[j] : sums[c][j] + v[j];

@@ -710,6 +710,7 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
     mbar_fence_init();
   }
   let_next_start();
+  __syncwarp();
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)), "r"(256) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -953,6 +954,7 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
           for (int q = 0; q < 2; ++q) {
             const int c = cb * 32 + q * 16;
             float v[16], x2[16];
+            __syncwarp();
             if constexpr (cross) tmem_ld16x2(tm_own + tP + c, tm_own + tO + c, v, x2);
             else tmem_ld16(tm_own + tP + c, v);
             if (cb != wr) {
@@ -1116,6 +1118,7 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
     }
     {
       float v[NS];
+      __syncwarp();                                      // lanes come from their own stores
       if constexpr (NS == 32) tmem_ld32(tm_own + tD + cs, v);
       else tmem_ld16(tm_own + tD + cs, v);
       const float keep = d.keep, keep_lo = d.keep_lo;

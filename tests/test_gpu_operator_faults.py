@@ -116,3 +116,38 @@ def test_a_decay_reaches_no_earlier_step(t, value, dtype):
         clean = torch.ones_like(x, dtype=torch.bool)
         clean[0, reached, head] = False                  # the first group is the first two heads
         within(name, x[clean], want[i][clean], ((F + 2 * u) * mag[i] + u * want[i].abs() + tiny)[clean])
+
+
+# ------------------------------------------------------------------------------------------------ waits
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_lanes_meet_before_accumulators_are_read(dtype):
+    """Sizes at which the lanes of a warp part right before an accumulator is read: columns that end inside 32, rows that cannot leave as a
+    tile, several chunks and chains; results as for any size, the same twice, and no bounded wait ran out."""
+    from lrnnx_b200 import _lib
+    from lrnnx_b200.ops import linear_attention_fn, linear_cross_entropy
+    h, w, labels = loss_operands(700, 1301, 509, dtype)
+    hh, ww = h.detach().requires_grad_(), w.detach().requires_grad_()
+    up = torch.tensor(700.0, device="cuda")
+    runs = [torch.autograd.grad(linear_cross_entropy(hh, ww, labels), (hh, ww), up) for _ in range(2)]
+    counted = int((labels != -100).sum())
+    check(runs[0], reference(h, w, labels, torch.full((700,), 700 / counted, device="cuda", dtype=torch.float64)), h, w, dtype)
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+    for dk, dv in ((33, 81), (121, 99)):
+        ops, dout, dlast = attn_operands(2, 391, 3, 1, dk, dv, dtype, "token", seed=21)
+        want = with_gradients(ops, 1.0, dout, dlast)
+        mag = with_gradients([x.abs() for x in ops[:3]] + [ops[3], ops[4].abs()], 1.0, dout.abs(), dlast.abs())
+        runs = []
+        for _ in range(2):
+            leaves = [x.detach().requires_grad_() for x in ops]
+            o, last = linear_attention_fn(*leaves[:4], initial_state=leaves[4], return_last_state=True)
+            runs.append([o.detach(), last.detach(), *torch.autograd.grad([o, last], leaves, [dout, dlast])])
+        assert all(torch.equal(a, b) for a, b in zip(*runs))
+        F, u = (391 / 16 + 200) * 2.0 ** -23, ATTN_HALF[dtype]
+        for i in (0, 2, 3, 4):
+            within(str(i), runs[0][i], want[i], (F + 2 * u) * mag[i] + u * want[i].abs() + TINY[dtype])
+        for i in (1, 6):
+            within(str(i), runs[0][i], want[i], F * mag[i])
+    torch.cuda.synchronize()
+    assert _lib.lib().b200_device_status() == 0
