@@ -826,8 +826,7 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
     if (grad && !cross && chunk % kSnapB == 0) snapshot(chunk / kSnapB, 1.f);
     fence_proxy_async();
     tc_fence_before();
-    __syncthreads();                                     // the state's terms are written, accumulators read
-    if (*(volatile int *)&fail) break;
+    if (__syncthreads_or(*(volatile int *)&fail)) break;     // the state's terms are written, accumulators read; a wait that ran out ends the walk for all
     if (!STATE_ONLY && tid < DO) {                       // the next chunk's
       odd[(it + 1) & 1] = 0;
       odd_from[(it + 1) & 1][tid] = BC;
@@ -1145,10 +1144,12 @@ template <int DI, int MODE> __global__ void __launch_bounds__(BT, DI == 128 && M
       }
     }
   }
-  if (grad && warp == sum_warp && i_end > i_begin && !*(volatile int *)&fail) chunk_runs(p, tile, bh, i_end - BC, lane, pairs, dot_sum);
+  const bool ok = !__syncthreads_or(*(volatile int *)&fail);
+  if (grad && warp == sum_warp && i_end > i_begin && ok) chunk_runs(p, tile, bh, i_end - BC, lane, pairs, dot_sum);
   if (!STATE_ONLY && issuer) bulk_wait<0>();
+  if (!ok && issuer)
+    for (int i = 0; i < 1 << 12; ++i) __nanosleep(256);  // copies and products in flight: a millisecond, many times what they take
   __syncwarp();
-  const bool ok = !*(volatile int *)&fail;
   if (STATE_ONLY && ok) {
     each([&](int c, float &x) { p.seg[(((int64_t)bh * p.nseg + seg) * p.di + rs) * p.dout + c] = x; });
     if (tile == 0 && tid == 0) p.seg_g[(int64_t)bh * p.nseg + seg] = total;

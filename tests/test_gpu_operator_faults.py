@@ -151,3 +151,21 @@ def test_lanes_meet_before_accumulators_are_read(dtype):
             within(str(i), runs[0][i], want[i], F * mag[i])
     torch.cuda.synchronize()
     assert _lib.lib().b200_device_status() == 0
+
+
+def test_waits_that_end_in_time_leave_no_status():
+    """A wait that ran out ends its block whole (all threads read the same decision) and sets the status word, which ordinary calls of every
+    path leave at zero: TMA or not, segments or not, with and without the gradient of the decays."""
+    from lrnnx_b200 import _lib
+    from lrnnx_b200.ops import linear_attention_fn
+    for b, n, heads, dk, dv, pad in ((1, 4000, 1, 64, 64, 0), (1, 4000, 1, 128, 128, 3), (8, 140, 24, 128, 64, 0), (2, 129, 2, 50, 30, 1)):
+        (q, k, v, g, s0), dout, dlast = attn_operands(b, n, heads, heads, dk, dv, torch.bfloat16, "token", seed=22)
+        if pad:
+            q, k, v = (torch.nn.functional.pad(x, (pad, pad))[..., pad:-pad] for x in (q, k, v))
+        for with_g in (False, True):
+            leaves = [x.detach().requires_grad_(i != 3 or with_g) for i, x in enumerate((q, k, v, g, s0))]
+            o, last = linear_attention_fn(*leaves[:4], initial_state=leaves[4], return_last_state=True)
+            grads = torch.autograd.grad([o, last], [x for x in leaves if x.requires_grad], [dout, dlast])
+            assert all(bool(torch.isfinite(x).all()) for x in (o, last, *grads))
+    torch.cuda.synchronize()
+    assert _lib.lib().b200_device_status() == 0
