@@ -12,7 +12,7 @@ import torch
 
 from .. import _lib
 from .mamba_block import _DT
-from .once import once
+from .once import once, recorded
 
 
 @functools.lru_cache(maxsize=None)
@@ -66,7 +66,7 @@ class TokenEmbeddingFn(torch.autograd.Function):
 def token_embedding(ids, weight, scale=1.0, padding_idx=None):
     """``scale * weight[ids]``: ids (...) int32 or int64, weight (classes, features) float32, float16 or
     bfloat16 -> (..., features).  The gradient of row ``padding_idx`` is zero.  An id outside
-    [0, classes) reads nothing: its row is NaN, and it adds to no gradient."""
+    [0, classes) reads nothing: its row is NaN, and it adds to no gradient.  Forward-mode derivatives are an error."""
     shape = weight.shape
     if len(shape) != 2 or 0 in shape:
         raise RuntimeError("token_embedding: weight (classes, features) expected")
@@ -84,6 +84,6 @@ def token_embedding(ids, weight, scale=1.0, padding_idx=None):
         raise RuntimeError("token_embedding: padding_idx must be a row of weight")
     if ids.numel() == 0:
         return weight[:0].sum() + weight.new_empty(ids.shape + (shape[1],))
-    if torch.is_grad_enabled() and weight.requires_grad:
+    if recorded(weight):
         return TokenEmbeddingFn.apply(ids, weight, float(scale), padding_idx)
     return _lookup(ids, weight, *shape, float(scale), padding_idx)[0]

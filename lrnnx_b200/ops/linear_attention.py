@@ -15,7 +15,7 @@ import torch
 
 from .. import _lib
 from .mamba_block import _DT
-from .once import once
+from .once import once, recorded
 
 MAX_SIZE = 128            # of dk and dv
 
@@ -114,7 +114,7 @@ def linear_attention_fn(q, k, v, g, scale=1.0, initial_state=None, return_last_s
     q; -inf starts from an empty state at that step (a new document).  ``initial_state`` float32 (batch, heads, dk, dv)
     is the state before the first step.  Returns out (batch, length, heads, dv), and with ``return_last_state`` the float32
     state after the last step.  An infinite or NaN value reaches its own step and later ones, no earlier result.  Gradients for q, k, v, g and
-    initial_state."""
+    initial_state; forward-mode derivatives are an error."""
     _check("linear_attention_fn", 4, q, k, v, g, initial_state)
     batch, length, heads, dv = v.shape
     if initial_state is not None and (tuple(initial_state.shape) != (batch, heads, q.shape[-1], dv) or initial_state.dtype != torch.float32):
@@ -126,8 +126,7 @@ def linear_attention_fn(q, k, v, g, scale=1.0, initial_state=None, return_last_s
         if not return_last_state:
             return out
         return out, initial_state.clone() if initial_state is not None else torch.zeros(batch, heads, q.shape[-1], dv, device=v.device)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad
-                                    or initial_state is not None and initial_state.requires_grad):
+    if recorded(q, k, v, g, initial_state):
         return LinearAttentionFn.apply(q, k, v, g, float(scale), initial_state, return_last_state)
     out, last = _forward(_inner(q), _inner(k), _inner(v), g, float(scale), None if initial_state is None else _inner(initial_state), return_last_state)
     return (out, last) if return_last_state else out

@@ -15,7 +15,7 @@ import torch
 
 from .. import _lib
 from .mamba_block import _DT
-from .once import once
+from .once import once, recorded
 
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
@@ -81,7 +81,8 @@ def linear_cross_entropy(hidden, weight, labels, ignore_index=-100, reduction="m
     that are not ``ignore_index`` (zero where there are none), their sum, or with ``reduction="none"``
     the loss of every row, zero for ignored ones.  hidden (..., features) and weight (classes,
     features) float32, float16 or bfloat16 alike; labels (...) integer.  A label outside [0, classes)
-    has no loss and no gradient, as in ``cross_entropy``; a row without a target may hold anything.  Gradients for hidden and weight."""
+    has no loss and no gradient, as in ``cross_entropy``; a row without a target may hold anything.  Gradients for hidden
+    and weight; forward-mode derivatives are an error."""
     if reduction not in _REDUCTIONS:
         raise RuntimeError(f"linear_cross_entropy: reduction must be one of {', '.join(_REDUCTIONS)}")
     if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1] or labels.shape != hidden.shape[:-1]:
@@ -97,7 +98,7 @@ def linear_cross_entropy(hidden, weight, labels, ignore_index=-100, reduction="m
     if labels.numel() == 0:                        # no rows: a sum over nothing, with gradients of zero
         zero = (hidden.sum() + weight[:0].sum()).float()
         return zero.expand(labels.shape) if reduction == "none" else zero
-    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+    if recorded(hidden, weight):
         return LinearCrossEntropyFn.apply(hidden, weight, labels, ignore_index, _REDUCTIONS[reduction])
     return _forward(_rows(hidden.reshape(-1, hidden.shape[-1])), _rows(weight), labels.reshape(-1).to(torch.int64).contiguous(), ignore_index,
                     _REDUCTIONS[reduction], labels.shape)[0]

@@ -169,3 +169,49 @@ def test_waits_that_end_in_time_leave_no_status():
             assert all(bool(torch.isfinite(x).all()) for x in (o, last, *grads))
     torch.cuda.synchronize()
     assert _lib.lib().b200_device_status() == 0
+
+
+# ------------------------------------------------------------------------------------------------ derivatives
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused(grad):
+    """A forward-mode tangent on any operand is an error, never dropped, whether gradients are recorded or not."""
+    import torch.autograd.forward_ad as fw
+    from lrnnx_b200.lm import MambaLMHeadModel
+    from lrnnx_b200.ops import linear_attention_fn, linear_cross_entropy, token_embedding
+    h, w, labels = loss_operands(6, 40, 24, torch.float32)
+    ids = labels.clamp(0, 39)
+    attn, _, _ = attn_operands(1, 5, 2, 1, 8, 8, torch.float32, "token")
+    calls = [(lambda x: token_embedding(ids, x), w), (lambda x: linear_cross_entropy(x, w, labels), h), (lambda x: linear_cross_entropy(h, x, labels), w)]
+    for i in range(5):
+        calls.append((lambda x, i=i: linear_attention_fn(*[x if j == i else t for j, t in enumerate(attn[:4])], initial_state=x if i == 4 else attn[4]), attn[i]))
+    model = MambaLMHeadModel(32, 1, 40, device="cuda")
+    calls.append((lambda x: torch.func.functional_call(model, {"backbone.embedding.weight": x}, (ids[None],)), model.lm_head.weight.detach()))
+    with torch.set_grad_enabled(grad), fw.dual_level():
+        for call, x in calls:
+            call(x)
+            with pytest.raises((NotImplementedError, RuntimeError), match="jvp|forward"):
+                call(fw.make_dual(x, torch.ones_like(x)))
+    # on the upstream gradient
+    x = w.clone().requires_grad_()
+    out = token_embedding(ids, x)
+    with fw.dual_level():
+        dout = torch.ones_like(out)
+        torch.autograd.grad(out, x, dout, retain_graph=True)
+        with pytest.raises((NotImplementedError, RuntimeError), match="jvp|forward"):
+            torch.autograd.grad(out, x, fw.make_dual(dout, dout))
+
+
+def test_transforms_are_refused():
+    """torch.func's transforms of the operators are errors."""
+    from lrnnx_b200.ops import linear_attention_fn, linear_cross_entropy, token_embedding
+    h, w, labels = loss_operands(6, 40, 24, torch.float32)
+    ids = labels.clamp(0, 39)
+    q, k, v, g, _ = attn_operands(1, 5, 2, 1, 8, 8, torch.float32, "token")[0]
+    for call, x in ((lambda x: token_embedding(ids, x).sum(), w), (lambda x: linear_cross_entropy(x, w, labels), h), (lambda x: linear_attention_fn(x, k, v, g).sum(), q)):
+        for transform in (lambda: torch.func.grad(call)(x), lambda: torch.func.jvp(call, (x,), (x,)), lambda: torch.vmap(call)(torch.stack([x, x]))):
+            with pytest.raises((NotImplementedError, RuntimeError)):
+                transform()
+    with pytest.raises(RuntimeError):
+        torch.vmap(lambda i: token_embedding(i, w))(torch.stack([ids, ids]))
