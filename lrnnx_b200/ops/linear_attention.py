@@ -126,9 +126,11 @@ def linear_attention_fn(q, k, v, g, scale=1.0, initial_state=None, return_last_s
         if not return_last_state:
             return out
         return out, initial_state.clone() if initial_state is not None else torch.zeros(batch, heads, q.shape[-1], dv, device=v.device)
-    if recorded(q, k, v, g, initial_state):
-        return LinearAttentionFn.apply(q, k, v, g, float(scale), initial_state, return_last_state)
-    out, last = _forward(_inner(q), _inner(k), _inner(v), g, float(scale), None if initial_state is None else _inner(initial_state), return_last_state)
+    # copies that the kernels need are made here, where autograd sees them: what is saved is then what came in, which second derivatives go by
+    q, k, v, s0 = _inner(q), _inner(k), _inner(v), None if initial_state is None else _inner(initial_state)
+    if recorded(q, k, v, g, s0):
+        return LinearAttentionFn.apply(q, k, v, g, float(scale), s0, return_last_state)
+    out, last = _forward(q, k, v, g, float(scale), s0, return_last_state)
     return (out, last) if return_last_state else out
 
 

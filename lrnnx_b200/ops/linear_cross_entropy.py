@@ -98,7 +98,8 @@ def linear_cross_entropy(hidden, weight, labels, ignore_index=-100, reduction="m
     if labels.numel() == 0:                        # no rows: a sum over nothing, with gradients of zero
         zero = (hidden.sum() + weight[:0].sum()).float()
         return zero.expand(labels.shape) if reduction == "none" else zero
+    # copies that the kernels need are made here, where autograd sees them: what is saved is then what came in, which second derivatives go by
+    hidden, weight = _rows(hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1])), _rows(weight)
     if recorded(hidden, weight):
         return LinearCrossEntropyFn.apply(hidden, weight, labels, ignore_index, _REDUCTIONS[reduction])
-    return _forward(_rows(hidden.reshape(-1, hidden.shape[-1])), _rows(weight), labels.reshape(-1).to(torch.int64).contiguous(), ignore_index,
-                    _REDUCTIONS[reduction], labels.shape)[0]
+    return _forward(hidden, weight, labels.reshape(-1).to(torch.int64).contiguous(), ignore_index, _REDUCTIONS[reduction], labels.shape)[0]

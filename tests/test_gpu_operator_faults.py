@@ -215,3 +215,23 @@ def test_transforms_are_refused():
                 transform()
     with pytest.raises(RuntimeError):
         torch.vmap(lambda i: token_embedding(i, w))(torch.stack([ids, ids]))
+
+
+def test_second_derivatives_of_copied_operands_are_refused():
+    """As for operands that are read in place: transposed ones, ones with other strides and more dimensions, one alone that requires a gradient."""
+    from lrnnx_b200.ops import linear_attention_fn, linear_cross_entropy, token_embedding
+    h, w, labels = loss_operands(6, 40, 24, torch.float32)
+    attn, _, _ = attn_operands(1, 5, 2, 1, 8, 8, torch.float32, "token")
+    turned = lambda x: x.transpose(-1, -2).contiguous().transpose(-1, -2)  # noqa: E731
+    calls = [(lambda x: linear_cross_entropy(turned(x), w, labels), h), (lambda x: linear_cross_entropy(h, turned(x), labels), w),
+             (lambda x: linear_cross_entropy(x.view(2, 3, 24), w, labels.view(2, 3)), h), (lambda x: linear_cross_entropy(turned(x.view(2, 3, 24)), w, labels.view(2, 3)), h),
+             (lambda x: linear_cross_entropy(x[0].expand(6, 24)[:1], w, labels[:1].clamp(min=0)), h), (lambda x: token_embedding(labels.clamp(0, 39), turned(x)).square().sum(), w)]
+    for i in range(5):
+        calls.append((lambda x, i=i: linear_attention_fn(*[(turned(x) if i != 3 else x) if j == i else t for j, t in enumerate(attn[:4])],
+                                                         initial_state=turned(x) if i == 4 else attn[4]).square().sum(), attn[i]))
+    for call, x in calls:
+        x = x.detach().clone().requires_grad_()
+        dx, = torch.autograd.grad(call(x), x, create_graph=True)
+        assert torch.equal(dx, torch.autograd.grad(call(x), x)[0]) and dx.requires_grad
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            (dx.sum() + x.sum()).backward()
