@@ -23,6 +23,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .ops.cross_entropy import cross_entropy
 from .ops.embedding import token_embedding
 from .ops.linear_cross_entropy import linear_cross_entropy
 from .ops.linear_step import linear_step
@@ -186,6 +187,29 @@ class Backbone(nn.Module):
         return self.norm_f(hidden, residual)
 
 
+def _is_bare_product(head):
+    """Whether calling ``head`` is hidden @ weight^T and nothing else."""
+    hooks = ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks")
+    return (type(head) is nn.Linear and head.bias is None and "forward" not in vars(head) and not any(getattr(head, n) for n in hooks)
+            and not torch.nn.modules.module._has_any_global_hook())
+
+
+def _loss_of_logits(logits, labels, ignore_index, reduction):
+    """``linear_cross_entropy`` of logits that a module has formed: the same rows count, in the same reductions."""
+    if reduction not in ("mean", "sum", "none"):
+        raise RuntimeError("loss: reduction must be one of none, mean, sum")
+    if labels.shape != logits.shape[:-1]:
+        raise RuntimeError("loss: labels must have the shape of the logits without their last dimension")
+    classes, flat = logits.shape[-1], labels.reshape(-1).to(torch.int64)
+    logits = logits.reshape(-1, classes)
+    if reduction == "mean" and len(flat):
+        return cross_entropy(logits, flat, ignore_index)
+    on = (flat != ignore_index) & (flat >= 0) & (flat < classes)
+    z = torch.where(on.unsqueeze(1), logits.float(), 0.0)                  # rows without a target may hold anything
+    rows = torch.where(on, torch.logsumexp(z, 1) - z.gather(1, torch.where(on, flat, 0).unsqueeze(1)).squeeze(1), 0.0)
+    return rows.view(labels.shape) if reduction == "none" else rows.sum()
+
+
 class MambaLMHeadModel(nn.Module):
     """``LRNNLMHeadModel(mixer_types=["Mamba"] * n_layer, rms_norm=True)`` of lrnnx on this package's kernels."""
 
@@ -212,17 +236,24 @@ class MambaLMHeadModel(nn.Module):
         sd.setdefault("lm_head.weight", sd["backbone.embedding.weight"])
         return super().load_state_dict(sd, strict=strict)
 
-    def forward(self, input_ids, caches=None, num_last_tokens=0):
+    def forward(self, input_ids, caches=None, num_last_tokens=0, labels=None, ignore_index=-100, reduction="mean"):
+        """Logits (batch, L, vocab); with ``labels`` what ``loss`` describes in their place, so that a wrapper that works in
+        ``forward`` (DistributedDataParallel) averages the gradients of the loss too."""
         hidden = self.backbone(input_ids, caches)
         if num_last_tokens > 0:
             hidden = hidden[:, -num_last_tokens:]
-        return self.lm_head(hidden)
+        if labels is None:
+            return self.lm_head(hidden)
+        if _is_bare_product(self.lm_head):
+            return linear_cross_entropy(hidden, self.lm_head.weight, labels, ignore_index, reduction)
+        return _loss_of_logits(self.lm_head(hidden), labels, ignore_index, reduction)
 
     def loss(self, input_ids, labels, ignore_index=-100, reduction="mean"):
         """``cross_entropy(self(input_ids), labels)`` without the logits: labels (batch, L) are the tokens
         that follow, ``ignore_index`` where none counts; the mean (``reduction``: "mean", "sum", "none") in
-        float32."""
-        return linear_cross_entropy(self.backbone(input_ids), self.lm_head.weight, labels, ignore_index, reduction)
+        float32.  A head that is more than a product with its weight (a bias, a hook, another module) is called, and its
+        logits are formed.  Inside a wrapper call it as ``wrapper(input_ids, labels=labels)``."""
+        return self(input_ids, labels=labels, ignore_index=ignore_index, reduction=reduction)
 
     def step(self, token_ids, caches):
         """token_ids (batch,) -> logits (batch, vocab); caches advance in place."""

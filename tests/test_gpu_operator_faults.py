@@ -235,3 +235,71 @@ def test_second_derivatives_of_copied_operands_are_refused():
         assert torch.equal(dx, torch.autograd.grad(call(x), x)[0]) and dx.requires_grad
         with pytest.raises(RuntimeError, match="differentiated again"):
             (dx.sum() + x.sum()).backward()
+
+
+# ------------------------------------------------------------------------------------------------ the model
+
+
+def _model(dtype, vocab=120):
+    from lrnnx_b200.lm import MambaLMHeadModel
+    torch.manual_seed(0)
+    model = MambaLMHeadModel(32, 1, vocab, device="cuda", dtype=dtype)
+    ids = torch.randint(0, vocab, (2, 19), device="cuda")
+    labels = ids.roll(-1, 1)
+    labels[0, 3:6], labels[1, 7] = -100, vocab + 5
+    return model, ids, labels
+
+
+def _of_logits(logits, labels, reduction):
+    """The definition in float64."""
+    z, y = logits.double().flatten(0, -2), labels.flatten()
+    on = (y >= 0) & (y < z.shape[1])
+    rows = torch.where(on, torch.logsumexp(z, 1) - z.gather(1, y.clamp(0, z.shape[1] - 1).unsqueeze(1)).squeeze(1), 0.0)
+    return rows.view(labels.shape) if reduction == "none" else rows.sum() / (int((y != -100).sum()) if reduction == "mean" else 1)
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("head", ["bias", "adapter", "hook", "pre_hook", "instance"])
+def test_model_loss_calls_its_head(head, reduction):
+    """``loss`` is the loss of ``model(ids)`` whatever module the head is: value and gradients, float32.  Logits are below 2 and losses near log 120, each
+    with a few float32 roundings (2^-24) of 120 terms; the sum has 38 rows."""
+    model, ids, labels = _model(torch.float32)
+    weight = model.lm_head.weight
+    if head == "bias":
+        model.lm_head = torch.nn.Linear(32, 120, device="cuda")
+        model.lm_head.weight = weight
+    elif head == "adapter":
+        model.lm_head = torch.nn.Sequential(torch.nn.Linear(32, 32, device="cuda"), model.lm_head)
+    elif head == "hook":
+        model.lm_head.register_forward_hook(lambda module, args, out: 3.0 * out + 1.0)
+    elif head == "pre_hook":
+        model.lm_head.register_forward_pre_hook(lambda module, args: (2.0 * args[0],))
+    else:
+        model.lm_head.forward = lambda x: torch.nn.functional.linear(x, weight) * 0.5
+    params = list(model.parameters())
+    want = _of_logits(model(ids), labels, reduction)
+    got = model.loss(ids, labels, reduction=reduction)
+    assert got.dtype == torch.float32 and got.shape == want.shape
+    rows = 38 if reduction == "sum" else 1
+    assert bool(((got.double() - want).abs() <= rows * 120 * 2.0 ** -22).all())
+    for a, b in zip(torch.autograd.grad(got.sum(), params), torch.autograd.grad(want.sum(), params)):
+        assert float((a - b).norm()) <= 2e-5 * float(b.norm()) + 1e-12
+
+
+def test_model_loss_goes_through_forward():
+    """What is hung on the model's own call sees the loss too, as a wrapper that calls ``forward`` does."""
+    model, ids, labels = _model(torch.float32)
+    seen = []
+    model.register_forward_hook(lambda module, args, out: seen.append(out.shape))
+    a, b = model.loss(ids, labels), model(ids, labels=labels)
+    assert torch.equal(a, b) and seen == [(), ()]
+    assert model(ids).shape == (2, 19, 120) and model.loss(ids, labels, reduction="none").shape == (2, 19)
+    with pytest.raises(RuntimeError):
+        model.loss(ids, labels[:, :-1])
+    with pytest.raises(RuntimeError):
+        model.loss(ids, labels, reduction="max")
+    model.lm_head = torch.nn.Linear(32, 120, device="cuda")
+    with pytest.raises(RuntimeError):
+        model.loss(ids, labels[:, :-1])
+    with pytest.raises(RuntimeError):
+        model.loss(ids, labels, reduction="max")
