@@ -244,7 +244,7 @@ class MambaLMHeadModel(nn.Module):
             hidden = hidden[:, -num_last_tokens:]
         if labels is None:
             return self.lm_head(hidden)
-        if _is_bare_product(self.lm_head):
+        if _is_bare_product(self.lm_head) and hidden.dtype == self.lm_head.weight.dtype:      # (autocast leaves them different)
             return linear_cross_entropy(hidden, self.lm_head.weight, labels, ignore_index, reduction)
         return _loss_of_logits(self.lm_head(hidden), labels, ignore_index, reduction)
 

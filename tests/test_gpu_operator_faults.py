@@ -303,3 +303,16 @@ def test_model_loss_goes_through_forward():
         model.loss(ids, labels[:, :-1])
     with pytest.raises(RuntimeError):
         model.loss(ids, labels, reduction="max")
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_model_loss_under_autocast(reduction):
+    """Float32 weights under autocast leave hidden states of another type than the head's weight, which the model's call takes and its loss
+    has to as well.  Logits below 2 are bfloat16, half a step 2^-8 of a value: a row's loss is off by two of them at most, with 38 rows in a sum."""
+    model, ids, labels = _model(torch.float32)
+    with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16):      # (the mixer's backward pass wants one type)
+        logits = model(ids)
+        got = model.loss(ids, labels, reduction=reduction)
+    assert logits.dtype == torch.bfloat16 and got.dtype == torch.float32
+    want = _of_logits(logits, labels, reduction)
+    assert bool(((got.double() - want).abs() <= (38 if reduction == "sum" else 1) * 2 * 2.0 ** -8 * 2).all())
