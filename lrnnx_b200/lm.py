@@ -27,7 +27,7 @@ from .ops.cross_entropy import cross_entropy
 from .ops.embedding import token_embedding
 from .ops.linear_cross_entropy import linear_cross_entropy
 from .ops.linear_step import linear_step
-from .ops.mamba_block import causal_conv1d_fn, causal_conv1d_update, rms_norm_fn
+from .ops.mamba_block import _DT, causal_conv1d_fn, causal_conv1d_update, rms_norm_fn
 from .ops.mamba_inner import mamba_inner_fn
 from .ops.selective_scan import selective_scan_fn
 from .ops.selective_state_update import selective_state_update
@@ -45,13 +45,14 @@ class RMSNorm(nn.Module):
 
 
 class TokenEmbedding(nn.Embedding):
-    """nn.Embedding whose lookup and gradient are this package's kernels (``token_embedding``)."""
-
-    def __init__(self, num_embeddings, embedding_dim, padding_idx=None, device=None, dtype=None):
-        super().__init__(num_embeddings, embedding_dim, padding_idx=padding_idx, device=device, dtype=dtype)
+    """nn.Embedding whose lookup and gradient are this package's kernels (``token_embedding``).  What they do not have (``max_norm``,
+    ``scale_grad_by_freq``, sparse gradients, weights of another type or not on a GPU) is nn.Embedding's own."""
 
     def forward(self, ids):
-        return token_embedding(ids, self.weight, padding_idx=self.padding_idx)
+        weight = self.weight
+        if not weight.is_cuda or weight.dtype not in _DT or self.max_norm is not None or self.scale_grad_by_freq or self.sparse:
+            return super().forward(ids)
+        return token_embedding(ids, weight, padding_idx=self.padding_idx)
 
 
 class _InProjFn(torch.autograd.Function):
