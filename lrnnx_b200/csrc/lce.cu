@@ -22,11 +22,15 @@
 // swizzled tiles, of K-major or of MN-major layout.
 //
 // float32 operands are split into three bfloat16 (8 bits of mantissa each) and multiplied as six products of the
-// planes, the small ones first; what is left out is below 2^-24.  The tensor core truncates when it adds into its
-// accumulator, an error to one side that grows with the length of the chain, so that long contractions are cut into
-// chains of kSegSteps whose sums are added up in float32, rounded to nearest: for the gradients in the epilogue's registers
-// (through memory they cost dz W 32 us of 204 at 2031 x 16411 x 509).  (An infinite float32 operand gives NaN
+// planes, the small ones first; what is left out is below 2^-24.  (An infinite float32 operand gives NaN
 // where its product with the rest of a split is none.)
+//
+// The tensor core truncates when it adds into its accumulator, an error to one side that grows with the length of the chain: over
+// 8192 features a loss came out 3e-5 too small.  So the contractions of float32 are cut into chains of at most kSegSteps stages, and that of z into
+// chains of kSegSteps16 for 16-bit operands, whose sums are added up in the epilogue's registers, rounded to nearest (through
+// memory they cost dz W 32 us of 204 at 2031 x 16411 x 509).  The gradients of 16-bit operands are rounded to 2^-8 or 2^-11 and stay one
+// chain, and so does z where one chain holds it: cut in two, the forward over 2048 features takes 2.5 % longer (333 x 50280 float16
+// 88.1 -> 90.5 us, 4096 x 50280 bfloat16 543 -> 557 us).
 //
 // Measured (one B200, 16384 x 50280 x 768 bfloat16, forward and backward 4.34 ms, 1.17 PFLOP/s over the four products, under the power
 // limit as a library product would be): z and its log-sum-exp 827-844 us (tensor pipe 82 %), the two pieces of dz 479 us each
@@ -55,12 +59,12 @@ constexpr int LCE_THREADS = 384;                 // 4 warps that issue, 8 that e
 constexpr int LCE_SMEM = NST * ST_BYTES + 8 * STAGING + 1024;
 constexpr uint32_t LCE_WAIT = 1u << 24;
 constexpr int64_t kPieceBytes = int64_t(1) << 30;
-constexpr int kSegSteps = 8;              // float32 only: stages (of 64) in one accumulation chain of the leading product
+constexpr int kSegSteps = 8;              // float32: most stages (of 64) of the contraction in one accumulation chain, which has their six products
+constexpr int kSegSteps16 = 16;           // float16 and bfloat16: the same of z
 constexpr int kPieceStages = 64;           // what a piece costs besides, in stages: launches, the sums of dH read and written
 constexpr int kMaxSplits = 32;            // blocks that share the contraction of a tile
 
-// EPI_SUM: as EPI_OUT, the sums of a tile's chains kept in registers
-enum { EPI_LSE = 0, EPI_DZ = 1, EPI_OUT = 2, EPI_SUM = 3 };
+enum { EPI_LSE = 0, EPI_DZ = 1, EPI_OUT = 2 };
 
 struct LceGemm {
   CUtensorMap a, b, out;       // (inner, rows, plane); out: dz
@@ -201,7 +205,8 @@ template <typename T> __device__ __forceinline__ void store_row(T *dst, const fl
   }
 }
 
-template <int EPI>
+// CUT: the contraction of a tile is more than one chain, whose sums are kept in registers
+template <int EPI, bool CUT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LCE_THREADS, 1) lce_gemm_kernel(const __grid_constant__ LceGemm p) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -313,12 +318,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LCE_THREADS, 1) lce_
       const int row = m0 + q * 32 + lane, c0 = n0 + half * (TN / 2);      // this thread's row and 128 columns
       const bool in = row < p.rows;
       const int kb = k_from(t), ke = k_to(t);
-      float sums[EPI == EPI_SUM ? TN / 64 : 1][32];
+      float sums[CUT ? TN / 64 : 1][32] = {};
       for (int k0 = kb; k0 < ke; k0 += p.seg, ++ch) {
+        const bool whole = !CUT || k0 + p.seg >= ke;                     // the tile's last chain
         // what the epilogue needs besides is loaded before the wait
         float lse2 = 0.f, sc = 0.f;
         int at = -1;                                                     // the label's column within this thread's columns
-        if (EPI < EPI_OUT && in) {
+        if (EPI < EPI_OUT && in && whole) {
           const int64_t label = p.labels[row];
           if (label != p.ignore_index && label >= 0 && label < p.classes) {
             const int64_t c = label - p.col0 - c0;
@@ -332,13 +338,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LCE_THREADS, 1) lce_
         if (!mbar_wait(&pipe.acc_full[ch & 1], (ch >> 1) & 1, LCE_WAIT)) { ok = false; break; }
         tc_fence_after();
         const uint32_t ta = tmem + (ch & 1) * TN + ((uint32_t)(q * 32) << 16) + half * (TN / 2);
+        const auto emptied = [&]() {                                     // the accumulator has been read
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_at(of_first(&pipe.acc_empty[ch & 1]));
+        };
+        if constexpr (CUT) {
+#pragma unroll
+          for (int c = 0; c < TN / 32; ++c) {           // 16 at a time: with 32 more registers beside the 128 sums are spilled
+            float v[16];
+            __syncwarp();                              // lanes come from their own waits, and from the last tile's stores
+            tmem_ld16(ta + c * 16, v);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) sums[c >> 1][(c & 1) * 16 + j] += v[j];
+          }
+          emptied();
+          if (!whole) continue;
+        }
         if constexpr (EPI == EPI_LSE) {
           float m = -INFINITY, sum = 0.f, target = 0.f;                   // m in units of log2
-#pragma unroll
-          for (int c = 0; c < TN / 64; ++c) {
-            float v[32];
-            __syncwarp();
-            tmem_ld32(ta + c * 32, v);
+          const auto take = [&](float (&v)[32], int c) {
             const int left = p.cols - (c0 + c * 32);
             if (left < 32) {
 #pragma unroll
@@ -361,21 +380,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LCE_THREADS, 1) lce_
             }
             sum = fmaf(sum, ex2(m - off), s0 + s1);                       // the first time 0 * 2^-inf
             m = nm;
+          };
+#pragma unroll
+          for (int c = 0; c < TN / 64; ++c) {
+            if constexpr (CUT) {
+              asm volatile("" : "+f"(m), "+f"(sum), "+f"(target)::"memory");      // one 32 after the other: together they do not fit the registers
+              take(sums[c], c);
+            } else {
+              float v[32];
+              __syncwarp();
+              tmem_ld32(ta + c * 32, v);
+              take(v, c);
+            }
           }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) arrive_at(of_first(&pipe.acc_empty[ch & 1]));
+          if constexpr (!CUT) emptied();
           if (in) {
             p.part[(int64_t)(n_of(t) * 2 + half) * p.rows + row] = make_float2(m, sum);
             if (at >= 0) p.target[row] = target;
           }
         } else if constexpr (EPI == EPI_DZ) {
-#pragma unroll 1
-          for (int c = 0; c < TN / 128; ++c) {
-            float v[64];
-            __syncwarp();
-            tmem_ld32(ta + c * 64, *reinterpret_cast<float(*)[32]>(v));
-            tmem_ld32(ta + c * 64 + 32, *reinterpret_cast<float(*)[32]>(v + 32));
+          const auto give = [&](float (&v)[64], int c) {
 #pragma unroll
             for (int j = 0; j < 64; ++j) v[j] = ex2(fmaf(v[j], kLog2e, -lse2));
             if ((at >> 6) == c) {
@@ -395,26 +419,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LCE_THREADS, 1) lce_
                 for (int j = 0; j < 64; ++j) v[j] -= __bfloat162float(__float2bfloat16_rn(v[j]));
               }
             }
+          };
+          if constexpr (CUT) {
+#pragma unroll
+            for (int c = 0; c < TN / 128; ++c) give(*reinterpret_cast<float(*)[64]>(sums[2 * c]), c);
+          } else {
+#pragma unroll 1
+            for (int c = 0; c < TN / 128; ++c) {
+              float v[64];
+              __syncwarp();
+              tmem_ld32(ta + c * 64, *reinterpret_cast<float(*)[32]>(v));
+              tmem_ld32(ta + c * 64 + 32, *reinterpret_cast<float(*)[32]>(v + 32));
+              give(v, c);
+            }
+            emptied();
           }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) arrive_at(of_first(&pipe.acc_empty[ch & 1]));
         } else {
           float *acc = p.acc + (int64_t)(t / (p.nt * p.mt)) * p.rows * p.acc_rs;
           const float unit = unit_back(p.common, p.dtype);
-          if constexpr (EPI == EPI_SUM) {
-#pragma unroll
-            for (int c = 0; c < TN / 64; ++c) {
-              float v[32];
-              __syncwarp();                              // lanes come from their own waits, and from the last tile's stores
-              tmem_ld32(ta + c * 32, v);
-#pragma unroll
-              for (int j = 0; j < 32; ++j) sums[c][j] = k0 == kb ? v[j] : sums[c][j] + v[j];
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) arrive_at(of_first(&pipe.acc_empty[ch & 1]));
-            if (k0 + p.seg < ke) continue;
+          if constexpr (CUT) {
             // 32 x 32 of them, a row a lane, are turned over in shared memory, so that a row leaves as one line
             float *turn = reinterpret_cast<float *>(staging);
             const int r0 = m0 + q * 32, n = min(32, p.rows - r0);
@@ -469,9 +492,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LCE_THREADS, 1) lce_
                 else store_row<__half>(reinterpret_cast<__half *>(p.dst) + i, v, n, vec);
               }
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) arrive_at(of_first(&pipe.acc_empty[ch & 1]));
+            emptied();
           }
         }
       }
@@ -750,12 +771,18 @@ int pack(const void *src, int64_t rs, int64_t rows, const b200_lce_args &a, cons
   return launch_status();
 }
 
-template <int EPI> int launch_gemm(const LceGemm &g, cudaStream_t st) {
-  cudaError_t e = cudaFuncSetAttribute(lce_gemm_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, LCE_SMEM);
+template <int EPI, bool CUT> int launch_gemm_of(const LceGemm &g, cudaStream_t st) {
+  cudaError_t e = cudaFuncSetAttribute(lce_gemm_kernel<EPI, CUT>, cudaFuncAttributeMaxDynamicSharedMemorySize, LCE_SMEM);
   if (e != cudaSuccess) { set_error("cudaFuncSetAttribute: %s", cudaGetErrorString(e)); return (int)e; }
   const int tiles = g.mt * g.nt * (EPI >= EPI_OUT ? g.splits : 1), sms = sm_count_current();
-  lce_gemm_kernel<EPI><<<(unsigned)(2 * (tiles < sms / 2 ? tiles : sms / 2)), LCE_THREADS, LCE_SMEM, st>>>(g);
+  lce_gemm_kernel<EPI, CUT><<<(unsigned)(2 * (tiles < sms / 2 ? tiles : sms / 2)), LCE_THREADS, LCE_SMEM, st>>>(g);
   return launch_status();
+}
+
+// (the sums of float32 gradients take the same path when they are one chain: their results leave a row a line)
+template <int EPI> int launch_gemm(const LceGemm &g, cudaStream_t st) {
+  const bool cut = EPI == EPI_OUT ? g.dtype == B200_F32 : g.seg < g.nk;
+  return cut ? launch_gemm_of<EPI, true>(g, st) : launch_gemm_of<EPI, false>(g, st);
 }
 
 uint32_t idesc_of(int dtype, bool a_mn, bool b_mn) { return idesc_f16(dtype == B200_F16 ? 0u : 1u, a_mn, b_mn, 2 * TM, TN); }
@@ -776,7 +803,8 @@ int gemm_z(LceGemm &g, const b200_lce_args &a, const Plan &q, const Operands &o,
   g.mt = (int)((a.rows + 2 * TM - 1) / (2 * TM));
   g.nt = (cols + TN - 1) / TN;
   g.nk = (a.features + TK - 1) / TK;
-  g.seg = g.nk;
+  const int chains = (g.nk + (q.planes == 3 ? kSegSteps : kSegSteps16) - 1) / (q.planes == 3 ? kSegSteps : kSegSteps16);
+  g.seg = (g.nk + chains - 1) / chains;
   g.passes = q.planes == 3 ? 6 : 1;
   g.b_row0 = c0;
   g.idesc = idesc_of(a.dtype, false, false);
@@ -915,7 +943,7 @@ extern "C" int b200_lce_bwd(const b200_lce_args *args, void *stream) {
       g.dst_rs = a.dhidden_rs;
       g.add = pc > 0;
       g.last = pc == q.n_pieces - 1 && g.splits == 1;
-      if (int e = a.dtype == B200_F32 ? launch_gemm<EPI_SUM>(g, st) : launch_gemm<EPI_OUT>(g, st)) return e;
+      if (int e = launch_gemm<EPI_OUT>(g, st)) return e;
       if (g.splits > 1 && pc == q.n_pieces - 1)
         if (int e = fold(g, st)) return e;
     }
@@ -936,7 +964,7 @@ extern "C" int b200_lce_bwd(const b200_lce_args *args, void *stream) {
       g.splits = q.splits_w;
       g.per = q.per_w;
       g.last = g.splits == 1;
-      if (int e = a.dtype == B200_F32 ? launch_gemm<EPI_SUM>(g, st) : launch_gemm<EPI_OUT>(g, st)) return e;
+      if (int e = launch_gemm<EPI_OUT>(g, st)) return e;
       if (g.splits > 1)
         if (int e = fold(g, st)) return e;
     }

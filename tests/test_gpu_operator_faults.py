@@ -91,6 +91,29 @@ def test_a_row_weight_that_is_not_finite_stays_in_its_row(value, dtype):
     assert torch.equal(got[rows], clean[rows]) and not bool(torch.isfinite(got[7]).any())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("features", [520, 1032, 1536, 8192])
+def test_long_contractions_are_not_one_chain(features, dtype):
+    """Every product is positive and the labels' class has none, so that what the tensor core truncates (2^-23 of the running sum at each 16
+    features) adds up to one side in the log-sum-exp alone.  Chains hold 512 features (float32, with 8 steps' worth for the
+    five small products) or 1024, and their sums are rounded."""
+    from lrnnx_b200.ops import linear_cross_entropy
+    gen = torch.Generator().manual_seed(features)
+    h = torch.randn(150, features, generator=gen).abs().to(dtype).cuda()
+    w = (torch.randn(600, features, generator=gen).abs() * (30 / (0.64 * features))).to(dtype).cuda()
+    w[0] = 0
+    labels = torch.zeros(150, dtype=torch.int64, device="cuda")
+    hh, ww = h.requires_grad_(), w.requires_grad_()
+    up = torch.full((150,), 4.0, device="cuda")
+    loss = linear_cross_entropy(hh, ww, labels, reduction="none")
+    ref = reference(h.detach(), w.detach(), labels, up)
+    chain = 512 if dtype == torch.float32 else 1024
+    z = (h.detach().double() @ w.detach().double().t()).amax(1)
+    Z = z * (min(features, chain) / 16 + 8 + features // chain + 1) * 2.0 ** -23
+    assert bool(((loss.detach().double() - ref["loss"]).abs() <= Z + 2.0 ** -21 * (1 + ref["lse"])).all())
+    check(torch.autograd.grad(loss, (hh, ww), up), ref, h.detach(), w.detach(), dtype)
+
+
 # ------------------------------------------------------------------------------------------------ linear attention
 
 
