@@ -145,6 +145,8 @@ def linear_attention_step(state, q, k, v, g, scale=1.0, state_batch_indices=None
     slots, ss = state.shape[0], state.stride()
     if state.shape[1:] != (heads, dk, dv) or ss[3] != 1 and dv > 1:
         raise RuntimeError("linear_attention_step: state must be (batch, heads, dk, dv) with dv contiguous")
+    if 0 in ss and any(x == 0 and n > 1 for x, n in zip(ss, state.shape)):
+        raise RuntimeError("linear_attention_step: elements of the state must not share memory, it is updated in place")
     if state.dtype != q.dtype and state.dtype != torch.float32:
         raise RuntimeError("linear_attention_step: the state must be float32 or of the dtype of q")
     if state_batch_indices is None:

@@ -141,6 +141,19 @@ def test_a_decay_reaches_no_earlier_step(t, value, dtype):
         within(name, x[clean], want[i][clean], ((F + 2 * u) * mag[i] + u * want[i].abs() + tiny)[clean])
 
 
+def test_step_refuses_a_state_that_shares_memory():
+    """A broadcast state would be read and written by several blocks at once."""
+    from lrnnx_b200.ops import linear_attention_step
+    (q, k, v, g, _), _, _ = attn_operands(3, 1, 4, 2, 16, 8, torch.float32, "token")
+    ops = [x[:, 0] for x in (q, k, v, g)]
+    one = torch.zeros(1, 4, 16, 8, device="cuda")
+    for state in (one.expand(3, -1, -1, -1), torch.zeros(3, 1, 16, 8, device="cuda").expand(-1, 4, -1, -1), torch.zeros(3, 4, 1, 8, device="cuda").expand(-1, -1, 16, -1)):
+        with pytest.raises(RuntimeError, match="share memory"):
+            linear_attention_step(state, *ops)
+    out = linear_attention_step(one.expand(1, 4, 16, 8), *[x[:1] for x in ops])            # a batch of one has no pitch to speak of
+    assert out.shape == (1, 4, 8) and bool(one.any())
+
+
 # ------------------------------------------------------------------------------------------------ waits
 
 
