@@ -154,6 +154,27 @@ def test_step_refuses_a_state_that_shares_memory():
     assert out.shape == (1, 4, 8) and bool(one.any())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("b,n,heads,groups,dk,dv,decay", [(2, 1500, 2, 1, 64, 48, "token"), (1, 2048, 2, 2, 128, 64, "token"), (1, 1500, 2, 2, 64, 64, "strong"),
+                                                          (2, 600, 3, 1, 40, 32, "strong")])
+def test_decay_gradients_keep_32_bits(b, n, heads, groups, dk, dv, decay, dtype):
+    """A decay's gradient is a sum over pairs of steps across it.  The 2-norm of its error against the root of the sums of the pairs' squares,
+    which the recurrence of squared operands and doubled decays gives: a pair's product is off by its operands' split (2^-22), the decays'
+    exponentials (2^-22) and the truncations of at most 16 partial sums on its way (2^-20), independent of one another: 2^-19 in all.  A
+    gradient from sums of q dq - k dk along the sequence has the error of those sums, which with strong decays are many times the pairs'."""
+    from lrnnx_b200.ops import linear_attention_fn
+    ops, dout, dlast = attn_operands(b, n, heads, groups, dk, dv, dtype, "token", seed=31)
+    if decay == "strong":
+        ops[3] = torch.full_like(ops[3], -3.0)
+    want = with_gradients(ops, 1.0, dout, dlast)[5]
+    square = lambda x: x.double().square()  # noqa: E731
+    pairs = with_gradients([square(x) for x in ops[:3]] + [2 * ops[3].double(), square(ops[4])], 1.0, square(dout), square(dlast))[5].sqrt()
+    leaves = [x.detach().requires_grad_() for x in ops]
+    o, last = linear_attention_fn(*leaves[:4], initial_state=leaves[4], return_last_state=True)
+    got, = torch.autograd.grad([o, last], leaves[3:4], [dout, dlast])
+    assert float((got.double() - want).norm()) <= 2.0 ** -19 * float(pairs.norm())
+
+
 # ------------------------------------------------------------------------------------------------ waits
 
 
