@@ -373,3 +373,48 @@ def test_model_loss_under_autocast(reduction):
     assert logits.dtype == torch.bfloat16 and got.dtype == torch.float32
     want = _of_logits(logits, labels, reduction)
     assert bool(((got.double() - want).abs() <= (38 if reduction == "sum" else 1) * 2 * 2.0 ** -8 * 2).all())
+
+
+def test_calls_of_two_threads_at_once():
+    """Threads with a stream each, which also look the driver's functions up for the first time together: the results of one thread alone."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    here = Path(__file__).resolve().parent
+    code = """
+import sys, threading, torch
+sys.path[:0] = [%r, %r]
+from test_gpu_linear_attention import make as attn_operands
+from test_gpu_linear_cross_entropy import make as loss_operands
+from lrnnx_b200 import _lib
+from lrnnx_b200.ops import linear_attention_fn, linear_attention_step, linear_cross_entropy, token_embedding
+dt = torch.bfloat16
+h, w, labels = loss_operands(300, 2000, 64, dt)
+ids = labels.clamp(min=0)
+(q, k, v, g, s0), dout, dlast = attn_operands(2, 700, 3, 1, 64, 64, dt, "token")
+def run():
+    L = [t.detach().requires_grad_() for t in (h, w, q, k, v, g)]
+    loss, e, o = linear_cross_entropy(L[0], L[1], labels), token_embedding(ids, L[1]), linear_attention_fn(*L[2:])
+    s = s0.clone()
+    y = linear_attention_step(s, q[:, 0], k[:, 0], v[:, 0], g[:, 0])
+    return [loss.detach(), o.detach(), y, s, *torch.autograd.grad([loss, e, o], L, [None, torch.ones_like(e), dout])]
+got, start = [None] * 6, threading.Barrier(6)
+def thread(i):
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        start.wait()
+        for _ in range(10):
+            got[i] = run()
+    stream.synchronize()
+torch.cuda.synchronize()
+threads = [threading.Thread(target=thread, args=(i,)) for i in range(6)]
+for t in threads: t.start()
+for t in threads: t.join()
+want = run()
+torch.cuda.synchronize()
+assert all(len(r) == len(want) and all(torch.equal(a, b) for a, b in zip(r, want)) for r in got)
+assert _lib.lib().b200_device_status() == 0
+print("same")
+""" % (str(here), str(here.parent))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "same" in r.stdout, r.stdout + r.stderr
