@@ -554,7 +554,7 @@ int b200_lce_bwd(const b200_lce_args *args, void *stream);
  * Embedding lookup with a scale, and its gradient by sorted tokens; replaces nn.Embedding in
  * lrnnx's backbone (lrnnx/architectures/language_model.py:198-511) and the scatter of its backward.
  *   out[t] = scale weight[ids[t]];  an id outside [0, classes) reads nothing and gives NaN
- *   dweight[v] = scale sum_{t: ids[t] = v} dout[t], float32 sums in the order of t; zero for other
+ *   dweight[v] = scale sum_{t: ids[t] = v} dout[t], float32 sums in an order that ids as a whole fixes; zero for other
  *   rows and for padding_idx (-1: none)
  *   ids (tokens) int64 (ids_wide 1) or int32;  weight, dweight (classes, features), out, dout
  *   (tokens, features): dtype, features contiguous;  dweight dense, written whole
@@ -581,7 +581,8 @@ int b200_embed_bwd(const b200_embed_args *args, void *stream);
  * its selective scan):  S_t = exp(g_t) S_{t-1} + k_t v_t^T,  out_t = scale S_t^T q_t.
  *   q, k (batch, seqlen, groups, dk), v, out (batch, seqlen, heads, dv): dtype, sizes contiguous, dk and dv up to
  *   128; head h reads group h / (heads / groups)
- *   g (batch, seqlen, heads): log decays, float32 or dtype, any strides (0 for a decay per head); -inf empties the state
+ *   g (batch, seqlen, heads): log decays, float32 or dtype, any strides (0 for a decay per head); -inf empties
+ *   the state (times zero: one that is infinite or NaN becomes NaN)
  *   s0 float32 (batch, heads, dk, dv), dv contiguous, nullable (zeros); last float32, dense: nullable
  *   backward: dout like out; dlast float32, dense, nullable;
  *   dq, dk_out, dv_out dense, dtype; dg (nullable) of g's dtype, dense (batch, seqlen, heads), or (heads) with

@@ -4,11 +4,12 @@
 //
 // Forward: a copy of rows, 16 bytes a thread; bound by HBM, and by the launch for the few tokens of a decoding step.
 // Backward: the (id, position) pairs are sorted by id, stably (least significant digit first, up to 9 bits a pass), so
-// that rows of one id are added in the order of their positions: no atomics, the same bits every time.  One cluster of eight
+// that rows of one id lie in the order of their positions: no atomics, the same bits every time.  One cluster of eight
 // thread blocks sorts, with its digit counts in distributed shared memory; the other SMs clear the gradient meanwhile.
 // Every 16 sorted pairs are a piece, whatever ids they hold, so a frequent token does not make one block slow: a thread
 // block adds up the runs of equal ids in its piece in float32 and writes a run that lies inside it; what a run crossing
-// borders has in a piece goes to the workspace and is joined by the piece where the run begins.  Each row is rounded
+// borders has in a piece goes to the workspace and is joined by the piece where the run begins, in eight interleaved shares.  Where
+// the borders fall within a run depends on the whole list of ids, and with them the order of its sums.  Each row is rounded
 // once.  Ids outside [0, classes) and the padding id sort behind all others and are not summed.
 //
 // Measured (one B200, 16384 tokens as frequent as in text, 50280 x 768 bfloat16): lookup 9 us, sort and clearing 24 us (77 MB cleared;

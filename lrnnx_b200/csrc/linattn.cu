@@ -92,7 +92,8 @@ __device__ __forceinline__ float ex2a(float x) {
   return y;
 }
 // A sum in two floats (the second what the first leaves out): 48 bits, at a tenth of the latency of 64-bit arithmetic in a
-// chain that a whole block waits for.
+// chain that a whole block waits for.  The error of a rounded sum by Knuth's two-sum (The Art of Computer Programming, 2, 4.2.2),
+// numbers of two parts added as Dekker does (Numerische Mathematik 18, 1971).
 struct Two { float h, l; };
 __device__ __forceinline__ Two two(float x) { return Two{x, 0.f}; }
 __device__ __forceinline__ Two operator+(Two a, Two b) {
@@ -178,7 +179,7 @@ __device__ __forceinline__ void chunk_decays(const Walk &p, int b, int h, int i0
 __device__ __forceinline__ float decay_between(const Decays &d, int r, int c) { return ex2a((d.hi[r] - d.hi[c]) + (d.lo[r] - d.lo[c])); }
 
 // The dots of a chunk's steps become what the pairs of steps on both sides of a step give to its decay, by one warp, N steps a
-// lane, in 64 bits.  Forwards (x . dq, pairs whose earlier step is before the chunk): the sum from the step on.  Backwards (x . dk,
+// lane, summed in two floats and kept as one.  Forwards (x . dq, pairs whose earlier step is before the chunk): the sum from the step on.  Backwards (x . dk,
 // pairs whose later step is after the chunk, and pairs within it, by row and column sums without the diagonal): the sum
 // over the steps before it in time.
 template <int N> __device__ __forceinline__ void chunk_runs(const Walk &p, int tile, int bh, int i0, int lane, const Two (&v)[N], float dots) {

@@ -2,7 +2,8 @@
 
 ``token_embedding(ids, weight)`` takes the place of nn.Embedding in the language model
 (lrnnx/architectures/language_model.py:198-511).  Its gradient adds the rows of each token in float32 in
-the order of their positions, so it is the same at every call, and rounds once.
+an order that the list of ids fixes (partial sums of up to 16 neighbours in the sorted list, then eight interleaved shares of those), so it
+is the same at every call, and rounds once; other ids in the list can change a row's last bits.
 """
 from __future__ import annotations
 
