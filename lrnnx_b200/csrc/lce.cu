@@ -36,7 +36,7 @@
 // limit as a library product would be): z and its log-sum-exp 827-844 us (tensor pipe 82 %), the two pieces of dz 479 us each
 // (74 %: the epilogue's stores), dz W 439-456 us each (90 %), dz^T H 510 and 438 us (80 %: 297
 // tiles on 74 pairs), with pieces of equal size; cut as piece_of does, 65 us less for the whole.  float32,
-// 2031 x 16411 x 509: 0.81 ms, six times the products: z 131 us, dz 153, dz W 163, dz^T H 171, operands split in both passes 57.
+// 2031 x 16411 x 509: 0.82 ms, six times the products: z 131 us, dz 153, dz W 163, dz^T H 171, operands split in both passes 57.
 #include "common.cuh"
 #include "dispatch.h"
 #include "tc_common.cuh"
@@ -384,7 +384,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LCE_THREADS, 1) lce_
 #pragma unroll
           for (int c = 0; c < TN / 64; ++c) {
             if constexpr (CUT) {
-              asm volatile("" : "+f"(m), "+f"(sum), "+f"(target)::"memory");      // one 32 after the other: together they do not fit the registers
               take(sums[c], c);
             } else {
               float v[32];

@@ -189,9 +189,9 @@ class Backbone(nn.Module):
 
 
 def _is_bare_product(head):
-    """Whether calling ``head`` is hidden @ weight^T and nothing else."""
+    """Whether calling ``head`` is hidden @ weight^T of an ordinary weight and nothing else."""
     hooks = ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks")
-    return (type(head) is nn.Linear and head.bias is None and "forward" not in vars(head) and not any(getattr(head, n) for n in hooks)
+    return (type(head) is nn.Linear and type(head.weight) in (nn.Parameter, torch.Tensor) and head.bias is None and "forward" not in vars(head) and not any(getattr(head, n) for n in hooks)
             and not torch.nn.modules.module._has_any_global_hook())
 
 

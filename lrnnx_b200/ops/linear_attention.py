@@ -111,9 +111,10 @@ def _check(name, dims, q, k, v, g, state):
 def linear_attention_fn(q, k, v, g, scale=1.0, initial_state=None, return_last_state=False):
     """q, k (batch, length, groups, dk), v (batch, length, heads, dv) of one dtype (float32, float16, bfloat16), any strides; heads a
     multiple of groups, dk and dv up to 128.  g: log decays, (batch, length, heads) or (heads,), float32 or the dtype of
-    q; -inf starts from an empty state at that step (a new document; the state is multiplied by zero, so that one that is not finite is NaN from there).  ``initial_state`` float32 (batch, heads, dk, dv)
-    is the state before the first step.  Returns out (batch, length, heads, dv), and with ``return_last_state`` the float32
-    state after the last step.  An infinite or NaN value reaches its own step and later ones, no earlier result.  Gradients for q, k, v, g and
+    q; -inf starts from an empty state at that step (a new document; the state is multiplied by zero, so that one that is
+    not finite is NaN from there).  ``initial_state`` float32 (batch, heads, dk, dv) is the state before the first step.
+    Returns out (batch, length, heads, dv), and with ``return_last_state`` the float32 state after the last step.  An
+    infinite or NaN value reaches its own step and later ones, no earlier result.  Gradients for q, k, v, g and
     initial_state; forward-mode derivatives are an error."""
     _check("linear_attention_fn", 4, q, k, v, g, initial_state)
     batch, length, heads, dv = v.shape
@@ -137,8 +138,10 @@ def linear_attention_fn(q, k, v, g, scale=1.0, initial_state=None, return_last_s
 def linear_attention_step(state, q, k, v, g, scale=1.0, state_batch_indices=None):
     """One token: state (batch, heads, dk, dv), float32 or the dtype of q, dv contiguous, is updated in place; q, k (batch,
     groups, dk), v (batch, heads, dv), g (batch, heads) or (heads,).  With ``state_batch_indices`` (batch,) int32 the
-    state is a pool and entry b advances slot ``state_batch_indices[b]``, no slot twice (blocks would race for it); an entry outside the pool has no
-    state and gives zeros.  A decay of -inf multiplies the state by zero: a slot to be used anew that may hold anything is cleared first.  Returns out (batch, heads, dv).  No gradient; legal inside CUDA-graph capture."""
+    state is a pool and entry b advances slot ``state_batch_indices[b]``, no slot twice (blocks would race for it); an
+    entry outside the pool has no state and gives zeros.  A decay of -inf multiplies the state by zero: a slot to be used
+    anew that may hold anything is cleared first.  Returns out (batch, heads, dv).  No gradient; legal inside CUDA-graph
+    capture."""
     _check("linear_attention_step", 3, q, k, v, g, state)
     batch, heads, dv = v.shape
     _, groups, dk = q.shape

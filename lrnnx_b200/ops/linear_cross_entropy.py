@@ -81,10 +81,10 @@ def linear_cross_entropy(hidden, weight, labels, ignore_index=-100, reduction="m
     that are not ``ignore_index`` (zero where there are none), their sum, or with ``reduction="none"``
     the loss of every row, zero for ignored ones.  hidden (..., features) and weight (classes,
     features) float32, float16 or bfloat16 alike; labels (...) integer.  A label outside [0, classes)
-    has no loss and no gradient, as in ``cross_entropy``; a row without a target may hold anything.  float32 operands
-    are multiplied as sums of three bfloat16, so that an infinite one gives NaN (also where a product with it is infinite): classes are not masked by
-    weights of -inf.  Gradients for hidden
-    and weight; forward-mode derivatives are an error."""
+    has no loss and no gradient, as in ``cross_entropy``; a row without a target may hold anything.
+    float32 operands are multiplied as sums of three bfloat16, so that an infinite one gives NaN (also where
+    a product with it is infinite): classes are not masked by weights of -inf.  Gradients for hidden and
+    weight; forward-mode derivatives are an error."""
     if reduction not in _REDUCTIONS:
         raise RuntimeError(f"linear_cross_entropy: reduction must be one of {', '.join(_REDUCTIONS)}")
     if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1] or labels.shape != hidden.shape[:-1]:
